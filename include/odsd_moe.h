@@ -37,6 +37,9 @@
  *                       parameter_loader.py:424-539 is where a loader would call it)
  *   odsd_kv_store      store_kvcache                           demo/src/layers/attention.py:32-79
  *   odsd_paged_attention  _fallback_decode_attention / flash_attn_with_kvcache   attention.py:252-352
+ *   odsd_linear        F.linear around the block               demo/src/layers/attention.py:169-288
+ *   odsd_rotary        q_norm / k_norm, rotary_emb, store      demo/src/layers/attention.py:209-228
+ *   odsd_verify_drafts  acceptance of a verify step            demo/src/execution/cb_executor.py:261-300
  */
 #ifndef ODSD_MOE_H
 #define ODSD_MOE_H
@@ -68,7 +71,11 @@ typedef enum odsd_status {
                                  ODSD_STATIC_SCRATCH_BYTES of scratch memory             */
 } odsd_status;
 
-enum { ODSD_DT_F32 = 0, ODSD_DT_BF16 = 1, ODSD_DT_F16 = 2 /* attention entry point only */ };
+enum { ODSD_DT_F32 = 0, ODSD_DT_BF16 = 1, ODSD_DT_F16 = 2 /* attention and dense entry points only */ };
+
+/* activations of odsd_linear: y, max(y, 0), y / (1 + exp(-y)), y Phi(y), and the latter's tanh form
+ * 0.5 y (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))) */
+enum { ODSD_ACT_NONE = 0, ODSD_ACT_RELU = 1, ODSD_ACT_SILU = 2, ODSD_ACT_GELU = 3, ODSD_ACT_GELU_TANH = 4 };
 
 /* Shape of one MoE layer call.  Rules: H % 128 == 0, I % 128 == 0, 1 <= K <= E <= 512,
  * K <= 64, T >= 0 (T == 0 is a no-op). */
@@ -320,6 +327,76 @@ int     odsd_varlen_attention(const void *q, const void *k, const void *v, const
                               void *workspace, size_t workspace_bytes, void *stream);
 size_t odsd_varlen_attention_workspace_bytes(int32_t n_seqs, int32_t max_seqlen_q, int32_t max_seqlen_k,
                                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+
+/* Matrix product with its epilogue: out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n].
+ *   x [M, K], w [N, K], residual and out [M, N]: rows ldx, ldw, ldr, ldo elements apart, a row's elements consecutive;
+ *   bias [N] and residual may be NULL; x, w, bias of `dtype` (ODSD_DT_BF16 or ODSD_DT_F16), residual and out of
+ *   `out_dtype` (dtype or ODSD_DT_F32); act: one of ODSD_ACT_*
+ * Any M >= 0 (0: nothing is done), N >= 1, K >= 1, up to M = 4 million; pointers aligned to their elements (with K, ldx and
+ * ldw multiples of 8 and x and w 16-byte aligned the fast kernels run).  Sums and epilogue in fp32, one rounding at the end.
+ * out may be the residual itself (the same rows); it overlaps no other operand.  The same inputs give the same bits.
+ * workspace: odsd_linear_workspace_bytes(M, N, K) bytes (0: a size is out of range), 16-byte aligned.
+ * Stands in for the F.linear calls around the block (demo/src/layers/attention.py:169-288). */
+int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *residual,
+                int64_t ldr, void *out, int64_t ldo, int32_t M, int32_t N, int32_t K, int32_t dtype,
+                int32_t out_dtype, int32_t act, void *workspace, size_t workspace_bytes, void *stream);
+size_t odsd_linear_workspace_bytes(int32_t M, int32_t N, int32_t K);
+
+/* Rotary positions of a step's queries and keys, with the per-head RMSNorm in front and the KV-cache store behind them.
+ *   q [n, num_heads, head_dim], k / v [n, num_kv_heads, head_dim]: a head's elements consecutive, tokens and heads any
+ *   number of elements apart (views of a fused projection); dtype ODSD_DT_BF16 or ODSD_DT_F16 for all tensors
+ *   positions    [n_axes] rows of n positions, position_stride elements apart, int32 or int64 (position_bytes 4 or 8)
+ *   inv_freq     fp64 [rotary_dim / 2]: radians per position of each frequency
+ *   sections     HOST int32 [n_axes] (NULL for one axis): the first sections[0] frequencies turn with the positions of axis
+ *                0, the next sections[1] with those of axis 1, ...; they add up to rotary_dim / 2; n_axes <= 4
+ *   frequency i turns columns i and i + rotary_dim / 2 of a head (interleaved: 2i and 2i + 1); columns from rotary_dim on pass
+ *   q_weight / k_weight  [head_dim] or NULL: x * rsqrt(mean(x^2) + eps) * weight over each head first
+ *   q_out        [n, num_heads, head_dim], contiguous;  k_out  [n, num_kv_heads, head_dim] or NULL
+ *   k_cache / v_cache  [num_slots, num_kv_heads * head_dim] or both NULL: row i of the n_store stored ones, token
+ *                src_index[i] (src_index NULL: token i, n_store == n), goes to slot slot_mapping[i]; rows without a slot
+ *                (negative, >= num_slots) or token are not stored.  k_out and src_index together are refused, and
+ *                n_store is 0 without a cache.  Slots are each named once.
+ * Angles in fp64 (in turns), the rest in fp32, one rounding at the end; v is copied.  Outputs overlap no input.
+ * Stands in for q_norm / k_norm and rotary_emb of Qwen3Attention.forward with the store that follows them
+ * (demo/src/layers/attention.py:209-228, rotary_embedding.py). */
+int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+                int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                int64_t v_head_stride, int32_t n, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                int32_t rotary_dim, int32_t interleaved, int32_t dtype, const void *positions,
+                int32_t position_bytes, int32_t n_axes, int64_t position_stride, const int32_t *sections,
+                const double *inv_freq, const void *q_weight, const void *k_weight, float eps, void *q_out,
+                void *k_out, void *k_cache, void *v_cache, const int32_t *slot_mapping,
+                const int32_t *src_index, int32_t n_store, int64_t num_slots, void *stream);
+
+/* Verification of drafted tokens against the target's probabilities from given random numbers (speculative sampling);
+ * without drafts, the sampling of a decode step.
+ *   logits       [n_rows, vocab], rows logits_stride apart, ODSD_DT_F32 / BF16 / F16: query_lens[s] rows for sequence s, one
+ *                after the other (query_lens NULL: one each): one per drafted token and one behind the last
+ *   draft_tokens int64 [n_drafts]: query_lens[s] - 1 for sequence s;  draft_logits [n_drafts, vocab] of the same type, or
+ *                NULL: the draft model's distribution is one-hot at its token
+ *   temperature  fp32 [n_seqs], or NULL: temperature_all for all; 0: greedy
+ *   accept_u     fp32 [n_drafts], sample_u fp32 [n_seqs]: random numbers in [0, 1)
+ * With p_j = softmax(logits_j / T), q_j = softmax(draft_logits_j / T): draft j is kept while accept_u_j < min(1, p_j(d_j) /
+ * q_j(d_j)); after the kept ones comes a token drawn with sample_u from max(p_j - q_j, 0) at the first draft j that is not
+ * kept (from p_j where that is zero everywhere), or from the row behind the last.  Drawn: the lowest token whose inclusive
+ * cumulative weight exceeds sample_u times the total.  Greedy: p is one-hot at the largest logit, the lowest index of equals.
+ * All in fp64.  -inf masks a token, NaN counts as -inf; a row with +inf has its weight on those; a draft outside the
+ * vocabulary is not kept; a row with no number above -inf keeps no draft and draws -1.
+ *   tokens       int64 [n_seqs, max_q_len]: the kept drafts, the drawn token, -1 behind it
+ *   num_accepted int32 [n_seqs];  accept_probs fp32 [n_drafts]: min(1, p / q) of every draft, kept or not
+ * max_q_len bounds query_lens (a longer sequence has its first max_q_len rows verified).  A sequence with query_lens 0 gets
+ * -1 only.  workspace: odsd_verify_workspace_bytes(...) bytes (0: sizes out of range), 16-byte aligned.
+ * Stands in for the acceptance of a verify step (demo/src/execution/cb_executor.py:261-300) in the sampled form of
+ * pre_exp/moe_spec_acc_rate_benchmark/spec_sampling.py:3-198. */
+int odsd_verify_drafts(const void *logits, int64_t logits_stride, const void *draft_logits,
+                       int64_t draft_stride, int32_t dtype, const int64_t *draft_tokens,
+                       const int32_t *query_lens, const float *temperature, float temperature_all,
+                       const float *accept_u, const float *sample_u, int32_t n_seqs, int32_t max_q_len,
+                       int32_t n_rows, int32_t n_drafts, int32_t vocab, int64_t *tokens,
+                       int32_t *num_accepted, float *accept_probs, void *workspace, size_t workspace_bytes,
+                       void *stream);
+size_t odsd_verify_workspace_bytes(int32_t n_seqs, int32_t max_q_len, int32_t n_rows, int32_t n_drafts,
+                                   int32_t vocab, int32_t has_draft_logits);
 
 /* The same call with every kernel timed, for measurement (no counterpart in the reference):
  * events = 2 * ODSD_N_KERNELS hipEvent_t handles created by the caller; the launch of kernel slot k

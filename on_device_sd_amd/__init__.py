@@ -12,8 +12,10 @@ from .placement import (ExpertActivation, LayerExpertActivations, build_draft_pl
                         build_layer_activations, build_prefill_placement)
 from .layers import W4MoELayer, W4MoELayerWithWeights, W4Operators
 from .cache import LRUStrategy, W4ExpertCache, cache_capacity
-from .kv import (SequenceSlots, attention_for_context, build_decode_context, build_prefill_context,
-                 build_verify_context, get_attention_context, paged_attention, store_kvcache, varlen_attention)
+from .kv import (SequenceSlots, apply_rotary, attention_for_context, build_decode_context, build_prefill_context,
+                 build_verify_context, get_attention_context, paged_attention, rotary_store_kvcache, store_kvcache,
+                 varlen_attention)
+from .verify import VerifyResult, verify_drafts
 
 __all__ = [
     "AttentionOutput", "ExpertID", "ExpertPlacement", "LayerOutput", "MoEConfig", "RoutingResult",
@@ -25,4 +27,5 @@ __all__ = [
     "LRUStrategy", "W4ExpertCache", "cache_capacity",
     "SequenceSlots", "build_verify_context", "build_prefill_context", "build_decode_context",
     "get_attention_context", "attention_for_context", "paged_attention", "store_kvcache", "varlen_attention",
+    "apply_rotary", "rotary_store_kvcache", "VerifyResult", "verify_drafts",
 ]

@@ -68,6 +68,14 @@ SIGNATURES = {
     "odsd_varlen_attention": (C.c_int, [_P, _P, _P, _P, _P] + [C.c_int32] * 6 + [C.c_float, C.c_int32, _P, _P,
                                                                                 C.c_size_t, _P]),
     "odsd_varlen_attention_workspace_bytes": (C.c_size_t, [C.c_int32] * 6),
+    "odsd_linear": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64, _P, C.c_int64] + [C.c_int32] * 6
+                    + [_P, C.c_size_t, _P]),
+    "odsd_linear_workspace_bytes": (C.c_size_t, [C.c_int32] * 3),
+    "odsd_rotary": (C.c_int, [_P, C.c_int64, C.c_int64] * 3 + [C.c_int32] * 7 + [_P, C.c_int32, C.c_int32, C.c_int64]
+                    + [_P] * 4 + [C.c_float] + [_P] * 6 + [C.c_int32, C.c_int64, _P]),
+    "odsd_verify_drafts": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int32, _P, _P, _P, C.c_float, _P, _P]
+                           + [C.c_int32] * 5 + [_P] * 4 + [C.c_size_t, _P]),
+    "odsd_verify_workspace_bytes": (C.c_size_t, [C.c_int32] * 6),
     "odsd_moe_forward_events": (C.c_int, [_SP, _P, _P, C.c_float, _P, _P, C.c_int32, _P, _P, _P, _P, _P,
                                           C.c_size_t, _P, _P, _P]),
     "odsd_moe_stack_workspace_bytes": (C.c_size_t, [_SP]),

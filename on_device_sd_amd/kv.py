@@ -14,12 +14,13 @@ Python and need no GPU; ``attention_for_context`` runs the attention kernel that
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence
+import ctypes as C
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from .ops import _stream, _wrote
+from .ops import _ptr, _raw_device, _same_device, _stream, _wrote
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -54,6 +55,120 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
                                  key.element_size(), k_cache.numel() // D,
                                  _stream()), "odsd_kv_store")
     _wrote(k_cache, v_cache)
+
+
+_ROTARY_DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, want_k, k_cache, v_cache,
+            slot_mapping, src_index):
+    dev = q.get_device()
+    _same_device(dev, k, v, positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slot_mapping, src_index)
+    if dev != _raw_device():
+        with torch.cuda.device(dev):
+            return _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, want_k, k_cache,
+                           v_cache, slot_mapping, src_index)
+    code = _ROTARY_DTYPES.get(q.dtype)
+    if code is None:
+        raise TypeError(f"rotary positions take bfloat16 or float16, got {q.dtype}")
+    n, heads, head_dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape != (n, kv_heads, head_dim) or k.dtype != q.dtype:
+        raise ValueError("q [n, heads, head_dim] and k [n, kv_heads, head_dim] must have the same tokens, head size and dtype")
+    rotary_dim = 2 * inv_freq.numel()
+    if inv_freq.dtype != torch.float64:
+        raise TypeError("inv_freq must be float64: an angle is a position times a frequency")
+    if not 0 < rotary_dim <= head_dim:
+        raise ValueError(f"{inv_freq.numel()} frequencies do not fit a head of {head_dim}")
+    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
+        raise TypeError("positions must be int32 or int64")
+    axes = 1 if positions.dim() == 1 else positions.shape[0]
+    if positions.shape[-1] != n or positions.dim() > 2:
+        raise ValueError(f"positions must be [{n}] or [axes, {n}]")
+    if sections is None:
+        if axes != 1:
+            raise ValueError("positions of several axes need sections")
+        counts = None
+    else:
+        if len(sections) != axes or sum(sections) != rotary_dim // 2 or min(sections) < 0 or axes > 4:
+            raise ValueError(f"sections {tuple(sections)}: one count per axis (at most 4), together {rotary_dim // 2}")
+        counts = (C.c_int32 * axes)(*sections)
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (head_dim,) or w.dtype != q.dtype):
+            raise ValueError("norm weights must be [head_dim] in the dtype of q")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    inv_freq = inv_freq.contiguous()
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    vs0 = vs1 = n_store = num_slots = 0
+    if k_cache is not None:
+        D = kv_heads * head_dim
+        if v.shape != k.shape or not v.dtype == k_cache.dtype == v_cache.dtype == q.dtype:
+            raise ValueError("k and v must have the same shape, and the caches their dtype")
+        if k_cache.shape != v_cache.shape or k_cache.shape[-1] != D or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+            raise ValueError(f"the caches must be contiguous rows of {D}")
+        if v.stride(2) != 1:
+            v = v.contiguous()
+        vs0, vs1 = v.stride(0), v.stride(1)
+        if slot_mapping.dtype != torch.int32:
+            slot_mapping = slot_mapping.to(torch.int32)
+        slot_mapping = slot_mapping.contiguous()
+        n_store, num_slots = slot_mapping.numel(), k_cache.numel() // D
+        if src_index is not None:
+            if src_index.dtype != torch.int32:
+                src_index = src_index.to(torch.int32)
+            src_index = src_index.contiguous()
+        if (n if src_index is None else src_index.numel()) != n_store:
+            raise ValueError("slot_mapping must name a slot (or -1) for every row that is stored")
+    q_out = torch.empty(n, heads, head_dim, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(n, kv_heads, head_dim, dtype=q.dtype, device=q.device) if want_k else None
+    if n == 0:
+        return q_out, k_out
+    rc = _lib.load().odsd_rotary(
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), _ptr(v), vs0, vs1, n, heads, kv_heads,
+        head_dim, rotary_dim, 1 if interleaved else 0, code, positions.data_ptr(), positions.element_size(), axes,
+        positions.stride(0) if axes > 1 else n, counts, inv_freq.data_ptr(), _ptr(q_weight), _ptr(k_weight), eps,
+        q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), _ptr(src_index), n_store, num_slots,
+        _stream())
+    if rc:
+        _lib.check(rc, "odsd_rotary")
+    if k_cache is not None:
+        _wrote(k_cache, v_cache)
+    return q_out, k_out
+
+
+def apply_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+                 sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions of q [n, heads, head_dim] and k [n, kv_heads, head_dim] (bfloat16 / float16; views of a fused
+    projection as they are), returned contiguous.  ``positions`` int32 / int64 [n], or [axes, n] (time, height, width) with
+    ``sections``: how many of the frequencies, in order, turn with each axis.  ``inv_freq`` float64 [rotary_dim / 2], radians
+    per position, for a plain ladder ``base ** (-arange(0, rotary_dim, 2) / rotary_dim)``; columns of a head from rotary_dim
+    on pass.  Frequency i turns columns i and i + rotary_dim / 2 (``interleaved``: 2i and 2i + 1).  With ``q_weight`` /
+    ``k_weight`` [head_dim] each head goes through RMSNorm first (``q_norm`` / ``k_norm`` of the reference's attention)."""
+    return _rotary(q, k, None, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, True, None, None, None, None)
+
+
+def rotary_store_kvcache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                         k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                         src_index: Optional[torch.Tensor] = None, *, sections: Optional[Sequence[int]] = None,
+                         interleaved: bool = False, q_weight: Optional[torch.Tensor] = None,
+                         k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, want_k: bool = False):
+    """``apply_rotary`` and ``store_kvcache`` in one kernel: the turned keys and the values go straight to their slots
+    (``slot_mapping`` / ``src_index`` as there), the turned queries are returned.  ``want_k``: the turned keys too, as
+    (q, k), for the packed attention of a prefill step (not together with ``src_index``)."""
+    if k_cache is None or v_cache is None or v is None or slot_mapping is None:
+        raise ValueError("the store needs v, both caches and slot_mapping; apply_rotary is the form without")
+    if want_k and src_index is not None:
+        raise ValueError("want_k returns every token's key; with src_index only those named are computed")
+    q_out, k_out = _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, want_k, k_cache,
+                           v_cache, slot_mapping, src_index)
+    return (q_out, k_out) if want_k else q_out
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, context: Dict[str, torch.Tensor],

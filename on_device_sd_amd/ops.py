@@ -179,6 +179,88 @@ def to_f16(x: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------------------------------
+# Projections
+# ------------------------------------------------------------------------------------------
+_LINEAR_DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}       # ODSD_ACT_*
+
+
+def _same_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor is on GPU ``dev`` (an index; -1 is the CPU)."""
+    for t in tensors:
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise RuntimeError("runs on the GPU only, all tensors on the same one (there is no CPU fallback)")
+
+
+def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int]:
+    """A matrix whose rows are dense, copied only if they are not, and the elements between two rows (the stride of a
+    single row says nothing)."""
+    if t.stride(1) != 1 or t.stride(0) < cols:         # (a broadcast or overlapping view is not a matrix of rows)
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else cols
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+           activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+           out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x @ weight.T + bias) + residual in one kernel: a projection around the attention with what follows it, or the
+    language-model head.  x [..., K] and weight [N, K] bfloat16 or float16 (the same), bias [N] like them, residual
+    [..., N] in the output's dtype (``out_dtype``: x's, the default, or float32).  ``activation``: None, "relu", "silu",
+    "gelu" (erf) or "gelu_tanh".  fp32 sums and epilogue, one rounding.  Rows may be any distance apart; with K and the row
+    distances multiples of 8 and 16-byte aligned tensors the fast kernels run.  No gradient flows through it."""
+    dev = x.get_device()
+    _same_device(dev, weight, bias, residual)
+    if dev != _raw_device():
+        with torch.cuda.device(dev):
+            return linear(x, weight, bias, activation=activation, residual=residual, out_dtype=out_dtype)
+    dtype = x.dtype
+    code = _LINEAR_DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"linear takes bfloat16 or float16, got {dtype}")
+    if weight.dtype != dtype or (bias is not None and bias.dtype != dtype):
+        raise TypeError("x, weight and bias must have the same dtype")
+    if out_dtype is None:
+        out_dtype = dtype
+    elif out_dtype != dtype and out_dtype != torch.float32:
+        raise TypeError(f"out_dtype is x's or float32, got {out_dtype}")
+    act = _ACTIVATIONS.get(activation, -1)
+    if act < 0:
+        raise ValueError(f"activation {activation!r} is none of {list(_ACTIVATIONS)}")
+    shape = x.shape
+    N, K = weight.shape
+    if x.dim() == 0 or shape[-1] != K:
+        raise ValueError(f"x {tuple(shape)} and weight {tuple(weight.shape)} do not belong together")
+    out = torch.empty(shape[:-1] + (N,), dtype=out_dtype, device=x.device)
+    if N == 0 or out.numel() == 0:
+        return out
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
+    M = x.shape[0]
+    x, ldx = _rows(x, K)
+    weight, ldw = _rows(weight, K)
+    if bias is not None:
+        if bias.shape != (N,):
+            raise ValueError(f"bias {tuple(bias.shape)} does not fit {N} outputs")
+        bias = bias.contiguous()
+    ldr = N
+    if residual is not None:
+        if residual.shape != out.shape or residual.dtype != out_dtype:
+            raise ValueError(f"the residual must be {tuple(out.shape)} {out_dtype}, like the output")
+        residual, ldr = _rows(residual.reshape(-1, N), N)
+    lib = _lib.load()
+    nbytes = lib.odsd_linear_workspace_bytes(M, N, K)
+    if nbytes == 0:
+        raise _lib.OdsdError(f"linear: unsupported shape M={M} N={N} K={K}")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    rc = lib.odsd_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr,
+                         out.data_ptr(), N, M, N, K, code, _lib.DT_F32 if out_dtype == torch.float32 else code, act,
+                         ws.data_ptr(), nbytes, _stream())
+    if rc:
+        _lib.check(rc, "odsd_linear")
+    return out
+
+
+# ------------------------------------------------------------------------------------------
 # Router / dispatch
 # ------------------------------------------------------------------------------------------
 def router_topk(x: torch.Tensor, gate_weight: torch.Tensor, top_k: int, renorm: bool,
