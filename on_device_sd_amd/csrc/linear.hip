@@ -77,185 +77,22 @@ __device__ __forceinline__ void finish8(const LinearParams &p, int m, int n, con
     }
 }
 
-// ---- tiles -----------------------------------------------------------------------------------
-// NWN x NWM wavefronts, each FA blocks of 32 n by FB blocks of 32 m on v_mfma_f32_32x32x16; steps of 64 along K.  Both
-// operands go to LDS without passing registers (buffer_load ... lds, 16 bytes a lane), STAGES buffers of them; a buffer's
-// rows are 128 bytes, whose 16-byte segments are XORed with the row's number, so that the fragment reads (eight lanes, eight
-// rows, one segment) meet eight different bank groups.  What is behind a row's end, the matrix's last row or the slice's
-// last step is addressed outside the buffer descriptor and arrives as zeros, without memory traffic, so every copy is
-// issued whatever follows and a count says which have landed.
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES>
-struct LinearTile {
-    static constexpr int NW = NWN * NWM, TN = NWN * FA * 32, TM = NWM * FB * 32;
-    static constexpr int A_BYTES = TN * 128, STAGE = (TN + TM) * 128;
-    static constexpr int LA = TN / 8 / NW, LB = TM / 8 / NW, L = LA + LB;   // copies of a wavefront per step: 8 rows each
-    static constexpr int CH = FA < 2 ? FA : 2;                             // blocks of n that leave together
-    static constexpr int OUT_WAVE = FB * 32 * CH * 32 * 4;
-    static constexpr int LDS = STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE;
-    static_assert(LA * 8 * NW == TN && LB * 8 * NW == TM && LB >= 1, "every wavefront copies whole groups of 8 rows");
-};
-
-__device__ __forceinline__ void copy16_to_lds(uint4_t rsrc, uint32_t off, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(lds_addr), "v"(off), "s"(rsrc) : "memory");
-}
-__device__ __forceinline__ uint4_t descriptor(const void *base, uint32_t bytes) {
-    const uint64_t a = (uint64_t)base;
-    uint4_t r;
-    r.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
-    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
-    r.z = __builtin_amdgcn_readfirstlane(bytes);
-    r.w = 0x00020000u;
-    return r;
-}
-
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES>
-__global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParams p) {
-    typedef LinearTile<T, O, NWN, NWM, FA, FB, STAGES> C;
-    typedef typename AttnT<T>::V8 V8;
-    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // neighbouring tiles on one XCD (workgroup i is on XCD i % 8), in groups of up to 8 along m that share their weights
-    const int total = p.tiles_n * p.tiles_m * p.slices, per = (total + 7) / 8;
-    const int b = blockIdx.x, t0 = (b & 7) * per + (b >> 3);
-    if ((b >> 3) >= per || t0 >= total) return;
-    const int slice = t0 / (p.tiles_n * p.tiles_m), t = t0 - slice * (p.tiles_n * p.tiles_m);
-    const int group = t / (8 * p.tiles_n), in_group = t - group * 8 * p.tiles_n;
-    const int gm = min(8, p.tiles_m - group * 8);
-    const int n0 = in_group / gm * C::TN, m0 = (group * 8 + in_group % gm) * C::TM;
-
-    const int k_begin = slice * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
-    const int steps = (k_end - k_begin + 63) / 64;
-    const uint32_t ldw = (uint32_t)p.ldw * 2u, ldx = (uint32_t)p.ldx * 2u;
-    const uint4_t rw = descriptor((const char *)p.w + (int64_t)n0 * p.ldw * 2, (uint32_t)(min(C::TN, p.N - n0) - 1) * ldw + p.K * 2);
-    const uint4_t rx = descriptor((const char *)p.x + (int64_t)m0 * p.ldx * 2, (uint32_t)(min(C::TM, p.M - m0) - 1) * ldx + p.K * 2);
-    const int seg = (lane & 7) ^ (lane >> 3);
-    const uint32_t row0 = wave * 8 + (lane >> 3);
-    const uint32_t off_w = row0 * ldw + seg * 16, off_x = row0 * ldx + seg * 16;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)lds;
-    auto copy_step = [&](int step, uint32_t buf) {
-        const int k = k_begin + step * 64;
-        const uint32_t ko = k + seg * 8 < k_end ? (uint32_t)k * 2u : 0x80000000u;
-#pragma unroll
-        for (int i = 0; i < C::LA; ++i) copy16_to_lds(rw, off_w + ko + i * (C::NW * 8) * ldw, lds0 + buf + (i * C::NW + wave) * 1024);
-#pragma unroll
-        for (int i = 0; i < C::LB; ++i) copy16_to_lds(rx, off_x + ko + i * (C::NW * 8) * ldx, lds0 + buf + C::A_BYTES + (i * C::NW + wave) * 1024);
-    };
-
-    const int wn = wave % NWN, wm = wave / NWN;
-    const uint32_t frag = (lane & 31) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
-    const uint32_t fa0 = wn * FA * 4096 + frag, fb0 = C::A_BYTES + wm * FB * 4096 + frag;
-    float16_t acc[FA][FB];
-#pragma unroll
-    for (int i = 0; i < FA; ++i)
-#pragma unroll
-        for (int j = 0; j < FB; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    V8 fa[2][FA], fb[2][FB];
-    auto read = [&](int par, uint32_t buf, int j) {
-#pragma unroll
-        for (int i = 0; i < FB; ++i) fb[par][i] = *(const V8 *)(lds + ((buf + fb0) ^ (j << 5)) + i * 4096);
-#pragma unroll
-        for (int i = 0; i < FA; ++i) fa[par][i] = *(const V8 *)(lds + ((buf + fa0) ^ (j << 5)) + i * 4096);
-    };
-
-    for (int s = 0; s < STAGES; ++s) copy_step(s, s * C::STAGE);
-    ODSD_WAIT_VMCNT_LGKM0((STAGES - 1) * C::L);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    uint32_t cur = 0;
-    read(0, cur, 0);
-    for (int step = 0; step < steps; ++step) {
-        uint32_t next = cur + C::STAGE;
-        if (next == C::STAGE * STAGES) next = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j == 3) {
-                // the next step's copies have landed and this step's last fragments are read: by every wavefront
-                __builtin_amdgcn_sched_barrier(0);
-                ODSD_WAIT_VMCNT_LGKM0((STAGES - 2) * C::L);
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                read(0, next, 0);
-                copy_step(step + STAGES, cur);
-            } else {
-                read((j + 1) & 1, cur, j + 1);
-            }
-#pragma unroll
-            for (int a = 0; a < FA; ++a)
-#pragma unroll
-                for (int c = 0; c < FB; ++c) acc[a][c] = AttnT<T>::mfma32(fa[j & 1][a], fb[j & 1][c], acc[a][c]);
-        }
-        cur = next;
-    }
-    ODSD_WAIT_VMCNT_LGKM0(0);                  // the copies past the end (zeros) have landed, too
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-
-    // The sums leave through LDS (each wavefront its own part): a lane gets eight consecutive n of one token.  16-byte pieces
-    // of a token's row are XORed with the token's number.
-    constexpr int PIECES = C::CH * 8;          // of 4 sums, per token
-    char *stage = lds + wave * C::OUT_WAVE;
-#pragma unroll
-    for (int a0 = 0; a0 < FA; a0 += C::CH) {
-#pragma unroll
-        for (int a = 0; a < C::CH; ++a)
-#pragma unroll
-            for (int c = 0; c < FB; ++c)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = c * 32 + (lane & 31), piece = a * 8 + q * 2 + (lane >> 5);
-                    float4_t v;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) v[u] = acc[a0 + a][c][4 * q + u];
-                    *(float4_t *)(stage + m * (PIECES * 16) + ((piece ^ (m & (PIECES - 1))) << 4)) = v;
-                }
-        // (a wavefront's own LDS accesses stay in order)
-        constexpr int LANES = PIECES / 2;      // lanes that share a token's row
-        for (int r = lane / LANES; r < FB * 32; r += 64 / LANES) {
-            const int pc = lane % LANES * 2;
-            float v[8];
-            *(float4_t *)v = *(const float4_t *)(stage + r * (PIECES * 16) + ((pc ^ (r & (PIECES - 1))) << 4));
-            *(float4_t *)(v + 4) = *(const float4_t *)(stage + r * (PIECES * 16) + (((pc + 1) ^ (r & (PIECES - 1))) << 4));
-            const int m = m0 + wm * FB * 32 + r, n = n0 + (wn * FA + a0) * 32 + pc * 4;
-            if (p.slices > 1) {
-                if (m < p.M && n < p.N) {
-                    float *part = p.part + ((int64_t)slice * p.M + m) * p.part_ld + n;
-                    *(float4_t *)part = *(float4_t *)v;
-                    *(float4_t *)(part + 4) = *(float4_t *)(v + 4);
-                }
-            } else {
-                finish8<T, O>(p, m, n, v);
-            }
-        }
-        asm volatile("" ::: "memory");
-    }
-}
-
-// the slices' sums together, in their order, and the epilogue
 template <typename T, typename O>
-__global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p) {
-    const int per_row = (p.N + 7) / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int m = (int)(i / per_row), n = (int)(i - (int64_t)m * per_row) * 8;
-    if (m >= p.M) return;
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < p.slices; ++s) {
-        const float *part = p.part + ((int64_t)s * p.M + m) * p.part_ld + n;
-        const float4_t a = *(const float4_t *)part, b = *(const float4_t *)(part + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] += a[e];
-            v[4 + e] += b[e];
-        }
+__device__ __forceinline__ void finish1(const LinearParams &p, int m, int n, float v) {
+    constexpr bool PRECISE = sizeof(O) == 4;
+    if (p.bias) v += (float)((const T *)p.bias)[n];
+    switch (p.act) {
+        case ODSD_ACT_RELU: v = activate<PRECISE, ODSD_ACT_RELU>(v); break;
+        case ODSD_ACT_SILU: v = activate<PRECISE, ODSD_ACT_SILU>(v); break;
+        case ODSD_ACT_GELU: v = activate<PRECISE, ODSD_ACT_GELU>(v); break;
+        case ODSD_ACT_GELU_TANH: v = activate<PRECISE, ODSD_ACT_GELU_TANH>(v); break;
+        default: break;
     }
-    finish8<T, O>(p, m, n, v);
+    if (p.res) v += (float)((const O *)p.res)[(int64_t)m * p.ldr + n];
+    ((O *)p.out)[(int64_t)m * p.ldo + n] = (O)v;
 }
 
-// ---- any shape, any alignment ----------------------------------------------------------------
-// 64 x 64 tile, steps of 64 along K, operands through registers into LDS (rows padded by 16 bytes).  Eight values of a row
-// that lie in K whole are one 16-byte load at the elements' own alignment; the row's end comes element by element.
+// eight values of a row from column k on, zeros behind its end; at the elements' own alignment
 template <typename T>
 __device__ __forceinline__ uint4_t load8_any(const T *row, int k, int K, bool row_ok) {
     uint4_t v = {0, 0, 0, 0};
@@ -273,6 +110,275 @@ __device__ __forceinline__ uint4_t load8_any(const T *row, int k, int K, bool ro
     return v;
 }
 
+// ---- few tokens ------------------------------------------------------------------------------
+// The weights' bytes bound it.  A workgroup takes 16 rows of w and all of K; its NWV wavefronts share K in blocks of 64
+// columns and add their sums up through LDS, so nothing is split over workgroups, there is one launch and no workspace.
+// Weights go to registers as the matrix instruction wants them (a lane: 16 consecutive columns of one row), DEPTH blocks of
+// them requested at once; a token's columns are used by one wavefront of the workgroup only, so they come to registers, too.
+// (Three or four groups of 16 tokens in this form: slower than tiles from 17 tokens on, K 2048, N 5120, M = 40 16.7 / 11.5 us.)
+template <typename T, typename O, int NWV, int DEPTH>
+__global__ __launch_bounds__(NWV * 64) void linear_rows_kernel(LinearParams p) {
+    typedef typename AttnT<T>::V8 V8;
+    __shared__ float sums[NWV][16][17];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+    const int full = p.K / 64, blocks = (p.K + 63) / 64;       // blocks that lie in K whole; all of them
+    const bool token = r < p.M;                                // (columns of the product that nobody stores are not read)
+    const T *w = (const T *)p.w + (int64_t)min(n0 + r, p.N - 1) * p.ldw;
+    const T *x = (const T *)p.x + (int64_t)min(r, p.M - 1) * p.ldx;
+    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    uint4_t a[DEPTH][2], c[DEPTH][2];
+    auto multiply = [&](int d) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) acc = AttnT<T>::mfma(__builtin_bit_cast(V8, a[d][u]), __builtin_bit_cast(V8, c[d][u]), acc);
+    };
+    int b = wave;
+    auto group = [&](auto count) {                             // this many blocks of the wavefront, all of them whole
+        constexpr int n = decltype(count)::value;
+#pragma unroll
+        for (int d = 0; d < n; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) __builtin_memcpy(&a[d][u], w + (b + d * NWV) * 64 + g * 16 + u * 8, 16);
+#pragma unroll
+        for (int d = 0; d < n; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                c[d][u] = uint4_t{0, 0, 0, 0};
+                if (token) __builtin_memcpy(&c[d][u], x + (b + d * NWV) * 64 + g * 16 + u * 8, 16);
+            }
+#pragma unroll
+        for (int d = 0; d < n; ++d) multiply(d);
+        b += n * NWV;
+    };
+    while (b + (DEPTH - 1) * NWV < full) group(std::integral_constant<int, DEPTH>{});
+    while (b < full) group(std::integral_constant<int, 1>{});
+    if (b < blocks) {                                          // the block that K ends in
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            a[0][u] = load8_any(w, b * 64 + g * 16 + u * 8, p.K, true);
+            c[0][u] = load8_any(x, b * 64 + g * 16 + u * 8, p.K, token);
+        }
+        multiply(0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[wave][r][g * 4 + e] = acc[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += NWV * 64) {
+        const int m = i >> 4, n = i & 15;
+        if (m >= p.M || n0 + n >= p.N) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NWV; ++q) v += sums[q][m][n];
+        finish1<T, O>(p, m, n0 + n, v);
+    }
+}
+
+// ---- tiles -----------------------------------------------------------------------------------
+// NWN x NWM wavefronts, each FA blocks of 32 n by FB blocks of 32 m on v_mfma_f32_32x32x16; steps of BK along K.  Both
+// operands go to LDS without passing registers (buffer_load ... lds, 16 bytes a lane), STAGES buffers of them; a buffer's
+// rows are 128 bytes (64 with steps of 32), whose 16-byte segments are XORed with bits of the row's number: the 16 lanes that
+// read together (rows 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of a block, one segment) then meet the 16 bank groups.  What is behind a row's end, the matrix's last row or the slice's
+// last step is addressed outside the buffer descriptor and arrives as zeros, without memory traffic, so every copy is
+// issued whatever follows and a count says which have landed.
+template <int NWN, int NWM, int FA, int FB, int BK, int STAGES>
+struct LinearTile {
+    static constexpr int NW = NWN * NWM, TN = NWN * FA * 32, TM = NWM * FB * 32;
+    static constexpr int ROW = BK * 2, SEGS = BK / 8, ROWS = 64 / SEGS;      // bytes and 16-byte segments of a row, rows of a copy
+    static constexpr int A_BYTES = TN * ROW, STAGE = (TN + TM) * ROW;
+    static constexpr int LA = TN / ROWS / NW, LB = TM / ROWS / NW, L = LA + LB;   // copies of a wavefront per step
+    static constexpr int CH = FA < 2 ? FA : 2;                             // blocks of n that leave together
+    static constexpr int OUT_WAVE = FB * 32 * CH * 32 * 4;
+    static constexpr int LDS = STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE;
+    static_assert(LA * ROWS * NW == TN && LB * ROWS * NW == TM && LB >= 1, "every wavefront makes the same number of copies");
+    static_assert((BK == 64 && NW % 2 == 0) || BK == 32, "the swizzle of a copied row does not depend on the copy");
+};
+
+__device__ __forceinline__ void copy16_to_lds(uint4_t rsrc, uint32_t off, uint32_t lds_addr) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(lds_addr), "v"(off), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ uint4_t descriptor(const void *base, uint32_t bytes) {
+    const uint64_t a = (uint64_t)base;
+    uint4_t r;
+    r.x = __builtin_amdgcn_readfirstlane((uint32_t)a);
+    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
+    r.z = __builtin_amdgcn_readfirstlane(bytes);
+    r.w = 0x00020000u;
+    return r;
+}
+
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES>
+__global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParams p) {
+    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES> C;
+    typedef typename AttnT<T>::V8 V8;
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // neighbouring tiles on one XCD (workgroup i is on XCD i % 8), in groups of up to 8 along m that share their weights
+    const int total = p.tiles_n * p.tiles_m * p.slices, per = (total + 7) / 8;
+    const int b = blockIdx.x, t0 = (b & 7) * per + (b >> 3);
+    if ((b >> 3) >= per || t0 >= total) return;
+    const int slice = t0 / (p.tiles_n * p.tiles_m), t = t0 - slice * (p.tiles_n * p.tiles_m);
+    const int group = t / (8 * p.tiles_n), in_group = t - group * 8 * p.tiles_n;
+    const int gm = min(8, p.tiles_m - group * 8);
+    const int n0 = in_group / gm * C::TN, m0 = (group * 8 + in_group % gm) * C::TM;
+
+    const int k_begin = slice * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
+    const int steps = (k_end - k_begin + BK - 1) / BK;
+    const uint32_t ldw = (uint32_t)p.ldw * 2u, ldx = (uint32_t)p.ldx * 2u;
+    const uint4_t rw = descriptor((const char *)p.w + (int64_t)n0 * p.ldw * 2, (uint32_t)(min(C::TN, p.N - n0) - 1) * ldw + p.K * 2);
+    const uint4_t rx = descriptor((const char *)p.x + (int64_t)m0 * p.ldx * 2, (uint32_t)(min(C::TM, p.M - m0) - 1) * ldx + p.K * 2);
+    // of the row that a lane copies (the same for all its copies: NW is even)
+    const int seg = BK == 64 ? (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)) : (lane & 3) ^ (lane >> 4);
+    const uint32_t row0 = wave * C::ROWS + lane / C::SEGS;
+    const uint32_t off_w = row0 * ldw + seg * 16, off_x = row0 * ldx + seg * 16;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)lds;
+    auto copy = [&](int step, uint32_t buf, int i) {            // copy i of a step's: first those of w, then those of x
+        const int k = k_begin + step * BK;
+        const uint32_t ko = k + seg * 8 < k_end ? (uint32_t)k * 2u : 0x80000000u;
+        if (i < C::LA) copy16_to_lds(rw, off_w + ko + i * (C::NW * C::ROWS) * ldw, lds0 + buf + (i * C::NW + wave) * 1024);
+        else copy16_to_lds(rx, off_x + ko + (i - C::LA) * (C::NW * C::ROWS) * ldx, lds0 + buf + C::A_BYTES + ((i - C::LA) * C::NW + wave) * 1024);
+    };
+
+    const int wn = wave % NWN, wm = wave / NWN;
+    const uint32_t frag = (lane & 31) * C::ROW + (((lane >> 5) ^ (BK == 64 ? (lane >> 1) & 7 : (lane >> 2) & 3)) << 4);
+    const uint32_t fa0 = wn * FA * 32 * C::ROW + frag, fb0 = C::A_BYTES + wm * FB * 32 * C::ROW + frag;
+    float16_t acc[FA][FB];
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    V8 fa[2][FA], fb[2][FB];
+    // fragment i of columns 16 j .. of a buffer, in the order in which the products want them: w's first, x's, the rest of w's
+    auto read = [&](int par, uint32_t buf, int j, int i) {
+        if (i > 0 && i <= FB) fb[par][i - 1] = *(const V8 *)(lds + ((buf + fb0) ^ (j << 5)) + (i - 1) * 32 * C::ROW);
+        else fa[par][i ? i - FB : 0] = *(const V8 *)(lds + ((buf + fa0) ^ (j << 5)) + (i ? i - FB : 0) * 32 * C::ROW);
+    };
+    // 16 columns: their products, and between those, one by one, the reads of the next 16 columns' fragments and the copies
+    // of the step that comes into the buffer that was left last.  (The compiler would request a fragment right before its
+    // use, and copies in a row stall the wavefront: a CU takes one per 16 cycles.)
+    constexpr int J = BK / 16, NM = FA * FB, NR = FA + FB, EARLY = (C::L + 1) / 2;
+    auto columns = [&](auto jc, int step, uint32_t cur, uint32_t next, uint32_t left) {
+        constexpr int j = decltype(jc)::value;
+        constexpr bool last = j == J - 1;
+        constexpr int NC = last ? EARLY : j == 0 ? C::L - EARLY : 0;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            acc[i / FB][i % FB] = AttnT<T>::mfma32(fa[j & 1][i / FB], fb[j & 1][i % FB], acc[i / FB][i % FB]);
+            if (last && i == 0) {
+                // the next step's copies have landed and this step's last fragments are read: by every wavefront
+                ODSD_WAIT_VMCNT_LGKM0((STAGES - 2) * C::L);
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+                if (r * NM / NR == i) read((j + 1) & 1, last ? next : cur, last ? 0 : j + 1, r);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (c * NM / NC == i) copy(last ? step + STAGES : step + STAGES - 1, last ? cur : left, last ? c : EARLY + c);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+#pragma unroll
+        for (int i = 0; i < (s < STAGES - 1 ? C::L : EARLY); ++i) copy(s, s * C::STAGE, i);
+    ODSD_WAIT_VMCNT_LGKM0((STAGES - 2) * C::L + EARLY);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    uint32_t cur = 0, left = (STAGES - 1) * C::STAGE;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) read(0, cur, 0, r);
+    for (int step = 0; step < steps; ++step) {
+        uint32_t next = cur + C::STAGE;
+        if (next == C::STAGE * STAGES) next = 0;
+        columns(std::integral_constant<int, 0>{}, step, cur, next, left);
+        columns(std::integral_constant<int, 1>{}, step, cur, next, left);
+        if constexpr (J == 4) {
+            columns(std::integral_constant<int, 2>{}, step, cur, next, left);
+            columns(std::integral_constant<int, 3>{}, step, cur, next, left);
+        }
+        left = cur;
+        cur = next;
+    }
+    ODSD_WAIT_VMCNT_LGKM0(0);                  // the copies past the end (zeros) have landed, too
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+
+    // The sums leave through LDS (each wavefront its own part): a lane gets eight consecutive n of one token.  16-byte pieces
+    // of a token's row are XORed with the token's number.
+    constexpr int PIECES = C::CH * 8;          // of 4 sums, per token
+    auto swz = [](int m) { return PIECES == 16 ? m & 15 : (m >> 1) & 7; };
+    char *stage = lds + wave * C::OUT_WAVE;
+#pragma unroll
+    for (int a0 = 0; a0 < FA; a0 += C::CH) {
+#pragma unroll
+        for (int a = 0; a < C::CH; ++a)
+#pragma unroll
+            for (int c = 0; c < FB; ++c)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int m = c * 32 + (lane & 31), piece = a * 8 + q * 2 + (lane >> 5);
+                    float4_t v;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] = acc[a0 + a][c][4 * q + u];
+                    *(float4_t *)(stage + m * (PIECES * 16) + ((piece ^ swz(m)) << 4)) = v;
+                }
+        // (a wavefront's own LDS accesses stay in order)
+        constexpr int LANES = PIECES / 2;      // lanes that share a token's row
+        for (int r = lane / LANES; r < FB * 32; r += 64 / LANES) {
+            const int pc = lane % LANES * 2;
+            float v[8];
+            *(float4_t *)v = *(const float4_t *)(stage + r * (PIECES * 16) + ((pc ^ swz(r)) << 4));
+            *(float4_t *)(v + 4) = *(const float4_t *)(stage + r * (PIECES * 16) + (((pc + 1) ^ swz(r)) << 4));
+            const int m = m0 + wm * FB * 32 + r, n = n0 + (wn * FA + a0) * 32 + pc * 4;
+            if (p.slices > 1) {
+                if (m < p.M && n < p.N) {
+                    float *part = p.part + ((int64_t)slice * p.M + m) * p.part_ld + n;
+                    *(float4_t *)part = *(float4_t *)v;
+                    *(float4_t *)(part + 4) = *(float4_t *)(v + 4);
+                }
+            } else {
+                finish8<T, O>(p, m, n, v);
+            }
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// the slices' sums together, in their order, and the epilogue
+template <typename T, typename O, int SLICES>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p) {
+    const int per_row = (p.N + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int m = (int)(i / per_row), n = (int)(i - (int64_t)m * per_row) * 8;
+    if (m >= p.M) return;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    float4_t a[SLICES], b[SLICES];             // requested together: the kernel is one latency long
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) {
+        const float *part = p.part + ((int64_t)min(s, p.slices - 1) * p.M + m) * p.part_ld + n;
+        a[s] = *(const float4_t *)part;
+        b[s] = *(const float4_t *)(part + 4);
+    }
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) {
+        if (s >= p.slices) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] += a[s][e];
+            v[4 + e] += b[s][e];
+        }
+    }
+    finish8<T, O>(p, m, n, v);
+}
+
+// ---- any shape, any alignment ----------------------------------------------------------------
+// 64 x 64 tile, steps of 64 along K, operands through registers into LDS (rows padded by 16 bytes).
 template <typename T, typename O>
 __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
     constexpr int LD = 72;
@@ -332,45 +438,86 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
+enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_128_32, LIN_TILE_128_64, LIN_TILE_64_64, LIN_TILE_128_128, LIN_TILE_256_256, LIN_KINDS };
+static const int TILE_N[LIN_KINDS] = {16, 64, 128, 128, 64, 128, 256}, TILE_M[LIN_KINDS] = {16, 64, 32, 64, 64, 128, 256};
 struct LinearPlan {
-    int tile;          // index of the tile shape below, -1: the kernel for any shape
-    int slices, slice_k;
+    int kind, slices, slice_k;
     int64_t part_ld;
     size_t bytes;      // of workspace
     bool fits;         // the launch's workgroups are counted in 31 bits
 };
-static const int TILE_N[] = {128, 128, 128, 256}, TILE_M[] = {32, 64, 128, 256};
-
-static LinearPlan linear_plan(int M, int N, int K) {
+static int64_t linear_tiles(int kind, int M, int N) {
+    return (int64_t)((M + TILE_M[kind] - 1) / TILE_M[kind]) * ((N + TILE_N[kind] - 1) / TILE_N[kind]);
+}
+static LinearPlan linear_plan_of(int kind, int slices, int M, int N, int K) {
     LinearPlan l;
-    l.tile = M <= 32 ? 0 : M <= 64 ? 1 : (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 192 ? 3 : 2;
-    const int64_t tiles = (int64_t)((M + TILE_M[l.tile] - 1) / TILE_M[l.tile]) * ((N + TILE_N[l.tile] - 1) / TILE_N[l.tile]);
-    const int steps = (K + 63) / 64;
-    int slices = 1;
-    while (slices < 16 && tiles * slices * 2 <= 512 && steps / (slices * 2) >= 4) slices *= 2;
-    const int per = (steps + slices - 1) / slices;
+    l.kind = kind;
+    const int steps = (K + 63) / 64, per = (steps + slices - 1) / slices;
     l.slice_k = per * 64;
     l.slices = (steps + per - 1) / per;
     l.part_ld = ((int64_t)N + 7) / 8 * 8;
-    l.fits = tiles * l.slices <= 0x7ffffff0LL;
+    l.fits = linear_tiles(kind, M, N) * l.slices <= 0x7ffffff0LL;
     l.bytes = l.slices > 1 ? (size_t)l.slices * M * l.part_ld * 4 : 0;
     return l;
 }
+static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
+    // Up to 4 tokens, and up to 16 on a few hundred workgroups, one pass over the weights' rows beats the tiles (us, rows /
+    // 128 x 32 tiles): M = 1: K 4096, N 2048 7.1 / 9.9, K 2048, N 131072 93 / 100; M = 16: K 4096, N 2048 8.4 / 10.4, K 2048,
+    // N 5120 10.1 / 10.2, K 4096, N 16384 36.6 / 28.6, K 2048, N 131072 123 / 105.
+    if (M <= 4 || (M <= 16 && N <= 6144)) return linear_plan_of(LIN_ROWS, 1, M, N, K);
+    if (!aligned) return linear_plan_of(LIN_ANY, 1, M, N, K);
+    const int steps = (K + 63) / 64;
+    // Up to 64 tokens the weights' bytes count: as many tokens in a tile as there are, and parts of K until the workgroups
+    // are two per CU.  64 x 64 tiles once they alone fill the chip (M = 64, K 2048, us, 128 x 64 / 64 x 64: N 5120 12.3 /
+    // 13.2, N 32768 36.0 / 33.1, N 131072 117 / 113).
+    if (M <= 64) {
+        const int kind = M <= 32 ? LIN_TILE_128_32 : N >= 24576 ? LIN_TILE_64_64 : LIN_TILE_128_64;
+        int slices = 1;
+        while (slices < 8 && linear_tiles(kind, M, N) * slices * 2 <= 512 && steps / (slices * 2) >= 8) slices *= 2;
+        return linear_plan_of(kind, slices, M, N, K);
+    }
+    // More tokens: the shape and the number of parts of K with the least estimated time.  A round of workgroups (512, or
+    // 256 of the largest tile) takes a step's time for every 64 columns and its epilogue; parts of K cost a second launch.
+    // Step and epilogue in us, as measured on full rounds (K 2048 and 4096, bf16).  us of the shape taken / of others, K 4096,
+    // N 4096: M = 2048 (128 x 128) 66 / 81 (128 x 64), M = 4096 (256 x 256) 111 / 128 (128 x 128); K 2048, N 5120: M = 200
+    // (64 x 64) 14 / 18 / 22, M = 500 (128 x 64) 21 / 25 / 27.
+    static const float STEP[LIN_KINDS] = {0, 0, 0, 0.68f, 0.42f, 1.06f, 1.58f}, END[LIN_KINDS] = {0, 0, 0, 2.0f, 1.5f, 4.0f, 10.0f};
+    LinearPlan best = {};
+    float best_us = 0.0f;
+    for (int kind = LIN_TILE_128_64; kind <= LIN_TILE_256_256; ++kind) {
+        const int64_t slots = kind == LIN_TILE_256_256 ? 256 : 512;
+        for (int slices = 1; slices <= 8 && (slices == 1 || steps / slices >= 8); slices *= 2) {
+            const LinearPlan l = linear_plan_of(kind, slices, M, N, K);
+            const float rounds = (float)((linear_tiles(kind, M, N) * l.slices + slots - 1) / slots);
+            const float us = rounds * (l.slice_k / 64 * STEP[kind] + END[kind]) + (l.slices > 1 ? 4.0f + l.bytes / 2e6f : 0.0f);
+            if (best_us == 0.0f || us < best_us) {
+                best_us = us;
+                best = l;
+            }
+        }
+    }
+    return best;
+}
 
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES>
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES>
 static void launch_tile(LinearParams &p, hipStream_t st) {
-    typedef LinearTile<T, O, NWN, NWM, FA, FB, STAGES> C;
+    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES> C;
     p.tiles_n = (p.N + C::TN - 1) / C::TN;
     p.tiles_m = (p.M + C::TM - 1) / C::TM;
     const int64_t total = (int64_t)p.tiles_n * p.tiles_m * p.slices;
-    linear_tile_kernel<T, O, NWN, NWM, FA, FB, STAGES><<<(unsigned)((total + 7) / 8 * 8), C::NW * 64, 0, st>>>(p);
+    linear_tile_kernel<T, O, NWN, NWM, FA, FB, BK, STAGES><<<(unsigned)((total + 7) / 8 * 8), C::NW * 64, 0, st>>>(p);
 }
 
 template <typename T, typename O> static int launch_linear(LinearParams &p, const LinearPlan &l, void *workspace, hipStream_t st) {
-    // rows of whole 16-byte segments, and a tile's rows within 31 bits of bytes
-    const bool aligned = ((p.K | p.ldx | p.ldw) & 7) == 0 && odsd_aligned16(p.x) && odsd_aligned16(p.w) &&
-                         p.ldx < (1 << 21) && p.ldw < (1 << 21);
-    if (!aligned) {
+    if (l.kind == LIN_ROWS) {
+        // blocks of 64 columns that each of the 16 wavefronts has: requested together where there are more than two
+        const unsigned grid = (unsigned)((p.N + 15) / 16);
+        if (p.K > 2048) linear_rows_kernel<T, O, 16, 4><<<grid, 1024, 0, st>>>(p);
+        else linear_rows_kernel<T, O, 16, 2><<<grid, 1024, 0, st>>>(p);
+        ODSD_CHECK_LAUNCH();
+        return ODSD_OK;
+    }
+    if (l.kind == LIN_ANY) {
         linear_any_kernel<T, O><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64)), 256, 0, st>>>(p);
         ODSD_CHECK_LAUNCH();
         return ODSD_OK;
@@ -379,15 +526,19 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
     p.slice_k = l.slice_k;
     p.part = (float *)workspace;
     p.part_ld = l.part_ld;
-    switch (l.tile) {
-        case 0: launch_tile<T, O, 4, 1, 1, 1, 4>(p, st); break;
-        case 1: launch_tile<T, O, 4, 1, 1, 2, 3>(p, st); break;
-        case 2: launch_tile<T, O, 2, 2, 2, 2, 2>(p, st); break;
-        default: launch_tile<T, O, 2, 4, 4, 2, 2>(p, st); break;
+    switch (l.kind) {
+        case LIN_TILE_128_32: launch_tile<T, O, 4, 1, 1, 1, 64, 4>(p, st); break;
+        case LIN_TILE_128_64: launch_tile<T, O, 4, 1, 1, 2, 64, 3>(p, st); break;
+        case LIN_TILE_64_64: launch_tile<T, O, 2, 2, 1, 1, 64, 4>(p, st); break;
+        case LIN_TILE_128_128: launch_tile<T, O, 2, 2, 2, 2, 64, 2>(p, st); break;
+        default: launch_tile<T, O, 2, 4, 4, 2, 64, 2>(p, st); break;
     }
     if (p.slices > 1) {
         const int64_t units = (int64_t)p.M * ((p.N + 7) / 8);
-        linear_join_kernel<T, O><<<(unsigned)((units + 255) / 256), 256, 0, st>>>(p);
+        const unsigned grid = (unsigned)((units + 255) / 256);
+        if (p.slices <= 2) linear_join_kernel<T, O, 2><<<grid, 256, 0, st>>>(p);
+        else if (p.slices <= 4) linear_join_kernel<T, O, 4><<<grid, 256, 0, st>>>(p);
+        else linear_join_kernel<T, O, 8><<<grid, 256, 0, st>>>(p);
     }
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
@@ -395,7 +546,7 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
 
 extern "C" size_t odsd_linear_workspace_bytes(int32_t M, int32_t N, int32_t K) {
     if (M < 0 || N <= 0 || K <= 0) return 0;
-    const LinearPlan l = linear_plan(M, N, K);
+    const LinearPlan l = linear_plan(M, N, K, true);
     return !l.fits ? 0 : l.bytes > 256 ? l.bytes : 256;
 }
 
@@ -416,7 +567,9 @@ extern "C" int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ld
         !odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
     if (workspace_bytes < odsd_linear_workspace_bytes(M, N, K)) return ODSD_ERR_WORKSPACE;
     LinearParams p{x, w, bias, residual, out, ldx, ldw, ldr, ldo, M, N, K, act, 0, 0, 1, 0, nullptr, 0};
-    const LinearPlan l = linear_plan(M, N, K);
+    // rows of whole 16-byte segments, and a tile's rows within 31 bits of bytes
+    const bool aligned = ((K | ldx | ldw) & 7) == 0 && odsd_aligned16(x) && odsd_aligned16(w) && ldx < (1 << 21) && ldw < (1 << 21);
+    const LinearPlan l = linear_plan(M, N, K, aligned);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == ODSD_DT_BF16)
         return out_dtype == ODSD_DT_F32 ? launch_linear<__bf16, float>(p, l, workspace, st) : launch_linear<__bf16, __bf16>(p, l, workspace, st);
