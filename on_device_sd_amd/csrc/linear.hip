@@ -92,21 +92,28 @@ __device__ __forceinline__ void finish1(const LinearParams &p, int m, int n, flo
     ((O *)p.out)[(int64_t)m * p.ldo + n] = (O)v;
 }
 
-// eight values of a row from column k on, zeros behind its end; at the elements' own alignment
-template <typename T>
-__device__ __forceinline__ uint4_t load8_any(const T *row, int k, int K, bool row_ok) {
+// Eight values of a row from column k on, at the elements' own alignment, without a branch before the load: at the row's end
+// its last eight, of which clip8() zeroes those in front of k (all, if k is behind the end).  Both operands of a product are
+// loaded so, so their columns stay together.  load8_short: K < 8, one by one.
+template <typename T> __device__ __forceinline__ uint4_t load8(const T *row, int k, int K) {
+    uint4_t v;
+    __builtin_memcpy(&v, row + min(k, K - 8), 16);
+    return v;
+}
+template <typename T> __device__ __forceinline__ uint4_t load8_short(const T *row, int k, int K) {
     uint4_t v = {0, 0, 0, 0};
-    if (!row_ok) return v;
-    if (k + 8 <= K) {
-        __builtin_memcpy(&v, row + k, 16);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            uint16_t e = 0;
-            if (k + i < K) __builtin_memcpy(&e, row + k + i, 2);
-            v[i >> 1] |= (uint32_t)e << (16 * (i & 1));
-        }
+    for (int i = 0; i < 8; ++i) {
+        uint16_t e = 0;
+        if (k + i < K) __builtin_memcpy(&e, row + k + i, 2);
+        v[i >> 1] |= (uint32_t)e << (16 * (i & 1));
     }
+    return v;
+}
+__device__ __forceinline__ uint4_t clip8(uint4_t v, int k, int K) {
+    const int skip = K >= 8 ? k - (K - 8) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = skip > 2 * i + 1 ? 0u : skip > 2 * i ? v[i] & 0xffff0000u : v[i];
     return v;
 }
 
@@ -153,10 +160,24 @@ __global__ __launch_bounds__(NWV * 64) void linear_rows_kernel(LinearParams p) {
     while (b + (DEPTH - 1) * NWV < full) group(std::integral_constant<int, DEPTH>{});
     while (b < full) group(std::integral_constant<int, 1>{});
     if (b < blocks) {                                          // the block that K ends in
+        const int k = b * 64 + g * 16;
+        if (p.K < 8) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            a[0][u] = load8_any(w, b * 64 + g * 16 + u * 8, p.K, true);
-            c[0][u] = load8_any(x, b * 64 + g * 16 + u * 8, p.K, token);
+            for (int u = 0; u < 2; ++u) {
+                a[0][u] = load8_short(w, k + u * 8, p.K);
+                c[0][u] = load8_short(x, k + u * 8, p.K);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                a[0][u] = load8(w, k + u * 8, p.K);
+                c[0][u] = load8(x, k + u * 8, p.K);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                a[0][u] = clip8(a[0][u], k + u * 8, p.K);
+                c[0][u] = clip8(c[0][u], k + u * 8, p.K);
+            }
         }
         multiply(0);
     }
@@ -390,12 +411,18 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
     const int row = tid >> 3, col = (tid & 7) * 8;       // rows `row` and `row + 32`, 8 values from `col` on
     const T *w = (const T *)p.w, *x = (const T *)p.x;
     uint4_t rw[2], rx[2];
+    // (rows past the last: products that nobody stores)
+    const T *wr[2], *xr[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        wr[i] = w + (int64_t)min(n0 + row + 32 * i, p.N - 1) * p.ldw;
+        xr[i] = x + (int64_t)min(m0 + row + 32 * i, p.M - 1) * p.ldx;
+    }
     auto fetch = [&](int k) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int n = n0 + row + 32 * i, m = m0 + row + 32 * i;
-            rw[i] = load8_any(w + (int64_t)min(n, p.N - 1) * p.ldw, k + col, p.K, n < p.N);
-            rx[i] = load8_any(x + (int64_t)min(m, p.M - 1) * p.ldx, k + col, p.K, m < p.M);
+            rw[i] = load8(wr[i], k + col, p.K);
+            rx[i] = load8(xr[i], k + col, p.K);
         }
     };
     const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32;
@@ -404,9 +431,24 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
     for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int b = 0; b < 2; ++b) acc[a][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    fetch(0);
+    if (p.K >= 8) {
+        fetch(0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            rw[i] = load8_short(wr[i], col, p.K);
+            rx[i] = load8_short(xr[i], col, p.K);
+        }
+    }
     for (int k = 0; k < p.K; k += 64) {
         __syncthreads();
+        if (k + 64 > p.K && p.K >= 8) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                rw[i] = clip8(rw[i], k + col, p.K);
+                rx[i] = clip8(rx[i], k + col, p.K);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             *(uint4_t *)(ws + (row + 32 * i) * LD + col) = rw[i];

@@ -7,16 +7,44 @@
 // p.  Drawn means: the lowest token whose inclusive cumulative weight exceeds r times the total.  T = 0: p is one-hot at the
 // largest logit (the lowest index of equals).
 //
-// All probabilities and sums are fp64.  A cumulative sum over 100 000 tokens in fp32 has borders that are off by more than
-// many tokens' probability, and p - q of two good models is a small difference; in fp64 a token does not depend on the
-// order of the sums or the accuracy of exp but with a probability of about 1e-11 a draw.  On this chip an fp64 FMA issues at
-// the rate of an unpacked fp32 one, so the 20 instructions of exp stay near the time that the logits take to arrive.
+// What a token is drawn from is fp64: a cumulative sum over 100 000 tokens in fp32 has borders that are off by more than many
+// tokens' probability, and p - q of two good models is a small difference; in fp64 a token depends on the order of the sums
+// and the accuracy of exp (2e-13) with a probability of about 1e-11 a draw.  Only the row that a sequence draws from needs
+// that; whether a draft is kept takes the statistics of every row, and those are one pass in fp32: exp2 by the hardware (1 ulp)
+// of an argument to 48 bits, sums in fp32 over 4 logits and by a tree over 32, in fp64 above that.  A sum is off by less than
+// 2^-23 + 6 2^-24 relative, plus 17 ln 2 2^-24 where l - top is not exact (16-bit logits 2^16 times below the largest).
+//
+// Launches: statistics of all rows (with drafts); which drafts stay, and the exact sums of p and q of the rows at hand (with
+// draft logits); sums of the weights, 512 tokens each; the draw.
 #include "common.h"
+#include <type_traits>
 
 #define VER_THREADS 256
 #define VER_CHUNK 8192          // logits of one row that a workgroup takes: 32 a thread, kept in registers
 #define VER_SUB 512             // granularity of the sums that the draw walks over: 8 consecutive logits a lane
 
+// of a chunk of a row: its largest logit, the lowest index that has it (greedy), else sum exp((l - top) / T)
+struct Stat {
+    float top;
+    int at;
+    double z;
+};
+// which distribution the next token of a sequence is drawn from
+struct Choice {
+    int row, draft;                 // row of the target, of the draft (-1: none); row -1: nothing to draw from
+    int count;                      // kept drafts
+    int greedy;                     // the token of the one-hot target, -1: not greedy
+    int one_hot;                    // refused draft without logits: its token, else -1
+    float top_p, top_q;             // the rows' largest logits (only with draft >= 0)
+    int pad;
+    double k;                       // log2(e) / T
+};
+// of VER_SUB tokens: the sum of their weights relative to exp((top - row's top) / T)
+struct Block {
+    double sum;
+    float top;
+    int pad;
+};
 struct VerifyParams {
     const void *logits, *draft_logits;
     int64_t ld_t, ld_d;
@@ -30,70 +58,132 @@ struct VerifyParams {
     int64_t *tokens;
     int32_t *num_accepted;
     float *accept_probs;
-    struct Stat *stats;             // [n_q + n_d][splits]
-    double *sums;                   // [S][subs]
-    struct Choice *choice;          // [S]
-};
-// of a chunk of a row: its largest logit, the lowest index that has it, and sum exp((l - max) / T)
-struct Stat {
-    float top;
-    int at;
-    double z;
-};
-// which distribution the next token of a sequence is drawn from
-struct Choice {
-    int row, draft;                 // row of the target, of the draft (-1: none); row -1: no row is left
-    int count;                      // accepted drafts
-    int greedy;                     // or token of the one-hot target, -1: not greedy
-    int one_hot;                    // draft without logits: the drafted token, else -1
-    float top_p, top_q;
-    int pad;
-    double z_p, z_q, k;             // k: log2(e) / T
+    Stat *stats;                    // [n_q + n_d][splits]
+    double *z;                      // [S][splits][2]: exact sums of the chunks of p and q of the chosen rows
+    Block *blocks;                  // [S][subs]
+    Choice *choice;                 // [S]
 };
 
-// e^(ln2 t) = 2^t for t <= 0 (anything below -1100, and NaN, gives 0): 2^n by the exponent, 2^f, |f| <= 1/2, as the Taylor
-// polynomial of degree 10 in f ln 2 (remainder 0.347^11 / 11! = 2e-13 relative)
+// 2^t for t <= 0, not far below -1100: 2^n by the exponent, 2^f, |f| <= 1/2, by its interpolation at the ten Chebyshev points of the
+// interval (degree 9, 1.9e-14 relative)
 __device__ __forceinline__ double exp2_neg(double t) {
-    t = fmax(t, -1100.0);
-    const double n = rint(t);
-    const double f = (t - n) * 0.69314718055994530942;
-    double e = 2.7557319223985891e-7;
-    e = fma(e, f, 2.7557319223985893e-6);
-    e = fma(e, f, 2.4801587301587302e-5);
-    e = fma(e, f, 1.9841269841269841e-4);
-    e = fma(e, f, 1.3888888888888889e-3);
-    e = fma(e, f, 8.3333333333333333e-3);
-    e = fma(e, f, 4.1666666666666667e-2);
-    e = fma(e, f, 1.6666666666666667e-1);
-    e = fma(e, f, 0.5);
-    e = fma(e, f, 1.0);
-    e = fma(e, f, 1.0);
+    const double n = rint(t), f = t - n;
+    double e = 1.0205905413765595e-07;
+    e = fma(e, f, 1.325964524488711e-06);
+    e = fma(e, f, 1.5252672924850737e-05);
+    e = fma(e, f, 0.0001540343375125101);
+    e = fma(e, f, 0.0013333558200794592);
+    e = fma(e, f, 0.009618129193934313);
+    e = fma(e, f, 0.05550410866465167);
+    e = fma(e, f, 0.2402265069564034);
+    e = fma(e, f, 0.6931471805599462);
+    e = fma(e, f, 1.0000000000000135);
     return ldexp(e, (int)n);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {      // a NaN counts as nothing
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float number(float l) { return l == l ? l : -INFINITY; }
 // exp((l - top) / T).  A row whose largest logit is +inf has its weight on the +inf entries; one without any number has none.
 __device__ __forceinline__ double weight_of(float l, float top, double k) {
     if (top == INFINITY) return l == INFINITY ? 1.0 : 0.0;
-    if (top == -INFINITY) return 0.0;
-    return exp2_neg(((double)l - (double)top) * k);
+    if (!(l > -INFINITY) || top == -INFINITY) return 0.0;
+    const double t = ((double)l - (double)top) * k;
+    return t > -1100.0 ? exp2_neg(t) : 0.0;
 }
-
-__device__ __forceinline__ float up(float v) { return v; }
-__device__ __forceinline__ float up(__bf16 v) { return (float)v; }
-__device__ __forceinline__ float up(half_t v) { return (float)v; }
-
-// eight consecutive logits of a row, at the elements' own alignment; NaN and what is behind the row's end count as -inf
-template <typename T> __device__ __forceinline__ void load8(const T *row, int i, int V, float *l) {
-    T e[8];
-    if (i + 8 <= V) {
-        __builtin_memcpy(e, row + i, sizeof e);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) l[j] = up(e[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) l[j] = i + j < V ? up(row[i + j]) : -INFINITY;
+// The same for many logits of a row: where nothing is out of the ordinary, a clamp in fp32 stands for all cases (NaN, -inf and
+// what weighs nothing become 2^-1200, which is 0), and (l - top) k is one FMA (top k is off by 2^-53 of itself).  Eight at a
+// time, so that the chains of FMAs hide each other's latency, with the coefficients in scalar registers (as literals they
+// cost two moves an FMA): 17 instructions a logit, 39 one by one.
+struct Weigh {
+    double k, shift;
+    float low, top;
+    bool plain;
+    __device__ __forceinline__ Weigh(float top_, double k_) : k(k_), top(top_) {
+        low = (float)((double)top - 1200.0 / k);
+        shift = -(double)top * k;
+        const double least = ((double)top - (double)low) * k;
+        plain = fabsf(top) < 1e30f && k > 1e-20 && k < 1e20 && least > 1100.0 && least < 1e6 && fabs(shift) < 1e4;
+        plain = __builtin_amdgcn_readfirstlane(plain);
     }
+    template <typename R> __device__ __forceinline__ void operator()(const R &r, double *w) const {
+        const double c[10] = {1.0000000000000135, 0.6931471805599462, 0.2402265069564034, 0.05550410866465167,
+                              0.009618129193934313, 0.0013333558200794592, 0.0001540343375125101,
+                              1.5252672924850737e-05, 1.325964524488711e-06, 1.0205905413765595e-07};
+        double f[8], n[8];
+        if (plain) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l[j] = l[j] == l[j] ? l[j] : -INFINITY;
+            for (int j = 0; j < 8; ++j) f[j] = fma((double)max3(r.get(j), low, low), k, shift);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float l = r.get(j);
+                const double t = top == INFINITY ? (l == INFINITY ? 0.0 : -1200.0) : ((double)l - (double)top) * k;
+                f[j] = t > -1200.0 ? t : -1200.0;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            n[j] = rint(f[j]);
+            f[j] -= n[j];
+            w[j] = c[9];
+        }
+#pragma unroll
+        for (int i = 8; i >= 0; --i) {
+            double ci = c[i];
+            asm("" : "+s"(ci));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = fma(w[j], f[j], ci);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = ldexp(w[j], (int)n[j]);
+    }
+};
+
+// Eight consecutive logits as they lie in memory, at the elements' own alignment.  A row's last eight are loaded where it
+// ends: `base` is where, and what is in front of the eight asked for (or all, behind the end) becomes -inf by clip().  No lane
+// branches before its loads, so those of a thread are on their way together.  (Rows have 8 logits at least: pad_kernel.)
+template <typename T> struct Raw8 {
+    uint32_t w[sizeof(T) * 2];
+    int base, skip;
+    __device__ __forceinline__ void load(const T *row, int i, int V) {
+        base = min(i, V - 8);
+        skip = i - base;
+        __builtin_memcpy(w, row + base, sizeof w);
+    }
+    __device__ __forceinline__ void clip() {
+        if (!__any(skip > 0)) return;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = j < skip ? 0xff800000u : w[j];
+        } else {
+            constexpr uint32_t low = std::is_same<T, __bf16>::value ? 0xff80u : 0xfc00u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (2 * j < skip) w[j] = (w[j] & 0xffff0000u) | low;
+                if (2 * j + 1 < skip) w[j] = (w[j] & 0xffffu) | (low << 16);
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[j]);
+        } else {
+            const uint32_t two = w[j >> 1];
+            if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
+            else return (float)__builtin_bit_cast(half_t, (uint16_t)(j & 1 ? two >> 16 : two));
+        }
+    }
+};
+template <typename T> __device__ __forceinline__ float largest8(const Raw8<T> &r) {
+    const float t = max3(max3(r.get(0), r.get(1), r.get(2)), max3(r.get(3), r.get(4), r.get(5)), max3(r.get(6), r.get(7), -INFINITY));
+    if (t == t) return t;
+    float m = -INFINITY;                                                // (signalling NaN come back from the hardware's maximum)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, number(r.get(j)));
+    return m;
 }
 
 // the larger logit, the lower index of equals
@@ -108,6 +198,15 @@ __device__ __forceinline__ float temperature_of(const VerifyParams &p, int s) { 
 __device__ __forceinline__ int len_of(const VerifyParams &p, int s) { return p.query_lens ? max(p.query_lens[s], 0) : 1; }
 // log2(e) / T; 0 says greedy
 __device__ __forceinline__ double factor_of(float t) { return t > 0.0f ? 1.4426950408889634074 / (double)t : 0.0; }
+
+// rows of fewer than 8 logits, as rows of 8
+template <typename T>
+__global__ __launch_bounds__(VER_THREADS) void verify_pad_kernel(const T *src, int64_t ld, T *dst, int rows, int V) {
+    const int64_t i = (int64_t)blockIdx.x * VER_THREADS + threadIdx.x;
+    const int64_t row = i >> 3;
+    const int j = (int)(i & 7);
+    if (row < rows) dst[i] = j < V ? src[row * ld + j] : (T)-INFINITY;
+}
 
 // the sequence that row `r` of the target (or of the drafts) belongs to: by the whole wavefront
 __device__ __forceinline__ int sequence_of(const VerifyParams &p, int r, bool draft) {
@@ -135,195 +234,354 @@ __global__ __launch_bounds__(VER_THREADS) void verify_stats_kernel(VerifyParams 
     __shared__ float s_top[4];
     __shared__ int s_at[4];
     __shared__ double s_z[4];
-    const int row = blockIdx.x / p.splits, c = blockIdx.x - row * p.splits;
+    const int row = blockIdx.x / p.splits, c = blockIdx.x - row * p.splits, wave = threadIdx.x >> 6;
     const bool draft = row >= p.n_q;
     const int r = draft ? row - p.n_q : row;
     const T *src = draft ? (const T *)p.draft_logits + (int64_t)r * p.ld_d : (const T *)p.logits + (int64_t)r * p.ld_t;
-    float l[32];
+    const int first = c * VER_CHUNK + (int)threadIdx.x * 8;
+    Raw8<T> raw[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load8(src, c * VER_CHUNK + i * (VER_THREADS * 8) + (int)threadIdx.x * 8, p.V, l + 8 * i);
+    for (int i = 0; i < 4; ++i) raw[i].load(src, first + i * (VER_THREADS * 8), p.V);
     float t = p.temperature_all;
     if (p.temperature) {
         const int s = sequence_of(p, r, draft);
         t = s < 0 ? 0.0f : p.temperature[s];
     }
     const double k = factor_of(t);
-    float top = -INFINITY;
-    int at = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) better(top, at, l[i], c * VER_CHUNK + (i >> 3) * (VER_THREADS * 8) + (int)threadIdx.x * 8 + (i & 7));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) better(top, at, __shfl_xor(top, o, ODSD_WAVE), __shfl_xor(at, o, ODSD_WAVE));
-    const int wave = threadIdx.x >> 6;
-    if (lane_id() == 0) {
-        s_top[wave] = top;
-        s_at[wave] = at;
-    }
+    for (int i = 0; i < 4; ++i) raw[i].clip();
+    float top = max3(largest8(raw[0]), largest8(raw[1]), fmaxf(largest8(raw[2]), largest8(raw[3])));
+    const float own = top;
+    top = wave_max(top);
+    if (lane_id() == 0) s_top[wave] = top;
     __syncthreads();
-    top = s_top[0];
-    at = s_at[0];
-    for (int w = 1; w < 4; ++w) better(top, at, s_top[w], s_at[w]);
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    int at = 0x7fffffff;
     double z = 0.0;
-    if (k > 0.0) {
+    if (!(k > 0.0)) {                                  // greedy: where it is, nothing else
+        if (own == top) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) z += weight_of(l[i], top, k);
+            for (int i = 3; i >= 0; --i)
+#pragma unroll
+                for (int j = 7; j >= 0; --j)
+                    if (raw[i].get(j) == top && j >= raw[i].skip) at = raw[i].base + j;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, ODSD_WAVE));
+        if (lane_id() == 0) s_at[wave] = at;
+    } else {
+        if (fabsf(top) < INFINITY && k > 1e-30 && k < 1e30) {
+            // x = (l - top) k to 48 bits: a part that exp2 takes as it is, and its rest times the derivative
+            const float kh = (float)k, kl = (float)(k - (double)kh), low = -160.0f / kh;
+            // sum e (1 + ln 2 lo) as sum e + ln 2 sum e lo
+            float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, more[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float l = raw[i].get(j), d0 = l - top;
+                    const float d = max3(d0, low, low);                          // (NaN and -inf: 2^-160)
+                    const float hi = d * kh;
+                    float lo = fmaf(d, kl, fmaf(d, kh, -hi));
+                    if (sizeof(T) == 4) {                                        // what l - top lost (16-bit logits: as good as nothing)
+                        const float b = l - d0;
+                        const float lost = (l - (d0 + b)) + (b - top);
+                        lo = d > low ? fmaf(lost, kh, lo) : lo;
+                    }
+                    const float e = __builtin_amdgcn_exp2f(hi);
+                    sum[j] += e;
+                    more[j & 1] = fmaf(e, lo, more[j & 1]);
+                }
+            z = (double)(((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]))) +
+                0.69314718055994530942 * (double)(more[0] + more[1]);
+        } else {
+            // (any temperature, any logits; read again, one by one)
+#pragma unroll 1
+            for (int i = 0; i < 32; ++i) {
+                const int at = first + (i >> 3) * (VER_THREADS * 8) + (i & 7);
+                if (at < p.V) z += weight_of(number((float)src[at]), top, k);
+            }
+        }
         z = wave_sum(z);
         if (lane_id() == 0) s_z[wave] = z;
-        __syncthreads();
-        z = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
     }
-    if (threadIdx.x == 0) p.stats[(int64_t)row * p.splits + c] = Stat{top, at, z};
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        Stat st{top, 0x7fffffff, 0.0};
+        if (k > 0.0) st.z = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
+        else st.at = min(min(s_at[0], s_at[1]), min(s_at[2], s_at[3]));
+        p.stats[(int64_t)row * p.splits + c] = st;
+    }
 }
 
-// the whole row's, by one wavefront
+// the whole row's, by 16 neighbouring lanes
 __device__ __forceinline__ Stat row_stat(const VerifyParams &p, int row, double k) {
-    Stat all{-INFINITY, 0x7fffffff, 0.0};
     const Stat *st = p.stats + (int64_t)row * p.splits;
-    for (int c = lane_id(); c < p.splits; c += 64) better(all.top, all.at, st[c].top, st[c].at);
+    const int l = lane_id() & 15;
+    Stat own{-INFINITY, 0x7fffffff, 0.0};
+    if (l < p.splits) own = st[l];
+    float top = own.top;
+    int at = own.at;
+    for (int c = l + 16; c < p.splits; c += 16) better(top, at, st[c].top, st[c].at);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) better(all.top, all.at, __shfl_xor(all.top, o, ODSD_WAVE), __shfl_xor(all.at, o, ODSD_WAVE));
-    for (int c = lane_id(); c < p.splits; c += 64) all.z += st[c].z * weight_of(st[c].top, all.top, k);
-    all.z = wave_sum(all.z);
-    return all;
+    for (int o = 8; o > 0; o >>= 1) better(top, at, __shfl_xor(top, o, ODSD_WAVE), __shfl_xor(at, o, ODSD_WAVE));
+    double z = 0.0;
+    if (k > 0.0) {
+        z = own.z * weight_of(own.top, top, k);
+        for (int c = l + 16; c < p.splits; c += 16) z += st[c].z * weight_of(st[c].top, top, k);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, ODSD_WAVE);
+    }
+    return Stat{top, at, z};
 }
 
 // ---- which drafts stay -----------------------------------------------------------------------------
-// One workgroup per sequence, a wavefront per draft.
+// By a whole workgroup; every workgroup of a sequence comes to the same answer, one (`writes`) leaves it.  Rows in batches of
+// 32: their statistics by 16 lanes each, then a lane per draft.  Without drafts in the call there are no statistics and
+// nothing to decide.
 template <typename T>
-__global__ __launch_bounds__(VER_THREADS) void verify_accept_kernel(VerifyParams p) {
-    __shared__ int s_start[4], s_dstart[4], s_first;
-    const int s = blockIdx.x, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) s_first = 0x7fffffff;
+__device__ Choice choose(const VerifyParams &p, const int s, const bool writes) {
+    __shared__ int s_start[4], s_dstart[4];
+    __shared__ Stat s_p[32], s_q[32];
+    __shared__ Choice s_choice;
+    __shared__ bool s_done;
+    const int wave = threadIdx.x >> 6;
     int start = 0, dstart = 0;
-    for (int i = threadIdx.x; i < s; i += VER_THREADS) {
-        const int n = len_of(p, i);
-        start += n;
-        dstart += max(n - 1, 0);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        start += __shfl_xor(start, o, ODSD_WAVE);
-        dstart += __shfl_xor(dstart, o, ODSD_WAVE);
-    }
-    if (lane_id() == 0) {
-        s_start[wave] = start;
-        s_dstart[wave] = dstart;
-    }
-    __syncthreads();
-    start = s_start[0] + s_start[1] + s_start[2] + s_start[3];
-    dstart = s_dstart[0] + s_dstart[1] + s_dstart[2] + s_dstart[3];
-    // rows and drafts that are really there; drafts that no row verifies are not accepted
-    int n = min(min(len_of(p, s), p.max_q), p.n_q - start);
-    n = min(n, p.n_d - dstart + 1);
-    const int d_end = s == p.S - 1 ? p.n_d : min(dstart + max(len_of(p, s) - 1, 0), p.n_d);
-    for (int j = dstart + max(n - 1, 0) + (int)threadIdx.x; j < d_end; j += VER_THREADS) p.accept_probs[j] = 0.0f;
     const float t = temperature_of(p, s);
-    const double k = factor_of(t);
-    for (int j = wave; j < n - 1; j += 4) {
-        const int64_t d = p.drafts[dstart + j];
-        double a = 0.0;
-        if (d >= 0 && d < p.V) {
-            const Stat sp = row_stat(p, start + j, k);
-            const float lp = up(((const T *)p.logits)[(int64_t)(start + j) * p.ld_t + d]);
-            double pd, qd = 1.0;
-            if (k > 0.0) {
-                pd = sp.z > 0.0 ? weight_of(lp, sp.top, k) / sp.z : 0.0;
-                if (p.draft_logits) {
-                    const Stat sq = row_stat(p, p.n_q + dstart + j, k);
-                    const float lq = up(((const T *)p.draft_logits)[(int64_t)(dstart + j) * p.ld_d + d]);
-                    qd = sq.z > 0.0 ? weight_of(lq, sq.top, k) / sq.z : 0.0;
-                }
-            } else {
-                pd = sp.top > -INFINITY && sp.at == (int)d ? 1.0 : 0.0;
-            }
-            a = pd >= qd ? (pd > 0.0 ? 1.0 : 0.0) : pd / qd;
+    const int len = len_of(p, s);
+    if (p.query_lens) {
+        for (int i = threadIdx.x; i < s; i += VER_THREADS) {
+            const int n = len_of(p, i);
+            start += n;
+            dstart += max(n - 1, 0);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            start += __shfl_xor(start, o, ODSD_WAVE);
+            dstart += __shfl_xor(dstart, o, ODSD_WAVE);
         }
         if (lane_id() == 0) {
-            p.accept_probs[dstart + j] = (float)a;
-            if (!((double)p.accept_u[dstart + j] < a)) atomicMin(&s_first, j);
+            s_start[wave] = start;
+            s_dstart[wave] = dstart;
         }
+        __syncthreads();
+        start = s_start[0] + s_start[1] + s_start[2] + s_start[3];
+        dstart = s_dstart[0] + s_dstart[1] + s_dstart[2] + s_dstart[3];
+    } else {
+        start = s;
+    }
+    // rows and drafts that are really there; drafts that no row verifies are not kept
+    const int n = max(min(min(min(len, p.max_q), p.n_q - start), p.n_d - dstart + 1), 0);
+    if (writes) {
+        const int d_end = s == p.S - 1 ? p.n_d : min(dstart + max(len - 1, 0), p.n_d);
+        for (int j = dstart + max(n - 1, 0) + (int)threadIdx.x; j < d_end; j += VER_THREADS) p.accept_probs[j] = 0.0f;
+    }
+    const double k = factor_of(t);
+    if (threadIdx.x == 0) {
+        s_choice = Choice{n > 0 ? start : -1, -1, 0, -1, -1, 0.0f, 0.0f, 0, k};
+        s_done = false;
     }
     __syncthreads();
-    const int count = max(min(s_first, n - 1), 0);
-    int64_t *out = p.tokens + (int64_t)s * p.max_q;
-    for (int j = threadIdx.x; j < p.max_q; j += VER_THREADS)
-        if (j != count) out[j] = j < count ? p.drafts[dstart + j] : -1;
-    if (wave != 0) return;
-    Choice c;
-    c.row = n > 0 ? start + count : -1;
-    c.draft = n > 0 && count < n - 1 && p.draft_logits && k > 0.0 ? dstart + count : -1;
-    c.one_hot = n > 0 && count < n - 1 && !p.draft_logits ? (int)min(max(p.drafts[dstart + count], (int64_t)-1), (int64_t)0x7fffffff) : -1;
-    c.count = count;
-    c.greedy = -1;
-    c.k = k;
-    c.pad = 0;
-    c.top_p = c.top_q = 0.0f;
-    c.z_p = c.z_q = 1.0;
-    if (n > 0) {
-        const Stat sp = row_stat(p, c.row, k);
-        c.top_p = sp.top;
-        c.z_p = sp.z;
-        if (!(sp.top > -INFINITY)) c.row = -1;                     // a row without a number: nothing to draw from
-        else if (!(k > 0.0)) c.greedy = sp.at;
-        if (c.draft >= 0) {
-            const Stat sq = row_stat(p, p.n_q + c.draft, k);
-            c.top_q = sq.top;
-            c.z_q = sq.z;
-            if (!(sq.z > 0.0)) c.draft = -1;                       // q is nowhere: p - q is p
+    if (p.n_d > 0) {
+        const bool with_q = p.draft_logits && k > 0.0;
+        for (int j0 = 0; j0 < n; j0 += 32) {
+            const int rows = min(32, n - j0), drafts = min(32, n - 1 - j0);
+            for (int g = threadIdx.x >> 4; g < (with_q ? 64 : 32); g += VER_THREADS / 16) {
+                const int j = g & 31;
+                if (g < 32 ? j >= rows : j >= drafts) continue;
+                const Stat st = row_stat(p, g < 32 ? start + j0 + j : p.n_q + dstart + j0 + j, k);
+                if ((lane_id() & 15) == 0) (g < 32 ? s_p : s_q)[j] = st;
+            }
+            // the drafts' own logits on their way meanwhile
+            const int j = lane_id();
+            int64_t d = -1;
+            float u = 0.0f, lp = -INFINITY, lq = -INFINITY;
+            if (wave == 0 && j < drafts) {
+                d = p.drafts[dstart + j0 + j];
+                u = p.accept_u[dstart + j0 + j];
+                if (d >= 0 && d < p.V) {
+                    lp = (float)((const T *)p.logits)[(int64_t)(start + j0 + j) * p.ld_t + d];
+                    if (with_q) lq = (float)((const T *)p.draft_logits)[(int64_t)(dstart + j0 + j) * p.ld_d + d];
+                }
+            }
+            __syncthreads();
+            if (wave == 0) {
+                double a = 0.0;
+                if (j < drafts && d >= 0 && d < p.V) {
+                    const Stat sp = s_p[j];
+                    double pd, qd = 1.0;
+                    if (k > 0.0) {
+                        pd = sp.z > 0.0 ? weight_of(lp, sp.top, k) / sp.z : 0.0;
+                        if (with_q) qd = s_q[j].z > 0.0 ? weight_of(lq, s_q[j].top, k) / s_q[j].z : 0.0;
+                    } else {
+                        pd = sp.top > -INFINITY && sp.at == (int)d ? 1.0 : 0.0;
+                    }
+                    a = pd >= qd ? (pd > 0.0 ? 1.0 : 0.0) : pd / qd;
+                }
+                if (writes && j < drafts) p.accept_probs[dstart + j0 + j] = (float)a;
+                const uint64_t refused = __ballot(j < drafts && !((double)u < a));
+                const bool ends = refused != 0 || j0 + rows == n;
+                if (!s_done && ends) {
+                    const int at = refused ? __builtin_ctzll(refused) : rows - 1;      // of the batch: the row that is drawn from
+                    const int64_t d_at = __shfl(d, at, ODSD_WAVE);
+                    if (j == 0) {
+                        Choice c = s_choice;
+                        c.row = start + j0 + at;
+                        c.count = j0 + at;
+                        c.top_p = s_p[at].top;
+                        if (!(c.top_p > -INFINITY)) c.row = -1;                        // a row without a number: nothing to draw from
+                        else if (!(k > 0.0)) c.greedy = s_p[at].at;
+                        if (refused && with_q) {
+                            c.top_q = s_q[at].top;
+                            if (s_q[at].z > 0.0) c.draft = dstart + j0 + at;           // (q is nowhere: p - q is p)
+                        }
+                        if (refused && !p.draft_logits && d_at >= 0 && d_at < p.V) c.one_hot = (int)d_at;
+                        s_choice = c;
+                        s_done = true;
+                    }
+                }
+            }
+            __syncthreads();
+            if (s_done && !writes) break;
         }
     }
-    if (lane_id() == 0) {
-        p.choice[s] = c;
-        p.num_accepted[s] = count;
-        if (c.row < 0 || c.greedy >= 0) {
-            if (count < p.max_q) out[count] = c.row < 0 ? -1 : c.greedy;
+    const Choice c = s_choice;
+    if (writes) {
+        int64_t *out = p.tokens + (int64_t)s * p.max_q;
+        // (the token behind the kept ones is the draw's, unless it is known here)
+        const bool drawn = c.row >= 0 && c.greedy < 0;
+        for (int j = threadIdx.x; j < p.max_q; j += VER_THREADS)
+            if (j != c.count || !drawn) out[j] = j < c.count ? p.drafts[dstart + j] : j == c.count && c.row >= 0 ? c.greedy : -1;
+        if (threadIdx.x == 0) {
+            p.choice[s] = c;
+            p.num_accepted[s] = c.count;
         }
+    }
+    return c;
+}
+
+// The exact sums of a chunk of p and of q of the rows that a refused draft leaves (with draft logits).
+template <typename T>
+__global__ __launch_bounds__(VER_THREADS) void verify_choose_kernel(VerifyParams p) {
+    __shared__ double s_z[2][4];
+    const int s = blockIdx.y;
+    const Choice c = choose<T>(p, s, blockIdx.x == 0);
+    if (c.row < 0 || c.greedy >= 0 || c.draft < 0) return;
+    Raw8<T> rp[4], rq[4];
+    const T *lp = (const T *)p.logits + (int64_t)c.row * p.ld_t, *lq = (const T *)p.draft_logits + (int64_t)c.draft * p.ld_d;
+    const int first = blockIdx.x * VER_CHUNK + (int)threadIdx.x * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        rp[i].load(lp, first + i * (VER_THREADS * 8), p.V);
+        rq[i].load(lq, first + i * (VER_THREADS * 8), p.V);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        rp[i].clip();
+        rq[i].clip();
+    }
+    double zp = 0.0, zq = 0.0;
+    const Weigh wp(c.top_p, c.k), wq(c.top_q, c.k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        double w[8], v[8];
+        wp(rp[i], w);
+        wq(rq[i], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            zp += w[j];
+            zq += v[j];
+        }
+    }
+    zp = wave_sum(zp);
+    zq = wave_sum(zq);
+    if (lane_id() == 0) {
+        s_z[0][threadIdx.x >> 6] = zp;
+        s_z[1][threadIdx.x >> 6] = zq;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const double *z = s_z[threadIdx.x];
+        p.z[((int64_t)s * p.splits + blockIdx.x) * 2 + threadIdx.x] = (z[0] + z[1]) + (z[2] + z[3]);
     }
 }
 
-// weights of eight consecutive tokens: p, and max(p - q, 0)
-template <typename T>
-__device__ __forceinline__ void weights8(const VerifyParams &p, const Choice &c, int i, bool rest, double *w) {
-    float l[8];
-    load8((const T *)p.logits + (int64_t)c.row * p.ld_t, i, p.V, l);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = weight_of(l[j], c.top_p, c.k) / c.z_p;
-    if (!rest) return;
-    if (c.draft >= 0) {
-        load8((const T *)p.draft_logits + (int64_t)c.draft * p.ld_d, i, p.V, l);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = fmax(w[j] - weight_of(l[j], c.top_q, c.k) / c.z_q, 0.0);
-    } else if (c.one_hot >= 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = i + j == c.one_hot ? 0.0 : w[j];
+// the row's sums from its chunks', in their order: by a whole wavefront
+__device__ __forceinline__ void exact_sums(const VerifyParams &p, int s, double &zp, double &zq) {
+    zp = zq = 0.0;
+    for (int c = lane_id(); c < p.splits; c += 64) {
+        zp += p.z[((int64_t)s * p.splits + c) * 2];
+        zq += p.z[((int64_t)s * p.splits + c) * 2 + 1];
     }
+    zp = wave_sum(zp);
+    zq = wave_sum(zq);
+}
+
+// The weights of eight consecutive tokens that one is drawn from, relative to exp((top - row's top) / T): max(p - q, 0) with
+// top = 0 by agreement (`rest`, with draft logits), else the exponentials, the refused draft's taken out; by a whole wavefront.
+// (`r` and `q`: loaded, q only with draft logits)
+template <typename T>
+__device__ __forceinline__ float weights8(const Choice &c, Raw8<T> &r, Raw8<T> &q, bool rest, double ip, double iq, double *w) {
+    r.clip();
+    if (rest && c.draft >= 0) {
+        q.clip();
+        const Weigh wp(c.top_p, c.k), wq(c.top_q, c.k);
+        double v[8];
+        wp(r, w);
+        wq(q, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double d = w[j] * ip - v[j] * iq;
+            w[j] = d > 0.0 ? d : 0.0;
+        }
+        return 0.0f;
+    }
+    const float top = wave_max(largest8(r));
+    if (c.k > 0.0) {
+        const Weigh wp(top, c.k);
+        wp(r, w);
+    } else {                                                            // greedy, in a call without statistics
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = top > -INFINITY && r.get(j) == top && j >= r.skip ? 1.0 : 0.0;
+    }
+    if (rest && c.one_hot >= 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = r.base + j == c.one_hot ? 0.0 : w[j];
+    }
+    return top;
+}
+template <typename T>
+__device__ __forceinline__ void load_pair(const VerifyParams &p, const Choice &c, int i, Raw8<T> &r, Raw8<T> &q) {
+    r.load((const T *)p.logits + (int64_t)c.row * p.ld_t, i, p.V);
+    if (c.draft >= 0) q.load((const T *)p.draft_logits + (int64_t)c.draft * p.ld_d, i, p.V);
 }
 
 // ---- sums of the weights that the next token is drawn from -------------------------------------------
-template <typename T>
+template <typename T, bool CHOSEN>
 __global__ __launch_bounds__(VER_THREADS) void verify_sums_kernel(VerifyParams p) {
     const int s = blockIdx.y;
-    const Choice c = p.choice[s];
+    Choice c;
+    if (CHOSEN) c = p.choice[s];
+    else c = choose<T>(p, s, blockIdx.x == 0);
     if (c.row < 0 || c.greedy >= 0) return;
-    const int wave = threadIdx.x >> 6;
-    for (int i = 0; i < 4; ++i) {
-        const int sub = blockIdx.x * (VER_CHUNK / VER_SUB) + i * 4 + wave;
-        if (sub >= p.subs) return;
-        double w[8], v[8];
-        weights8<T>(p, c, sub * VER_SUB + lane_id() * 8, true, w);
-        weights8<T>(p, c, sub * VER_SUB + lane_id() * 8, false, v);
-        double a = 0.0, b = 0.0;
+    Raw8<T> r[4], q[4];
+    const int sub0 = blockIdx.x * (VER_CHUNK / VER_SUB) + (int)(threadIdx.x >> 6);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            a += w[j];
-            b += v[j];
-        }
-        a = wave_sum(a);
-        b = wave_sum(b);
-        if (lane_id() == 0) {
-            p.sums[(int64_t)s * 2 * p.subs + sub] = a;
-            p.sums[((int64_t)s * 2 + 1) * p.subs + sub] = b;
-        }
+    for (int i = 0; i < 4; ++i) load_pair(p, c, (sub0 + i * 4) * VER_SUB + lane_id() * 8, r[i], q[i]);
+    double ip = 0.0, iq = 0.0;
+    if (c.draft >= 0) {
+        exact_sums(p, s, ip, iq);
+        ip = 1.0 / ip;
+        iq = 1.0 / iq;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int sub = sub0 + i * 4;
+        if (sub >= p.subs) return;
+        double w[8];
+        const float top = weights8<T>(c, r[i], q[i], true, ip, iq, w);
+        const double a = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        if (lane_id() == 0) p.blocks[(int64_t)s * p.subs + sub] = Block{a, top, 0};
     }
 }
 
@@ -337,64 +595,101 @@ __device__ __forceinline__ double wave_scan(double v) {       // inclusive
 }
 
 // ---- the draw: one wavefront per sequence --------------------------------------------------------------
+// A lane has `per` neighbouring blocks; one scan over the lanes finds whose, that lane its block, the wavefront the token in it.
 template <typename T>
 __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
-    const int s = blockIdx.x;
+    const int s = blockIdx.x, per = (p.subs + 63) / 64, b0 = min((int)lane_id() * per, p.subs), b1 = min(b0 + per, p.subs);
+    Block *blocks = p.blocks + (int64_t)s * p.subs;
     const Choice c = p.choice[s];
+    const float u = p.sample_u[s];
     if (c.row < 0 || c.greedy >= 0) return;
-    bool rest = c.draft >= 0 || c.one_hot >= 0;
-    const double *sums = p.sums + (int64_t)s * 2 * p.subs;
-    double total = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
-        if (pass == 1 || !rest) {                              // nothing of p exceeds q: p itself
-            rest = false;
-            sums = p.sums + ((int64_t)s * 2 + 1) * p.subs;
+    double ip = 0.0, iq = 0.0;
+    if (c.draft >= 0) {
+        exact_sums(p, s, ip, iq);
+        ip = 1.0 / ip;
+        iq = 1.0 / iq;
+    }
+    bool rest = true;
+    double lane_sum, total;
+    float top;
+    auto block_weight = [&](int b) {                          // of block b, relative to the largest block's top
+        const Block v = blocks[b];
+        return c.k > 0.0 ? v.sum * weight_of(v.top, top, c.k) : v.top == top ? v.sum : 0.0;
+    };
+    for (;;) {
+        top = -INFINITY;
+        if (rest && c.draft >= 0) {
+            top = 0.0f;                                       // (by agreement: these sums are absolute)
+        } else {
+            for (int b = b0; b < b1; ++b) top = fmaxf(top, blocks[b].sum > 0.0 ? blocks[b].top : -INFINITY);
+            top = wave_max(top);
         }
-        total = 0.0;
-        for (int b = 0; b < p.subs; b += 64) total += __shfl(wave_scan(b + lane_id() < p.subs ? sums[b + lane_id()] : 0.0), 63, ODSD_WAVE);
+        lane_sum = 0.0;
+        for (int b = b0; b < b1; ++b) lane_sum += block_weight(b);
+        total = wave_sum(lane_sum);
         if (total > 0.0 || !rest) break;
+        // nothing of p exceeds q: p itself.  (Two equal distributions keep every draft, so this is rare: the sums are made here.)
+        rest = false;
+        for (int b = 0; b < p.subs; ++b) {
+            double w[8];
+            Raw8<T> r1, q1;
+            load_pair(p, c, b * VER_SUB + lane_id() * 8, r1, q1);
+            const float t = weights8<T>(c, r1, q1, false, ip, iq, w);
+            const double a = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+            if (lane_id() == 0) blocks[b] = Block{a, t, 0};
+        }
+        __threadfence();
     }
-    const double aim = (double)p.sample_u[s] * total;
-    // the first block of VER_SUB tokens whose inclusive sum exceeds the aim (else the last one that has any weight)
-    double before = 0.0, at_before = 0.0;
+    int64_t *out = p.tokens + (int64_t)s * p.max_q + c.count;
+    if (!(total > 0.0)) {
+        if (lane_id() == 0) *out = -1;
+        return;
+    }
+    const double aim = c.k > 0.0 ? (double)u * total : 0.0;    // (greedy: the first of the largest)
+    // the first lane whose inclusive sum exceeds the aim (else the last that has any weight), and of its blocks likewise
+    const double run = wave_scan(lane_sum);
+    const uint64_t past = __ballot(run > aim && lane_sum > 0.0), any = __ballot(lane_sum > 0.0);
+    const int owner = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
     int sub = -1;
-    for (int b = 0; b < p.subs && sub < 0; b += 64) {
-        const double own = b + lane_id() < p.subs ? sums[b + lane_id()] : 0.0;
-        const double run = wave_scan(own);
-        const uint64_t past = __ballot(before + run > aim && own > 0.0);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            sub = b + l;
-            at_before = before + __shfl(run - own, l, ODSD_WAVE);
+    double before = run - lane_sum;
+    if ((int)lane_id() == owner) {
+        int last = -1;
+        double last_before = 0.0, sum = before;
+        for (int b = b0; b < b1 && sub < 0; ++b) {
+            const double w = block_weight(b);
+            if (w > 0.0) {
+                last = b;
+                last_before = sum;
+                if (past && sum + w > aim) sub = b;
+            }
+            sum += w;
         }
-        before += __shfl(run, 63, ODSD_WAVE);
+        // (rounding between the scan and this sum, or no block past the aim: the last token with a weight is taken)
+        before = sub >= 0 ? last_before : -INFINITY;
+        if (sub < 0) sub = last;
     }
-    if (sub < 0) {
-        for (int b = (p.subs - 1) / 64 * 64; b >= 0 && sub < 0; b -= 64) {
-            const uint64_t any = __ballot(b + lane_id() < p.subs && sums[b + lane_id()] > 0.0);
-            if (any) sub = b + 63 - __builtin_clzll(any);
-        }
-        at_before = -INFINITY;                                 // no sum exceeds the aim: the last token with a weight is taken
-        if (sub < 0) {
-            if (lane_id() == 0) p.tokens[(int64_t)s * p.max_q + c.count] = -1;
-            return;
-        }
-    }
+    sub = __shfl(sub, owner, ODSD_WAVE);
+    before = __shfl(before, owner, ODSD_WAVE);
     double w[8], own = 0.0;
-    const int i0 = sub * VER_SUB + lane_id() * 8;
-    weights8<T>(p, c, i0, rest, w);
+    Raw8<T> r1, q1;
+    load_pair(p, c, sub * VER_SUB + lane_id() * 8, r1, q1);
+    const float block_top = weights8<T>(c, r1, q1, rest, ip, iq, w);
+    const double scale = c.k > 0.0 ? weight_of(block_top, top, c.k) : 1.0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) own += w[j];
-    const double run = at_before + (wave_scan(own) - own);
+    for (int j = 0; j < 8; ++j) {
+        w[j] *= scale;
+        own += w[j];
+    }
     // the first token of this lane whose cumulative weight exceeds the aim, and the last that has any weight
+    const double up_to = before + (wave_scan(own) - own);
     int hit = 0x7fffffff, last = -1;
     double cum = 0.0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         cum += w[j];
         if (w[j] > 0.0) {
-            if (hit == 0x7fffffff && run + cum > aim) hit = i0 + j;
-            last = i0 + j;
+            if (hit == 0x7fffffff && up_to + cum > aim) hit = r1.base + j;
+            last = r1.base + j;
         }
     }
 #pragma unroll
@@ -402,12 +697,12 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
         hit = min(hit, __shfl_xor(hit, o, ODSD_WAVE));
         last = max(last, __shfl_xor(last, o, ODSD_WAVE));
     }
-    if (lane_id() == 0) p.tokens[(int64_t)s * p.max_q + c.count] = hit != 0x7fffffff ? hit : last;
+    if (lane_id() == 0) *out = hit != 0x7fffffff ? hit : last;
 }
 
 // ---- entry points ------------------------------------------------------------------------------------
 struct VerifyLayout {
-    size_t stats, sums, choice, total;
+    size_t stats, z, blocks, choice, padded, total;
     int splits, subs;
 };
 static bool verify_layout(int64_t S, int64_t n_q, int64_t n_d, int64_t V, bool draft_logits, VerifyLayout &l) {
@@ -415,9 +710,11 @@ static bool verify_layout(int64_t S, int64_t n_q, int64_t n_d, int64_t V, bool d
     l.subs = (int)((V + VER_SUB - 1) / VER_SUB);
     size_t o = 0;
     auto take = [&](size_t bytes) { const size_t at = o; o += odsd_round_up(bytes, 256); return at; };
-    l.stats = take((size_t)(n_q + (draft_logits ? n_d : 0)) * l.splits * sizeof(Stat));
-    l.sums = take((size_t)S * 2 * l.subs * 8);
+    l.stats = take(n_d ? (size_t)(n_q + (draft_logits ? n_d : 0)) * l.splits * sizeof(Stat) : 0);
+    l.z = take(draft_logits ? (size_t)S * l.splits * 16 : 0);
+    l.blocks = take((size_t)S * l.subs * sizeof(Block));
     l.choice = take((size_t)S * sizeof(Choice));
+    l.padded = take(V < 8 ? (size_t)(n_q + n_d) * 8 * 4 : 0);
     l.total = o;
     return (n_q + n_d) * l.splits <= 0x7fffffffLL && S <= 65535;
 }
@@ -433,11 +730,28 @@ extern "C" size_t odsd_verify_workspace_bytes(int32_t n_seqs, int32_t max_q_len,
     return l.total > 256 ? l.total : 256;
 }
 
-template <typename T> static int launch_verify(const VerifyParams &p, hipStream_t st) {
-    const int rows = p.n_q + (p.draft_logits ? p.n_d : 0);
-    if (rows > 0) verify_stats_kernel<T><<<(unsigned)(rows * p.splits), VER_THREADS, 0, st>>>(p);
-    verify_accept_kernel<T><<<(unsigned)p.S, VER_THREADS, 0, st>>>(p);
-    verify_sums_kernel<T><<<dim3((unsigned)p.splits, (unsigned)p.S), VER_THREADS, 0, st>>>(p);
+template <typename T> static int launch_verify(VerifyParams &p, void *padded, hipStream_t st) {
+    if (p.V < 8) {
+        T *rows = (T *)padded, *draft_rows = rows + (int64_t)p.n_q * 8;
+        auto pad = [&](const void *src, int64_t ld, T *dst, int n) {
+            if (n > 0) verify_pad_kernel<T><<<(unsigned)(((int64_t)n * 8 + VER_THREADS - 1) / VER_THREADS), VER_THREADS, 0, st>>>((const T *)src, ld, dst, n, p.V);
+        };
+        pad(p.logits, p.ld_t, rows, p.n_q);
+        if (p.draft_logits) {
+            pad(p.draft_logits, p.ld_d, draft_rows, p.n_d);
+            p.draft_logits = draft_rows;
+        }
+        p.logits = rows;
+        p.ld_t = p.ld_d = p.V = 8;
+    }
+    const dim3 chunks((unsigned)p.splits, (unsigned)p.S);
+    if (p.n_d > 0 && p.n_q > 0) verify_stats_kernel<T><<<(unsigned)((p.n_q + (p.draft_logits ? p.n_d : 0)) * p.splits), VER_THREADS, 0, st>>>(p);
+    if (p.draft_logits) {
+        verify_choose_kernel<T><<<chunks, VER_THREADS, 0, st>>>(p);
+        verify_sums_kernel<T, true><<<chunks, VER_THREADS, 0, st>>>(p);
+    } else {
+        verify_sums_kernel<T, false><<<chunks, VER_THREADS, 0, st>>>(p);
+    }
     verify_draw_kernel<T><<<(unsigned)p.S, 64, 0, st>>>(p);
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
@@ -467,10 +781,10 @@ extern "C" int odsd_verify_drafts(const void *logits, int64_t logits_stride, con
     char *ws = (char *)workspace;
     VerifyParams p{logits, draft_logits, logits_stride, draft_stride, draft_tokens, query_lens, temperature,
                    temperature_all, accept_u, sample_u, n_seqs, max_q_len, n_rows, n_drafts, vocab, l.splits, l.subs,
-                   tokens, num_accepted, accept_probs, (Stat *)(ws + l.stats), (double *)(ws + l.sums),
-                   (Choice *)(ws + l.choice)};
+                   tokens, num_accepted, accept_probs, (Stat *)(ws + l.stats), (double *)(ws + l.z),
+                   (Block *)(ws + l.blocks), (Choice *)(ws + l.choice)};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == ODSD_DT_F32) return launch_verify<float>(p, st);
-    if (dtype == ODSD_DT_BF16) return launch_verify<__bf16>(p, st);
-    return launch_verify<half_t>(p, st);
+    if (dtype == ODSD_DT_F32) return launch_verify<float>(p, ws + l.padded, st);
+    if (dtype == ODSD_DT_BF16) return launch_verify<__bf16>(p, ws + l.padded, st);
+    return launch_verify<half_t>(p, ws + l.padded, st);
 }

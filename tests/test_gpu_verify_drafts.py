@@ -1,5 +1,7 @@
-"""verify_drafts against the 64-bit definition: kept drafts and drawn tokens exactly, probabilities to one fp32 rounding (half
-a step, 2^-24, and 1e-11 for exp and the order of the sums)."""
+"""verify_drafts against the 64-bit definition: kept drafts and drawn tokens exactly, probabilities to what their sums' fp32
+statistics allow: each of the two sums of a probability's ratio is off by at most 2^-23 (the hardware's exp2, 1 ulp) + 6 2^-24
+(roundings of a sum of 32: 3 along 4 logits, 3 up the tree) + 17 ln 2 2^-24 (a difference of logits rounded to fp32, 17 bits
+below the largest, where 131 072 tokens still weigh as much as it), 1.2e-6; the ratio of two 2.4e-6, rounded to fp32 (2^-24)."""
 import numpy as np
 import pytest
 import torch
@@ -9,6 +11,7 @@ from oracle import dense_oracle as orc
 
 pytestmark = pytest.mark.gpu
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+PROB_TOL = 2 * (2.0 ** -23 + 6 * 2.0 ** -24 + 17 * 0.6932 * 2.0 ** -24) + 2.0 ** -24
 
 
 def make(lens, V, dtype="bf16", seed=0, with_q=True, near=0.7, T=0.8):
@@ -40,7 +43,7 @@ def check(dev, m, temperature=0.8, width=None, logits=None, draft_logits=None):
     # (a temperature is an fp32 number, as the kernel gets it)
     tokens, accepted, probs = orc.verify(m["logits"].double().numpy(), m["drafts"].numpy(), lens, m["accept_u"].numpy(), m["sample_u"].numpy(),
                                          None if q is None else q.double().numpy(), np.float32(temperature), width)
-    assert np.allclose(r.accept_probs.cpu().double().numpy(), probs, rtol=2.0 ** -24 + 1e-11, atol=1e-40)
+    assert np.allclose(r.accept_probs.cpu().double().numpy(), probs, rtol=PROB_TOL, atol=1e-40)
     assert r.num_accepted.cpu().tolist() == accepted.tolist()
     assert r.tokens.cpu().tolist() == tokens.tolist()
     return r
@@ -158,6 +161,46 @@ def test_sampling_of_a_decode_step(dev):
     share = np.bincount(r.tokens[:, 0].cpu().numpy(), minlength=50) / n
     assert np.abs(share - p).max() <= 1.0 / n + 1e-9 and r.accept_probs.numel() == 0 and not r.num_accepted.any()
     assert odsd.verify_drafts(row[:0].to(dev), None, {}, None, u[:0].to(dev)).tokens.shape == (0, 1)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_sampling_with_temperatures_masks_and_empty_rows(dev, dtype):
+    g = torch.Generator().manual_seed(3)
+    n, V = 37, 5001
+    x = (torch.randn(n, V, generator=g) * 3).to(DT[dtype])
+    x[:, 2::3] = -float("inf")
+    x[4] = -float("inf")
+    x[5] = float("nan")
+    x[6, 100] = x[6, 4000] = float("inf")
+    x[7, 50] = x[7, 4500] = 40.0
+    x[8, :] = torch.finfo(DT[dtype]).min
+    x[9, 10] = float("nan")
+    t = torch.rand(n, generator=g) * 2
+    t[::4] = 0.0
+    t[7], t[30], t[31], t[33] = 0.0, 1e-35, 1e35, 3e38
+    u = torch.rand(n, generator=g)
+    u[10], u[11] = 0.0, 1.0 - 2.0 ** -24
+    r = odsd.verify_drafts(x.to(dev), None, {}, None, u.to(dev), temperature=t.to(dev))
+    want, _, _ = orc.verify(x.double().numpy(), None, [1] * n, None, u.numpy(), None, t.double().numpy())
+    assert r.tokens.cpu().tolist() == want.tolist() and not r.num_accepted.any()
+
+
+def test_extreme_temperatures_with_drafts(dev):
+    lens = [3, 2, 4, 2, 3]
+    m = make(lens, 2000, "fp32", seed=21)
+    m["logits"][0, 5] = m["draft_logits"][1, 7] = -float("inf")
+    check(dev, m, [1e-35, 1e35, 3e38, 1e-44, 50.0])
+
+
+def test_all_tokens_alike(dev):
+    """Rows whose logits are all equal, or equal but one: every rounding of the statistics falls the same way."""
+    for V in (131072, 100003):
+        m = make([3, 2], V, "fp32", seed=22)
+        m["logits"][:] = 1.37
+        m["draft_logits"][:] = -0.61
+        m["logits"][1, 17] = 12.9
+        m["draft_logits"][1, 5] = 13.3
+        check(dev, m, 0.77)
 
 
 def test_many_sequences(dev):
