@@ -335,7 +335,8 @@ size_t odsd_varlen_attention_workspace_bytes(int32_t n_seqs, int32_t max_seqlen_
  * Any M >= 0 (0: nothing is done), N >= 1, K >= 1, up to M = 4 million; pointers aligned to their elements (with K, ldx and
  * ldw multiples of 8 and x and w 16-byte aligned the fast kernels run).  Sums and epilogue in fp32, one rounding at the end.
  * out may be the residual itself (the same rows); it overlaps no other operand.  The same inputs give the same bits.
- * workspace: odsd_linear_workspace_bytes(M, N, K) bytes (0: a size is out of range), 16-byte aligned.
+ * workspace: odsd_linear_workspace_bytes(M, N, K) bytes (0: a size is out of range; 256: none is used, NULL will do),
+ * 16-byte aligned.
  * Stands in for the F.linear calls around the block (demo/src/layers/attention.py:169-288). */
 int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *residual,
                 int64_t ldr, void *out, int64_t ldo, int32_t M, int32_t N, int32_t K, int32_t dtype,

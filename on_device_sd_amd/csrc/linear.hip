@@ -602,16 +602,17 @@ extern "C" int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ld
     // the grid's second dimension and the 32-bit products inside the kernels
     if (M > 64 * 65535 || N > 0x7fffffff - 256 || K > 0x7fffffff - 256) return ODSD_ERR_UNSUPPORTED;
     if (M == 0) return ODSD_OK;
-    if (odsd_linear_workspace_bytes(M, N, K) == 0) return ODSD_ERR_UNSUPPORTED;
-    if (!x || !w || !out || !workspace) return ODSD_ERR_NULL;
+    if (!x || !w || !out) return ODSD_ERR_NULL;
     const uintptr_t oe = out_dtype == ODSD_DT_F32 ? 4 : 2;
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias) & 1) || (((uintptr_t)out | (uintptr_t)residual) & (oe - 1)) ||
         !odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
-    if (workspace_bytes < odsd_linear_workspace_bytes(M, N, K)) return ODSD_ERR_WORKSPACE;
     LinearParams p{x, w, bias, residual, out, ldx, ldw, ldr, ldo, M, N, K, act, 0, 0, 1, 0, nullptr, 0};
     // rows of whole 16-byte segments, and a tile's rows within 31 bits of bytes
     const bool aligned = ((K | ldx | ldw) & 7) == 0 && odsd_aligned16(x) && odsd_aligned16(w) && ldx < (1 << 21) && ldw < (1 << 21);
     const LinearPlan l = linear_plan(M, N, K, aligned);
+    if (!l.fits) return ODSD_ERR_UNSUPPORTED;
+    if (l.bytes && !workspace) return ODSD_ERR_NULL;
+    if (workspace_bytes < l.bytes) return ODSD_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == ODSD_DT_BF16)
         return out_dtype == ODSD_DT_F32 ? launch_linear<__bf16, float>(p, l, workspace, st) : launch_linear<__bf16, __bf16>(p, l, workspace, st);

@@ -25,7 +25,7 @@ struct RotaryParams {
     int64_t num_slots;
     int n, n_store;                 // tokens; rows that are stored
     int Hq, Hk, D, R;
-    int tokens_per_wg, q_wgs;
+    int q_tokens, kv_tokens, q_wgs; // tokens of a workgroup, workgroups that have queries
 };
 
 // sin and cos of t turns, |t| <= 1/2: reduced to an eighth of a turn and the quarter it lies in, Taylor polynomials there
@@ -42,139 +42,235 @@ __device__ __forceinline__ void sincos_turns(float t, float &s, float &c) {
     c = (iq + 1) & 2 ? -b : b;
 }
 
-// V: values per access (8: 16-bit elements, everything 16-byte aligned, R and D - R multiples of 16; else 1).
-// A unit is 2 V columns of a head: V frequencies with both members of their pairs, or 2 V columns that pass.  The units of a
-// head lie on LG neighbouring lanes (a power of two), which add up its squares.
-template <typename T, int V, bool SIDE, typename POS>
-__global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryParams p, int LG) {
-    typedef T TV __attribute__((ext_vector_type(V)));
-    extern __shared__ float2 trig[];                      // [tokens_per_wg][R / 2]: (cos, sin)
+// What a workgroup has: the heads of `rows` tokens of q, or of rows that go to k_out and the cache with the values beside them.
+struct RotaryPart {
+    bool is_q;
+    int row0, rows, H;
+    const void *src, *weight;
+    int64_t token_ld, head_ld;
+};
+__device__ __forceinline__ RotaryPart rotary_part(const RotaryParams &p) {
+    RotaryPart w;
+    w.is_q = (int)blockIdx.x < p.q_wgs;
+    const int per = w.is_q ? p.q_tokens : p.kv_tokens;
+    w.row0 = (w.is_q ? blockIdx.x : blockIdx.x - p.q_wgs) * per;
+    w.rows = min(per, (w.is_q ? p.n : p.n_store) - w.row0);
+    w.H = w.is_q ? p.Hq : p.Hk;
+    w.src = w.is_q ? p.q : p.k;
+    w.weight = w.is_q ? p.q_weight : p.k_weight;
+    w.token_ld = w.is_q ? p.q_token : p.k_token;
+    w.head_ld = w.is_q ? p.q_head : p.k_head;
+    return w;
+}
+__device__ __forceinline__ int rotary_token(const RotaryParams &p, const RotaryPart &w, int r) {
+    const int t = w.is_q || !p.src ? w.row0 + r : p.src[w.row0 + r];
+    return t >= 0 && t < p.n ? t : -1;
+}
+__device__ __forceinline__ int64_t rotary_slot(const RotaryParams &p, const RotaryPart &w, int r) {
+    const int64_t slot = p.slots[w.row0 + r];
+    return slot >= 0 && slot < p.num_slots ? slot : -1;
+}
+// (cos, sin) of every frequency of the workgroup's tokens
+template <typename POS>
+__device__ __forceinline__ void rotary_angles(const RotaryParams &p, const RotaryPart &w, float2 *trig) {
     const int half = p.R / 2;
-    const bool is_q = (int)blockIdx.x < p.q_wgs;
-    const int row0 = (is_q ? blockIdx.x : blockIdx.x - p.q_wgs) * p.tokens_per_wg;
-    const int rows = min(p.tokens_per_wg, (is_q ? p.n : p.n_store) - row0);
-    auto token_of = [&](int r) { return is_q || !p.src ? row0 + r : p.src[row0 + r]; };
-    for (int i = threadIdx.x; i < rows * half; i += ROT_THREADS) {
+    for (int i = threadIdx.x; i < w.rows * half; i += ROT_THREADS) {
         const int r = i / half, f = i - r * half;
-        const int t = token_of(r);
+        const int t = rotary_token(p, w, r);
         float s = 0.0f, c = 1.0f;
-        if (t >= 0 && t < p.n) {
+        if (t >= 0) {
             const int axis = (f >= p.sec_end[0]) + (f >= p.sec_end[1]) + (f >= p.sec_end[2]);
             const double turns = (double)((const POS *)p.positions)[axis * p.pos_ld + t] * (p.inv_freq[f] * 0.15915494309189533577);
             sincos_turns((float)(turns - rint(turns)), s, c);
         }
         trig[i] = make_float2(c, s);
     }
-    __syncthreads();
+}
+// Where a head of a token goes: its place in q_out or k_out, and in the cache, if its row has one.
+template <typename T>
+__device__ __forceinline__ void rotary_targets(const RotaryParams &p, const RotaryPart &w, int r, int t, int h, T *&dst, T *&dst2) {
+    dst = w.is_q ? (T *)p.q_out + ((int64_t)t * p.Hq + h) * p.D : p.k_out ? (T *)p.k_out + ((int64_t)t * p.Hk + h) * p.D : nullptr;
+    dst2 = nullptr;
+    if (!w.is_q && p.k_cache) {
+        const int64_t slot = rotary_slot(p, w, r);
+        if (slot >= 0) dst2 = (T *)p.k_cache + (slot * p.Hk + h) * p.D;
+    }
+}
+// The first columns of the two halves of unit u: V frequencies with both members of their pairs, or 2 V columns that pass.
+template <int V, bool SIDE>
+__device__ __forceinline__ void rotary_columns(const RotaryParams &p, int u, int &c0, int &c1) {
+    const int half = p.R / 2;
+    if (u < half / V) {
+        c0 = SIDE ? 2 * V * u : V * u;
+        c1 = SIDE ? c0 + V : c0 + half;
+    } else {
+        c0 = p.R + (u - half / V) * 2 * V;
+        c1 = c0 + V;
+    }
+}
+template <int V, bool SIDE>
+__device__ __forceinline__ void rotary_turn(float *x, const float2 *cs) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int lo = SIDE ? 2 * i : i, hi = SIDE ? 2 * i + 1 : V + i;
+        const float c = cs[i].x, s = cs[i].y, x1 = x[lo], x2 = x[hi];
+        x[lo] = x1 * c - x2 * s;
+        x[hi] = x2 * c + x1 * s;
+    }
+}
 
-    const int units = half / V + (p.D - p.R) / (2 * V);
-    const int H = is_q ? p.Hq : p.Hk;
-    const int per_pass = ROT_THREADS / LG;
-    const int sub = threadIdx.x % LG;
-    const T *src = (const T *)(is_q ? p.q : p.k), *weight = (const T *)(is_q ? p.q_weight : p.k_weight);
-    const int64_t token_ld = is_q ? p.q_token : p.k_token, head_ld = is_q ? p.q_head : p.k_head;
-    for (int hr = threadIdx.x / LG; hr < rows * H; hr += per_pass) {
-        const int r = hr / H, h = hr - r * H;
-        const int t = token_of(r);
-        if (t < 0 || t >= p.n) continue;                  // (all LG lanes of the head agree)
-        T *dst = is_q ? (T *)p.q_out + ((int64_t)t * p.Hq + h) * p.D
-                      : p.k_out ? (T *)p.k_out + ((int64_t)t * p.Hk + h) * p.D : nullptr;
-        T *dst2 = nullptr;                                // the head's place in the cache, if its row has one
-        if (!is_q && p.k_cache) {
-            const int64_t slot = p.slots[row0 + r];
-            if (slot >= 0 && slot < p.num_slots) dst2 = (T *)p.k_cache + (slot * p.Hk + h) * p.D;
+// Everything in pieces of eight 16-bit values, 16-byte aligned.  A head's units (two pieces each) lie on LG neighbouring lanes,
+// which add up its squares; a thread's first unit is requested before the angles are made, so that its way from memory and
+// the sines hide each other.  Bytes bound it: 16384 tokens of 32 + 4 heads of 128 on three axes in 54 to 59 us, 5.1 to
+// 5.6 TB/s; two units a thread 60, four 69 (fewer workgroups at once); one token a workgroup for the keys, too, 73 to 84.
+template <typename T, bool SIDE, typename POS>
+__global__ __launch_bounds__(ROT_THREADS) void rotary_wide_kernel(RotaryParams p, int LG) {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    extern __shared__ float2 trig[];                      // [rows][R / 2]: (cos, sin)
+    const RotaryPart w = rotary_part(p);
+    const int half = p.R / 2, units = p.D / 16, per_pass = ROT_THREADS / LG, total = w.rows * w.H;
+    const int sub = threadIdx.x % LG, first = threadIdx.x / LG;
+    int c0, c1;
+    rotary_columns<8, SIDE>(p, min(sub, units - 1), c0, c1);
+    T8 a, b, wa, wb;
+    int token;
+    auto fetch = [&](int hr) {
+        const int r = min(hr, total - 1) / w.H, h = min(hr, total - 1) - r * w.H;
+        token = rotary_token(p, w, r);
+        const T *row = (const T *)w.src + max(token, 0) * w.token_ld + h * w.head_ld;
+        a = *(const T8 *)(row + c0);
+        b = *(const T8 *)(row + c1);
+    };
+    fetch(first);
+    if (w.weight) {
+        wa = *(const T8 *)((const T *)w.weight + c0);
+        wb = *(const T8 *)((const T *)w.weight + c1);
+    }
+    if (!w.is_q && p.v_cache) {
+        const int chunks = p.Hk * (p.D / 8);
+        for (int i = threadIdx.x; i < w.rows * chunks; i += ROT_THREADS) {
+            const int r = i / chunks, c = i - r * chunks, h = c / (p.D / 8), at = (c - h * (p.D / 8)) * 8;
+            const int t = rotary_token(p, w, r);
+            const int64_t slot = rotary_slot(p, w, r);
+            if (t >= 0 && slot >= 0)
+                *(T8 *)((T *)p.v_cache + (slot * p.Hk + h) * p.D + at) = *(const T8 *)((const T *)p.v + t * p.v_token + h * p.v_head + at);
         }
-        if (!dst && !dst2) continue;
-        const T *row = src + t * token_ld + h * head_ld;
-        float scale = 1.0f;
-        auto columns = [&](int u, int &c0, int &c1) {     // the first columns of a unit's two halves
-            if (u < half / V) {
-                c0 = SIDE ? 2 * V * u : V * u;
-                c1 = SIDE ? c0 + V : c0 + half;
-            } else {
-                c0 = p.R + (u - half / V) * 2 * V;
-                c1 = c0 + V;
+    }
+    rotary_angles<POS>(p, w, trig);
+    __syncthreads();
+    for (int hr = first; hr < total; hr += per_pass) {
+        if (hr != first) fetch(hr);
+        const int r = hr / w.H, h = hr - r * w.H;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = (float)a[e];
+            x[8 + e] = (float)b[e];
+        }
+        if (w.weight) {
+            float ss = 0.0f;
+            if (sub < units) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
             }
-        };
+            for (int o = LG / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, ODSD_WAVE);   // (all LG lanes of a head are here)
+            const float scale = rsqrtf(ss / (float)p.D + p.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] *= scale * (float)wa[e];
+                x[8 + e] *= scale * (float)wb[e];
+            }
+        }
+        if (sub >= units || token < 0) continue;
+        if (sub < half / 8) rotary_turn<8, SIDE>(x, trig + r * half + sub * 8);
+        T8 ya, yb;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ya[e] = (T)x[e];
+            yb[e] = (T)x[8 + e];
+        }
+        T *dst, *dst2;
+        rotary_targets(p, w, r, token, h, dst, dst2);
+        if (dst) {
+            *(T8 *)(dst + c0) = ya;
+            *(T8 *)(dst + c1) = yb;
+        }
+        if (dst2) {
+            *(T8 *)(dst2 + c0) = ya;
+            *(T8 *)(dst2 + c1) = yb;
+        }
+    }
+}
+
+// Any head size, strides and alignment: value by value, a unit is one pair; a head's units lie on LG lanes in turns.
+template <typename T, bool SIDE, typename POS>
+__global__ __launch_bounds__(ROT_THREADS) void rotary_any_kernel(RotaryParams p, int LG) {
+    extern __shared__ float2 trig[];
+    const RotaryPart w = rotary_part(p);
+    rotary_angles<POS>(p, w, trig);
+    __syncthreads();
+    const int half = p.R / 2, units = p.D / 2, sub = threadIdx.x % LG;
+    for (int hr = threadIdx.x / LG; hr < w.rows * w.H; hr += ROT_THREADS / LG) {
+        const int r = hr / w.H, h = hr - r * w.H;
+        const int t = rotary_token(p, w, r);
+        if (t < 0) continue;                              // (all LG lanes of the head agree)
+        T *dst, *dst2;
+        rotary_targets(p, w, r, t, h, dst, dst2);
+        const T *row = (const T *)w.src + t * w.token_ld + h * w.head_ld, *weight = (const T *)w.weight;
+        float scale = 1.0f;
+        int c0, c1;
         if (weight) {
             float ss = 0.0f;
             for (int u = sub; u < units; u += LG) {
-                int c0, c1;
-                columns(u, c0, c1);
-                const TV a = *(const TV *)(row + c0), b = *(const TV *)(row + c1);
-#pragma unroll
-                for (int i = 0; i < V; ++i) ss += (float)a[i] * (float)a[i] + (float)b[i] * (float)b[i];
+                rotary_columns<1, SIDE>(p, u, c0, c1);
+                ss += (float)row[c0] * (float)row[c0] + (float)row[c1] * (float)row[c1];
             }
             for (int o = LG / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, ODSD_WAVE);
             scale = rsqrtf(ss / (float)p.D + p.eps);
         }
         for (int u = sub; u < units; u += LG) {
-            int c0, c1;
-            columns(u, c0, c1);
-            const TV a = *(const TV *)(row + c0), b = *(const TV *)(row + c1);
-            float x[2 * V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[i] = (float)a[i];
-                x[V + i] = (float)b[i];
-            }
+            rotary_columns<1, SIDE>(p, u, c0, c1);
+            float x[2] = {(float)row[c0], (float)row[c1]};
             if (weight) {
-                const TV wa = *(const TV *)(weight + c0), wb = *(const TV *)(weight + c1);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[i] *= scale * (float)wa[i];
-                    x[V + i] *= scale * (float)wb[i];
-                }
+                x[0] *= scale * (float)weight[c0];
+                x[1] *= scale * (float)weight[c1];
             }
-            if (u < half / V) {
-                const float2 *cs = trig + r * half + u * V;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int lo = SIDE ? 2 * i : i, hi = SIDE ? 2 * i + 1 : V + i;
-                    const float c = cs[i].x, s = cs[i].y, x1 = x[lo], x2 = x[hi];
-                    x[lo] = x1 * c - x2 * s;
-                    x[hi] = x2 * c + x1 * s;
-                }
-            }
-            TV ya, yb;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                ya[i] = (T)x[i];
-                yb[i] = (T)x[V + i];
-            }
+            if (u < half) rotary_turn<1, SIDE>(x, trig + r * half + u);
             if (dst) {
-                *(TV *)(dst + c0) = ya;
-                *(TV *)(dst + c1) = yb;
+                dst[c0] = (T)x[0];
+                dst[c1] = (T)x[1];
             }
             if (dst2) {
-                *(TV *)(dst2 + c0) = ya;
-                *(TV *)(dst2 + c1) = yb;
+                dst2[c0] = (T)x[0];
+                dst2[c1] = (T)x[1];
             }
         }
     }
-    if (is_q || !p.v_cache) return;
-    const int chunks = p.D / V;
-    for (int i = threadIdx.x; i < rows * p.Hk * chunks; i += ROT_THREADS) {
-        const int r = i / (p.Hk * chunks), c = i - r * (p.Hk * chunks);
-        const int t = token_of(r);
-        const int64_t slot = p.slots[row0 + r];
-        if (t < 0 || t >= p.n || slot < 0 || slot >= p.num_slots) continue;
-        const int h = c / chunks, at = (c - h * chunks) * V;
-        *(TV *)((T *)p.v_cache + (slot * p.Hk + h) * p.D + at) = *(const TV *)((const T *)p.v + t * p.v_token + h * p.v_head + at);
+    if (w.is_q || !p.v_cache) return;
+    for (int i = threadIdx.x; i < w.rows * p.Hk * p.D; i += ROT_THREADS) {
+        const int r = i / (p.Hk * p.D), c = i - r * (p.Hk * p.D), h = c / p.D, at = c - h * p.D;
+        const int t = rotary_token(p, w, r);
+        const int64_t slot = rotary_slot(p, w, r);
+        if (t >= 0 && slot >= 0) ((T *)p.v_cache)[(slot * p.Hk + h) * p.D + at] = ((const T *)p.v)[t * p.v_token + h * p.v_head + at];
     }
 }
 
-template <typename T, int V, bool SIDE>
-static void launch_rotary(RotaryParams &p, int pos_bytes, hipStream_t st) {
-    const int units = p.R / 2 / V + (p.D - p.R) / (2 * V);
+template <typename T, bool SIDE, typename POS>
+static void launch_rotary(RotaryParams &p, bool wide, hipStream_t st) {
+    const int units = wide ? p.D / 16 : p.D / 2;
     int LG = 1;
     while (LG < units && LG < 64) LG *= 2;
-    p.tokens_per_wg = 1;
-    p.q_wgs = p.n;
-    const int kv_wgs = p.n_store;
-    const size_t lds = (size_t)p.tokens_per_wg * (p.R / 2) * sizeof(float2);
-    if (pos_bytes == 8) rotary_kernel<T, V, SIDE, int64_t><<<p.q_wgs + kv_wgs, ROT_THREADS, lds, st>>>(p, LG);
-    else rotary_kernel<T, V, SIDE, int32_t><<<p.q_wgs + kv_wgs, ROT_THREADS, lds, st>>>(p, LG);
+    // Tokens of a workgroup: one while there are few workgroups, else as many as give each thread a unit (at most 32: their
+    // angles, 4 KB a token for 1024 columns, stay within the LDS)
+    const bool many = wide && (int64_t)p.n + p.n_store >= 2048;
+    auto tokens = [&](int H) { return many ? max(1, min(ROT_THREADS / (LG * H), 32)) : 1; };
+    p.q_tokens = tokens(p.Hq);
+    p.kv_tokens = tokens(p.Hk);
+    p.q_wgs = (p.n + p.q_tokens - 1) / p.q_tokens;
+    const unsigned grid = (unsigned)(p.q_wgs + (p.n_store + p.kv_tokens - 1) / p.kv_tokens);
+    const size_t lds = (size_t)max(p.q_tokens, p.kv_tokens) * (p.R / 2) * sizeof(float2);
+    if (wide) rotary_wide_kernel<T, SIDE, POS><<<grid, ROT_THREADS, lds, st>>>(p, LG);
+    else rotary_any_kernel<T, SIDE, POS><<<grid, ROT_THREADS, lds, st>>>(p, LG);
 }
 
 extern "C" int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
@@ -229,18 +325,18 @@ extern "C" int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head
     if (((uintptr_t)positions & (position_bytes - 1)) || ((uintptr_t)inv_freq & 7)) return ODSD_ERR_ALIGN;
     const bool wide = (bytes & 15) == 0 && (elems & 7) == 0 && rotary_dim % 16 == 0 && head_dim % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-#define ROT_GO(T)                                                                        \
-    do {                                                                                 \
-        if (wide) {                                                                      \
-            if (interleaved) launch_rotary<T, 8, true>(p, position_bytes, st);           \
-            else launch_rotary<T, 8, false>(p, position_bytes, st);                      \
-        } else {                                                                         \
-            if (interleaved) launch_rotary<T, 1, true>(p, position_bytes, st);           \
-            else launch_rotary<T, 1, false>(p, position_bytes, st);                      \
-        }                                                                                \
+#define ROT_GO(T, POS)                                               \
+    do {                                                             \
+        if (interleaved) launch_rotary<T, true, POS>(p, wide, st);   \
+        else launch_rotary<T, false, POS>(p, wide, st);              \
     } while (0)
-    if (dtype == ODSD_DT_BF16) ROT_GO(__bf16);
-    else ROT_GO(half_t);
+    if (dtype == ODSD_DT_BF16) {
+        if (position_bytes == 8) ROT_GO(__bf16, int64_t);
+        else ROT_GO(__bf16, int32_t);
+    } else {
+        if (position_bytes == 8) ROT_GO(half_t, int64_t);
+        else ROT_GO(half_t, int32_t);
+    }
 #undef ROT_GO
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;

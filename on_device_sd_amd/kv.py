@@ -58,82 +58,99 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 
 
 _ROTARY_DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_POSITION_BYTES = {torch.int64: 8, torch.int32: 4}
+
+
+def _int32_row(t: torch.Tensor) -> torch.Tensor:
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
 
 
 def _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, want_k, k_cache, v_cache,
             slot_mapping, src_index):
+    # (a decode step's kernel takes 4 us, so the host's share is kept small: each attribute of a tensor is read once)
     dev = q.get_device()
     _same_device(dev, k, v, positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slot_mapping, src_index)
     if dev != _raw_device():
         with torch.cuda.device(dev):
             return _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, want_k, k_cache,
                            v_cache, slot_mapping, src_index)
-    code = _ROTARY_DTYPES.get(q.dtype)
+    dtype = q.dtype
+    code = _ROTARY_DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"rotary positions take bfloat16 or float16, got {q.dtype}")
-    n, heads, head_dim = q.shape
-    kv_heads = k.shape[1]
-    if k.shape != (n, kv_heads, head_dim) or k.dtype != q.dtype:
+        raise TypeError(f"rotary positions take bfloat16 or float16, got {dtype}")
+    shape, k_shape = q.shape, k.shape
+    n, heads, head_dim = shape
+    kv_heads = k_shape[1]
+    if k_shape != (n, kv_heads, head_dim) or k.dtype != dtype:
         raise ValueError("q [n, heads, head_dim] and k [n, kv_heads, head_dim] must have the same tokens, head size and dtype")
     rotary_dim = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float64:
         raise TypeError("inv_freq must be float64: an angle is a position times a frequency")
     if not 0 < rotary_dim <= head_dim:
-        raise ValueError(f"{inv_freq.numel()} frequencies do not fit a head of {head_dim}")
-    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
+        raise ValueError(f"{rotary_dim // 2} frequencies do not fit a head of {head_dim}")
+    pos_bytes = _POSITION_BYTES.get(positions.dtype)
+    if pos_bytes is None:
         raise TypeError("positions must be int32 or int64")
-    axes = 1 if positions.dim() == 1 else positions.shape[0]
-    if positions.shape[-1] != n or positions.dim() > 2:
+    pos_shape = positions.shape
+    axes = 1 if len(pos_shape) == 1 else pos_shape[0]
+    if pos_shape[-1] != n or len(pos_shape) > 2:
         raise ValueError(f"positions must be [{n}] or [axes, {n}]")
-    if sections is None:
-        if axes != 1:
-            raise ValueError("positions of several axes need sections")
-        counts = None
-    else:
+    counts = None
+    if sections is not None:
         if len(sections) != axes or sum(sections) != rotary_dim // 2 or min(sections) < 0 or axes > 4:
             raise ValueError(f"sections {tuple(sections)}: one count per axis (at most 4), together {rotary_dim // 2}")
         counts = (C.c_int32 * axes)(*sections)
-    for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (head_dim,) or w.dtype != q.dtype):
-            raise ValueError("norm weights must be [head_dim] in the dtype of q")
-    if q.stride(2) != 1:
+    elif axes != 1:
+        raise ValueError("positions of several axes need sections")
+    qw = kw = None
+    if q_weight is not None or k_weight is not None:
+        for w in (q_weight, k_weight):
+            if w is not None and (w.shape != (head_dim,) or w.dtype != dtype):
+                raise ValueError("norm weights must be [head_dim] in the dtype of q")
+        q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+        qw, kw = _ptr(q_weight), _ptr(k_weight)
+    q_strides, k_strides, pos_strides = q.stride(), k.stride(), positions.stride()
+    if q_strides[2] != 1:
         q = q.contiguous()
-    if k.stride(2) != 1:
+        q_strides = q.stride()
+    if k_strides[2] != 1:
         k = k.contiguous()
-    if positions.stride(-1) != 1:
+        k_strides = k.stride()
+    if pos_strides[-1] != 1:
         positions = positions.contiguous()
+        pos_strides = positions.stride()
     inv_freq = inv_freq.contiguous()
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    vp = kcp = vcp = slots = src = None
     vs0 = vs1 = n_store = num_slots = 0
     if k_cache is not None:
         D = kv_heads * head_dim
-        if v.shape != k.shape or not v.dtype == k_cache.dtype == v_cache.dtype == q.dtype:
+        cache_shape = k_cache.shape
+        if v.shape != k_shape or not v.dtype == k_cache.dtype == v_cache.dtype == dtype:
             raise ValueError("k and v must have the same shape, and the caches their dtype")
-        if k_cache.shape != v_cache.shape or k_cache.shape[-1] != D or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        if cache_shape != v_cache.shape or cache_shape[-1] != D or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
             raise ValueError(f"the caches must be contiguous rows of {D}")
-        if v.stride(2) != 1:
+        v_strides = v.stride()
+        if v_strides[2] != 1:
             v = v.contiguous()
-        vs0, vs1 = v.stride(0), v.stride(1)
-        if slot_mapping.dtype != torch.int32:
-            slot_mapping = slot_mapping.to(torch.int32)
-        slot_mapping = slot_mapping.contiguous()
+            v_strides = v.stride()
+        vs0, vs1 = v_strides[0], v_strides[1]
+        slot_mapping = _int32_row(slot_mapping)
         n_store, num_slots = slot_mapping.numel(), k_cache.numel() // D
         if src_index is not None:
-            if src_index.dtype != torch.int32:
-                src_index = src_index.to(torch.int32)
-            src_index = src_index.contiguous()
+            src_index = _int32_row(src_index)
+            src = src_index.data_ptr()
         if (n if src_index is None else src_index.numel()) != n_store:
             raise ValueError("slot_mapping must name a slot (or -1) for every row that is stored")
-    q_out = torch.empty(n, heads, head_dim, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(n, kv_heads, head_dim, dtype=q.dtype, device=q.device) if want_k else None
+        vp, kcp, vcp, slots = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr()
+    q_out = torch.empty(shape, dtype=dtype, device=q.device)
+    k_out = torch.empty(k_shape, dtype=dtype, device=q.device) if want_k else None
     if n == 0:
         return q_out, k_out
     rc = _lib.load().odsd_rotary(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), _ptr(v), vs0, vs1, n, heads, kv_heads,
-        head_dim, rotary_dim, 1 if interleaved else 0, code, positions.data_ptr(), positions.element_size(), axes,
-        positions.stride(0) if axes > 1 else n, counts, inv_freq.data_ptr(), _ptr(q_weight), _ptr(k_weight), eps,
-        q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), _ptr(src_index), n_store, num_slots,
-        _stream())
+        q.data_ptr(), q_strides[0], q_strides[1], k.data_ptr(), k_strides[0], k_strides[1], vp, vs0, vs1, n, heads, kv_heads,
+        head_dim, rotary_dim, 1 if interleaved else 0, code, positions.data_ptr(), pos_bytes, axes,
+        pos_strides[0] if axes > 1 else n, counts, inv_freq.data_ptr(), qw, kw, eps, q_out.data_ptr(), _ptr(k_out), kcp, vcp,
+        slots, src, n_store, num_slots, _stream())
     if rc:
         _lib.check(rc, "odsd_rotary")
     if k_cache is not None:

@@ -192,12 +192,17 @@ def _same_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError("runs on the GPU only, all tensors on the same one (there is no CPU fallback)")
 
 
-def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int]:
+_NO_WORKSPACE = 256                    # what odsd_linear_workspace_bytes answers where nothing is split
+
+
+def _rows(t: torch.Tensor, rows: int, cols: int) -> Tuple[torch.Tensor, int]:
     """A matrix whose rows are dense, copied only if they are not, and the elements between two rows (the stride of a
     single row says nothing)."""
-    if t.stride(1) != 1 or t.stride(0) < cols:         # (a broadcast or overlapping view is not a matrix of rows)
+    ld, step = t.stride()
+    if step != 1 or ld < cols:                         # (a broadcast or overlapping view is not a matrix of rows)
         t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else cols
+        ld = cols
+    return t, ld if rows > 1 else cols
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -219,42 +224,49 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         raise TypeError(f"linear takes bfloat16 or float16, got {dtype}")
     if weight.dtype != dtype or (bias is not None and bias.dtype != dtype):
         raise TypeError("x, weight and bias must have the same dtype")
+    out_code = code
     if out_dtype is None:
         out_dtype = dtype
-    elif out_dtype != dtype and out_dtype != torch.float32:
-        raise TypeError(f"out_dtype is x's or float32, got {out_dtype}")
-    act = _ACTIVATIONS.get(activation, -1)
-    if act < 0:
+    elif out_dtype != dtype:
+        if out_dtype != torch.float32:
+            raise TypeError(f"out_dtype is x's or float32, got {out_dtype}")
+        out_code = _lib.DT_F32
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation {activation!r} is none of {list(_ACTIVATIONS)}")
     shape = x.shape
     N, K = weight.shape
-    if x.dim() == 0 or shape[-1] != K:
+    if not shape or shape[-1] != K:
         raise ValueError(f"x {tuple(shape)} and weight {tuple(weight.shape)} do not belong together")
-    out = torch.empty(shape[:-1] + (N,), dtype=out_dtype, device=x.device)
-    if N == 0 or out.numel() == 0:
-        return out
-    if x.dim() != 2:
-        x = x.reshape(-1, K)
-    M = x.shape[0]
-    x, ldx = _rows(x, K)
-    weight, ldw = _rows(weight, K)
+    out_shape = shape[:-1] + (N,)
+    bp = rp = None
     if bias is not None:
         if bias.shape != (N,):
             raise ValueError(f"bias {tuple(bias.shape)} does not fit {N} outputs")
         bias = bias.contiguous()
+        bp = bias.data_ptr()
+    if residual is not None and (residual.shape != out_shape or residual.dtype != out_dtype):
+        raise ValueError(f"the residual must be {tuple(out_shape)} {out_dtype}, like the output")
+    out = torch.empty(out_shape, dtype=out_dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    if len(shape) != 2:
+        x = x.reshape(-1, K)
+    M = x.shape[0]
+    x, ldx = _rows(x, M, K)
+    weight, ldw = _rows(weight, N, K)
     ldr = N
     if residual is not None:
-        if residual.shape != out.shape or residual.dtype != out_dtype:
-            raise ValueError(f"the residual must be {tuple(out.shape)} {out_dtype}, like the output")
-        residual, ldr = _rows(residual.reshape(-1, N), N)
+        residual, ldr = _rows(residual if len(shape) == 2 else residual.reshape(-1, N), M, N)
+        rp = residual.data_ptr()
     lib = _lib.load()
     nbytes = lib.odsd_linear_workspace_bytes(M, N, K)
-    if nbytes == 0:
-        raise _lib.OdsdError(f"linear: unsupported shape M={M} N={N} K={K}")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    rc = lib.odsd_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr,
-                         out.data_ptr(), N, M, N, K, code, _lib.DT_F32 if out_dtype == torch.float32 else code, act,
-                         ws.data_ptr(), nbytes, _stream())
+    wp = None
+    if nbytes > _NO_WORKSPACE:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        wp = ws.data_ptr()
+    rc = lib.odsd_linear(x.data_ptr(), ldx, weight.data_ptr(), ldw, bp, rp, ldr, out.data_ptr(), N, M, N, K, code, out_code, act,
+                         wp, nbytes, _stream())
     if rc:
         _lib.check(rc, "odsd_linear")
     return out

@@ -76,13 +76,15 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
                 raise ValueError(f"query lengths {host} do not fit {rows} rows and {n_drafts} drafts")
             if context.get("max_query_len", rows) < max(host):
                 raise ValueError("max_query_len is below the longest query")
-        lens = lens.to(device=logits.device, dtype=torch.int32).contiguous()
+        if lens.get_device() != dev or lens.dtype != torch.int32:
+            lens = lens.to(device=logits.device, dtype=torch.int32)
+        lens = lens.contiguous()
         longest = context.get("max_query_len", rows)
     ld_draft = vocab
     if draft_logits is not None:
         if draft_logits.shape != (n_drafts, vocab) or draft_logits.dtype != logits.dtype:
             raise ValueError(f"draft_logits must be [{n_drafts}, {vocab}] in the dtype of logits")
-        draft_logits, ld_draft = _rows(draft_logits, vocab) if n_drafts else (None, vocab)
+        draft_logits, ld_draft = _rows(draft_logits, n_drafts, vocab) if n_drafts else (None, vocab)
     if t_tensor is not None:
         if t_tensor.dtype != torch.float32 or t_tensor.numel() != n_seqs:
             raise ValueError(f"temperature must be a number or float32 [{n_seqs}]")
@@ -92,21 +94,24 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
         t_all = float(temperature)
         if not t_all >= 0.0:
             raise ValueError(f"temperature {temperature} is negative")
-    logits, ld = _rows(logits, vocab)
+    logits, ld = _rows(logits, rows, vocab)
     if draft_tokens is not None:
-        draft_tokens = draft_tokens.to(torch.int64).contiguous()
+        if draft_tokens.dtype != torch.int64:
+            draft_tokens = draft_tokens.to(torch.int64)
+        draft_tokens = draft_tokens.contiguous()
         accept_u = accept_u.contiguous()
     sample_u = sample_u.contiguous()
-    out = VerifyResult(torch.empty(n_seqs, longest, dtype=torch.int64, device=logits.device),
-                       torch.empty(n_seqs, dtype=torch.int32, device=logits.device),
-                       torch.empty(n_drafts, dtype=torch.float32, device=logits.device))
+    device = logits.device
+    out = VerifyResult(torch.empty((n_seqs, longest), dtype=torch.int64, device=device),
+                       torch.empty(n_seqs, dtype=torch.int32, device=device),
+                       torch.empty(n_drafts, dtype=torch.float32, device=device))
     if n_seqs == 0:
         return out
     lib = _lib.load()
     nbytes = lib.odsd_verify_workspace_bytes(n_seqs, longest, rows, n_drafts, vocab, 0 if draft_logits is None else 1)
     if nbytes == 0:
         raise _lib.OdsdError(f"verify_drafts: unsupported sizes: {n_seqs} sequences, {rows} rows of {vocab}")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     rc = lib.odsd_verify_drafts(logits.data_ptr(), ld, _ptr(draft_logits), ld_draft, code, _ptr(draft_tokens), _ptr(lens),
                                 _ptr(t_tensor), t_all, _ptr(accept_u), sample_u.data_ptr(), n_seqs, longest, rows,
                                 n_drafts, vocab, out.tokens.data_ptr(), out.num_accepted.data_ptr(),
