@@ -200,8 +200,9 @@ __global__ __launch_bounds__(NWV * 64) void linear_rows_kernel(LinearParams p) {
 // rows are 128 bytes (64 with steps of 32), whose 16-byte segments are XORed with bits of the row's number: the 16 lanes that
 // read together (rows 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of a block, one segment) then meet the 16 bank groups.  What is behind a row's end, the matrix's last row or the slice's
 // last step is addressed outside the buffer descriptor and arrives as zeros, without memory traffic, so every copy is
-// issued whatever follows and a count says which have landed.
-template <int NWN, int NWM, int FA, int FB, int BK, int STAGES>
+// issued whatever follows and a count says which have landed.  KS groups of such wavefronts take every KS-th step each, with
+// buffers of their own, and add their sums up at the end: for few tokens, where a step is a chain of latencies.
+template <int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS>
 struct LinearTile {
     static constexpr int NW = NWN * NWM, TN = NWN * FA * 32, TM = NWM * FB * 32;
     static constexpr int ROW = BK * 2, SEGS = BK / 8, ROWS = 64 / SEGS;      // bytes and 16-byte segments of a row, rows of a copy
@@ -209,7 +210,7 @@ struct LinearTile {
     static constexpr int LA = TN / ROWS / NW, LB = TM / ROWS / NW, L = LA + LB;   // copies of a wavefront per step
     static constexpr int CH = FA < 2 ? FA : 2;                             // blocks of n that leave together
     static constexpr int OUT_WAVE = FB * 32 * CH * 32 * 4;
-    static constexpr int LDS = STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE;
+    static constexpr int LDS = KS * (STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE);
     static_assert(LA * ROWS * NW == TN && LB * ROWS * NW == TM && LB >= 1, "every wavefront makes the same number of copies");
     static_assert((BK == 64 && NW % 2 == 0) || BK == 32, "the swizzle of a copied row does not depend on the copy");
 };
@@ -228,12 +229,13 @@ __device__ __forceinline__ uint4_t descriptor(const void *base, uint32_t bytes) 
     return r;
 }
 
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES>
-__global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParams p) {
-    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES> C;
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS>
+__global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(LinearParams p) {
+    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES, KS> C;
     typedef typename AttnT<T>::V8 V8;
     __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = lane_id(), any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = any_wave % C::NW, part = any_wave / C::NW;      // of a share of K, and which share
     // neighbouring tiles on one XCD (workgroup i is on XCD i % 8), in groups of up to 8 along m that share their weights
     const int total = p.tiles_n * p.tiles_m * p.slices, per = (total + 7) / 8;
     const int b = blockIdx.x, t0 = (b & 7) * per + (b >> 3);
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParam
     const int n0 = in_group / gm * C::TN, m0 = (group * 8 + in_group % gm) * C::TM;
 
     const int k_begin = slice * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
-    const int steps = (k_end - k_begin + BK - 1) / BK;
+    const int steps = (k_end - k_begin + BK * KS - 1) / (BK * KS);   // of a share: every KS-th
     const uint32_t ldw = (uint32_t)p.ldw * 2u, ldx = (uint32_t)p.ldx * 2u;
     const uint4_t rw = descriptor((const char *)p.w + (int64_t)n0 * p.ldw * 2, (uint32_t)(min(C::TN, p.N - n0) - 1) * ldw + p.K * 2);
     const uint4_t rx = descriptor((const char *)p.x + (int64_t)m0 * p.ldx * 2, (uint32_t)(min(C::TM, p.M - m0) - 1) * ldx + p.K * 2);
@@ -252,9 +254,10 @@ __global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParam
     const int seg = BK == 64 ? (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)) : (lane & 3) ^ (lane >> 4);
     const uint32_t row0 = wave * C::ROWS + lane / C::SEGS;
     const uint32_t off_w = row0 * ldw + seg * 16, off_x = row0 * ldx + seg * 16;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)lds;
+    char *const mine = lds + part * (C::STAGE * STAGES);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)mine;
     auto copy = [&](int step, uint32_t buf, int i) {            // copy i of a step's: first those of w, then those of x
-        const int k = k_begin + step * BK;
+        const int k = k_begin + (step * KS + part) * BK;
         const uint32_t ko = k + seg * 8 < k_end ? (uint32_t)k * 2u : 0x80000000u;
         if (i < C::LA) copy16_to_lds(rw, off_w + ko + i * (C::NW * C::ROWS) * ldw, lds0 + buf + (i * C::NW + wave) * 1024);
         else copy16_to_lds(rx, off_x + ko + (i - C::LA) * (C::NW * C::ROWS) * ldx, lds0 + buf + C::A_BYTES + ((i - C::LA) * C::NW + wave) * 1024);
@@ -273,8 +276,8 @@ __global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParam
     V8 fa[2][FA], fb[2][FB];
     // fragment i of columns 16 j .. of a buffer, in the order in which the products want them: w's first, x's, the rest of w's
     auto read = [&](int par, uint32_t buf, int j, int i) {
-        if (i > 0 && i <= FB) fb[par][i - 1] = *(const V8 *)(lds + ((buf + fb0) ^ (j << 5)) + (i - 1) * 32 * C::ROW);
-        else fa[par][i ? i - FB : 0] = *(const V8 *)(lds + ((buf + fa0) ^ (j << 5)) + (i ? i - FB : 0) * 32 * C::ROW);
+        if (i > 0 && i <= FB) fb[par][i - 1] = *(const V8 *)(mine + ((buf + fb0) ^ (j << 5)) + (i - 1) * 32 * C::ROW);
+        else fa[par][i ? i - FB : 0] = *(const V8 *)(mine + ((buf + fa0) ^ (j << 5)) + (i ? i - FB : 0) * 32 * C::ROW);
     };
     // 16 columns: their products, and between those, one by one, the reads of the next 16 columns' fragments and the copies
     // of the step that comes into the buffer that was left last.  (The compiler would request a fragment right before its
@@ -334,7 +337,7 @@ __global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParam
     // of a token's row are XORed with the token's number.
     constexpr int PIECES = C::CH * 8;          // of 4 sums, per token
     auto swz = [](int m) { return PIECES == 16 ? m & 15 : (m >> 1) & 7; };
-    char *stage = lds + wave * C::OUT_WAVE;
+    char *stage = lds + any_wave * C::OUT_WAVE;
 #pragma unroll
     for (int a0 = 0; a0 < FA; a0 += C::CH) {
 #pragma unroll
@@ -349,13 +352,23 @@ __global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParam
                     for (int u = 0; u < 4; ++u) v[u] = acc[a0 + a][c][4 * q + u];
                     *(float4_t *)(stage + m * (PIECES * 16) + ((piece ^ swz(m)) << 4)) = v;
                 }
-        // (a wavefront's own LDS accesses stay in order)
+        // one share of K: a wavefront's own LDS accesses stay in order; several: each adds up its part of the tokens
+        if (KS > 1) __syncthreads();
         constexpr int LANES = PIECES / 2;      // lanes that share a token's row
-        for (int r = lane / LANES; r < FB * 32; r += 64 / LANES) {
+        for (int r = part * (64 / LANES) + lane / LANES; r < FB * 32; r += KS * (64 / LANES)) {
             const int pc = lane % LANES * 2;
+            float4_t lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const char *from = KS > 1 ? lds + (s * C::NW + wave) * C::OUT_WAVE : stage;
+                const float4_t a = *(const float4_t *)(from + r * (PIECES * 16) + ((pc ^ swz(r)) << 4));
+                const float4_t b = *(const float4_t *)(from + r * (PIECES * 16) + (((pc + 1) ^ swz(r)) << 4));
+                lo = s ? lo + a : a;
+                hi = s ? hi + b : b;
+            }
             float v[8];
-            *(float4_t *)v = *(const float4_t *)(stage + r * (PIECES * 16) + ((pc ^ swz(r)) << 4));
-            *(float4_t *)(v + 4) = *(const float4_t *)(stage + r * (PIECES * 16) + (((pc + 1) ^ swz(r)) << 4));
+            *(float4_t *)v = lo;
+            *(float4_t *)(v + 4) = hi;
             const int m = m0 + wm * FB * 32 + r, n = n0 + (wn * FA + a0) * 32 + pc * 4;
             if (p.slices > 1) {
                 if (m < p.M && n < p.N) {
@@ -367,6 +380,7 @@ __global__ __launch_bounds__(NWN * NWM * 64) void linear_tile_kernel(LinearParam
                 finish8<T, O>(p, m, n, v);
             }
         }
+        if (KS > 1 && FA > C::CH) __syncthreads();
         asm volatile("" ::: "memory");
     }
 }
@@ -480,8 +494,11 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
-enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_128_32, LIN_TILE_128_64, LIN_TILE_64_64, LIN_TILE_128_128, LIN_TILE_256_256, LIN_KINDS };
-static const int TILE_N[LIN_KINDS] = {16, 64, 128, 128, 64, 128, 256}, TILE_M[LIN_KINDS] = {16, 64, 32, 64, 64, 128, 256};
+// tiles n x m; K4, K2: K shared by groups of wavefronts of the workgroup
+enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_32_64_K4, LIN_TILE_32_64_K2, LIN_TILE_128_32, LIN_TILE_128_64, LIN_TILE_64_64,
+       LIN_TILE_128_128, LIN_TILE_256_256, LIN_KINDS };
+static const int TILE_N[LIN_KINDS] = {16, 64, 32, 32, 128, 128, 64, 128, 256};
+static const int TILE_M[LIN_KINDS] = {16, 64, 64, 64, 32, 64, 64, 128, 256};
 struct LinearPlan {
     int kind, slices, slice_k;
     int64_t part_ld;
@@ -503,15 +520,20 @@ static LinearPlan linear_plan_of(int kind, int slices, int M, int N, int K) {
     return l;
 }
 static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
-    // Up to 4 tokens, and up to 16 on a few hundred workgroups, one pass over the weights' rows beats the tiles (us, rows /
-    // 128 x 32 tiles): M = 1: K 4096, N 2048 7.1 / 9.9, K 2048, N 131072 93 / 100; M = 16: K 4096, N 2048 8.4 / 10.4, K 2048,
-    // N 5120 10.1 / 10.2, K 4096, N 16384 36.6 / 28.6, K 2048, N 131072 123 / 105.
-    if (M <= 4 || (M <= 16 && N <= 6144)) return linear_plan_of(LIN_ROWS, 1, M, N, K);
+    // Up to 4 tokens one pass over the weights' rows, also where their segments are not aligned (up to 16, there).  us, rows /
+    // the tiles that follow: M = 1: K 4096, N 2048 7.1 / 11.0, K 2048, N 131072 93 / 100; M = 4: K 2048, N 5120 8.3 / 8.0;
+    // M = 16: K 2048, N 5120 10.0 / 8.0, N 131072 123 / 105.
+    if (M <= 4 || (M <= 16 && !aligned)) return linear_plan_of(LIN_ROWS, 1, M, N, K);
     if (!aligned) return linear_plan_of(LIN_ANY, 1, M, N, K);
     const int steps = (K + 63) / 64;
-    // Up to 64 tokens the weights' bytes count: as many tokens in a tile as there are, and parts of K until the workgroups
-    // are two per CU.  64 x 64 tiles once they alone fill the chip (M = 64, K 2048, us, 128 x 64 / 64 x 64: N 5120 12.3 /
-    // 13.2, N 32768 36.0 / 33.1, N 131072 117 / 113).
+    // Up to 64 tokens the weights' bytes count, and how many of them are on their way.  While 32-row tiles are at most one
+    // (two) per CU, K is shared inside the workgroup, in one launch; beyond that, as many tokens in a tile as there are, and
+    // parts of K until the workgroups are two per CU; 64 x 64 tiles once they alone fill the chip.  us at M = 64, K shared by
+    // 4 / by 2 / parts of K in two launches: K 2048: N 5120 8.5 / 8.6 / 13.0, N 8192 10.2 / 9.8 / 13.8, N 16384 18.1 / 14.5 /
+    // 21.2, N 24576 29.5 / 27.4 / 27.7; K 4096: N 2048 11.4 / 12.1 / 13.0, N 12288 30.6 / 29.1 / 28.0; K 8192: N 2048 18.3 /
+    // 20.7 / 14.4, N 8192 33.3 / 36.0 / 36.4.  (128 x 64 / 64 x 64 tiles: N 32768 36.0 / 33.1, N 131072 117 / 113.)
+    if (M <= 64 && N <= 8192 && (K <= 4096 || K <= N)) return linear_plan_of(LIN_TILE_32_64_K4, 1, M, N, K);
+    if (M <= 64 && N <= 16384 && K <= 2048) return linear_plan_of(LIN_TILE_32_64_K2, 1, M, N, K);
     if (M <= 64) {
         const int kind = M <= 32 ? LIN_TILE_128_32 : N >= 24576 ? LIN_TILE_64_64 : LIN_TILE_128_64;
         int slices = 1;
@@ -523,7 +545,8 @@ static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
     // Step and epilogue in us, as measured on full rounds (K 2048 and 4096, bf16).  us of the shape taken / of others, K 4096,
     // N 4096: M = 2048 (128 x 128) 66 / 81 (128 x 64), M = 4096 (256 x 256) 111 / 128 (128 x 128); K 2048, N 5120: M = 200
     // (64 x 64) 14 / 18 / 22, M = 500 (128 x 64) 21 / 25 / 27.
-    static const float STEP[LIN_KINDS] = {0, 0, 0, 0.68f, 0.42f, 1.06f, 1.58f}, END[LIN_KINDS] = {0, 0, 0, 2.0f, 1.5f, 4.0f, 10.0f};
+    static const float STEP[LIN_KINDS] = {0, 0, 0, 0, 0, 0.68f, 0.42f, 1.06f, 1.58f};
+    static const float END[LIN_KINDS] = {0, 0, 0, 0, 0, 2.0f, 1.5f, 4.0f, 10.0f};
     LinearPlan best = {};
     float best_us = 0.0f;
     for (int kind = LIN_TILE_128_64; kind <= LIN_TILE_256_256; ++kind) {
@@ -541,13 +564,13 @@ static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
     return best;
 }
 
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES>
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS = 1>
 static void launch_tile(LinearParams &p, hipStream_t st) {
-    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES> C;
+    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES, KS> C;
     p.tiles_n = (p.N + C::TN - 1) / C::TN;
     p.tiles_m = (p.M + C::TM - 1) / C::TM;
     const int64_t total = (int64_t)p.tiles_n * p.tiles_m * p.slices;
-    linear_tile_kernel<T, O, NWN, NWM, FA, FB, BK, STAGES><<<(unsigned)((total + 7) / 8 * 8), C::NW * 64, 0, st>>>(p);
+    linear_tile_kernel<T, O, NWN, NWM, FA, FB, BK, STAGES, KS><<<(unsigned)((total + 7) / 8 * 8), C::NW * KS * 64, 0, st>>>(p);
 }
 
 template <typename T, typename O> static int launch_linear(LinearParams &p, const LinearPlan &l, void *workspace, hipStream_t st) {
@@ -569,6 +592,8 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
     p.part = (float *)workspace;
     p.part_ld = l.part_ld;
     switch (l.kind) {
+        case LIN_TILE_32_64_K4: launch_tile<T, O, 1, 2, 1, 1, 64, 3, 4>(p, st); break;
+        case LIN_TILE_32_64_K2: launch_tile<T, O, 1, 2, 1, 1, 64, 3, 2>(p, st); break;
         case LIN_TILE_128_32: launch_tile<T, O, 4, 1, 1, 1, 64, 4>(p, st); break;
         case LIN_TILE_128_64: launch_tile<T, O, 4, 1, 1, 2, 64, 3>(p, st); break;
         case LIN_TILE_64_64: launch_tile<T, O, 2, 2, 1, 1, 64, 4>(p, st); break;

@@ -18,8 +18,8 @@ def test_linear_status_codes():
     assert f(dt=0) == f(dt=9) == f(odt=2) == f(odt=9) == 7
     assert f(act=5) == f(act=-1) == 3 and f(M=5_000_000) == 3
     assert f(x=None) == f(w=None) == f(out=None) == 1
-    split = dict(M=40, N=512, K=4096, ldx=4096, ldw=4096, ldo=512)             # parts of K: a workspace is needed
-    assert lib.odsd_linear_workspace_bytes(40, 512, 4096) > 256 and f(ws=None, **split) == 1 and f(nb=256, **split) == 5
+    split = dict(M=40, N=512, K=8192, ldx=8192, ldw=8192, ldo=512)             # parts of K: a workspace is needed
+    assert lib.odsd_linear_workspace_bytes(40, 512, 8192) > 256 and f(ws=None, **split) == 1 and f(nb=256, **split) == 5
     assert f(x=P + 1) == f(out=P + 1) == f(odt=0, out=P + 2) == f(ws=P + 8) == 4
     assert f(M=0, x=None, out=None) == 0
     assert lib.odsd_linear_workspace_bytes(4, 16, 0) == 0 and lib.odsd_linear_workspace_bytes(4, 16, 64) >= 256

@@ -53,7 +53,10 @@ def run(dev, M, K, N, dtype="bf16", out=None, act=None, bias=True, residual=True
 SHAPES = [(1, 2048, 4096), (1, 8, 1), (1, 1, 1), (2, 64, 16), (3, 100, 7), (5, 2048, 5120), (7, 2056, 130), (8, 4096, 2048), (15, 512, 333),
           (16, 1288, 1000), (17, 1288, 1001), (31, 640, 260), (33, 264, 515), (40, 2048, 512), (64, 2048, 1024), (64, 72, 40), (65, 512, 512),
           (100, 1000, 300), (128, 4096, 256), (129, 64, 129), (200, 512, 384), (256, 256, 256), (257, 1288, 513), (333, 1288, 2053),
-          (512, 32, 512), (1000, 520, 1000), (1, 520, 40000), (20, 4096, 64), (300, 4104, 128), (700, 1536, 700)]
+          (512, 32, 512), (1000, 520, 1000), (1, 520, 40000), (20, 4096, 64), (300, 4104, 128), (700, 1536, 700),
+          # the borders of the choice of kernels: tokens, rows of w, parts of K
+          (4, 256, 300), (5, 256, 300), (16, 8200, 520), (33, 8192, 512), (64, 2048, 8192), (64, 2048, 8193), (48, 1032, 16384), (64, 1032, 16392),
+          (32, 2056, 16640), (64, 520, 24576), (65, 4096, 512), (256, 2048, 2048), (128, 8192, 128), (2048, 256, 2048), (1500, 192, 5000)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
