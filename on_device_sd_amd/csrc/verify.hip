@@ -186,6 +186,46 @@ template <typename T> __device__ __forceinline__ float largest8(const Raw8<T> &r
     return m;
 }
 
+// Reductions by DPP: a step is one or two vector instructions, where a shuffle through the LDS hardware waits for it; these
+// kernels are chains of them.  Within a row of 16 lanes (every lane has the result): rotations.  Over the wavefront (the result
+// is uniform): shifts within the rows, then the rows' last lanes.
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ int dpp(int old, int v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ float dpp(float old, float v) {
+    return __int_as_float(dpp<CTRL, ROWS>(__float_as_int(old), __float_as_int(v)));
+}
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ double dpp(double old, double v) {
+    return __hiloint2double(dpp<CTRL, ROWS>(__double2hiint(old), __double2hiint(v)), dpp<CTRL, ROWS>(__double2loint(old), __double2loint(v)));
+}
+enum { ROW_SHR = 0x110, ROW_ROR = 0x120, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143 };
+template <typename V, typename F> __device__ __forceinline__ V row_all(V v, F f) {
+    v = f(v, dpp<ROW_ROR + 8>(v, v));
+    v = f(v, dpp<ROW_ROR + 4>(v, v));
+    v = f(v, dpp<ROW_ROR + 2>(v, v));
+    return f(v, dpp<ROW_ROR + 1>(v, v));
+}
+// inclusive, over the lanes; `zero` leaves f's other argument as it is
+template <typename V, typename F> __device__ __forceinline__ V scan_all(V v, V zero, F f) {
+    v = f(dpp<ROW_SHR + 1>(zero, v), v);
+    v = f(dpp<ROW_SHR + 2>(zero, v), v);
+    v = f(dpp<ROW_SHR + 4>(zero, v), v);
+    v = f(dpp<ROW_SHR + 8>(zero, v), v);
+    v = f(dpp<ROW_BCAST15, 0xa>(zero, v), v);
+    return f(dpp<ROW_BCAST31, 0xc>(zero, v), v);
+}
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ double last_lane(double v) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+template <typename V> __device__ __forceinline__ V plus(V a, V b) { return a + b; }
+__device__ __forceinline__ double all_sum(double v) { return last_lane(scan_all(v, 0.0, plus<double>)); }
+__device__ __forceinline__ int all_sum(int v) { return last_lane(scan_all(v, 0, plus<int>)); }
+__device__ __forceinline__ float all_max(float v) { return last_lane(scan_all(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); })); }
+__device__ __forceinline__ int all_min(int v) { return last_lane(scan_all(v, 0x7fffffff, [](int a, int b) { return min(a, b); })); }
+__device__ __forceinline__ int all_max(int v) { return last_lane(scan_all(v, -0x7fffffff - 1, [](int a, int b) { return max(a, b); })); }
+
 // the larger logit, the lower index of equals
 __device__ __forceinline__ void better(float &top, int &at, float t2, int a2) {
     if (t2 > top || (t2 == top && a2 < at)) {
@@ -215,15 +255,10 @@ __device__ __forceinline__ int sequence_of(const VerifyParams &p, int r, bool dr
         const int s = s0 + lane_id();
         int n = s < p.S ? len_of(p, s) : 0;
         if (draft) n = max(n - 1, 0);
-        int sum = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(sum, o, ODSD_WAVE);
-            if (lane_id() >= o) sum += v;
-        }
+        const int sum = scan_all(n, 0, plus<int>);
         const uint64_t past = __ballot(before + sum > r);
         if (past) return s0 + __builtin_ctzll(past);
-        before += __shfl(sum, 63, ODSD_WAVE);
+        before += last_lane(sum);
     }
     return -1;
 }
@@ -252,7 +287,7 @@ __global__ __launch_bounds__(VER_THREADS) void verify_stats_kernel(VerifyParams 
     for (int i = 0; i < 4; ++i) raw[i].clip();
     float top = max3(largest8(raw[0]), largest8(raw[1]), fmaxf(largest8(raw[2]), largest8(raw[3])));
     const float own = top;
-    top = wave_max(top);
+    top = all_max(top);
     if (lane_id() == 0) s_top[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
@@ -266,8 +301,7 @@ __global__ __launch_bounds__(VER_THREADS) void verify_stats_kernel(VerifyParams 
                 for (int j = 7; j >= 0; --j)
                     if (raw[i].get(j) == top && j >= raw[i].skip) at = raw[i].base + j;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, ODSD_WAVE));
+        at = all_min(at);
         if (lane_id() == 0) s_at[wave] = at;
     } else {
         if (fabsf(top) < INFINITY && k > 1e-30 && k < 1e30) {
@@ -302,7 +336,7 @@ __global__ __launch_bounds__(VER_THREADS) void verify_stats_kernel(VerifyParams 
                 if (at < p.V) z += weight_of(number((float)src[at]), top, k);
             }
         }
-        z = wave_sum(z);
+        z = all_sum(z);
         if (lane_id() == 0) s_z[wave] = z;
     }
     __syncthreads();
@@ -322,15 +356,17 @@ __device__ __forceinline__ Stat row_stat(const VerifyParams &p, int row, double 
     if (l < p.splits) own = st[l];
     float top = own.top;
     int at = own.at;
-    for (int c = l + 16; c < p.splits; c += 16) better(top, at, st[c].top, st[c].at);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) better(top, at, __shfl_xor(top, o, ODSD_WAVE), __shfl_xor(at, o, ODSD_WAVE));
     double z = 0.0;
     if (k > 0.0) {
+        for (int c = l + 16; c < p.splits; c += 16) top = fmaxf(top, st[c].top);
+        top = row_all(top, [](float a, float b) { return fmaxf(a, b); });
         z = own.z * weight_of(own.top, top, k);
         for (int c = l + 16; c < p.splits; c += 16) z += st[c].z * weight_of(st[c].top, top, k);
+        z = row_all(z, plus<double>);
+    } else {
+        for (int c = l + 16; c < p.splits; c += 16) better(top, at, st[c].top, st[c].at);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, ODSD_WAVE);
+        for (int o = 8; o > 0; o >>= 1) better(top, at, __shfl_xor(top, o, ODSD_WAVE), __shfl_xor(at, o, ODSD_WAVE));
     }
     return Stat{top, at, z};
 }
@@ -355,11 +391,8 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
             start += n;
             dstart += max(n - 1, 0);
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            start += __shfl_xor(start, o, ODSD_WAVE);
-            dstart += __shfl_xor(dstart, o, ODSD_WAVE);
-        }
+        start = all_sum(start);
+        dstart = all_sum(dstart);
         if (lane_id() == 0) {
             s_start[wave] = start;
             s_dstart[wave] = dstart;
@@ -386,17 +419,11 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
         const bool with_q = p.draft_logits && k > 0.0;
         for (int j0 = 0; j0 < n; j0 += 32) {
             const int rows = min(32, n - j0), drafts = min(32, n - 1 - j0);
-            for (int g = threadIdx.x >> 4; g < (with_q ? 64 : 32); g += VER_THREADS / 16) {
-                const int j = g & 31;
-                if (g < 32 ? j >= rows : j >= drafts) continue;
-                const Stat st = row_stat(p, g < 32 ? start + j0 + j : p.n_q + dstart + j0 + j, k);
-                if ((lane_id() & 15) == 0) (g < 32 ? s_p : s_q)[j] = st;
-            }
-            // the drafts' own logits on their way meanwhile
+            // the drafts' own logits, on their way meanwhile: by the wavefront that has rows last
             const int j = lane_id();
             int64_t d = -1;
             float u = 0.0f, lp = -INFINITY, lq = -INFINITY;
-            if (wave == 0 && j < drafts) {
+            if (wave == 3 && j < drafts) {
                 d = p.drafts[dstart + j0 + j];
                 u = p.accept_u[dstart + j0 + j];
                 if (d >= 0 && d < p.V) {
@@ -404,8 +431,14 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
                     if (with_q) lq = (float)((const T *)p.draft_logits)[(int64_t)(dstart + j0 + j) * p.ld_d + d];
                 }
             }
+            for (int g = threadIdx.x >> 4; g < (with_q ? 64 : 32); g += VER_THREADS / 16) {
+                const int j = g & 31;
+                if (g < 32 ? j >= rows : j >= drafts) continue;
+                const Stat st = row_stat(p, g < 32 ? start + j0 + j : p.n_q + dstart + j0 + j, k);
+                if ((lane_id() & 15) == 0) (g < 32 ? s_p : s_q)[j] = st;
+            }
             __syncthreads();
-            if (wave == 0) {
+            if (wave == 3) {
                 double a = 0.0;
                 if (j < drafts && d >= 0 && d < p.V) {
                     const Stat sp = s_p[j];
@@ -493,8 +526,8 @@ __global__ __launch_bounds__(VER_THREADS) void verify_choose_kernel(VerifyParams
             zq += v[j];
         }
     }
-    zp = wave_sum(zp);
-    zq = wave_sum(zq);
+    zp = all_sum(zp);
+    zq = all_sum(zq);
     if (lane_id() == 0) {
         s_z[0][threadIdx.x >> 6] = zp;
         s_z[1][threadIdx.x >> 6] = zq;
@@ -513,8 +546,8 @@ __device__ __forceinline__ void exact_sums(const VerifyParams &p, int s, double 
         zp += p.z[((int64_t)s * p.splits + c) * 2];
         zq += p.z[((int64_t)s * p.splits + c) * 2 + 1];
     }
-    zp = wave_sum(zp);
-    zq = wave_sum(zq);
+    zp = all_sum(zp);
+    zq = all_sum(zq);
 }
 
 // The weights of eight consecutive tokens that one is drawn from, relative to exp((top - row's top) / T): max(p - q, 0) with
@@ -536,7 +569,7 @@ __device__ __forceinline__ float weights8(const Choice &c, Raw8<T> &r, Raw8<T> &
         }
         return 0.0f;
     }
-    const float top = wave_max(largest8(r));
+    const float top = all_max(largest8(r));
     if (c.k > 0.0) {
         const Weigh wp(top, c.k);
         wp(r, w);
@@ -577,21 +610,11 @@ __global__ __launch_bounds__(VER_THREADS) void verify_sums_kernel(VerifyParams p
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int sub = sub0 + i * 4;
-        if (sub >= p.subs) return;
         double w[8];
         const float top = weights8<T>(c, r[i], q[i], true, ip, iq, w);
-        const double a = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-        if (lane_id() == 0) p.blocks[(int64_t)s * p.subs + sub] = Block{a, top, 0};
+        const double a = all_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        if (sub < p.subs && lane_id() == 0) p.blocks[(int64_t)s * p.subs + sub] = Block{a, top, 0};
     }
-}
-
-__device__ __forceinline__ double wave_scan(double v) {       // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(v, o, ODSD_WAVE);
-        if (lane_id() >= o) v += u;
-    }
-    return v;
 }
 
 // ---- the draw: one wavefront per sequence --------------------------------------------------------------
@@ -612,21 +635,28 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
     bool rest = true;
     double lane_sum, total;
     float top;
-    auto block_weight = [&](int b) {                          // of block b, relative to the largest block's top
-        const Block v = blocks[b];
+    constexpr int KEEP = 4;                                   // blocks of a lane that stay in registers (131 072 tokens)
+    Block v[KEEP];
+    auto block_weight = [&](const Block &v) {                 // relative to the largest block's top
         return c.k > 0.0 ? v.sum * weight_of(v.top, top, c.k) : v.top == top ? v.sum : 0.0;
     };
     for (;;) {
-        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) v[i] = b0 + i < b1 ? blocks[b0 + i] : Block{0.0, -INFINITY, 0};
         if (rest && c.draft >= 0) {
             top = 0.0f;                                       // (by agreement: these sums are absolute)
         } else {
-            for (int b = b0; b < b1; ++b) top = fmaxf(top, blocks[b].sum > 0.0 ? blocks[b].top : -INFINITY);
-            top = wave_max(top);
+            top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) top = fmaxf(top, v[i].sum > 0.0 ? v[i].top : -INFINITY);
+            for (int b = b0 + KEEP; b < b1; ++b) top = fmaxf(top, blocks[b].sum > 0.0 ? blocks[b].top : -INFINITY);
+            top = all_max(top);
         }
         lane_sum = 0.0;
-        for (int b = b0; b < b1; ++b) lane_sum += block_weight(b);
-        total = wave_sum(lane_sum);
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) lane_sum += v[i].sum = block_weight(v[i]);
+        for (int b = b0 + KEEP; b < b1; ++b) lane_sum += block_weight(blocks[b]);
+        total = all_sum(lane_sum);
         if (total > 0.0 || !rest) break;
         // nothing of p exceeds q: p itself.  (Two equal distributions keep every draft, so this is rare: the sums are made here.)
         rest = false;
@@ -635,7 +665,7 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
             Raw8<T> r1, q1;
             load_pair(p, c, b * VER_SUB + lane_id() * 8, r1, q1);
             const float t = weights8<T>(c, r1, q1, false, ip, iq, w);
-            const double a = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+            const double a = all_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
             if (lane_id() == 0) blocks[b] = Block{a, t, 0};
         }
         __threadfence();
@@ -647,7 +677,7 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
     }
     const double aim = c.k > 0.0 ? (double)u * total : 0.0;    // (greedy: the first of the largest)
     // the first lane whose inclusive sum exceeds the aim (else the last that has any weight), and of its blocks likewise
-    const double run = wave_scan(lane_sum);
+    const double run = scan_all(lane_sum, 0.0, plus<double>);
     const uint64_t past = __ballot(run > aim && lane_sum > 0.0), any = __ballot(lane_sum > 0.0);
     const int owner = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
     int sub = -1;
@@ -655,21 +685,24 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
     if ((int)lane_id() == owner) {
         int last = -1;
         double last_before = 0.0, sum = before;
-        for (int b = b0; b < b1 && sub < 0; ++b) {
-            const double w = block_weight(b);
+        auto step = [&](int b, double w) {
+            if (sub >= 0) return;
             if (w > 0.0) {
                 last = b;
                 last_before = sum;
                 if (past && sum + w > aim) sub = b;
             }
             sum += w;
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) step(b0 + i, v[i].sum);
+        for (int b = b0 + KEEP; b < b1; ++b) step(b, block_weight(blocks[b]));
         // (rounding between the scan and this sum, or no block past the aim: the last token with a weight is taken)
         before = sub >= 0 ? last_before : -INFINITY;
         if (sub < 0) sub = last;
     }
-    sub = __shfl(sub, owner, ODSD_WAVE);
-    before = __shfl(before, owner, ODSD_WAVE);
+    sub = __builtin_amdgcn_readlane(sub, owner);
+    before = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(before), owner), __builtin_amdgcn_readlane(__double2loint(before), owner));
     double w[8], own = 0.0;
     Raw8<T> r1, q1;
     load_pair(p, c, sub * VER_SUB + lane_id() * 8, r1, q1);
@@ -681,7 +714,7 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
         own += w[j];
     }
     // the first token of this lane whose cumulative weight exceeds the aim, and the last that has any weight
-    const double up_to = before + (wave_scan(own) - own);
+    const double up_to = before + (scan_all(own, 0.0, plus<double>) - own);
     int hit = 0x7fffffff, last = -1;
     double cum = 0.0;
 #pragma unroll
@@ -692,11 +725,8 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyParams p) {
             last = r1.base + j;
         }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        hit = min(hit, __shfl_xor(hit, o, ODSD_WAVE));
-        last = max(last, __shfl_xor(last, o, ODSD_WAVE));
-    }
+    hit = all_min(hit);
+    last = all_max(last);
     if (lane_id() == 0) *out = hit != 0x7fffffff ? hit : last;
 }
 
@@ -776,6 +806,8 @@ extern "C" int odsd_verify_drafts(const void *logits, int64_t logits_stride, con
     const uintptr_t mask = dtype == ODSD_DT_F32 ? 3 : 1;
     if ((((uintptr_t)logits | (uintptr_t)draft_logits) & mask) || !odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
     if (workspace_bytes < need) return ODSD_ERR_WORKSPACE;
+    // (no drafts, a row for every sequence: their lengths are 1)
+    if (n_drafts == 0 && n_rows == n_seqs) query_lens = nullptr;
     VerifyLayout l;
     verify_layout(n_seqs, n_rows, n_drafts, vocab, draft_logits != nullptr, l);
     char *ws = (char *)workspace;
