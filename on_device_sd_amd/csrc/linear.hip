@@ -42,53 +42,69 @@ template <typename O> struct Vec8 { typedef O type __attribute__((ext_vector_typ
 
 // y[m][n .. n + 7] from their sums.  Eight consecutive values are one access at the elements' own alignment (the hardware
 // takes any), so neither N nor the rows' distances need be multiples of anything.
+template <typename T> __device__ __forceinline__ void load_bias8(const LinearParams &p, int n, float *b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+    if (!p.bias) return;
+    const T *bias = (const T *)p.bias + n;
+    if (n + 8 <= p.N) {
+        typename Vec8<T>::type v;
+        __builtin_memcpy(&v, bias, sizeof v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n + i < p.N) b[i] = (float)bias[i];
+    }
+}
 template <typename T, typename O, int ACT>
-__device__ __forceinline__ void finish8(const LinearParams &p, int m, int n, const float *v) {
+__device__ __forceinline__ void finish8(const LinearParams &p, int m, int n, const float *v, const float *b) {
     if (m >= p.M || n >= p.N) return;
-    const T *bias = p.bias ? (const T *)p.bias + n : nullptr;
     const O *res = p.res ? (const O *)p.res + (int64_t)m * p.ldr + n : nullptr;
     O *out = (O *)p.out + (int64_t)m * p.ldo + n;
     constexpr bool PRECISE = sizeof(O) == 4;
     if (n + 8 <= p.N) {
-        typename Vec8<T>::type b;
         typename Vec8<O>::type r, y;
-        if (bias) __builtin_memcpy(&b, bias, sizeof b);
         if (res) __builtin_memcpy(&r, res, sizeof r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float a = activate<PRECISE, ACT>(bias ? v[i] + (float)b[i] : v[i]);
+            const float a = activate<PRECISE, ACT>(v[i] + b[i]);
             y[i] = (O)(res ? a + (float)r[i] : a);
         }
         __builtin_memcpy(out, &y, sizeof y);
         return;
     }
-    for (int i = 0; i < 8 && n + i < p.N; ++i) {
-        const float a = activate<PRECISE, ACT>(bias ? v[i] + (float)bias[i] : v[i]);
-        out[i] = (O)(res ? a + (float)res[i] : a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (n + i < p.N) {
+            const float a = activate<PRECISE, ACT>(v[i] + b[i]);
+            out[i] = (O)(res ? a + (float)res[i] : a);
+        }
+}
+// f with the call's activation as a constant
+template <typename F> __device__ __forceinline__ void with_activation(int act, F f) {
+    switch (act) {
+        case ODSD_ACT_RELU: return f(std::integral_constant<int, ODSD_ACT_RELU>{});
+        case ODSD_ACT_SILU: return f(std::integral_constant<int, ODSD_ACT_SILU>{});
+        case ODSD_ACT_GELU: return f(std::integral_constant<int, ODSD_ACT_GELU>{});
+        case ODSD_ACT_GELU_TANH: return f(std::integral_constant<int, ODSD_ACT_GELU_TANH>{});
+        default: return f(std::integral_constant<int, ODSD_ACT_NONE>{});
     }
 }
 template <typename T, typename O>
 __device__ __forceinline__ void finish8(const LinearParams &p, int m, int n, const float *v) {
-    switch (p.act) {
-        case ODSD_ACT_RELU: return finish8<T, O, ODSD_ACT_RELU>(p, m, n, v);
-        case ODSD_ACT_SILU: return finish8<T, O, ODSD_ACT_SILU>(p, m, n, v);
-        case ODSD_ACT_GELU: return finish8<T, O, ODSD_ACT_GELU>(p, m, n, v);
-        case ODSD_ACT_GELU_TANH: return finish8<T, O, ODSD_ACT_GELU_TANH>(p, m, n, v);
-        default: return finish8<T, O, ODSD_ACT_NONE>(p, m, n, v);
-    }
+    with_activation(p.act, [&](auto act) {
+        float b[8];
+        load_bias8<T>(p, n, b);
+        finish8<T, O, decltype(act)::value>(p, m, n, v, b);
+    });
 }
-
 template <typename T, typename O>
 __device__ __forceinline__ void finish1(const LinearParams &p, int m, int n, float v) {
     constexpr bool PRECISE = sizeof(O) == 4;
     if (p.bias) v += (float)((const T *)p.bias)[n];
-    switch (p.act) {
-        case ODSD_ACT_RELU: v = activate<PRECISE, ODSD_ACT_RELU>(v); break;
-        case ODSD_ACT_SILU: v = activate<PRECISE, ODSD_ACT_SILU>(v); break;
-        case ODSD_ACT_GELU: v = activate<PRECISE, ODSD_ACT_GELU>(v); break;
-        case ODSD_ACT_GELU_TANH: v = activate<PRECISE, ODSD_ACT_GELU_TANH>(v); break;
-        default: break;
-    }
+    with_activation(p.act, [&](auto act) { v = activate<PRECISE, decltype(act)::value>(v); });
     if (p.res) v += (float)((const O *)p.res)[(int64_t)m * p.ldr + n];
     ((O *)p.out)[(int64_t)m * p.ldo + n] = (O)v;
 }
@@ -363,31 +379,39 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
                 }
         // one share of K: a wavefront's own LDS accesses stay in order; several: each adds up its part of the tokens
         if (KS > 1) __syncthreads();
-        constexpr int LANES = PIECES / 2;      // lanes that share a token's row
-        for (int r = part * (64 / LANES) + lane / LANES; r < FB * 32; r += KS * (64 / LANES)) {
-            const int pc = lane % LANES * 2;
-            float4_t lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+        constexpr int LANES = PIECES / 2, ROUND = 64 / LANES;  // lanes that share a token's row, rows at a time
+        const int pc = lane % LANES * 2, n = n0 + (wn * FA + a0) * 32 + pc * 4;
+        auto rows = [&](auto leave) {
+#pragma unroll 2                               // (all of them: the largest tile spills)
+            for (int i = 0; i < (FB * 32 / ROUND + KS - 1) / KS; ++i) {
+                const int r = (i * KS + part) * ROUND + lane / LANES;
+                if (r >= FB * 32) return;
+                float4_t lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const char *from = KS > 1 ? lds + (s * C::NW + wave) * C::OUT_WAVE : stage;
-                const float4_t a = *(const float4_t *)(from + r * (PIECES * 16) + ((pc ^ swz(r)) << 4));
-                const float4_t b = *(const float4_t *)(from + r * (PIECES * 16) + (((pc + 1) ^ swz(r)) << 4));
-                lo = s ? lo + a : a;
-                hi = s ? hi + b : b;
-            }
-            float v[8];
-            *(float4_t *)v = lo;
-            *(float4_t *)(v + 4) = hi;
-            const int m = m0 + wm * FB * 32 + r, n = n0 + (wn * FA + a0) * 32 + pc * 4;
-            if (p.slices > 1) {
-                if (m < p.M && n < p.N) {
-                    float *part = p.part + ((int64_t)slice * p.M + m) * p.part_ld + n;
-                    *(float4_t *)part = *(float4_t *)v;
-                    *(float4_t *)(part + 4) = *(float4_t *)(v + 4);
+                for (int s = 0; s < KS; ++s) {
+                    const char *from = KS > 1 ? lds + (s * C::NW + wave) * C::OUT_WAVE : stage;
+                    const float4_t a = *(const float4_t *)(from + r * (PIECES * 16) + ((pc ^ swz(r)) << 4));
+                    const float4_t b = *(const float4_t *)(from + r * (PIECES * 16) + (((pc + 1) ^ swz(r)) << 4));
+                    lo = s ? lo + a : a;
+                    hi = s ? hi + b : b;
                 }
-            } else {
-                finish8<T, O>(p, m, n, v);
+                float v[8];
+                *(float4_t *)v = lo;
+                *(float4_t *)(v + 4) = hi;
+                leave(m0 + wm * FB * 32 + r, v);
             }
+        };
+        if (p.slices > 1) {
+            rows([&](int m, const float *v) {
+                if (m >= p.M || n >= p.N) return;
+                float *to = p.part + ((int64_t)slice * p.M + m) * p.part_ld + n;
+                *(float4_t *)to = *(const float4_t *)v;
+                *(float4_t *)(to + 4) = *(const float4_t *)(v + 4);
+            });
+        } else {
+            float bias[8];
+            load_bias8<T>(p, n, bias);
+            with_activation(p.act, [&](auto act) { rows([&](int m, const float *v) { finish8<T, O, decltype(act)::value>(p, m, n, v, bias); }); });
         }
         if (KS > 1 && FA > C::CH) __syncthreads();
         asm volatile("" ::: "memory");
