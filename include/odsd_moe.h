@@ -55,7 +55,9 @@ extern "C" {
  * 112: odsd_moe_shape.max_rows (was reserved, 0 keeps the old meaning), odsd_experts_one_launch
  * 113: odsd_moe_static_init
  * 114: odsd_moe_stack_forward, odsd_moe_stack_forward_events
- * 115: odsd_route_dispatch_host_counts */
+ * 115: odsd_route_dispatch_host_counts
+ * (odsd_linear, odsd_rotary and odsd_verify_drafts came under the same number: a host that may meet an older library looks
+ * their symbols up) */
 #define ODSD_VERSION 115
 
 typedef enum odsd_status {
@@ -375,7 +377,7 @@ int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, co
  *                after the other (query_lens NULL: one each): one per drafted token and one behind the last
  *   draft_tokens int64 [n_drafts]: query_lens[s] - 1 for sequence s;  draft_logits [n_drafts, vocab] of the same type, or
  *                NULL: the draft model's distribution is one-hot at its token
- *   temperature  fp32 [n_seqs], or NULL: temperature_all for all; 0: greedy
+ *   temperature  fp32 [n_seqs], or NULL: temperature_all for all; 0 (and below, and NaN): greedy
  *   accept_u     fp32 [n_drafts], sample_u fp32 [n_seqs]: random numbers in [0, 1)
  * With p_j = softmax(logits_j / T), q_j = softmax(draft_logits_j / T): draft j is kept while accept_u_j < min(1, p_j(d_j) /
  * q_j(d_j)); after the kept ones comes a token drawn with sample_u from max(p_j - q_j, 0) at the first draft j that is not
@@ -385,8 +387,8 @@ int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, co
  * vocabulary is not kept; a row with no number above -inf keeps no draft and draws -1.
  *   tokens       int64 [n_seqs, max_q_len]: the kept drafts, the drawn token, -1 behind it
  *   num_accepted int32 [n_seqs];  accept_probs fp32 [n_drafts]: min(1, p / q) of every draft, kept or not
- * max_q_len bounds query_lens (a longer sequence has its first max_q_len rows verified).  A sequence with query_lens 0 gets
- * -1 only.  workspace: odsd_verify_workspace_bytes(...) bytes (0: sizes out of range), 16-byte aligned.
+ * max_q_len bounds query_lens (a longer sequence has its first max_q_len rows verified; 0: nothing is done or written).  A
+ * sequence with query_lens 0 gets -1 only.  Without drafts and with as many rows as sequences query_lens is not read.  workspace: odsd_verify_workspace_bytes(...) bytes (0: sizes out of range), 16-byte aligned.
  * Stands in for the acceptance of a verify step (demo/src/execution/cb_executor.py:261-300) in the sampled form of
  * pre_exp/moe_spec_acc_rate_benchmark/spec_sampling.py:3-198. */
 int odsd_verify_drafts(const void *logits, int64_t logits_stride, const void *draft_logits,

@@ -9,7 +9,7 @@
 //
 // What a token is drawn from is fp64: a cumulative sum over 100 000 tokens in fp32 has borders that are off by more than many
 // tokens' probability, and p - q of two good models is a small difference; in fp64 a token depends on the order of the sums
-// and the accuracy of exp (2e-13) with a probability of about 1e-11 a draw.  Only the row that a sequence draws from needs
+// and the accuracy of exp (4e-14) with a probability of about 1e-11 a draw.  Only the row that a sequence draws from needs
 // that; whether a draft is kept takes the statistics of every row, and those are one pass in fp32: exp2 by the hardware (1 ulp)
 // of an argument to 48 bits, sums in fp32 over 4 logits and by a tree over 32, in fp64 above that.  A sum is off by less than
 // 2^-23 + 6 2^-24 relative, plus 17 ln 2 2^-24 where l - top is not exact (16-bit logits 2^16 times below the largest).
@@ -64,20 +64,30 @@ struct VerifyParams {
     Choice *choice;                 // [S]
 };
 
-// 2^t for t <= 0, not far below -1100: 2^n by the exponent, 2^f, |f| <= 1/2, by its interpolation at the ten Chebyshev points of the
-// interval (degree 9, 1.9e-14 relative)
+// 2^t for t <= 0, not far below -1100: 2^n by the exponent, 2^f, |f| <= 1/2, as 1 + f P(f), P the interpolation of
+// (2^f - 1) / f at the nine Chebyshev points of the interval (3.7e-14 relative).  2^0 is exactly 1: equal logits weigh the same
+// whole number, so sums of them are exact.
+#define EXP2_1 0.6931471805599453
+#define EXP2_2 0.2402265069581299
+#define EXP2_3 0.055504108664760424
+#define EXP2_4 0.009618129159402558
+#define EXP2_5 0.0013333558179043112
+#define EXP2_6 0.00015403455852453838
+#define EXP2_7 1.525268684626772e-05
+#define EXP2_8 1.3255224878668817e-06
+#define EXP2_9 1.0203121063391729e-07
 __device__ __forceinline__ double exp2_neg(double t) {
     const double n = rint(t), f = t - n;
-    double e = 1.0205905413765595e-07;
-    e = fma(e, f, 1.325964524488711e-06);
-    e = fma(e, f, 1.5252672924850737e-05);
-    e = fma(e, f, 0.0001540343375125101);
-    e = fma(e, f, 0.0013333558200794592);
-    e = fma(e, f, 0.009618129193934313);
-    e = fma(e, f, 0.05550410866465167);
-    e = fma(e, f, 0.2402265069564034);
-    e = fma(e, f, 0.6931471805599462);
-    e = fma(e, f, 1.0000000000000135);
+    double e = EXP2_9;
+    e = fma(e, f, EXP2_8);
+    e = fma(e, f, EXP2_7);
+    e = fma(e, f, EXP2_6);
+    e = fma(e, f, EXP2_5);
+    e = fma(e, f, EXP2_4);
+    e = fma(e, f, EXP2_3);
+    e = fma(e, f, EXP2_2);
+    e = fma(e, f, EXP2_1);
+    e = fma(e, f, 1.0);
     return ldexp(e, (int)n);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {      // a NaN counts as nothing
@@ -109,9 +119,7 @@ struct Weigh {
         plain = __builtin_amdgcn_readfirstlane(plain);
     }
     template <typename R> __device__ __forceinline__ void operator()(const R &r, double *w) const {
-        const double c[10] = {1.0000000000000135, 0.6931471805599462, 0.2402265069564034, 0.05550410866465167,
-                              0.009618129193934313, 0.0013333558200794592, 0.0001540343375125101,
-                              1.5252672924850737e-05, 1.325964524488711e-06, 1.0205905413765595e-07};
+        const double c[10] = {1.0, EXP2_1, EXP2_2, EXP2_3, EXP2_4, EXP2_5, EXP2_6, EXP2_7, EXP2_8, EXP2_9};
         double f[8], n[8];
         if (plain) {
 #pragma unroll
@@ -236,8 +244,8 @@ __device__ __forceinline__ void better(float &top, int &at, float t2, int a2) {
 
 __device__ __forceinline__ float temperature_of(const VerifyParams &p, int s) { return p.temperature ? p.temperature[s] : p.temperature_all; }
 __device__ __forceinline__ int len_of(const VerifyParams &p, int s) { return p.query_lens ? max(p.query_lens[s], 0) : 1; }
-// log2(e) / T; 0 says greedy
-__device__ __forceinline__ double factor_of(float t) { return t > 0.0f ? 1.4426950408889634074 / (double)t : 0.0; }
+// log2(e) / T; 0 says greedy (an infinite T: all finite logits alike)
+__device__ __forceinline__ double factor_of(float t) { return t > 0.0f ? fmax(1.4426950408889634074 / (double)t, 1e-300) : 0.0; }
 
 // rows of fewer than 8 logits, as rows of 8
 template <typename T>

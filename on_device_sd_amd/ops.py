@@ -236,7 +236,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         raise ValueError(f"activation {activation!r} is none of {list(_ACTIVATIONS)}")
     shape = x.shape
     N, K = weight.shape
-    if not shape or shape[-1] != K:
+    if not shape or shape[-1] != K or K == 0:
         raise ValueError(f"x {tuple(shape)} and weight {tuple(weight.shape)} do not belong together")
     out_shape = shape[:-1] + (N,)
     bp = rp = None

@@ -34,7 +34,8 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
     token and one behind the last.  ``draft_tokens`` [n_drafts]: those tokens, sequence after sequence; ``draft_logits``
     [n_drafts, vocab] in the dtype of logits: what they were drawn from (None: each was certain, an n-gram table's or a
     greedy draft).  ``accept_u`` float32 [n_drafts], ``sample_u`` float32 [n_seqs]: random numbers in [0, 1).
-    ``temperature``: one number or float32 [n_seqs], 0 for greedy; it divides both models' logits.
+    ``temperature``: one number or float32 [n_seqs], 0 (in a tensor also what is below, or NaN) for greedy; it divides both
+    models' logits.
 
     Draft j of a sequence is kept while accept_u_j < min(1, p_j / q_j) of its token; then one token is drawn, from
     max(p - q, 0) at the first draft that is not kept, or from p behind the last: the lowest token whose cumulative weight
@@ -93,7 +94,7 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
     else:
         t_all = float(temperature)
         if not t_all >= 0.0:
-            raise ValueError(f"temperature {temperature} is negative")
+            raise ValueError(f"temperature {temperature} is negative or no number")
     logits, ld = _rows(logits, rows, vocab)
     if draft_tokens is not None:
         if draft_tokens.dtype != torch.int64:
@@ -105,7 +106,9 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
     out = VerifyResult(torch.empty((n_seqs, longest), dtype=torch.int64, device=device),
                        torch.empty(n_seqs, dtype=torch.int32, device=device),
                        torch.empty(n_drafts, dtype=torch.float32, device=device))
-    if n_seqs == 0:
+    if n_seqs == 0 or longest == 0:
+        out.num_accepted.zero_()
+        out.accept_probs.zero_()
         return out
     lib = _lib.load()
     nbytes = lib.odsd_verify_workspace_bytes(n_seqs, longest, rows, n_drafts, vocab, 0 if draft_logits is None else 1)

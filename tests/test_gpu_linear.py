@@ -146,13 +146,24 @@ def test_leading_dimensions_single_rows_and_empty(dev):
     assert torch.equal(ops.linear(x[0, :1].expand(5, 64), w), ops.linear(x[0, :1].repeat(5, 1), w))
 
 
+def test_rows_far_apart(dev):
+    """Rows 2^21 elements apart and more do not fit the tiles' 32-bit offsets: another kernel takes them."""
+    g = torch.Generator(device=dev).manual_seed(2)
+    far = torch.randn(70, 1 << 21, generator=g, device=dev, dtype=torch.float16)
+    x, w = far[:, :256], torch.randn(96, 256, generator=g, device=dev).half()
+    assert torch.equal(ops.linear(x[:3], w), ops.linear(x[:3].clone(), w))
+    for a, b in ((x, w), (w, x)):
+        y, z = ops.linear(a, b, out_dtype=torch.float32).double(), a.double() @ b.double().t()
+        assert ((y - z).abs() <= 32 * 2.0 ** -23 * (a.double().abs() @ b.double().abs().t())).all()
+
+
 def test_refusals(dev):
     x, w = torch.randn(4, 64, device=dev).half(), torch.randn(8, 64, device=dev).half()
     for bad in (lambda: ops.linear(x.float(), w.float()), lambda: ops.linear(x, w.bfloat16()), lambda: ops.linear(x, w, w[0, :8].float()),
                 lambda: ops.linear(x, w, out_dtype=torch.bfloat16)):
         with pytest.raises(TypeError):
             bad()
-    for bad in (lambda: ops.linear(x[:, :32], w), lambda: ops.linear(x, w, x[0, :7]), lambda: ops.linear(x, w, activation="tanh"),
+    for bad in (lambda: ops.linear(x[:, :32], w), lambda: ops.linear(x[:, :0], w[:, :0]), lambda: ops.linear(x, w, x[0, :7]), lambda: ops.linear(x, w, activation="tanh"),
                 lambda: ops.linear(x, w, residual=x[:, :7]), lambda: ops.linear(x, w, residual=x[:, :8].float())):
         with pytest.raises(ValueError):
             bad()

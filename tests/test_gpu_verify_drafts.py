@@ -125,6 +125,26 @@ def test_empty_sequences_and_wider_tokens(dev):
     assert r.tokens[0].tolist() == [-1] * 5 and r.tokens[5].tolist() == [-1] * 5
 
 
+def test_no_rows_at_all(dev):
+    none = torch.zeros(0, device=dev)
+    ctx = {"verify_query_lens": torch.zeros(2, dtype=torch.int32, device=dev), "max_query_len": 0}
+    r = odsd.verify_drafts(torch.zeros(0, 10, device=dev), None, ctx, None, torch.rand(2, device=dev))
+    assert r.tokens.shape == (2, 0) and r.num_accepted.tolist() == [0, 0] and r.accept_probs.numel() == 0
+    ctx["max_query_len"] = 3
+    r = odsd.verify_drafts(torch.zeros(0, 10, device=dev), none.long(), ctx, none, torch.rand(2, device=dev))
+    assert r.tokens.tolist() == [[-1] * 3] * 2 and r.num_accepted.tolist() == [0, 0]
+
+
+def test_infinite_temperature_is_uniform(dev):
+    x = torch.randn(5, 40, device=dev)
+    x[:, ::4] = -float("inf")
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.999], device=dev)
+    r = odsd.verify_drafts(x, None, {}, None, u, temperature=torch.full((5,), float("inf"), device=dev))
+    free = [i for i in range(40) if i % 4]
+    assert r.tokens[:, 0].tolist() == [free[int(v * 30)] for v in (0.0, 0.25, 0.5, 0.75, 0.999)]
+    assert torch.equal(odsd.verify_drafts(x, None, {}, None, u, temperature=float("inf")).tokens, r.tokens)
+
+
 def test_longer_sequences_than_stated(dev):
     """max_query_len below a length: its first rows are verified, as far as they go; nothing is written elsewhere."""
     m = make([5, 3], 400, "fp32", seed=9)
