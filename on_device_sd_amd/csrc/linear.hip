@@ -327,7 +327,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
                 if (r * NM / NR == i) read((j + 1) & 1, last ? next : cur, last ? 0 : j + 1, r);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                if (c * NM / NC == i) copy(last ? step + STAGES : step + STAGES - 1, last ? cur : left, last ? c : EARLY + c);
+                if (c * NM / (NC ? NC : 1) == i) copy(last ? step + STAGES : step + STAGES - 1, last ? cur : left, last ? c : EARLY + c);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -526,6 +526,20 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
     for (int r = row; r < 64; r += 32) finish8<T, O>(p, m0 + r, n0 + col, ys + r * 68 + col);
 }
 
+// Rows of x and of w whose K is no multiple of 8, as rows that are one (zeros behind K): 16 bytes a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pack_kernel(LinearParams p, T *x, T *w, int Kp) {
+    const int per_row = Kp / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
+    const int k = (int)(i - row * per_row) * 8;
+    if (row >= (int64_t)p.M + p.N) return;
+    const T *src = row < p.M ? (const T *)p.x + row * p.ldx : (const T *)p.w + (row - p.M) * p.ldw;
+    uint4_t v;
+    if (k + 8 <= p.K) __builtin_memcpy(&v, src + k, 16);
+    else v = load8_short(src, k, p.K);
+    *(uint4_t *)((row < p.M ? x + row * Kp : w + (row - p.M) * Kp) + k) = v;
+}
+
 // ---- which kernel ------------------------------------------------------------------------------
 // tiles n x m; K4, K2: K shared by groups of wavefronts of the workgroup
 enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_32_64_K4, LIN_TILE_32_64_K2, LIN_TILE_128_32, LIN_TILE_128_64, LIN_TILE_64_64,
@@ -535,6 +549,7 @@ static const int TILE_M[LIN_KINDS] = {16, 64, 64, 64, 32, 64, 64, 128, 256};
 struct LinearPlan {
     int kind, slices, slice_k;
     int64_t part_ld;
+    int Kp;            // not 0: x and w are packed into rows of this many columns first
     size_t bytes;      // of workspace
     bool fits;         // the launch's workgroups are counted in 31 bits
 };
@@ -548,16 +563,18 @@ static LinearPlan linear_plan_of(int kind, int slices, int M, int N, int K) {
     l.slice_k = per * 64;
     l.slices = (steps + per - 1) / per;
     l.part_ld = ((int64_t)N + 7) / 8 * 8;
+    l.Kp = 0;
     l.fits = linear_tiles(kind, M, N) * l.slices <= 0x7ffffff0LL;
     l.bytes = l.slices > 1 ? (size_t)l.slices * M * l.part_ld * 4 : 0;
     return l;
 }
-static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
-    // Up to 4 tokens one pass over the weights' rows, also where their segments are not aligned (up to 16, there).  us, rows /
-    // the tiles that follow: M = 1: K 4096, N 2048 7.1 / 11.0, K 2048, N 131072 93 / 100; M = 4: K 2048, N 5120 8.3 / 8.0;
-    // M = 16: K 2048, N 5120 10.0 / 8.0, N 131072 123 / 105.
-    if (M <= 4 || (M <= 16 && !aligned)) return linear_plan_of(LIN_ROWS, 1, M, N, K);
-    if (!aligned) return linear_plan_of(LIN_ANY, 1, M, N, K);
+static size_t linear_packed_bytes(int rows, int Kp) { return odsd_round_up((size_t)rows * Kp * 2, 256); }
+// For operands whose rows are whole 16-byte segments; *us: about how long it takes.
+static LinearPlan linear_plan_aligned(int M, int N, int K, float *us) {
+    *us = 8.0f + (float)N * K * 2 / 4.5e6f;
+    // Up to 4 tokens one pass over the weights' rows.  us, rows / the tiles that follow: M = 1: K 4096, N 2048 7.1 / 11.0, K
+    // 2048, N 131072 93 / 100; M = 4: K 2048, N 5120 8.3 / 8.0; M = 16: K 2048, N 5120 10.0 / 8.0, N 131072 123 / 105.
+    if (M <= 4) return linear_plan_of(LIN_ROWS, 1, M, N, K);
     const int steps = (K + 63) / 64;
     // Up to 64 tokens the weights' bytes count, and how many of them are on their way.  While 32-row tiles are at most one
     // (two) per CU, K is shared inside the workgroup, in one launch; beyond that, as many tokens in a tile as there are, and
@@ -581,20 +598,42 @@ static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
     static const float STEP[LIN_KINDS] = {0, 0, 0, 0, 0, 0.68f, 0.42f, 1.06f, 1.58f};
     static const float END[LIN_KINDS] = {0, 0, 0, 0, 0, 2.0f, 1.5f, 4.0f, 10.0f};
     LinearPlan best = {};
-    float best_us = 0.0f;
+    float best_us = 0.0f;              // (without the launch)
     for (int kind = LIN_TILE_128_64; kind <= LIN_TILE_256_256; ++kind) {
         const int64_t slots = kind == LIN_TILE_256_256 ? 256 : 512;
         for (int slices = 1; slices <= 8 && (slices == 1 || steps / slices >= 8); slices *= 2) {
             const LinearPlan l = linear_plan_of(kind, slices, M, N, K);
             const float rounds = (float)((linear_tiles(kind, M, N) * l.slices + slots - 1) / slots);
-            const float us = rounds * (l.slice_k / 64 * STEP[kind] + END[kind]) + (l.slices > 1 ? 4.0f + l.bytes / 2e6f : 0.0f);
-            if (best_us == 0.0f || us < best_us) {
-                best_us = us;
+            const float t = rounds * (l.slice_k / 64 * STEP[kind] + END[kind]) + (l.slices > 1 ? 4.0f + l.bytes / 2e6f : 0.0f);
+            if (best_us == 0.0f || t < best_us) {
+                best_us = t;
                 best = l;
             }
         }
     }
+    *us = 2.0f + best_us;
     return best;
+}
+static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
+    float us;
+    if (aligned) return linear_plan_aligned(M, N, K, &us);
+    if (M <= 16) return linear_plan_of(LIN_ROWS, 1, M, N, K);
+    // Columns that are no whole number of segments: both operands are packed into such rows first, which costs their bytes
+    // twice and a launch, where the tiles win more than that over the kernel for any shape (0.8 us a step and round of 512
+    // workgroups).  us, that kernel / packed: K 3809: M = 20, N 5000 46 / 33, M = 453, N 768 42 / 25; K 2047: M = 65, N 65536
+    // 127 / 172, M = 1000, N 5000 75 / 41; K 4095, M = 8192, N 4096 694 / 255.
+    if (K % 8 != 0 && K < (1 << 21) - 8) {
+        const int Kp = (K + 7) / 8 * 8;
+        LinearPlan l = linear_plan_aligned(M, N, Kp, &us);
+        const float pack = 4.0f + ((float)M + (float)N) * K * 4 / 4.5e6f;
+        const float any = (float)((linear_tiles(LIN_ANY, M, N) + 511) / 512) * ((K + 63) / 64) * 0.8f;
+        if (us + pack < any && l.fits && ((int64_t)M + N) * (Kp / 8) / 256 <= 0x7fffff00LL) {
+            l.Kp = Kp;
+            l.bytes = odsd_round_up(l.bytes, 256) + linear_packed_bytes(M, Kp) + linear_packed_bytes(N, Kp);
+            return l;
+        }
+    }
+    return linear_plan_of(LIN_ANY, 1, M, N, K);
 }
 
 template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS = 1>
@@ -624,6 +663,15 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
         ODSD_CHECK_LAUNCH();
         return ODSD_OK;
     }
+    if (l.Kp) {
+        const size_t parts = odsd_round_up(l.slices > 1 ? (size_t)l.slices * p.M * l.part_ld * 4 : 0, 256);
+        T *x = (T *)((char *)workspace + parts), *w = (T *)((char *)x + linear_packed_bytes(p.M, l.Kp));
+        const int64_t units = ((int64_t)p.M + p.N) * (l.Kp / 8);
+        linear_pack_kernel<T><<<(unsigned)((units + 255) / 256), 256, 0, st>>>(p, x, w, l.Kp);
+        p.x = x;
+        p.w = w;
+        p.ldx = p.ldw = p.K = l.Kp;
+    }
     p.slices = l.slices;
     p.slice_k = l.slice_k;
     p.part = (float *)workspace;
@@ -650,7 +698,7 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
 
 extern "C" size_t odsd_linear_workspace_bytes(int32_t M, int32_t N, int32_t K) {
     if (M < 0 || N <= 0 || K <= 0) return 0;
-    const LinearPlan l = linear_plan(M, N, K, true);
+    const LinearPlan l = linear_plan(M, N, K, K % 8 == 0);      // (pointers that are not aligned need no more)
     return !l.fits ? 0 : l.bytes > 256 ? l.bytes : 256;
 }
 

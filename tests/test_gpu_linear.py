@@ -72,7 +72,8 @@ def test_types_and_activations(dev, M, act, dtype, out):
     run(dev, M, 256, 320, dtype, out, act, bias=False, residual=False, seed=M + 1, scale=0.4)
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 2049, 65), (4, 333, 100), (16, 1111, 514), (50, 777, 201), (130, 513, 260), (400, 1027, 300)])
+@pytest.mark.parametrize("M,K,N", [(1, 2049, 65), (4, 333, 100), (16, 1111, 514), (50, 777, 201), (130, 513, 260), (400, 1027, 300),
+                                   (20, 3809, 700), (300, 2999, 520), (70, 2047, 9000), (257, 9, 257), (600, 4100, 1030)])
 def test_odd_columns(dev, M, K, N):
     run(dev, M, K, N, "bf16")
     run(dev, M, K, N, "fp16", "fp32", "gelu")
