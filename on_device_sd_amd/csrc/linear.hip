@@ -258,14 +258,15 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
     __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
     const int lane = lane_id(), any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = any_wave % C::NW, part = any_wave / C::NW;      // of a share of K, and which share
-    // neighbouring tiles on one XCD (workgroup i is on XCD i % 8), in groups of up to 8 along m that share their weights
+    // neighbouring tiles on one XCD (workgroup i is on XCD i % 8), in groups of up to 6 along m that share their weights: 6 x 5
+    // of the 32 tiles that its CUs have at once (8 x 4: 8192 x 4096 x 16384 3 % slower, other shapes within 1 %)
     const int total = p.tiles_n * p.tiles_m * p.slices, per = (total + 7) / 8;
     const int b = blockIdx.x, t0 = (b & 7) * per + (b >> 3);
     if ((b >> 3) >= per || t0 >= total) return;
     const int slice = t0 / (p.tiles_n * p.tiles_m), t = t0 - slice * (p.tiles_n * p.tiles_m);
-    const int group = t / (8 * p.tiles_n), in_group = t - group * 8 * p.tiles_n;
-    const int gm = min(8, p.tiles_m - group * 8);
-    const int n0 = in_group / gm * C::TN, m0 = (group * 8 + in_group % gm) * C::TM;
+    const int group = t / (6 * p.tiles_n), in_group = t - group * 6 * p.tiles_n;
+    const int gm = min(6, p.tiles_m - group * 6);
+    const int n0 = in_group / gm * C::TN, m0 = (group * 6 + in_group % gm) * C::TM;
 
     const int k_begin = slice * p.slice_k, k_end = min(p.K, k_begin + p.slice_k);
     const int steps = (k_end - k_begin + BK * KS - 1) / (BK * KS);   // of a share: every KS-th
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
     // 16 columns: their products, and between those, one by one, the reads of the next 16 columns' fragments and the copies
     // of the step that comes into the buffer that was left last.  (The compiler would request a fragment right before its
     // use, and copies in a row stall the wavefront: a CU takes one per 16 cycles.)
-    constexpr int J = BK / 16, NM = FA * FB, NR = FA + FB, EARLY = (C::L + 1) / 2;
+    constexpr int J = BK / 16, NM = FA * FB, NR = FA + FB, EARLY = C::L * 3 / 4;
     auto columns = [&](auto jc, int step, uint32_t cur, uint32_t next, uint32_t left) {
         constexpr int j = decltype(jc)::value;
         constexpr bool last = j == J - 1;
