@@ -90,12 +90,16 @@ __device__ __forceinline__ double exp2_neg(double t) {
     e = fma(e, f, 1.0);
     return ldexp(e, (int)n);
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {      // a NaN counts as nothing
+__device__ __forceinline__ float max3(float a, float b, float c) {      // a NaN in front of numbers counts as nothing
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
-__device__ __forceinline__ float number(float l) { return l == l ? l : -INFINITY; }
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
+    float r;
+    asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // exp((l - top) / T).  A row whose largest logit is +inf has its weight on the +inf entries; one without any number has none.
 __device__ __forceinline__ double weight_of(float l, float top, double k) {
     if (top == INFINITY) return l == INFINITY ? 1.0 : 0.0;
@@ -185,12 +189,17 @@ template <typename T> struct Raw8 {
         }
     }
 };
+// The largest of eight, NaN none of them.  (Told by the bits: a signalling NaN as an operand of the hardware's ordinary maximum
+// makes the result NaN, and the other operand is lost.)
 template <typename T> __device__ __forceinline__ float largest8(const Raw8<T> &r) {
-    const float t = max3(max3(r.get(0), r.get(1), r.get(2)), max3(r.get(3), r.get(4), r.get(5)), max3(r.get(6), r.get(7), -INFINITY));
+    const float t = max3_or_nan(max3_or_nan(r.get(0), r.get(1), r.get(2)), max3_or_nan(r.get(3), r.get(4), r.get(5)), max3_or_nan(r.get(6), r.get(7), -INFINITY));
     if (t == t) return t;
-    float m = -INFINITY;                                                // (signalling NaN come back from the hardware's maximum)
+    float m = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, number(r.get(j)));
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t bits = __float_as_uint(r.get(j));
+        m = fmaxf(m, __uint_as_float((bits & 0x7fffffffu) > 0x7f800000u ? 0xff800000u : bits));
+    }
     return m;
 }
 
@@ -229,7 +238,9 @@ __device__ __forceinline__ double last_lane(double v) {
 }
 template <typename V> __device__ __forceinline__ V plus(V a, V b) { return a + b; }
 __device__ __forceinline__ double all_sum(double v) { return last_lane(scan_all(v, 0.0, plus<double>)); }
-__device__ __forceinline__ int all_sum(int v) { return last_lane(scan_all(v, 0, plus<int>)); }
+// (modulo 2^32: lengths are the caller's)
+__device__ __forceinline__ int wrapping_plus(int a, int b) { return (int)((uint32_t)a + (uint32_t)b); }
+__device__ __forceinline__ int all_sum(int v) { return last_lane(scan_all(v, 0, wrapping_plus)); }
 __device__ __forceinline__ float all_max(float v) { return last_lane(scan_all(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); })); }
 __device__ __forceinline__ int all_min(int v) { return last_lane(scan_all(v, 0x7fffffff, [](int a, int b) { return min(a, b); })); }
 __device__ __forceinline__ int all_max(int v) { return last_lane(scan_all(v, -0x7fffffff - 1, [](int a, int b) { return max(a, b); })); }
@@ -263,10 +274,10 @@ __device__ __forceinline__ int sequence_of(const VerifyParams &p, int r, bool dr
         const int s = s0 + lane_id();
         int n = s < p.S ? len_of(p, s) : 0;
         if (draft) n = max(n - 1, 0);
-        const int sum = scan_all(n, 0, plus<int>);
-        const uint64_t past = __ballot(before + sum > r);
+        const int sum = scan_all(n, 0, wrapping_plus);
+        const uint64_t past = __ballot(wrapping_plus(before, sum) > r);
         if (past) return s0 + __builtin_ctzll(past);
-        before += last_lane(sum);
+        before = wrapping_plus(before, last_lane(sum));
     }
     return -1;
 }
@@ -341,7 +352,7 @@ __global__ __launch_bounds__(VER_THREADS) void verify_stats_kernel(VerifyParams 
 #pragma unroll 1
             for (int i = 0; i < 32; ++i) {
                 const int at = first + (i >> 3) * (VER_THREADS * 8) + (i & 7);
-                if (at < p.V) z += weight_of(number((float)src[at]), top, k);
+                if (at < p.V) z += weight_of((float)src[at], top, k);
             }
         }
         z = all_sum(z);
@@ -396,8 +407,8 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
     if (p.query_lens) {
         for (int i = threadIdx.x; i < s; i += VER_THREADS) {
             const int n = len_of(p, i);
-            start += n;
-            dstart += max(n - 1, 0);
+            start = wrapping_plus(start, n);
+            dstart = wrapping_plus(dstart, max(n - 1, 0));
         }
         start = all_sum(start);
         dstart = all_sum(dstart);
@@ -406,15 +417,18 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
             s_dstart[wave] = dstart;
         }
         __syncthreads();
-        start = s_start[0] + s_start[1] + s_start[2] + s_start[3];
-        dstart = s_dstart[0] + s_dstart[1] + s_dstart[2] + s_dstart[3];
+        start = wrapping_plus(wrapping_plus(s_start[0], s_start[1]), wrapping_plus(s_start[2], s_start[3]));
+        dstart = wrapping_plus(wrapping_plus(s_dstart[0], s_dstart[1]), wrapping_plus(s_dstart[2], s_dstart[3]));
+        // behind the last row, however far (lengths that do not belong to these rows): the sequence has none
+        if ((uint32_t)start > (uint32_t)p.n_q) start = p.n_q;
+        if ((uint32_t)dstart > (uint32_t)p.n_d) dstart = p.n_d;
     } else {
         start = s;
     }
     // rows and drafts that are really there; drafts that no row verifies are not kept
     const int n = max(min(min(min(len, p.max_q), p.n_q - start), p.n_d - dstart + 1), 0);
     if (writes) {
-        const int d_end = s == p.S - 1 ? p.n_d : min(dstart + max(len - 1, 0), p.n_d);
+        const int d_end = s == p.S - 1 ? p.n_d : dstart + min(max(len - 1, 0), p.n_d - dstart);
         for (int j = dstart + max(n - 1, 0) + (int)threadIdx.x; j < d_end; j += VER_THREADS) p.accept_probs[j] = 0.0f;
     }
     const double k = factor_of(t);
@@ -754,7 +768,7 @@ static bool verify_layout(int64_t S, int64_t n_q, int64_t n_d, int64_t V, bool d
     l.choice = take((size_t)S * sizeof(Choice));
     l.padded = take(V < 8 ? (size_t)(n_q + n_d) * 8 * 4 : 0);
     l.total = o;
-    return (n_q + n_d) * l.splits <= 0x7fffffffLL && S <= 65535;
+    return (n_q + n_d) * l.splits < (1LL << 32) / VER_THREADS && S <= 65535;      // a launch has fewer than 2^32 threads
 }
 static bool verify_sizes_ok(int32_t S, int32_t max_q, int32_t n_q, int32_t n_d, int32_t V) {
     return S >= 0 && max_q >= 0 && n_q >= 0 && n_d >= 0 && V > 0;

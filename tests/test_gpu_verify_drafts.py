@@ -104,6 +104,21 @@ def test_masked_rows(dev, dtype):
     check(dev, m)
 
 
+@pytest.mark.parametrize("dtype,bits,raw", [("fp32", 0x7fa00000, torch.int32), ("bf16", 0x7f81, torch.int16), ("fp16", 0x7d01, torch.int16)])
+@pytest.mark.parametrize("with_q", [True, False])
+def test_signalling_nan_counts_as_nothing(dev, dtype, bits, raw, with_q):
+    m = make([3, 2, 1], 2000, dtype, seed=31, with_q=with_q)
+    for t in (m["logits"], m["draft_logits"]):
+        if t is not None:
+            t.view(raw)[:, 5::7] = bits
+            assert torch.isnan(t[:, 5::7]).all()
+    m["logits"].view(raw)[5, 700:1999] = bits
+    for u in (0.3, 0.999999):
+        m["accept_u"][:] = u
+        check(dev, m)
+    check(dev, m, 0.0)
+
+
 def test_drafts_outside_the_vocabulary_and_equal_models(dev):
     m = make([4, 4, 2], 700, "fp32", seed=3)
     m["drafts"][1], m["drafts"][4], m["drafts"][6] = 700, -1, 2 ** 40
@@ -155,6 +170,41 @@ def test_longer_sequences_than_stated(dev):
     w = orc.verify(full["logits"].double().numpy()[5:], full["drafts"].numpy()[4:], [3], full["accept_u"].numpy()[4:], full["sample_u"].numpy()[1:],
                    full["draft_logits"].double().numpy()[4:])
     assert r.tokens[1].tolist() == w[0][0].tolist()
+
+
+@pytest.mark.parametrize("lens", [[2 ** 30] * 5, [2 ** 31 - 1, 2 ** 31 - 1, 1, 4], [3, 2 ** 31 - 1, 2 ** 31 - 1, 5]])
+def test_lengths_that_do_not_belong_to_the_rows(dev, lens):
+    """Lengths on the device are not checked; the first sequence's rows are verified as far as there are any, nobody else's are
+    taken for it, and sums of lengths past 31 bits find no row."""
+    m = make([4, 4], 300, "fp32", seed=14)
+    ctx = {"verify_query_lens": torch.tensor(lens, dtype=torch.int32, device=dev), "max_query_len": 3}
+    su = torch.rand(len(lens), device=dev)
+    for q in (m["draft_logits"].to(dev), None):
+        r = odsd.verify_drafts(m["logits"].to(dev), m["drafts"].to(dev), ctx, m["accept_u"].to(dev), su, draft_logits=q,
+                               temperature=torch.full((len(lens),), 0.8, device=dev))
+        tokens = r.tokens.cpu()
+        assert (tokens >= -1).all() and (tokens < 300).all() and tokens[0, 0] >= 0 and (r.num_accepted <= 2).all()
+        if lens[0] > 3:
+            assert (tokens[1] == -1).all()
+
+
+def test_two_calls_at_once(dev):
+    """Calls on two streams have workspaces of their own."""
+    ms = [make([4, 2, 5], 70000, "bf16", seed=s) for s in (41, 42)]
+    args = [{k: v.to(dev) for k, v in m.items() if k != "lens"} for m in ms]
+    ctx = {"verify_query_lens": torch.tensor([4, 2, 5], dtype=torch.int32, device=dev), "max_query_len": 5}
+    call = lambda a: odsd.verify_drafts(a["logits"], a["drafts"], ctx, a["accept_u"], a["sample_u"], draft_logits=a["draft_logits"], temperature=0.8)  # noqa: E731
+    alone = [call(a) for a in args]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in ms], [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(args[i]))
+    torch.cuda.synchronize()
+    for want, rs in zip(alone, got):
+        for r in rs:
+            assert torch.equal(r.tokens, want.tokens) and torch.equal(r.accept_probs, want.accept_probs)
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
