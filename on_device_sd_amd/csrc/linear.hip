@@ -212,24 +212,24 @@ __global__ __launch_bounds__(NWV * 64) void linear_rows_kernel(LinearParams p) {
 }
 
 // ---- tiles -----------------------------------------------------------------------------------
-// NWN x NWM wavefronts, each FA blocks of 32 n by FB blocks of 32 m on v_mfma_f32_32x32x16; steps of BK along K.  Both
+// NWN x NWM wavefronts, each FA blocks of 32 n by FB blocks of 32 m on v_mfma_f32_32x32x16; steps of 64 along K.  Both
 // operands go to LDS without passing registers (buffer_load ... lds, 16 bytes a lane), STAGES buffers of them; a buffer's
-// rows are 128 bytes (64 with steps of 32), whose 16-byte segments are XORed with bits of the row's number: the 16 lanes that
+// rows are 128 bytes, whose 16-byte segments are XORed with bits of the row's number: the 16 lanes that
 // read together (rows 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of a block, one segment) then meet the 16 bank groups.  What is behind a row's end, the matrix's last row or the slice's
 // last step is addressed outside the buffer descriptor and arrives as zeros, without memory traffic, so every copy is
 // issued whatever follows and a count says which have landed.  KS groups of such wavefronts take every KS-th step each, with
 // buffers of their own, and add their sums up at the end: for few tokens, where a step is a chain of latencies.
-template <int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS>
+template <int NWN, int NWM, int FA, int FB, int STAGES, int KS>
 struct LinearTile {
     static constexpr int NW = NWN * NWM, TN = NWN * FA * 32, TM = NWM * FB * 32;
-    static constexpr int ROW = BK * 2, SEGS = BK / 8, ROWS = 64 / SEGS;      // bytes and 16-byte segments of a row, rows of a copy
+    static constexpr int BK = 64, ROW = BK * 2, SEGS = BK / 8, ROWS = 64 / SEGS;   // bytes and 16-byte segments of a row, rows of a copy
     static constexpr int A_BYTES = TN * ROW, STAGE = (TN + TM) * ROW;
     static constexpr int LA = TN / ROWS / NW, LB = TM / ROWS / NW, L = LA + LB;   // copies of a wavefront per step
     static constexpr int CH = FA < 2 ? FA : 2;                             // blocks of n that leave together
     static constexpr int OUT_WAVE = FB * 32 * CH * 32 * 4;
     static constexpr int LDS = KS * (STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE);
     static_assert(LA * ROWS * NW == TN && LB * ROWS * NW == TM && LB >= 1, "every wavefront makes the same number of copies");
-    static_assert((BK == 64 && NW % 2 == 0) || BK == 32, "the swizzle of a copied row does not depend on the copy");
+    static_assert(NW % 2 == 0, "the swizzle of a copied row does not depend on the copy");
 };
 
 __device__ __forceinline__ void copy16_to_lds(uint4_t rsrc, uint32_t off, uint32_t lds_addr) {
@@ -251,10 +251,11 @@ __device__ __forceinline__ uint4_t descriptor(const void *base, uint32_t bytes) 
     return r;
 }
 
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS>
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES, int KS>
 __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(LinearParams p) {
-    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES, KS> C;
+    typedef LinearTile<NWN, NWM, FA, FB, STAGES, KS> C;
     typedef typename AttnT<T>::V8 V8;
+    constexpr int BK = C::BK;
     __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
     const int lane = lane_id(), any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = any_wave % C::NW, part = any_wave / C::NW;      // of a share of K, and which share
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
     const uint4_t rw = descriptor((const char *)p.w + (int64_t)n0 * p.ldw * 2, (uint32_t)(min(C::TN, p.N - n0) - 1) * ldw + p.K * 2);
     const uint4_t rx = descriptor((const char *)p.x + (int64_t)m0 * p.ldx * 2, (uint32_t)(min(C::TM, p.M - m0) - 1) * ldx + p.K * 2);
     // of the row that a lane copies (the same for all its copies: NW is even)
-    const int seg = BK == 64 ? (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)) : (lane & 3) ^ (lane >> 4);
+    const int seg = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4));
     const uint32_t row0 = wave * C::ROWS + lane / C::SEGS;
     const uint32_t off_w = row0 * ldw + seg * 16, off_x = row0 * ldx + seg * 16;
     char *const mine = lds + part * (C::STAGE * STAGES);
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
     };
 
     const int wn = wave % NWN, wm = wave / NWN;
-    const uint32_t frag = (lane & 31) * C::ROW + (((lane >> 5) ^ (BK == 64 ? (lane >> 1) & 7 : (lane >> 2) & 3)) << 4);
+    const uint32_t frag = (lane & 31) * C::ROW + (((lane >> 5) ^ ((lane >> 1) & 7)) << 4);
     const uint32_t fa0 = wn * FA * 32 * C::ROW + frag, fb0 = C::A_BYTES + wm * FB * 32 * C::ROW + frag;
     float16_t acc[FA][FB];
 #pragma unroll
@@ -348,10 +349,8 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
         if (next == C::STAGE * STAGES) next = 0;
         columns(std::integral_constant<int, 0>{}, step, cur, next, left);
         columns(std::integral_constant<int, 1>{}, step, cur, next, left);
-        if constexpr (J == 4) {
-            columns(std::integral_constant<int, 2>{}, step, cur, next, left);
-            columns(std::integral_constant<int, 3>{}, step, cur, next, left);
-        }
+        columns(std::integral_constant<int, 2>{}, step, cur, next, left);
+        columns(std::integral_constant<int, 3>{}, step, cur, next, left);
         left = cur;
         cur = next;
     }
@@ -547,12 +546,13 @@ enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_32_64_K4, LIN_TILE_32_64_K2, LIN_TILE_128
        LIN_TILE_128_128, LIN_TILE_256_256, LIN_KINDS };
 static const int TILE_N[LIN_KINDS] = {16, 64, 32, 32, 128, 128, 64, 128, 256};
 static const int TILE_M[LIN_KINDS] = {16, 64, 64, 64, 32, 64, 64, 128, 256};
+static const int THREADS[LIN_KINDS] = {1024, 256, 512, 256, 256, 256, 256, 256, 512};
 struct LinearPlan {
     int kind, slices, slice_k;
     int64_t part_ld;
     int Kp;            // not 0: x and w are packed into rows of this many columns first
     size_t bytes;      // of workspace
-    bool fits;         // the launch's workgroups are counted in 31 bits
+    bool fits;         // a launch has fewer than 2^32 threads
 };
 static int64_t linear_tiles(int kind, int M, int N) {
     return (int64_t)((M + TILE_M[kind] - 1) / TILE_M[kind]) * ((N + TILE_N[kind] - 1) / TILE_N[kind]);
@@ -565,7 +565,7 @@ static LinearPlan linear_plan_of(int kind, int slices, int M, int N, int K) {
     l.slices = (steps + per - 1) / per;
     l.part_ld = ((int64_t)N + 7) / 8 * 8;
     l.Kp = 0;
-    l.fits = linear_tiles(kind, M, N) * l.slices <= 0x7ffffff0LL;
+    l.fits = (linear_tiles(kind, M, N) * l.slices + 7) * THREADS[kind] < 1LL << 32;
     l.bytes = l.slices > 1 ? (size_t)l.slices * M * l.part_ld * 4 : 0;
     return l;
 }
@@ -628,7 +628,7 @@ static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
         LinearPlan l = linear_plan_aligned(M, N, Kp, &us);
         const float pack = 4.0f + ((float)M + (float)N) * K * 4 / 4.5e6f;
         const float any = (float)((linear_tiles(LIN_ANY, M, N) + 511) / 512) * ((K + 63) / 64) * 0.8f;
-        if (us + pack < any && l.fits && ((int64_t)M + N) * (Kp / 8) / 256 <= 0x7fffff00LL) {
+        if (us + pack < any && l.fits && ((int64_t)M + N) * (Kp / 8) < (1LL << 32) - 256) {
             l.Kp = Kp;
             l.bytes = odsd_round_up(l.bytes, 256) + linear_packed_bytes(M, Kp) + linear_packed_bytes(N, Kp);
             return l;
@@ -637,9 +637,9 @@ static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
     return linear_plan_of(LIN_ANY, 1, M, N, K);
 }
 
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int BK, int STAGES, int KS = 1>
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES, int KS = 1>
 static void launch_tile(LinearParams &p, hipStream_t st) {
-    typedef LinearTile<NWN, NWM, FA, FB, BK, STAGES, KS> C;
+    typedef LinearTile<NWN, NWM, FA, FB, STAGES, KS> C;
     p.tiles_n = (p.N + C::TN - 1) / C::TN;
     p.tiles_m = (p.M + C::TM - 1) / C::TM;
     // One pass over weights of more than a third of the 256 MB cache: nothing of them is there at the next call, so they do
@@ -647,7 +647,7 @@ static void launch_tile(LinearParams &p, hipStream_t st) {
     // again soon, come out of it (M = 64, K 2048, N 16384 15.0, past it 20.5; not called again 21.1 / 19.6).
     p.w_once = p.tiles_m == 1 && (int64_t)p.N * p.K * 2 >= (96 << 20);
     const int64_t total = (int64_t)p.tiles_n * p.tiles_m * p.slices;
-    linear_tile_kernel<T, O, NWN, NWM, FA, FB, BK, STAGES, KS><<<(unsigned)((total + 7) / 8 * 8), C::NW * KS * 64, 0, st>>>(p);
+    linear_tile_kernel<T, O, NWN, NWM, FA, FB, STAGES, KS><<<(unsigned)((total + 7) / 8 * 8), C::NW * KS * 64, 0, st>>>(p);
 }
 
 template <typename T, typename O> static int launch_linear(LinearParams &p, const LinearPlan &l, void *workspace, hipStream_t st) {
@@ -678,13 +678,13 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
     p.part = (float *)workspace;
     p.part_ld = l.part_ld;
     switch (l.kind) {
-        case LIN_TILE_32_64_K4: launch_tile<T, O, 1, 2, 1, 1, 64, 3, 4>(p, st); break;
-        case LIN_TILE_32_64_K2: launch_tile<T, O, 1, 2, 1, 1, 64, 3, 2>(p, st); break;
-        case LIN_TILE_128_32: launch_tile<T, O, 4, 1, 1, 1, 64, 4>(p, st); break;
-        case LIN_TILE_128_64: launch_tile<T, O, 4, 1, 1, 2, 64, 3>(p, st); break;
-        case LIN_TILE_64_64: launch_tile<T, O, 2, 2, 1, 1, 64, 4>(p, st); break;
-        case LIN_TILE_128_128: launch_tile<T, O, 2, 2, 2, 2, 64, 2>(p, st); break;
-        default: launch_tile<T, O, 2, 4, 4, 2, 64, 2>(p, st); break;
+        case LIN_TILE_32_64_K4: launch_tile<T, O, 1, 2, 1, 1, 3, 4>(p, st); break;
+        case LIN_TILE_32_64_K2: launch_tile<T, O, 1, 2, 1, 1, 3, 2>(p, st); break;
+        case LIN_TILE_128_32: launch_tile<T, O, 4, 1, 1, 1, 4>(p, st); break;
+        case LIN_TILE_128_64: launch_tile<T, O, 4, 1, 1, 2, 3>(p, st); break;
+        case LIN_TILE_64_64: launch_tile<T, O, 2, 2, 1, 1, 4>(p, st); break;
+        case LIN_TILE_128_128: launch_tile<T, O, 2, 2, 2, 2, 2>(p, st); break;
+        default: launch_tile<T, O, 2, 4, 4, 2, 2>(p, st); break;
     }
     if (p.slices > 1) {
         const int64_t units = (int64_t)p.M * ((p.N + 7) / 8);

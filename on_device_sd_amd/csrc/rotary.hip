@@ -256,7 +256,7 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_any_kernel(RotaryParams p,
 }
 
 template <typename T, bool SIDE, typename POS>
-static void launch_rotary(RotaryParams &p, bool wide, hipStream_t st) {
+static int launch_rotary(RotaryParams &p, bool wide, hipStream_t st) {
     const int units = wide ? p.D / 16 : p.D / 2;
     int LG = 1;
     while (LG < units && LG < 64) LG *= 2;
@@ -268,9 +268,12 @@ static void launch_rotary(RotaryParams &p, bool wide, hipStream_t st) {
     p.kv_tokens = tokens(p.Hk);
     p.q_wgs = (p.n + p.q_tokens - 1) / p.q_tokens;
     const unsigned grid = (unsigned)(p.q_wgs + (p.n_store + p.kv_tokens - 1) / p.kv_tokens);
+    if (grid >= (1u << 24)) return ODSD_ERR_UNSUPPORTED;       // 2^32 threads
     const size_t lds = (size_t)max(p.q_tokens, p.kv_tokens) * (p.R / 2) * sizeof(float2);
     if (wide) rotary_wide_kernel<T, SIDE, POS><<<grid, ROT_THREADS, lds, st>>>(p, LG);
     else rotary_any_kernel<T, SIDE, POS><<<grid, ROT_THREADS, lds, st>>>(p, LG);
+    ODSD_CHECK_LAUNCH();
+    return ODSD_OK;
 }
 
 extern "C" int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
@@ -283,7 +286,9 @@ extern "C" int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head
                            const int32_t *src_index, int32_t n_store, int64_t num_slots, void *stream) {
     if (n < 0 || n_store < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || rotary_dim <= 0 || (rotary_dim & 1) ||
         (head_dim & 1) || rotary_dim > head_dim || n_axes < 1 || num_slots < 0) return ODSD_ERR_SHAPE;
-    if (head_dim > 1024 || n_axes > 4 || (int64_t)n + n_store > 0x7fffffffLL) return ODSD_ERR_UNSUPPORTED;
+    // a token's columns and the rows of a call are counted in 31 bits
+    if (head_dim > 1024 || n_axes > 4 || (int64_t)n + n_store > 0x7fffffffLL ||
+        (int64_t)max(num_heads, num_kv_heads) * head_dim > 0x7fffffffLL) return ODSD_ERR_UNSUPPORTED;
     if (dtype != ODSD_DT_BF16 && dtype != ODSD_DT_F16) return ODSD_ERR_DTYPE;
     if (position_bytes != 4 && position_bytes != 8) return ODSD_ERR_DTYPE;
     RotaryParams p;
@@ -325,19 +330,8 @@ extern "C" int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head
     if (((uintptr_t)positions & (position_bytes - 1)) || ((uintptr_t)inv_freq & 7)) return ODSD_ERR_ALIGN;
     const bool wide = (bytes & 15) == 0 && (elems & 7) == 0 && rotary_dim % 16 == 0 && head_dim % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-#define ROT_GO(T, POS)                                               \
-    do {                                                             \
-        if (interleaved) launch_rotary<T, true, POS>(p, wide, st);   \
-        else launch_rotary<T, false, POS>(p, wide, st);              \
-    } while (0)
-    if (dtype == ODSD_DT_BF16) {
-        if (position_bytes == 8) ROT_GO(__bf16, int64_t);
-        else ROT_GO(__bf16, int32_t);
-    } else {
-        if (position_bytes == 8) ROT_GO(half_t, int64_t);
-        else ROT_GO(half_t, int32_t);
-    }
+#define ROT_GO(T, POS) (interleaved ? launch_rotary<T, true, POS>(p, wide, st) : launch_rotary<T, false, POS>(p, wide, st))
+    if (dtype == ODSD_DT_BF16) return position_bytes == 8 ? ROT_GO(__bf16, int64_t) : ROT_GO(__bf16, int32_t);
+    return position_bytes == 8 ? ROT_GO(half_t, int64_t) : ROT_GO(half_t, int32_t);
 #undef ROT_GO
-    ODSD_CHECK_LAUNCH();
-    return ODSD_OK;
 }

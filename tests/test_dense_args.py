@@ -59,6 +59,19 @@ def test_verify_status_codes():
     assert ws(64, 9, 576, 512, 131072, 1) > ws(64, 9, 576, 512, 131072, 0)
 
 
+def test_launches_of_too_many_threads_are_refused():
+    """2^32 threads and more, before anything is launched."""
+    lib = _lib.load()
+    n = 1 << 26
+    assert lib.odsd_linear_workspace_bytes(1, n, 64) == 0
+    assert lib.odsd_linear(P, 64, P, 64, None, None, n, P, n, 1, n, 64, 1, 1, 0, P, 1 << 30, None) == 3
+    for n, heads in ((1 << 24, 4), (4, 1 << 27)):
+        assert lib.odsd_rotary(P, heads * 20, 20, P, 40, 20, P, 40, 20, n, heads, 2, 20, 20, 0, 1, P, 8, 1, n, None, P, None, None, 1e-6, P, P,
+                               None, None, None, None, 0, 64, None) == 3
+    assert lib.odsd_verify_workspace_bytes(2, 3, 1 << 24, 4, 100, 0) == 0
+    assert lib.odsd_verify_workspace_bytes(2, 3, 1 << 20, 4, 131072, 0) == 0
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)

@@ -131,6 +131,41 @@ def test_same_bits_every_time_and_in_a_graph(dev):
             assert torch.equal(z, ops.linear(x, w, activation="silu")), (M, k)
 
 
+def test_two_calls_at_once(dev):
+    """Calls on two streams, of the forms with a workspace (parts of K; packed columns), have workspaces of their own."""
+    for M, K, N in [(64, 8192, 2048), (300, 4097, 2000)]:
+        g = torch.Generator(device=dev).manual_seed(9)
+        xs = [torch.randn(M, K, generator=g, device=dev).bfloat16() for _ in range(2)]
+        w = torch.randn(N, K, generator=g, device=dev).bfloat16()
+        alone = [ops.linear(x, w) for x in xs]
+        torch.cuda.synchronize()
+        streams, got = [torch.cuda.Stream() for _ in xs], [[], []]
+        for _ in range(8):
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    got[i].append(ops.linear(xs[i], w))
+        torch.cuda.synchronize()
+        for want, ys in zip(alone, got):
+            assert all(torch.equal(y, want) for y in ys)
+
+
+def test_the_output_may_be_the_residual_of_the_next_call(dev):
+    """Calls one after the other on one stream share freed workspaces in order: a chain equals its steps."""
+    g = torch.Generator(device=dev).manual_seed(10)
+    x = torch.randn(48, 8192, generator=g, device=dev).half()
+    w = torch.randn(1024, 8192, generator=g, device=dev).half() / 90
+    y = torch.zeros(48, 1024, device=dev).half()
+    steps = []
+    for _ in range(5):
+        y = ops.linear(x, w, residual=y, activation="relu")
+        steps.append(y)
+    once = ops.linear(x, w, activation="relu", out_dtype=torch.float32)
+    want = torch.zeros(48, 1024, device=dev).half()
+    for y in steps:                                     # the sums of every call are the same bits; one rounding a call
+        want = (once + want.float()).half()
+        assert torch.equal(y, want)
+
+
 def test_leading_dimensions_single_rows_and_empty(dev):
     w = torch.randn(24, 64, device=dev).half()
     x = torch.randn(2, 3, 64, device=dev).half()

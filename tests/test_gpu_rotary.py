@@ -122,6 +122,20 @@ def test_rows_without_a_token(dev):
     assert torch.equal(kc, before)
 
 
+@pytest.mark.parametrize("D", [64, 20])
+def test_one_token_in_several_slots(dev, D):
+    """src_index names a token twice: both slots get its rows."""
+    qkv, pos, inv, _, _ = inputs(6, 2, 2, D, D, "bf16")
+    q, k, v = heads(qkv.to(dev), 2, 2, D)
+    _, ko = odsd.apply_rotary(q, k, pos.to(dev), inv.to(dev))
+    kc, vc = torch.zeros(9, 2 * D, device=dev).bfloat16(), torch.zeros(9, 2 * D, device=dev).bfloat16()
+    src = torch.tensor([3, 0, 3, 3, 5, 0, 1, 2], dtype=torch.int32, device=dev)
+    slots = torch.tensor([8, 1, 0, 3, 4, 5, 6, 7], dtype=torch.int32, device=dev)
+    odsd.rotary_store_kvcache(q, k, v, pos.to(dev), inv.to(dev), kc, vc, slots, src)
+    assert torch.equal(kc[slots.long()], ko[src.long()].flatten(1)) and torch.equal(vc[slots.long()], v[src.long()].flatten(1))
+    assert not kc[2].any() and not vc[2].any()
+
+
 @pytest.mark.parametrize("offset", [0, 1, 8])
 def test_unaligned_views(dev, offset):
     H, KV, D, n = 4, 2, 64, 11
