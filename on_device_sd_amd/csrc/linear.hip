@@ -225,7 +225,7 @@ struct LinearTile {
     static constexpr int BK = 64, ROW = BK * 2, SEGS = BK / 8, ROWS = 64 / SEGS;   // bytes and 16-byte segments of a row, rows of a copy
     static constexpr int A_BYTES = TN * ROW, STAGE = (TN + TM) * ROW;
     static constexpr int LA = TN / ROWS / NW, LB = TM / ROWS / NW, L = LA + LB;   // copies of a wavefront per step
-    static constexpr int CH = FA < 2 ? FA : 2;                             // blocks of n that leave together
+    static constexpr int CH = FA < 2 || FB > 2 ? 1 : 2;                    // blocks of n that leave together
     static constexpr int OUT_WAVE = FB * 32 * CH * 32 * 4;
     static constexpr int LDS = KS * (STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE);
     static_assert(LA * ROWS * NW == TN && LB * ROWS * NW == TM && LB >= 1, "every wavefront makes the same number of copies");
@@ -542,11 +542,12 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(LinearParams p, T *x, 
 
 // ---- which kernel ------------------------------------------------------------------------------
 // tiles n x m; K4, K2: K shared by groups of wavefronts of the workgroup
-enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_32_64_K4, LIN_TILE_32_64_K2, LIN_TILE_128_32, LIN_TILE_128_64, LIN_TILE_64_64,
-       LIN_TILE_128_128, LIN_TILE_256_256, LIN_KINDS };
-static const int TILE_N[LIN_KINDS] = {16, 64, 32, 32, 128, 128, 64, 128, 256};
-static const int TILE_M[LIN_KINDS] = {16, 64, 64, 64, 32, 64, 64, 128, 256};
-static const int THREADS[LIN_KINDS] = {1024, 256, 512, 256, 256, 256, 256, 256, 512};
+enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_32_64_K4, LIN_TILE_64_32_K2, LIN_TILE_64_64, LIN_TILE_64_64_K2, LIN_TILE_64_128_K2,
+       LIN_TILE_128_128, LIN_TILE_128_192, LIN_TILE_256_128, LIN_TILE_256_192, LIN_TILE_256_256, LIN_KINDS };
+static const int TILE_N[LIN_KINDS] = {16, 64, 32, 64, 64, 64, 64, 128, 128, 256, 256, 256};
+static const int TILE_M[LIN_KINDS] = {16, 64, 64, 32, 64, 64, 128, 128, 192, 128, 192, 256};
+static const int THREADS[LIN_KINDS] = {1024, 256, 512, 256, 256, 512, 512, 256, 256, 512, 512, 512};
+static const int SHARES[LIN_KINDS] = {1, 1, 4, 2, 1, 2, 2, 1, 1, 1, 1, 1};     // of K in the workgroup
 struct LinearPlan {
     int kind, slices, slice_k;
     int64_t part_ld;
@@ -555,7 +556,7 @@ struct LinearPlan {
     bool fits;         // a launch has fewer than 2^32 threads
 };
 static int64_t linear_tiles(int kind, int M, int N) {
-    return (int64_t)((M + TILE_M[kind] - 1) / TILE_M[kind]) * ((N + TILE_N[kind] - 1) / TILE_N[kind]);
+    return (int64_t)((uint32_t)(M + TILE_M[kind] - 1) / (uint32_t)TILE_M[kind]) * ((uint32_t)(N + TILE_N[kind] - 1) / (uint32_t)TILE_N[kind]);
 }
 static LinearPlan linear_plan_of(int kind, int slices, int M, int N, int K) {
     LinearPlan l;
@@ -572,48 +573,43 @@ static LinearPlan linear_plan_of(int kind, int slices, int M, int N, int K) {
 static size_t linear_packed_bytes(int rows, int Kp) { return odsd_round_up((size_t)rows * Kp * 2, 256); }
 // For operands whose rows are whole 16-byte segments; *us: about how long it takes.
 static LinearPlan linear_plan_aligned(int M, int N, int K, float *us) {
-    *us = 8.0f + (float)N * K * 2 / 4.5e6f;
-    // Up to 4 tokens one pass over the weights' rows.  us, rows / the tiles that follow: M = 1: K 4096, N 2048 7.1 / 11.0, K
-    // 2048, N 131072 93 / 100; M = 4: K 2048, N 5120 8.3 / 8.0; M = 16: K 2048, N 5120 10.0 / 8.0, N 131072 123 / 105.
-    if (M <= 4) return linear_plan_of(LIN_ROWS, 1, M, N, K);
+    *us = 0.0f;
+    // Few tokens and little work: one pass over the weights' rows, every token's columns read again for 16 of them.  us, rows /
+    // the best tile: M = 1: K 4096, N 2048 6.9 / 9.4, K 2048, N 131072 83 / 95; M = 4: K 2048, N 5120 7.8 / 8.2; M = 16: K 1288,
+    // N 2056 4.2 / 7.1, K 4096, N 2048 9.6 / 10.2, K 2048, N 5120 10.0 / 9.2, K 4096, N 12288 30 / 20.
+    if (M <= 4 || (M <= 16 && (double)M * N * K <= 1.5e8)) return linear_plan_of(LIN_ROWS, 1, M, N, K);
+    // Else the shape and the number of parts of K with the least estimated time.  A round of workgroups (256, one per CU; two of
+    // 64 x 64, which is for single m tiles: the weights' bytes count there, and how many are on their way) takes a step's time
+    // for every 64 columns of a share of K, and its epilogue.  The bytes are a second bound; what the shorter one adds is a root of
+    // fourth powers.  Parts of K cost a launch and their sums' way through memory.  The constants are fitted to 370 shapes of 8 to
+    // 6000 tokens (bf16, weights from memory); the estimate's choice is 1.3 % slower than the best shape on average, 24 % at worst.
+    // us of the shape taken / others, K 4096, N 4096: M = 200 (64 x 64, K shared by 2) 18 / 21 (64 x 128), 23 (64 x 64); M = 512
+    // (64 x 128) 29 / 32 (128 x 128, 2 parts), 38 (64 x 64); M = 1024 (128 x 128) 43 / 49 (128 x 192), 53 (two workgroups of it with
+    // half the copies in flight per CU); M = 1536 (128 x 192) 56 / 57 (256 x 128), 66 (128 x 128); M = 4096 (256 x 256) 111 / 124
+    // (256 x 128); K 2048, N 5120, M = 4096 (256 x 192) 90 / 94 (256 x 128), 105 (256 x 256).
+    static const float STEP[LIN_KINDS] = {0, 0, 0.52f, 0.29f, 0.19f, 0.45f, 0.66f, 0.50f, 0.67f, 0.88f, 1.34f, 1.58f};
+    static const float END[LIN_KINDS] = {0, 0, 2.9f, 3.1f, 4.2f, 3.0f, 3.9f, 6.0f, 8.2f, 6.5f, 8.0f, 9.7f};
     const int steps = (K + 63) / 64;
-    // Up to 64 tokens the weights' bytes count, and how many of them are on their way.  While 32-row tiles are at most one
-    // (two) per CU, K is shared inside the workgroup, in one launch; beyond that, as many tokens in a tile as there are, and
-    // parts of K until the workgroups are two per CU; 64 x 64 tiles once they alone fill the chip.  us at M = 64, K shared by
-    // 4 / by 2 / parts of K in two launches: K 2048: N 5120 8.5 / 8.6 / 13.0, N 8192 10.2 / 9.8 / 13.8, N 16384 18.1 / 14.5 /
-    // 21.2, N 24576 29.5 / 27.4 / 27.7; K 4096: N 2048 11.4 / 12.1 / 13.0, N 12288 30.6 / 29.1 / 28.0; K 8192: N 2048 18.3 /
-    // 20.7 / 14.4, N 8192 33.3 / 36.0 / 36.4.  (128 x 64 / 64 x 64 tiles: N 32768 36.0 / 33.1, N 131072 117 / 113.)
-    if (M <= 64 && N <= 8192 && (K <= 4096 || K <= N)) return linear_plan_of(LIN_TILE_32_64_K4, 1, M, N, K);
-    if (M <= 64 && N <= 16384 && K <= 2048) return linear_plan_of(LIN_TILE_32_64_K2, 1, M, N, K);
-    if (M <= 64) {
-        const int kind = M <= 32 ? LIN_TILE_128_32 : N >= 24576 ? LIN_TILE_64_64 : LIN_TILE_128_64;
-        int slices = 1;
-        while (slices < 8 && linear_tiles(kind, M, N) * slices * 2 <= 512 && steps / (slices * 2) >= 8) slices *= 2;
-        return linear_plan_of(kind, slices, M, N, K);
-    }
-    // More tokens: the shape and the number of parts of K with the least estimated time.  A round of workgroups (512, or
-    // 256 of the largest tile) takes a step's time for every 64 columns and its epilogue; parts of K cost a second launch.
-    // Step and epilogue in us, as measured on full rounds (K 2048 and 4096, bf16).  us of the shape taken / of others, K 4096,
-    // N 4096: M = 2048 (128 x 128) 66 / 81 (128 x 64), M = 4096 (256 x 256) 111 / 128 (128 x 128); K 2048, N 5120: M = 200
-    // (64 x 64) 14 / 18 / 22, M = 500 (128 x 64) 21 / 25 / 27.
-    static const float STEP[LIN_KINDS] = {0, 0, 0, 0, 0, 0.68f, 0.42f, 1.06f, 1.58f};
-    static const float END[LIN_KINDS] = {0, 0, 0, 0, 0, 2.0f, 1.5f, 4.0f, 10.0f};
-    LinearPlan best = {};
-    float best_us = 0.0f;              // (without the launch)
-    for (int kind = LIN_TILE_128_64; kind <= LIN_TILE_256_256; ++kind) {
-        const int64_t slots = kind == LIN_TILE_256_256 ? 256 : 512;
-        for (int slices = 1; slices <= 8 && (slices == 1 || steps / slices >= 8); slices *= 2) {
-            const LinearPlan l = linear_plan_of(kind, slices, M, N, K);
-            const float rounds = (float)((linear_tiles(kind, M, N) * l.slices + slots - 1) / slots);
-            const float t = rounds * (l.slice_k / 64 * STEP[kind] + END[kind]) + (l.slices > 1 ? 4.0f + l.bytes / 2e6f : 0.0f);
-            if (best_us == 0.0f || t < best_us) {
-                best_us = t;
-                best = l;
+    const float bytes_us = ((float)M * K + (float)N * K + (float)M * N) * 2 / 6.7e6f + 5.2f, bytes2 = bytes_us * bytes_us;
+    const float join_us = (float)M * N * 4 / 3.5e6f;           // of a part
+    int kind = 0, parts = 1;
+    for (int k = LIN_TILE_32_64_K4; k < LIN_KINDS; ++k) {
+        if ((k == LIN_TILE_64_32_K2 && M > 32) || (k == LIN_TILE_64_64 && M > 64)) continue;
+        const int64_t tiles = linear_tiles(k, M, N);
+        for (int slices = 1; slices <= 8; slices *= 2) {
+            if (slices > 1 && (tiles * slices > 640 || steps / slices < 4)) break;
+            const float rounds = (float)(k == LIN_TILE_64_64 ? (tiles * slices + 511) / 512 : (tiles * slices + 255) / 256);
+            const int per_share = ((steps + slices - 1) / slices + SHARES[k] - 1) / SHARES[k];
+            const float t = rounds * (per_share * STEP[k] + END[k]);
+            const float total = sqrtf(sqrtf(t * t * t * t + bytes2 * bytes2)) + (slices > 1 ? 2.0f + slices * join_us : 0.0f);
+            if (*us == 0.0f || total < *us) {
+                *us = total;
+                kind = k;
+                parts = slices;
             }
         }
     }
-    *us = 2.0f + best_us;
-    return best;
+    return linear_plan_of(kind, parts, M, N, K);
 }
 static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
     float us;
@@ -679,11 +675,14 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
     p.part_ld = l.part_ld;
     switch (l.kind) {
         case LIN_TILE_32_64_K4: launch_tile<T, O, 1, 2, 1, 1, 3, 4>(p, st); break;
-        case LIN_TILE_32_64_K2: launch_tile<T, O, 1, 2, 1, 1, 3, 2>(p, st); break;
-        case LIN_TILE_128_32: launch_tile<T, O, 4, 1, 1, 1, 4>(p, st); break;
-        case LIN_TILE_128_64: launch_tile<T, O, 4, 1, 1, 2, 3>(p, st); break;
+        case LIN_TILE_64_32_K2: launch_tile<T, O, 2, 1, 1, 1, 4, 2>(p, st); break;
         case LIN_TILE_64_64: launch_tile<T, O, 2, 2, 1, 1, 4>(p, st); break;
-        case LIN_TILE_128_128: launch_tile<T, O, 2, 2, 2, 2, 2>(p, st); break;
+        case LIN_TILE_64_64_K2: launch_tile<T, O, 2, 2, 1, 1, 3, 2>(p, st); break;
+        case LIN_TILE_64_128_K2: launch_tile<T, O, 1, 4, 2, 1, 3, 2>(p, st); break;
+        case LIN_TILE_128_128: launch_tile<T, O, 2, 2, 2, 2, 4>(p, st); break;
+        case LIN_TILE_128_192: launch_tile<T, O, 2, 2, 2, 3, 3>(p, st); break;
+        case LIN_TILE_256_128: launch_tile<T, O, 4, 2, 2, 2, 3>(p, st); break;
+        case LIN_TILE_256_192: launch_tile<T, O, 4, 2, 2, 3, 2>(p, st); break;
         default: launch_tile<T, O, 2, 4, 4, 2, 2>(p, st); break;
     }
     if (p.slices > 1) {

@@ -64,6 +64,26 @@ def test_shapes(dev, M, K, N):
     run(dev, M, K, N, act="silu")
 
 
+# every tile shape, in one part of K and in several, with edges that are no multiple of it
+TILES = [(37, 72, 72), (18, 2168, 85), (67, 2888, 1173), (1341, 3008, 79), (19, 72, 65), (28, 6296, 5539), (14, 3800, 2822), (17, 2584, 1206),
+         (24, 64, 16930), (33, 4368, 8795), (7, 5008, 4990), (8, 7536, 2495), (38, 72, 8198), (77, 3368, 1037), (33, 7872, 1034), (72, 72, 8460),
+         (83, 4496, 4222), (198, 6072, 1032), (69, 8288, 1321), (134, 64, 9036), (218, 5216, 4446), (67, 5496, 4701), (143, 728, 17065),
+         (139, 4152, 9634), (134, 4808, 6065), (2316, 7120, 194), (133, 64, 18196), (66, 5200, 9058), (229, 9016, 2126), (258, 80, 22286),
+         (622, 64, 16930), (5433, 344, 2113)]
+
+
+@pytest.mark.parametrize("M,K,N", TILES)
+def test_tile_shapes(dev, M, K, N):
+    run(dev, M, K, N, "fp16", act="relu")
+
+
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
+@pytest.mark.parametrize("M,K,N", [(37, 136, 72), (19, 72, 65), (24, 72, 16930), (38, 72, 8198), (72, 72, 8460), (134, 64, 9036), (143, 728, 17065),
+                                   (133, 64, 18196), (258, 80, 22286), (622, 64, 16930)])
+def test_tile_shapes_of_every_type(dev, M, K, N, dtype, out):
+    run(dev, M, K, N, dtype, out, "gelu_tanh", seed=M)
+
+
 @pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("M", [1, 24, 150, 600])
