@@ -213,21 +213,24 @@ __global__ __launch_bounds__(NWV * 64) void linear_rows_kernel(LinearParams p) {
 
 // ---- tiles -----------------------------------------------------------------------------------
 // NWN x NWM wavefronts, each FA blocks of 32 n by FB blocks of 32 m on v_mfma_f32_32x32x16; steps of 64 along K.  Both
-// operands go to LDS without passing registers (buffer_load ... lds, 16 bytes a lane), STAGES buffers of them; a buffer's
-// rows are 128 bytes, whose 16-byte segments are XORed with bits of the row's number: the 16 lanes that
-// read together (rows 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of a block, one segment) then meet the 16 bank groups.  What is behind a row's end, the matrix's last row or the slice's
-// last step is addressed outside the buffer descriptor and arrives as zeros, without memory traffic, so every copy is
-// issued whatever follows and a count says which have landed.  KS groups of such wavefronts take every KS-th step each, with
-// buffers of their own, and add their sums up at the end: for few tokens, where a step is a chain of latencies.
+// operands go to LDS without passing registers (buffer_load ... lds, 16 bytes a lane): STAGES buffers of a step's x, one more of
+// w.  A buffer's rows are 128 bytes, whose 16-byte segments are XORed with bits of the row's number: the 16 lanes that read
+// together (rows 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of a block, one segment) then meet the 16 bank groups.  What is behind
+// a row's end, the matrix's last row or the slice's last step is addressed outside the buffer descriptor and arrives as zeros,
+// without memory traffic, so every copy is issued whatever follows and a count says which have landed.  KS groups of such
+// wavefronts take every KS-th step each, with buffers of their own, and add their sums up at the end: for few tokens, where a
+// step is a chain of latencies, and for small tiles, which leave a CU with one workgroup.
 template <int NWN, int NWM, int FA, int FB, int STAGES, int KS>
 struct LinearTile {
     static constexpr int NW = NWN * NWM, TN = NWN * FA * 32, TM = NWM * FB * 32;
     static constexpr int BK = 64, ROW = BK * 2, SEGS = BK / 8, ROWS = 64 / SEGS;   // bytes and 16-byte segments of a row, rows of a copy
-    static constexpr int A_BYTES = TN * ROW, STAGE = (TN + TM) * ROW;
+    static constexpr int A_BYTES = TN * ROW, B_BYTES = TM * ROW;
+    static constexpr int A_RING = (STAGES + 1) * A_BYTES, B_RING = STAGES * B_BYTES, RING = A_RING + B_RING;
     static constexpr int LA = TN / ROWS / NW, LB = TM / ROWS / NW, L = LA + LB;   // copies of a wavefront per step
-    static constexpr int CH = FA < 2 || FB > 2 ? 1 : 2;                    // blocks of n that leave together
+    // blocks of n that leave together (one where FB is 3; one block of m at a time and two of n are as fast within 1 %)
+    static constexpr int CH = FA < 2 || FB > 2 ? 1 : 2;
     static constexpr int OUT_WAVE = FB * 32 * CH * 32 * 4;
-    static constexpr int LDS = KS * (STAGE * STAGES > NW * OUT_WAVE ? STAGE * STAGES : NW * OUT_WAVE);
+    static constexpr int LDS = KS * (RING > NW * OUT_WAVE ? RING : NW * OUT_WAVE);
     static_assert(LA * ROWS * NW == TN && LB * ROWS * NW == TM && LB >= 1, "every wavefront makes the same number of copies");
     static_assert(NW % 2 == 0, "the swizzle of a copied row does not depend on the copy");
 };
@@ -278,21 +281,22 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
     const int seg = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4));
     const uint32_t row0 = wave * C::ROWS + lane / C::SEGS;
     const uint32_t off_w = row0 * ldw + seg * 16, off_x = row0 * ldx + seg * 16;
-    char *const mine = lds + part * (C::STAGE * STAGES);
+    char *const mine = lds + part * C::RING;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)mine;
-    auto copy = [&](int step, uint32_t buf, int i) {            // copy i of a step's: first those of w, then those of x
+    struct Place { uint32_t a, b; };                            // of a step's w and x in the rings
+    auto copy = [&](int step, Place to, int i) {                // copy i of a step's: first those of w, then those of x
         const int k = k_begin + (step * KS + part) * BK;
         const uint32_t ko = k + seg * 8 < k_end ? (uint32_t)k * 2u : 0x80000000u;
         if (i < C::LA) {
-            const uint32_t off = off_w + ko + i * (C::NW * C::ROWS) * ldw, at = lds0 + buf + (i * C::NW + wave) * 1024;
+            const uint32_t off = off_w + ko + i * (C::NW * C::ROWS) * ldw, at = lds0 + to.a + (i * C::NW + wave) * 1024;
             if (C::TM <= 64 && p.w_once) copy16_to_lds_nt(rw, off, at);
             else copy16_to_lds(rw, off, at);
-        } else copy16_to_lds(rx, off_x + ko + (i - C::LA) * (C::NW * C::ROWS) * ldx, lds0 + buf + C::A_BYTES + ((i - C::LA) * C::NW + wave) * 1024);
+        } else copy16_to_lds(rx, off_x + ko + (i - C::LA) * (C::NW * C::ROWS) * ldx, lds0 + to.b + ((i - C::LA) * C::NW + wave) * 1024);
     };
 
     const int wn = wave % NWN, wm = wave / NWN;
     const uint32_t frag = (lane & 31) * C::ROW + (((lane >> 5) ^ ((lane >> 1) & 7)) << 4);
-    const uint32_t fa0 = wn * FA * 32 * C::ROW + frag, fb0 = C::A_BYTES + wm * FB * 32 * C::ROW + frag;
+    const uint32_t fa0 = wn * FA * 32 * C::ROW + frag, fb0 = wm * FB * 32 * C::ROW + frag;
     float16_t acc[FA][FB];
 #pragma unroll
     for (int i = 0; i < FA; ++i)
@@ -302,25 +306,28 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     V8 fa[2][FA], fb[2][FB];
     // fragment i of columns 16 j .. of a buffer, in the order in which the products want them: w's first, x's, the rest of w's
-    auto read = [&](int par, uint32_t buf, int j, int i) {
-        if (i > 0 && i <= FB) fb[par][i - 1] = *(const V8 *)(mine + ((buf + fb0) ^ (j << 5)) + (i - 1) * 32 * C::ROW);
-        else fa[par][i ? i - FB : 0] = *(const V8 *)(mine + ((buf + fa0) ^ (j << 5)) + (i ? i - FB : 0) * 32 * C::ROW);
+    auto read = [&](int par, Place at, int j, int i) {
+        if (i > 0 && i <= FB) fb[par][i - 1] = *(const V8 *)(mine + ((at.b + fb0) ^ (j << 5)) + (i - 1) * 32 * C::ROW);
+        else fa[par][i ? i - FB : 0] = *(const V8 *)(mine + ((at.a + fa0) ^ (j << 5)) + (i ? i - FB : 0) * 32 * C::ROW);
     };
-    // 16 columns: their products, and between those, one by one, the reads of the next 16 columns' fragments and the copies
-    // of the step that comes into the buffer that was left last.  (The compiler would request a fragment right before its
-    // use, and copies in a row stall the wavefront: a CU takes one per 16 cycles.)
-    constexpr int J = BK / 16, NM = FA * FB, NR = FA + FB, EARLY = C::L * 3 / 4;
-    auto columns = [&](auto jc, int step, uint32_t cur, uint32_t next, uint32_t left) {
+    // 16 columns: their products, and between those, one by one, the reads of the next 16 columns' fragments and copies.  (The
+    // compiler would request a fragment right before its use, and copies in a row stall the wavefront: a CU takes one per 16
+    // cycles.)  Copies: in the second 16 columns w of the step that is STAGES ahead, into the buffer that the step before left;
+    // behind the barrier its x, into the buffer that this step leaves.  With as many buffers of w as of x, three quarters of a
+    // step's copies waited for the barrier and had a step less to arrive: 8192 x 4096 x 16384 890 us, now 856; 1536 x 8192 x 8192
+    // 189 and 162.
+    constexpr int J = C::BK / 16, NM = FA * FB, NR = FA + FB;
+    auto columns = [&](auto jc, int step, Place cur, Place next, uint32_t left) {
         constexpr int j = decltype(jc)::value;
         constexpr bool last = j == J - 1;
-        constexpr int NC = last ? EARLY : j == 0 ? C::L - EARLY : 0;
+        constexpr int NC = last ? C::LB : j == 1 ? C::LA : 0;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
             acc[i / FB][i % FB] = AttnT<T>::mfma32(fa[j & 1][i / FB], fb[j & 1][i % FB], acc[i / FB][i % FB]);
             if (last && i == 0) {
                 // the next step's copies have landed and this step's last fragments are read: by every wavefront
-                ODSD_WAIT_VMCNT_LGKM0((STAGES - 2) * C::L);
+                ODSD_WAIT_VMCNT_LGKM0((STAGES - 2) * C::L + C::LA);
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             }
@@ -329,7 +336,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
                 if (r * NM / NR == i) read((j + 1) & 1, last ? next : cur, last ? 0 : j + 1, r);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                if (c * NM / (NC ? NC : 1) == i) copy(last ? step + STAGES : step + STAGES - 1, last ? cur : left, last ? c : EARLY + c);
+                if (c * NM / (NC ? NC : 1) == i) copy(step + STAGES, Place{left, cur.b}, last ? C::LA + c : c);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -337,21 +344,22 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
 #pragma unroll
     for (int s = 0; s < STAGES; ++s)
 #pragma unroll
-        for (int i = 0; i < (s < STAGES - 1 ? C::L : EARLY); ++i) copy(s, s * C::STAGE, i);
-    ODSD_WAIT_VMCNT_LGKM0((STAGES - 2) * C::L + EARLY);
+        for (int i = 0; i < C::L; ++i) copy(s, Place{(uint32_t)(s * C::A_BYTES), (uint32_t)(C::A_RING + s * C::B_BYTES)}, i);
+    ODSD_WAIT_VMCNT_LGKM0((STAGES - 1) * C::L);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    uint32_t cur = 0, left = (STAGES - 1) * C::STAGE;
+    Place cur = {0, C::A_RING};
+    uint32_t left = C::A_RING - C::A_BYTES;                    // where w of the step before lay
 #pragma unroll
     for (int r = 0; r < NR; ++r) read(0, cur, 0, r);
     for (int step = 0; step < steps; ++step) {
-        uint32_t next = cur + C::STAGE;
-        if (next == C::STAGE * STAGES) next = 0;
+        const Place next = {cur.a + C::A_BYTES == C::A_RING ? 0u : cur.a + C::A_BYTES,
+                            cur.b + C::B_BYTES == C::RING ? (uint32_t)C::A_RING : cur.b + C::B_BYTES};
         columns(std::integral_constant<int, 0>{}, step, cur, next, left);
         columns(std::integral_constant<int, 1>{}, step, cur, next, left);
         columns(std::integral_constant<int, 2>{}, step, cur, next, left);
         columns(std::integral_constant<int, 3>{}, step, cur, next, left);
-        left = cur;
+        left = cur.a;
         cur = next;
     }
     ODSD_WAIT_VMCNT_LGKM0(0);                  // the copies past the end (zeros) have landed, too
@@ -543,9 +551,9 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(LinearParams p, T *x, 
 // ---- which kernel ------------------------------------------------------------------------------
 // tiles n x m; K4, K2: K shared by groups of wavefronts of the workgroup
 enum { LIN_ROWS = 0, LIN_ANY, LIN_TILE_32_64_K4, LIN_TILE_64_32_K2, LIN_TILE_64_64, LIN_TILE_64_64_K2, LIN_TILE_64_128_K2,
-       LIN_TILE_128_128, LIN_TILE_128_192, LIN_TILE_256_128, LIN_TILE_256_192, LIN_TILE_256_256, LIN_KINDS };
-static const int TILE_N[LIN_KINDS] = {16, 64, 32, 64, 64, 64, 64, 128, 128, 256, 256, 256};
-static const int TILE_M[LIN_KINDS] = {16, 64, 64, 32, 64, 64, 128, 128, 192, 128, 192, 256};
+       LIN_TILE_128_128, LIN_TILE_128_192, LIN_TILE_128_256, LIN_TILE_256_192, LIN_TILE_256_256, LIN_KINDS };
+static const int TILE_N[LIN_KINDS] = {16, 64, 32, 64, 64, 64, 64, 128, 128, 128, 256, 256};
+static const int TILE_M[LIN_KINDS] = {16, 64, 64, 32, 64, 64, 128, 128, 192, 256, 192, 256};
 static const int THREADS[LIN_KINDS] = {1024, 256, 512, 256, 256, 512, 512, 256, 256, 512, 512, 512};
 static const int SHARES[LIN_KINDS] = {1, 1, 4, 2, 1, 2, 2, 1, 1, 1, 1, 1};     // of K in the workgroup
 struct LinearPlan {
@@ -580,18 +588,19 @@ static LinearPlan linear_plan_aligned(int M, int N, int K, float *us) {
     if (M <= 4 || (M <= 16 && (double)M * N * K <= 1.5e8)) return linear_plan_of(LIN_ROWS, 1, M, N, K);
     // Else the shape and the number of parts of K with the least estimated time.  A round of workgroups (256, one per CU; two of
     // 64 x 64, which is for single m tiles: the weights' bytes count there, and how many are on their way) takes a step's time
-    // for every 64 columns of a share of K, and its epilogue.  The bytes are a second bound; what the shorter one adds is a root of
-    // fourth powers.  Parts of K cost a launch and their sums' way through memory.  The constants are fitted to 370 shapes of 8 to
-    // 6000 tokens (bf16, weights from memory); the estimate's choice is 1.3 % slower than the best shape on average, 24 % at worst.
-    // us of the shape taken / others, K 4096, N 4096: M = 200 (64 x 64, K shared by 2) 18 / 21 (64 x 128), 23 (64 x 64); M = 512
-    // (64 x 128) 29 / 32 (128 x 128, 2 parts), 38 (64 x 64); M = 1024 (128 x 128) 43 / 49 (128 x 192), 53 (two workgroups of it with
-    // half the copies in flight per CU); M = 1536 (128 x 192) 56 / 57 (256 x 128), 66 (128 x 128); M = 4096 (256 x 256) 111 / 124
-    // (256 x 128); K 2048, N 5120, M = 4096 (256 x 192) 90 / 94 (256 x 128), 105 (256 x 256).
-    static const float STEP[LIN_KINDS] = {0, 0, 0.52f, 0.29f, 0.19f, 0.45f, 0.66f, 0.50f, 0.67f, 0.88f, 1.34f, 1.58f};
-    static const float END[LIN_KINDS] = {0, 0, 2.9f, 3.1f, 4.2f, 3.0f, 3.9f, 6.0f, 8.2f, 6.5f, 8.0f, 9.7f};
+    // for every 64 columns of a share of K, and its epilogue.  The bytes are a second bound; what the shorter one adds is a root
+    // of fourth powers.  Parts of K cost a launch and their sums' way through memory.  The constants are fitted to 913 shapes of
+    // 5 to 8192 tokens (bf16, weights from memory); the estimate's choice is 0.9 % slower than the best on average, 20 % at worst.
+    // us of the shape taken / others, K 4096, N 4096: M = 200 (64 x 64, K shared by 2) 17.5 / 20 (64 x 128, 2 parts), 22 (128 x
+    // 128, 4 parts); M = 512 (64 x 128) 28 / 31 (128 x 128, 2 parts), 39 (64 x 64); M = 1000 (128 x 128) 40 / 43 (128 x 192), 53
+    // (64 x 128); M = 1536 (128 x 192) 52 / 56 (128 x 256), 73 (128 x 128); M = 4096 (256 x 256) 110 / 124 (128 x 256).  K 2048, N
+    // 5120: M = 48 (32 x 64) 8.2 / 9.3 (64 x 64), M = 4096 (256 x 192) 85 / 95 (128 x 256), 102 (256 x 256).  K 2048, N 131072, M =
+    // 64 (64 x 64) 118 / 130 (the same with K shared by 2).
+    static const float STEP[LIN_KINDS] = {0, 0, 0.58f, 0.69f, 0.41f, 0.43f, 0.68f, 0.52f, 0.66f, 0.85f, 1.16f, 1.36f};
+    static const float END[LIN_KINDS] = {0, 0, 3.3f, 2.3f, 4.4f, 3.9f, 3.6f, 5.7f, 8.9f, 5.6f, 8.2f, 9.4f};
     const int steps = (K + 63) / 64;
-    const float bytes_us = ((float)M * K + (float)N * K + (float)M * N) * 2 / 6.7e6f + 5.2f, bytes2 = bytes_us * bytes_us;
-    const float join_us = (float)M * N * 4 / 3.5e6f;           // of a part
+    const float bytes_us = ((float)M * K + (float)N * K + (float)M * N) * 2 / 7.4e6f + 6.7f, bytes2 = bytes_us * bytes_us;
+    const float join_us = (float)M * N * 4 / 3.7e6f;           // of a part
     int kind = 0, parts = 1;
     for (int k = LIN_TILE_32_64_K4; k < LIN_KINDS; ++k) {
         if ((k == LIN_TILE_64_32_K2 && M > 32) || (k == LIN_TILE_64_64 && M > 64)) continue;
@@ -601,7 +610,7 @@ static LinearPlan linear_plan_aligned(int M, int N, int K, float *us) {
             const float rounds = (float)(k == LIN_TILE_64_64 ? (tiles * slices + 511) / 512 : (tiles * slices + 255) / 256);
             const int per_share = ((steps + slices - 1) / slices + SHARES[k] - 1) / SHARES[k];
             const float t = rounds * (per_share * STEP[k] + END[k]);
-            const float total = sqrtf(sqrtf(t * t * t * t + bytes2 * bytes2)) + (slices > 1 ? 2.0f + slices * join_us : 0.0f);
+            const float total = sqrtf(sqrtf(t * t * t * t + bytes2 * bytes2)) + (slices > 1 ? 3.1f + slices * join_us : 0.0f);
             if (*us == 0.0f || total < *us) {
                 *us = total;
                 kind = k;
@@ -681,7 +690,7 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
         case LIN_TILE_64_128_K2: launch_tile<T, O, 1, 4, 2, 1, 3, 2>(p, st); break;
         case LIN_TILE_128_128: launch_tile<T, O, 2, 2, 2, 2, 4>(p, st); break;
         case LIN_TILE_128_192: launch_tile<T, O, 2, 2, 2, 3, 3>(p, st); break;
-        case LIN_TILE_256_128: launch_tile<T, O, 4, 2, 2, 2, 3>(p, st); break;
+        case LIN_TILE_128_256: launch_tile<T, O, 2, 4, 2, 2, 3>(p, st); break;
         case LIN_TILE_256_192: launch_tile<T, O, 4, 2, 2, 3, 2>(p, st); break;
         default: launch_tile<T, O, 2, 4, 4, 2, 2>(p, st); break;
     }

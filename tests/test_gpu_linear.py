@@ -69,7 +69,11 @@ TILES = [(37, 72, 72), (18, 2168, 85), (67, 2888, 1173), (1341, 3008, 79), (19, 
          (24, 64, 16930), (33, 4368, 8795), (7, 5008, 4990), (8, 7536, 2495), (38, 72, 8198), (77, 3368, 1037), (33, 7872, 1034), (72, 72, 8460),
          (83, 4496, 4222), (198, 6072, 1032), (69, 8288, 1321), (134, 64, 9036), (218, 5216, 4446), (67, 5496, 4701), (143, 728, 17065),
          (139, 4152, 9634), (134, 4808, 6065), (2316, 7120, 194), (133, 64, 18196), (66, 5200, 9058), (229, 9016, 2126), (258, 80, 22286),
-         (622, 64, 16930), (5433, 344, 2113)]
+         (622, 64, 16930), (5433, 344, 2113), (35, 3392, 2317), (18, 72, 8309), (5, 6296, 4790), (17, 3736, 1080), (33, 7240, 4410),
+         (35, 4648, 2232), (67, 392, 4290), (133, 6296, 1054), (72, 6056, 2231), (75, 3944, 1085), (151, 64, 8799), (65, 6592, 8199),
+         (67, 6576, 4446), (143, 968, 18257), (134, 3688, 11100), (158, 5144, 5560), (478, 8920, 1122), (137, 72, 18111), (195, 6304, 4171),
+         (133, 7600, 2787), (132, 4544, 5737), (404, 64, 22868), (140, 1104, 16903), (1353, 3872, 110), (111, 2880, 332), (6, 8888, 4382),
+         (16, 9048, 4574), (4267, 6848, 153), (129, 4904, 8293), (17, 2592, 78)]
 
 
 @pytest.mark.parametrize("M,K,N", TILES)
@@ -79,7 +83,8 @@ def test_tile_shapes(dev, M, K, N):
 
 @pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
 @pytest.mark.parametrize("M,K,N", [(37, 136, 72), (19, 72, 65), (24, 72, 16930), (38, 72, 8198), (72, 72, 8460), (134, 64, 9036), (143, 728, 17065),
-                                   (133, 64, 18196), (258, 80, 22286), (622, 64, 16930)])
+                                   (133, 64, 18196), (258, 80, 22286), (622, 64, 16930), (18, 72, 8309), (67, 392, 4290), (143, 968, 18257),
+                                   (137, 72, 18111), (140, 1104, 16903)])
 def test_tile_shapes_of_every_type(dev, M, K, N, dtype, out):
     run(dev, M, K, N, dtype, out, "gelu_tanh", seed=M)
 
