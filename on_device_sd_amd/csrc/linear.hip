@@ -14,7 +14,6 @@ struct LinearParams {
     int64_t ldx, ldw, ldr, ldo;    // elements between two rows
     int M, N, K, act;
     int tiles_n, tiles_m, slices, slice_k;   // tile kernel: K in `slices` parts of slice_k columns (a multiple of 64)
-    int w_once;                    // the weights are read past the caches
     float *part;                   // their sums, [slices][M][part_ld], when there are several
     int64_t part_ld;               // N rounded up to 8
 };
@@ -254,7 +253,8 @@ __device__ __forceinline__ uint4_t descriptor(const void *base, uint32_t bytes) 
     return r;
 }
 
-template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES, int KS>
+// ONCE: the weights are read past the caches
+template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES, int KS, bool ONCE>
 __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(LinearParams p) {
     typedef LinearTile<NWN, NWM, FA, FB, STAGES, KS> C;
     typedef typename AttnT<T>::V8 V8;
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
         const uint32_t ko = k + seg * 8 < k_end ? (uint32_t)k * 2u : 0x80000000u;
         if (i < C::LA) {
             const uint32_t off = off_w + ko + i * (C::NW * C::ROWS) * ldw, at = lds0 + to.a + (i * C::NW + wave) * 1024;
-            if (C::TM <= 64 && p.w_once) copy16_to_lds_nt(rw, off, at);
+            if (ONCE) copy16_to_lds_nt(rw, off, at);
             else copy16_to_lds(rw, off, at);
         } else copy16_to_lds(rx, off_x + ko + (i - C::LA) * (C::NW * C::ROWS) * ldx, lds0 + to.b + ((i - C::LA) * C::NW + wave) * 1024);
     };
@@ -647,12 +647,19 @@ static void launch_tile(LinearParams &p, hipStream_t st) {
     typedef LinearTile<NWN, NWM, FA, FB, STAGES, KS> C;
     p.tiles_n = (p.N + C::TN - 1) / C::TN;
     p.tiles_m = (p.M + C::TM - 1) / C::TM;
-    // One pass over weights of more than a third of the 256 MB cache: nothing of them is there at the next call, so they do
-    // not displace what is (M = 64, K 2048, N 32768 33.9 -> 31.4 us, M = 33, K 4096, N 65536 107 -> 93).  Smaller ones, called
-    // again soon, come out of it (M = 64, K 2048, N 16384 15.0, past it 20.5; not called again 21.1 / 19.6).
-    p.w_once = p.tiles_m == 1 && (int64_t)p.N * p.K * 2 >= (96 << 20);
     const int64_t total = (int64_t)p.tiles_n * p.tiles_m * p.slices;
-    linear_tile_kernel<T, O, NWN, NWM, FA, FB, STAGES, KS><<<(unsigned)((total + 7) / 8 * 8), C::NW * KS * 64, 0, st>>>(p);
+    const unsigned grid = (unsigned)((total + 7) / 8 * 8), threads = C::NW * KS * 64;
+    // One pass over weights of more than a third of the 256 MB cache: nothing of them is there at the next call, so they do
+    // not displace what is (M = 64, K 2048, N 32768 33.9 -> 31.4 us, M = 33, K 4096, N 65536 107 -> 93, M = 180, K 2048, N 65536
+    // 82 -> 74).  Smaller ones, called again soon, come out of it (M = 64, K 2048, N 16384 15.0, past it 20.5; not called again
+    // 21.1 / 19.6), and so do the ends of rows that are no whole lines of 128 bytes (M = 96, K 3000, N 36000 89 / 92).
+    if constexpr (C::TM < 256) {
+        if (p.tiles_m == 1 && (int64_t)p.N * p.K * 2 >= (96 << 20) && p.ldw % 64 == 0) {
+            linear_tile_kernel<T, O, NWN, NWM, FA, FB, STAGES, KS, true><<<grid, threads, 0, st>>>(p);
+            return;
+        }
+    }
+    linear_tile_kernel<T, O, NWN, NWM, FA, FB, STAGES, KS, false><<<grid, threads, 0, st>>>(p);
 }
 
 template <typename T, typename O> static int launch_linear(LinearParams &p, const LinearPlan &l, void *workspace, hipStream_t st) {
@@ -725,7 +732,7 @@ extern "C" int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ld
     const uintptr_t oe = out_dtype == ODSD_DT_F32 ? 4 : 2;
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias) & 1) || (((uintptr_t)out | (uintptr_t)residual) & (oe - 1)) ||
         !odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
-    LinearParams p{x, w, bias, residual, out, ldx, ldw, ldr, ldo, M, N, K, act, 0, 0, 1, 0, 0, nullptr, 0};
+    LinearParams p{x, w, bias, residual, out, ldx, ldw, ldr, ldo, M, N, K, act, 0, 0, 1, 0, nullptr, 0};
     // rows of whole 16-byte segments, and a tile's rows within 31 bits of bytes
     const bool aligned = ((K | ldx | ldw) & 7) == 0 && odsd_aligned16(x) && odsd_aligned16(w) && ldx < (1 << 21) && ldw < (1 << 21);
     const LinearPlan l = linear_plan(M, N, K, aligned);

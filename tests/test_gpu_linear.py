@@ -81,6 +81,13 @@ def test_tile_shapes(dev, M, K, N):
     run(dev, M, K, N, "fp16", act="relu")
 
 
+@pytest.mark.parametrize("M,K,N", [(12, 8192, 8000), (20, 12288, 4300), (40, 2048, 25700), (60, 4096, 12900), (100, 2048, 25700), (120, 4096, 12900),
+                                   (190, 2048, 25700), (190, 1024, 51300)])
+def test_weights_of_more_than_96_mb_in_one_pass(dev, M, K, N):
+    """they are read past the caches"""
+    run(dev, M, K, N, "bf16", "fp32")
+
+
 @pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
 @pytest.mark.parametrize("M,K,N", [(37, 136, 72), (19, 72, 65), (24, 72, 16930), (38, 72, 8198), (72, 72, 8460), (134, 64, 9036), (143, 728, 17065),
                                    (133, 64, 18196), (258, 80, 22286), (622, 64, 16930), (18, 72, 8309), (67, 392, 4290), (143, 968, 18257),
