@@ -65,8 +65,9 @@ struct VerifyParams {
 };
 
 // 2^t for t <= 0, not far below -1100: 2^n by the exponent, 2^f, |f| <= 1/2, as 1 + f P(f), P the interpolation of
-// (2^f - 1) / f at the nine Chebyshev points of the interval (3.7e-14 relative).  2^0 is exactly 1: equal logits weigh the same
-// whole number, so sums of them are exact.
+// (2^f - 1) / f at the nine Chebyshev points of the interval (3.7e-14 relative).  2^0 is exactly 1, and every t here is a
+// difference of logits times k, so a row's largest logits weigh exactly 1: sums over a row of equals are whole numbers, and a
+// token at a border of theirs is the definition's.
 #define EXP2_1 0.6931471805599453
 #define EXP2_2 0.2402265069581299
 #define EXP2_3 0.055504108664760424
@@ -108,18 +109,17 @@ __device__ __forceinline__ double weight_of(float l, float top, double k) {
     return t > -1100.0 ? exp2_neg(t) : 0.0;
 }
 // The same for many logits of a row: where nothing is out of the ordinary, a clamp in fp32 stands for all cases (NaN, -inf and
-// what weighs nothing become 2^-1200, which is 0), and (l - top) k is one FMA (top k is off by 2^-53 of itself).  Eight at a
-// time, so that the chains of FMAs hide each other's latency, with the coefficients in scalar registers (as literals they
-// cost two moves an FMA): 17 instructions a logit, 39 one by one.
+// what weighs nothing become 2^-1200, which is 0).  (l k - top k as one FMA saves an instruction, but leaves the rounding of
+// top k in the weight of the largest logit.)  Eight at a time, so that the chains of FMAs hide each other's latency, with the
+// coefficients in scalar registers (as literals they cost two moves an FMA): 18 instructions a logit, 39 one by one.
 struct Weigh {
-    double k, shift;
+    double k;
     float low, top;
     bool plain;
     __device__ __forceinline__ Weigh(float top_, double k_) : k(k_), top(top_) {
         low = (float)((double)top - 1200.0 / k);
-        shift = -(double)top * k;
         const double least = ((double)top - (double)low) * k;
-        plain = fabsf(top) < 1e30f && k > 1e-20 && k < 1e20 && least > 1100.0 && least < 1e6 && fabs(shift) < 1e4;
+        plain = fabsf(top) < 1e30f && k > 1e-20 && k < 1e20 && least > 1100.0 && least < 1e6;
         plain = __builtin_amdgcn_readfirstlane(plain);
     }
     template <typename R> __device__ __forceinline__ void operator()(const R &r, double *w) const {
@@ -127,7 +127,7 @@ struct Weigh {
         double f[8], n[8];
         if (plain) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = fma((double)max3(r.get(j), low, low), k, shift);
+            for (int j = 0; j < 8; ++j) f[j] = ((double)max3(r.get(j), low, low) - (double)top) * k;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
