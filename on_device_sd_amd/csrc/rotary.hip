@@ -286,9 +286,9 @@ extern "C" int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head
                            const int32_t *src_index, int32_t n_store, int64_t num_slots, void *stream) {
     if (n < 0 || n_store < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || rotary_dim <= 0 || (rotary_dim & 1) ||
         (head_dim & 1) || rotary_dim > head_dim || n_axes < 1 || num_slots < 0) return ODSD_ERR_SHAPE;
-    // a token's columns and the rows of a call are counted in 31 bits
+    // a token's columns and the rows of a call are counted in 31 bits, the columns in steps of a workgroup's threads
     if (head_dim > 1024 || n_axes > 4 || (int64_t)n + n_store > 0x7fffffffLL ||
-        (int64_t)max(num_heads, num_kv_heads) * head_dim > 0x7fffffffLL) return ODSD_ERR_UNSUPPORTED;
+        (int64_t)max(num_heads, num_kv_heads) * head_dim > 0x7fffffffLL - ROT_THREADS) return ODSD_ERR_UNSUPPORTED;
     if (dtype != ODSD_DT_BF16 && dtype != ODSD_DT_F16) return ODSD_ERR_DTYPE;
     if (position_bytes != 4 && position_bytes != 8) return ODSD_ERR_DTYPE;
     RotaryParams p;
