@@ -777,8 +777,9 @@ static bool verify_sizes_ok(int32_t S, int32_t max_q, int32_t n_q, int32_t n_d, 
 extern "C" size_t odsd_verify_workspace_bytes(int32_t n_seqs, int32_t max_q_len, int32_t n_rows, int32_t n_drafts,
                                               int32_t vocab, int32_t has_draft_logits) {
     VerifyLayout l;
+    // a row of logits and one of tokens are stepped over in 31 bits, by chunks and by a workgroup's threads
     if (!verify_sizes_ok(n_seqs, max_q_len, n_rows, n_drafts, vocab) || vocab > 0x7fffffff - VER_CHUNK ||
-        !verify_layout(n_seqs, n_rows, n_drafts, vocab, has_draft_logits != 0, l)) return 0;
+        max_q_len > 0x7fffffff - VER_THREADS || !verify_layout(n_seqs, n_rows, n_drafts, vocab, has_draft_logits != 0, l)) return 0;
     return l.total > 256 ? l.total : 256;
 }
 

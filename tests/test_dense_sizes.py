@@ -10,3 +10,11 @@ def test_rotary_rows_of_values_that_31_bits_cannot_step_over():
     for kv_heads, D in ((2 ** 30 - 1, 2), (2 ** 30 - 100, 2), ((2 ** 31 - 2) // 6, 6)):
         assert lib.odsd_rotary(P, D, D, P, kv_heads * D, D, P, kv_heads * D, D, 1, 1, kv_heads, D, D, 0, 1, P, 8, 1, 1, None, P, None, None, 1e-6, P,
                                None, P, P, P, None, 1, 64, None) == 3
+
+
+def test_verify_token_rows_that_31_bits_cannot_step_over():
+    lib = _lib.load()
+    for longest in (2 ** 31 - 1, 2 ** 31 - 256):
+        assert lib.odsd_verify_workspace_bytes(1, longest, 1, 0, 100, 0) == 0
+        assert lib.odsd_verify_drafts(P, 100, None, 100, 0, None, None, None, 1.0, None, P, 1, longest, 1, 0, 100, P, P, None, P, 1 << 30, None) == 3
+    assert lib.odsd_verify_workspace_bytes(1, 2 ** 31 - 257, 1, 0, 100, 0) >= 256
