@@ -712,8 +712,11 @@ template <typename T, typename O> static int launch_linear(LinearParams &p, cons
     return ODSD_OK;
 }
 
+// the grid's second dimension and the 32-bit products inside the kernels
+static bool linear_sizes_supported(int M, int N, int K) { return M <= 64 * 65535 && N <= 0x7fffffff - 256 && K <= 0x7fffffff - 256; }
+
 extern "C" size_t odsd_linear_workspace_bytes(int32_t M, int32_t N, int32_t K) {
-    if (M < 0 || N <= 0 || K <= 0) return 0;
+    if (M < 0 || N <= 0 || K <= 0 || !linear_sizes_supported(M, N, K)) return 0;
     const LinearPlan l = linear_plan(M, N, K, K % 8 == 0);      // (pointers that are not aligned need no more)
     return !l.fits ? 0 : l.bytes > 256 ? l.bytes : 256;
 }
@@ -725,8 +728,7 @@ extern "C" int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ld
     if (dtype != ODSD_DT_BF16 && dtype != ODSD_DT_F16) return ODSD_ERR_DTYPE;
     if (out_dtype != dtype && out_dtype != ODSD_DT_F32) return ODSD_ERR_DTYPE;
     if (act < ODSD_ACT_NONE || act > ODSD_ACT_GELU_TANH) return ODSD_ERR_UNSUPPORTED;
-    // the grid's second dimension and the 32-bit products inside the kernels
-    if (M > 64 * 65535 || N > 0x7fffffff - 256 || K > 0x7fffffff - 256) return ODSD_ERR_UNSUPPORTED;
+    if (!linear_sizes_supported(M, N, K)) return ODSD_ERR_UNSUPPORTED;
     if (M == 0) return ODSD_OK;
     if (!x || !w || !out) return ODSD_ERR_NULL;
     const uintptr_t oe = out_dtype == ODSD_DT_F32 ? 4 : 2;

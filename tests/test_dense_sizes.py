@@ -18,3 +18,12 @@ def test_verify_token_rows_that_31_bits_cannot_step_over():
         assert lib.odsd_verify_workspace_bytes(1, longest, 1, 0, 100, 0) == 0
         assert lib.odsd_verify_drafts(P, 100, None, 100, 0, None, None, None, 1.0, None, P, 1, longest, 1, 0, 100, P, P, None, P, 1 << 30, None) == 3
     assert lib.odsd_verify_workspace_bytes(1, 2 ** 31 - 257, 1, 0, 100, 0) >= 256
+
+
+def test_linear_workspace_query_answers_0_where_the_call_refuses():
+    lib = _lib.load()
+    for M, N, K in ((64 * 65535 + 1, 16, 64), (5_000_000, 7, 9), (2 ** 31 - 1, 16, 64), (4, 2 ** 31 - 1, 64), (4, 2 ** 31 - 256, 8), (4, 16, 2 ** 31 - 1),
+                    (100, 16, 2 ** 31 - 256)):
+        assert lib.odsd_linear(P, K, P, K, None, None, N, P, N, M, N, K, 1, 1, 0, P, 1 << 40, None) == 3, (M, N, K)
+        assert lib.odsd_linear_workspace_bytes(M, N, K) == 0, (M, N, K)
+    assert lib.odsd_linear_workspace_bytes(64 * 65535, 16, 64) >= 256
