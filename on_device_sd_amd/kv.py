@@ -20,7 +20,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .ops import _ptr, _raw_device, _same_device, _stream, _wrote
+from .ops import _INT32_MAX, _ptr, _raw_device, _same_device, _stream, _wrote
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -83,6 +83,8 @@ def _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_wei
     kv_heads = k_shape[1]
     if k_shape != (n, kv_heads, head_dim) or k.dtype != dtype:
         raise ValueError("q [n, heads, head_dim] and k [n, kv_heads, head_dim] must have the same tokens, head size and dtype")
+    if max(n, heads, kv_heads, head_dim, 0 if slot_mapping is None else slot_mapping.numel()) > _INT32_MAX:
+        raise _lib.OdsdError(f"rotary: unsupported sizes: {n} tokens of {heads} and {kv_heads} heads of {head_dim}")
     rotary_dim = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float64:
         raise TypeError("inv_freq must be float64: an angle is a position times a frequency")
