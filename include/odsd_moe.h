@@ -388,7 +388,8 @@ int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, co
  *   tokens       int64 [n_seqs, max_q_len]: the kept drafts, the drawn token, -1 behind it
  *   num_accepted int32 [n_seqs];  accept_probs fp32 [n_drafts]: min(1, p / q) of every draft, kept or not
  * max_q_len bounds query_lens (a longer sequence has its first max_q_len rows verified; 0: nothing is done or written).  A
- * sequence with query_lens 0 gets -1 only.  Without drafts and with as many rows as sequences query_lens is not read.  workspace: odsd_verify_workspace_bytes(...) bytes (0: sizes out of range), 16-byte aligned.
+ * sequence with query_lens 0 gets -1 only and takes no row (a batch with free places); rows behind the last sequence's are not
+ * drawn from.  workspace: odsd_verify_workspace_bytes(...) bytes (0: sizes out of range), 16-byte aligned.
  * Stands in for the acceptance of a verify step (demo/src/execution/cb_executor.py:261-300) in the sampled form of
  * pre_exp/moe_spec_acc_rate_benchmark/spec_sampling.py:3-198. */
 int odsd_verify_drafts(const void *logits, int64_t logits_stride, const void *draft_logits,

@@ -432,12 +432,13 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
         for (int j = dstart + max(n - 1, 0) + (int)threadIdx.x; j < d_end; j += VER_THREADS) p.accept_probs[j] = 0.0f;
     }
     const double k = factor_of(t);
-    if (threadIdx.x == 0) {
-        s_choice = Choice{n > 0 ? start : -1, -1, 0, -1, -1, 0.0f, 0.0f, 0, k};
-        s_done = false;
-    }
-    __syncthreads();
+    Choice c{n > 0 ? start : -1, -1, 0, -1, -1, 0.0f, 0.0f, 0, k};
     if (p.n_d > 0) {
+        if (threadIdx.x == 0) {
+            s_choice = c;
+            s_done = false;
+        }
+        __syncthreads();
         const bool with_q = p.draft_logits && k > 0.0;
         for (int j0 = 0; j0 < n; j0 += 32) {
             const int rows = min(32, n - j0), drafts = min(32, n - 1 - j0);
@@ -499,8 +500,8 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
             __syncthreads();
             if (s_done && !writes) break;
         }
+        c = s_choice;
     }
-    const Choice c = s_choice;
     if (writes) {
         int64_t *out = p.tokens + (int64_t)s * p.max_q;
         // (the token behind the kept ones is the draw's, unless it is known here)
@@ -829,8 +830,6 @@ extern "C" int odsd_verify_drafts(const void *logits, int64_t logits_stride, con
     const uintptr_t mask = dtype == ODSD_DT_F32 ? 3 : 1;
     if ((((uintptr_t)logits | (uintptr_t)draft_logits) & mask) || !odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
     if (workspace_bytes < need) return ODSD_ERR_WORKSPACE;
-    // (no drafts, a row for every sequence: their lengths are 1)
-    if (n_drafts == 0 && n_rows == n_seqs) query_lens = nullptr;
     VerifyLayout l;
     verify_layout(n_seqs, n_rows, n_drafts, vocab, draft_logits != nullptr, l);
     char *ws = (char *)workspace;

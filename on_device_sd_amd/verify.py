@@ -41,7 +41,8 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
     max(p - q, 0) at the first draft that is not kept, or from p behind the last: the lowest token whose cumulative weight
     exceeds sample_u times the total.  All sums in fp64.  -inf masks a token (a filter for the likeliest tokens is applied
     to the logits before).  Without drafts (``draft_tokens`` and ``accept_u`` None; a decode context) one token per row is
-    drawn.  ``max_query_len`` is read from the context; without it tokens has as many columns as there are rows."""
+    drawn; lengths of 0 and 1, where the context has them, say which sequences of a padded batch have a row (the others get -1).
+    ``max_query_len`` is read from the context; without it tokens has as many columns as there are rows."""
     dev = logits.get_device()
     lens = context.get("verify_query_lens")
     t_tensor = temperature if isinstance(temperature, torch.Tensor) else None
