@@ -253,6 +253,13 @@ __device__ __forceinline__ uint4_t descriptor(const void *base, uint32_t bytes) 
     return r;
 }
 
+// What the lanes of a wavefront wrote to LDS before is what its lanes read behind (and the other way round): the hardware keeps
+// a wavefront's LDS accesses in order, this keeps the compiler from moving them; no instruction.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ONCE: the weights are read past the caches
 template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES, int KS, bool ONCE>
 __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(LinearParams p) {
@@ -385,8 +392,9 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
                     for (int u = 0; u < 4; ++u) v[u] = acc[a0 + a][c][4 * q + u];
                     *(float4_t *)(stage + m * (PIECES * 16) + ((piece ^ swz(m)) << 4)) = v;
                 }
-        // one share of K: a wavefront's own LDS accesses stay in order; several: each adds up its part of the tokens
+        // several shares of K: each adds up its part of the tokens; one: a wavefront's own LDS accesses stay in order
         if (KS > 1) __syncthreads();
+        else wave_lds_order();
         constexpr int LANES = PIECES / 2, ROUND = 64 / LANES;  // lanes that share a token's row, rows at a time
         const int pc = lane % LANES * 2, n = n0 + (wn * FA + a0) * 32 + pc * 4;
         auto rows = [&](auto leave) {
@@ -422,7 +430,7 @@ __global__ __launch_bounds__(NWN * NWM * KS * 64) void linear_tile_kernel(Linear
             with_activation(p.act, [&](auto act) { rows([&](int m, const float *v) { finish8<T, O, decltype(act)::value>(p, m, n, v, bias); }); });
         }
         if (KS > 1 && FA > C::CH) __syncthreads();
-        asm volatile("" ::: "memory");
+        else wave_lds_order();
     }
 }
 
