@@ -56,8 +56,8 @@ extern "C" {
  * 113: odsd_moe_static_init
  * 114: odsd_moe_stack_forward, odsd_moe_stack_forward_events
  * 115: odsd_route_dispatch_host_counts
- * (odsd_linear, odsd_rotary and odsd_verify_drafts came under the same number: a host that may meet an older library looks
- * their symbols up) */
+ * (odsd_linear, odsd_linear_plan, odsd_rotary and odsd_verify_drafts came under the same number: a host that may meet an
+ * older library looks their symbols up) */
 #define ODSD_VERSION 115
 
 typedef enum odsd_status {
@@ -344,6 +344,14 @@ int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const vo
                 int64_t ldr, void *out, int64_t ldo, int32_t M, int32_t N, int32_t K, int32_t dtype,
                 int32_t out_dtype, int32_t act, void *workspace, size_t workspace_bytes, void *stream);
 size_t odsd_linear_workspace_bytes(int32_t M, int32_t N, int32_t K);
+/* How odsd_linear runs a call of these sizes and row distances (aligned: x and w lie at multiples of 16 bytes), as 7 numbers:
+ *   plan[0]  0: rows of w, for few tokens; 1: the kernel for any alignment; 2: tiles of n by m
+ *   plan[1], plan[2]  n and m of a workgroup;  plan[3]  groups of its wavefronts that share K (2: tiles);  plan[4]  parts of K
+ *            (more than 1: their sums are joined by a second launch)
+ *   plan[5]  columns that both operands are packed to first, or 0;  plan[6]  1 if the weights are read past the caches
+ * ODSD_ERR_SHAPE or ODSD_ERR_UNSUPPORTED for sizes that the call does not take (M = 0 among them).  A planning query for tests and
+ * measurement; the answers change with the estimates behind them. */
+int odsd_linear_plan(int32_t M, int32_t N, int32_t K, int64_t ldx, int64_t ldw, int32_t aligned, int32_t *plan);
 
 /* Rotary positions of a step's queries and keys, with the per-head RMSNorm in front and the KV-cache store behind them.
  *   q [n, num_heads, head_dim], k / v [n, num_kv_heads, head_dim]: a head's elements consecutive, tokens and heads any

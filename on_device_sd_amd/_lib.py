@@ -71,6 +71,7 @@ SIGNATURES = {
     "odsd_linear": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64, _P, C.c_int64] + [C.c_int32] * 6
                     + [_P, C.c_size_t, _P]),
     "odsd_linear_workspace_bytes": (C.c_size_t, [C.c_int32] * 3),
+    "odsd_linear_plan": (C.c_int, [C.c_int32] * 3 + [C.c_int64] * 2 + [C.c_int32, C.POINTER(C.c_int32)]),
     "odsd_rotary": (C.c_int, [_P, C.c_int64, C.c_int64] * 3 + [C.c_int32] * 7 + [_P, C.c_int32, C.c_int32, C.c_int64]
                     + [_P] * 4 + [C.c_float] + [_P] * 6 + [C.c_int32, C.c_int64, _P]),
     "odsd_verify_drafts": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int32, _P, _P, _P, C.c_float, _P, _P]

@@ -650,6 +650,14 @@ static LinearPlan linear_plan(int M, int N, int K, bool aligned) {
     return linear_plan_of(LIN_ANY, 1, M, N, K);
 }
 
+// One pass over weights of more than a third of the 256 MB cache: nothing of them is there at the next call, so they do not
+// displace what is (M = 64, K 2048, N 32768 33.9 -> 31.4 us, M = 33, K 4096, N 65536 107 -> 93, M = 180, K 2048, N 65536 82 ->
+// 74).  Smaller ones, called again soon, come out of it (M = 64, K 2048, N 16384 15.0, past it 20.5; not called again 21.1 /
+// 19.6), and so do the ends of rows that are no whole lines of 128 bytes (M = 96, K 3000, N 36000 89 / 92).
+static bool linear_past_caches(int tile_m, int M, int N, int K, int64_t ldw) {
+    return tile_m < 256 && M <= tile_m && (int64_t)N * K * 2 >= (96 << 20) && ldw % 64 == 0;
+}
+
 template <typename T, typename O, int NWN, int NWM, int FA, int FB, int STAGES, int KS = 1>
 static void launch_tile(LinearParams &p, hipStream_t st) {
     typedef LinearTile<NWN, NWM, FA, FB, STAGES, KS> C;
@@ -657,12 +665,8 @@ static void launch_tile(LinearParams &p, hipStream_t st) {
     p.tiles_m = (p.M + C::TM - 1) / C::TM;
     const int64_t total = (int64_t)p.tiles_n * p.tiles_m * p.slices;
     const unsigned grid = (unsigned)((total + 7) / 8 * 8), threads = C::NW * KS * 64;
-    // One pass over weights of more than a third of the 256 MB cache: nothing of them is there at the next call, so they do
-    // not displace what is (M = 64, K 2048, N 32768 33.9 -> 31.4 us, M = 33, K 4096, N 65536 107 -> 93, M = 180, K 2048, N 65536
-    // 82 -> 74).  Smaller ones, called again soon, come out of it (M = 64, K 2048, N 16384 15.0, past it 20.5; not called again
-    // 21.1 / 19.6), and so do the ends of rows that are no whole lines of 128 bytes (M = 96, K 3000, N 36000 89 / 92).
     if constexpr (C::TM < 256) {
-        if (p.tiles_m == 1 && (int64_t)p.N * p.K * 2 >= (96 << 20) && p.ldw % 64 == 0) {
+        if (linear_past_caches(C::TM, p.M, p.N, p.K, p.ldw)) {
             linear_tile_kernel<T, O, NWN, NWM, FA, FB, STAGES, KS, true><<<grid, threads, 0, st>>>(p);
             return;
         }
@@ -729,6 +733,26 @@ extern "C" size_t odsd_linear_workspace_bytes(int32_t M, int32_t N, int32_t K) {
     return !l.fits ? 0 : l.bytes > 256 ? l.bytes : 256;
 }
 
+// rows of whole 16-byte segments, and a tile's rows within 31 bits of bytes
+static bool linear_rows_aligned(int K, int64_t ldx, int64_t ldw) { return ((K | ldx | ldw) & 7) == 0 && ldx < (1 << 21) && ldw < (1 << 21); }
+
+extern "C" int odsd_linear_plan(int32_t M, int32_t N, int32_t K, int64_t ldx, int64_t ldw, int32_t aligned, int32_t *plan) {
+    if (!plan) return ODSD_ERR_NULL;
+    if (M <= 0 || N <= 0 || K <= 0 || ldx < K || ldw < K) return ODSD_ERR_SHAPE;
+    if (!linear_sizes_supported(M, N, K)) return ODSD_ERR_UNSUPPORTED;
+    const LinearPlan l = linear_plan(M, N, K, aligned && linear_rows_aligned(K, ldx, ldw));
+    if (!l.fits) return ODSD_ERR_UNSUPPORTED;
+    const bool tiles = l.kind > LIN_ANY;
+    plan[0] = tiles ? 2 : l.kind;
+    plan[1] = TILE_N[l.kind];
+    plan[2] = TILE_M[l.kind];
+    plan[3] = SHARES[l.kind];
+    plan[4] = l.slices;
+    plan[5] = l.Kp;
+    plan[6] = tiles && linear_past_caches(TILE_M[l.kind], M, N, l.Kp ? l.Kp : K, l.Kp ? l.Kp : ldw);
+    return ODSD_OK;
+}
+
 extern "C" int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *residual,
                            int64_t ldr, void *out, int64_t ldo, int32_t M, int32_t N, int32_t K, int32_t dtype,
                            int32_t out_dtype, int32_t act, void *workspace, size_t workspace_bytes, void *stream) {
@@ -743,8 +767,7 @@ extern "C" int odsd_linear(const void *x, int64_t ldx, const void *w, int64_t ld
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias) & 1) || (((uintptr_t)out | (uintptr_t)residual) & (oe - 1)) ||
         !odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
     LinearParams p{x, w, bias, residual, out, ldx, ldw, ldr, ldo, M, N, K, act, 0, 0, 1, 0, nullptr, 0};
-    // rows of whole 16-byte segments, and a tile's rows within 31 bits of bytes
-    const bool aligned = ((K | ldx | ldw) & 7) == 0 && odsd_aligned16(x) && odsd_aligned16(w) && ldx < (1 << 21) && ldw < (1 << 21);
+    const bool aligned = odsd_aligned16(x) && odsd_aligned16(w) && linear_rows_aligned(K, ldx, ldw);
     const LinearPlan l = linear_plan(M, N, K, aligned);
     if (!l.fits) return ODSD_ERR_UNSUPPORTED;
     if (l.bytes && !workspace) return ODSD_ERR_NULL;
