@@ -39,8 +39,9 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
 
     Draft j of a sequence is kept while accept_u_j < min(1, p_j / q_j) of its token; then one token is drawn, from
     max(p - q, 0) at the first draft that is not kept, or from p behind the last: the lowest token whose cumulative weight
-    exceeds sample_u times the total.  All sums in fp64.  -inf masks a token (a filter for the likeliest tokens is applied
-    to the logits before).  Without drafts (``draft_tokens`` and ``accept_u`` None; a decode context) one token per row is
+    exceeds sample_u times the total.  What a token is drawn from is summed in fp64; whether a draft is kept, and accept_probs,
+    come from fp32 statistics, good to 2.4e-6 of p / q.  -inf masks a token (a filter for the likeliest tokens is applied to
+    the logits before).  Without drafts (``draft_tokens`` and ``accept_u`` None; a decode context) one token per row is
     drawn; lengths of 0 and 1, where the context has them, say which sequences of a padded batch have a row (the others get -1).
     ``max_query_len`` is read from the context; without it tokens has as many columns as there are rows."""
     dev = logits.get_device()
