@@ -20,7 +20,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .ops import _INT32_MAX, _ptr, _raw_device, _same_device, _stream, _wrote
+from .ops import _ptr, _raw_device, _same_device, _stream, _wrote
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -83,7 +83,8 @@ def _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_wei
     kv_heads = k_shape[1]
     if k_shape != (n, kv_heads, head_dim) or k.dtype != dtype:
         raise ValueError("q [n, heads, head_dim] and k [n, kv_heads, head_dim] must have the same tokens, head size and dtype")
-    if max(n, heads, kv_heads, head_dim, 0 if slot_mapping is None else slot_mapping.numel()) > _INT32_MAX:
+    n_store = 0 if slot_mapping is None else slot_mapping.numel()
+    if (n | heads | kv_heads | head_dim | n_store) >> 31:      # (sizes are 31 bits in the library)
         raise _lib.OdsdError(f"rotary: unsupported sizes: {n} tokens of {heads} and {kv_heads} heads of {head_dim}")
     rotary_dim = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float64:
@@ -123,7 +124,7 @@ def _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_wei
         pos_strides = positions.stride()
     inv_freq = inv_freq.contiguous()
     vp = kcp = vcp = slots = src = None
-    vs0 = vs1 = n_store = num_slots = 0
+    vs0 = vs1 = num_slots = 0
     if k_cache is not None:
         D = kv_heads * head_dim
         cache_shape = k_cache.shape
@@ -137,7 +138,7 @@ def _rotary(q, k, v, positions, inv_freq, sections, interleaved, q_weight, k_wei
             v_strides = v.stride()
         vs0, vs1 = v_strides[0], v_strides[1]
         slot_mapping = _int32_row(slot_mapping)
-        n_store, num_slots = slot_mapping.numel(), k_cache.numel() // D
+        num_slots = k_cache.numel() // D
         if src_index is not None:
             src_index = _int32_row(src_index)
             src = src_index.data_ptr()

@@ -192,7 +192,6 @@ def _same_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError("runs on the GPU only, all tensors on the same one (there is no CPU fallback)")
 
 
-_INT32_MAX = 0x7fffffff                # sizes are 32 bits in the library; ctypes cuts a larger number off without an error
 _NO_WORKSPACE = 256                    # what odsd_linear_workspace_bytes answers where nothing is split
 
 
@@ -240,7 +239,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if not shape or shape[-1] != K or K == 0:
         raise ValueError(f"x {tuple(shape)} and weight {tuple(weight.shape)} do not belong together")
     M = shape[0] if len(shape) == 2 else x.numel() // K
-    if M > _INT32_MAX or N > _INT32_MAX or K > _INT32_MAX:
+    if (M | N | K) >> 31:                              # (sizes are 31 bits in the library; ctypes cuts more off without an error)
         raise _lib.OdsdError(f"linear: unsupported sizes: {M} rows of {K} by {N}")
     out_shape = shape[:-1] + (N,)
     bp = rp = None

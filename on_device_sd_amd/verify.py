@@ -13,7 +13,7 @@ from typing import Dict, Optional, Union
 import torch
 
 from . import _lib
-from .ops import _INT32_MAX, _ptr, _raw_device, _rows, _same_device, _stream
+from .ops import _ptr, _raw_device, _rows, _same_device, _stream
 
 _DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
@@ -83,7 +83,7 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: Optional[torch.Tensor], co
             lens = lens.to(device=logits.device, dtype=torch.int32)
         lens = lens.contiguous()
         longest = context.get("max_query_len", rows)
-    if max(n_seqs, longest, rows, n_drafts, vocab) > _INT32_MAX:
+    if (n_seqs | longest | rows | n_drafts | vocab) >> 31:     # (sizes are 31 bits in the library)
         raise _lib.OdsdError(f"verify_drafts: unsupported sizes: {n_seqs} sequences of up to {longest} rows, {n_drafts} drafts, "
                              f"{rows} rows of {vocab}")
     ld_draft = vocab
