@@ -392,9 +392,9 @@ __device__ __forceinline__ Stat row_stat(const VerifyParams &p, int row, double 
 
 // ---- which drafts stay -----------------------------------------------------------------------------
 // By a whole workgroup; every workgroup of a sequence comes to the same answer, one (`writes`) leaves it.  Rows in batches of
-// 32: their statistics by 16 lanes each, then a lane per draft.  Without drafts in the call there are no statistics and
-// nothing to decide.
-template <typename T>
+// 32: their statistics by 16 lanes each, then a lane per draft.  Without drafts in the call (DRAFTS: there may be some) there are
+// no statistics and nothing to decide but the row.
+template <typename T, bool DRAFTS>
 __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) {
     __shared__ int s_start[4], s_dstart[4];
     __shared__ Stat s_p[32], s_q[32];
@@ -408,10 +408,10 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
         for (int i = threadIdx.x; i < s; i += VER_THREADS) {
             const int n = len_of(p, i);
             start = wrapping_plus(start, n);
-            dstart = wrapping_plus(dstart, max(n - 1, 0));
+            if (DRAFTS) dstart = wrapping_plus(dstart, max(n - 1, 0));
         }
         start = all_sum(start);
-        dstart = all_sum(dstart);
+        if (DRAFTS) dstart = all_sum(dstart);
         if (lane_id() == 0) {
             s_start[wave] = start;
             s_dstart[wave] = dstart;
@@ -433,7 +433,7 @@ __device__ Choice choose(const VerifyParams &p, const int s, const bool writes) 
     }
     const double k = factor_of(t);
     Choice c{n > 0 ? start : -1, -1, 0, -1, -1, 0.0f, 0.0f, 0, k};
-    if (p.n_d > 0) {
+    if (DRAFTS && p.n_d > 0) {
         if (threadIdx.x == 0) {
             s_choice = c;
             s_done = false;
@@ -521,7 +521,7 @@ template <typename T>
 __global__ __launch_bounds__(VER_THREADS) void verify_choose_kernel(VerifyParams p) {
     __shared__ double s_z[2][4];
     const int s = blockIdx.y;
-    const Choice c = choose<T>(p, s, blockIdx.x == 0);
+    const Choice c = choose<T, true>(p, s, blockIdx.x == 0);
     if (c.row < 0 || c.greedy >= 0 || c.draft < 0) return;
     Raw8<T> rp[4], rq[4];
     const T *lp = (const T *)p.logits + (int64_t)c.row * p.ld_t, *lq = (const T *)p.draft_logits + (int64_t)c.draft * p.ld_d;
@@ -613,12 +613,15 @@ __device__ __forceinline__ void load_pair(const VerifyParams &p, const Choice &c
 }
 
 // ---- sums of the weights that the next token is drawn from -------------------------------------------
-template <typename T, bool CHOSEN>
+// Which row: chosen by the launch before (draft logits), by this one (drafts without), or no drafts in the call.  (The last as
+// an instance of its own: without the drafts' registers a CU holds five workgroups of fp32 logits instead of three.)
+enum { VER_CHOSEN, VER_CHOOSE, VER_SAMPLE };
+template <typename T, int ROW>
 __global__ __launch_bounds__(VER_THREADS) void verify_sums_kernel(VerifyParams p) {
     const int s = blockIdx.y;
     Choice c;
-    if (CHOSEN) c = p.choice[s];
-    else c = choose<T>(p, s, blockIdx.x == 0);
+    if (ROW == VER_CHOSEN) c = p.choice[s];
+    else c = choose<T, ROW == VER_CHOOSE>(p, s, blockIdx.x == 0);
     if (c.row < 0 || c.greedy >= 0) return;
     Raw8<T> r[4], q[4];
     const int sub0 = blockIdx.x * (VER_CHUNK / VER_SUB) + (int)(threadIdx.x >> 6);
@@ -802,9 +805,11 @@ template <typename T> static int launch_verify(VerifyParams &p, void *padded, hi
     if (p.n_d > 0 && p.n_q > 0) verify_stats_kernel<T><<<(unsigned)((p.n_q + (p.draft_logits ? p.n_d : 0)) * p.splits), VER_THREADS, 0, st>>>(p);
     if (p.draft_logits) {
         verify_choose_kernel<T><<<chunks, VER_THREADS, 0, st>>>(p);
-        verify_sums_kernel<T, true><<<chunks, VER_THREADS, 0, st>>>(p);
+        verify_sums_kernel<T, VER_CHOSEN><<<chunks, VER_THREADS, 0, st>>>(p);
+    } else if (p.n_d > 0) {
+        verify_sums_kernel<T, VER_CHOOSE><<<chunks, VER_THREADS, 0, st>>>(p);
     } else {
-        verify_sums_kernel<T, false><<<chunks, VER_THREADS, 0, st>>>(p);
+        verify_sums_kernel<T, VER_SAMPLE><<<chunks, VER_THREADS, 0, st>>>(p);
     }
     verify_draw_kernel<T><<<(unsigned)p.S, 64, 0, st>>>(p);
     ODSD_CHECK_LAUNCH();
