@@ -600,7 +600,7 @@ static LinearPlan linear_plan_aligned(int M, int N, int K, float *us) {
     // 64 x 64, which is for single m tiles: the weights' bytes count there, and how many are on their way) takes a step's time
     // for every 64 columns of a share of K, and its epilogue.  The bytes are a second bound; what the shorter one adds is a root
     // of fourth powers.  Parts of K cost a launch and their sums' way through memory.  The constants are fitted to 913 shapes of
-    // 5 to 8192 tokens (bf16, weights from memory); the estimate's choice is 0.9 % slower than the best on average, 20 % at worst.
+    // 5 to 8192 tokens (bf16, weights from memory), before the rule for weights read past the caches.
     // us of the shape taken / others, K 4096, N 4096: M = 200 (64 x 64, K shared by 2) 17.5 / 20 (64 x 128, 2 parts), 22 (128 x
     // 128, 4 parts); M = 512 (64 x 128) 28 / 31 (128 x 128, 2 parts), 39 (64 x 64); M = 1000 (128 x 128) 40 / 43 (128 x 192), 53
     // (64 x 128); M = 1536 (128 x 192) 52 / 56 (128 x 256), 73 (128 x 128); M = 4096 (256 x 256) 110 / 124 (128 x 256).  K 2048, N

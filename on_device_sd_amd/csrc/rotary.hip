@@ -122,8 +122,8 @@ __device__ __forceinline__ void rotary_turn(float *x, const float2 *cs) {
 
 // Everything in pieces of eight 16-bit values, 16-byte aligned.  A head's units (two pieces each) lie on LG neighbouring lanes,
 // which add up its squares; a thread's first unit is requested before the angles are made, so that its way from memory and
-// the sines hide each other.  Bytes bound it: 16384 tokens of 32 + 4 heads of 128 on three axes in 54 to 59 us, 5.1 to
-// 5.6 TB/s; two units a thread 60, four 69 (fewer workgroups at once); one token a workgroup for the keys, too, 73 to 84.
+// the sines hide each other.  Bytes bound it: 16384 tokens of 32 + 4 heads of 128 on three axes in 57 to 61 us, 4.9 to
+// 5.3 TB/s; two units a thread 60, four 69 (fewer workgroups at once); one token a workgroup for the keys, too, 73 to 84.
 template <typename T, bool SIDE, typename POS>
 __global__ __launch_bounds__(ROT_THREADS) void rotary_wide_kernel(RotaryParams p, int LG) {
     typedef T T8 __attribute__((ext_vector_type(8)));
@@ -203,7 +203,8 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_wide_kernel(RotaryParams p
     }
 }
 
-// Any head size, strides and alignment: value by value, a unit is one pair; a head's units lie on LG lanes in turns.
+// Any head size, strides and alignment: value by value, a unit is one pair; a head's units lie on LG lanes in turns.  16384 tokens
+// of 32 + 4 heads of 128 without norms, 2 bytes off alignment: 142 us, 2.1 TB/s (aligned, by the kernel above: 60).
 template <typename T, bool SIDE, typename POS>
 __global__ __launch_bounds__(ROT_THREADS) void rotary_any_kernel(RotaryParams p, int LG) {
     extern __shared__ float2 trig[];
