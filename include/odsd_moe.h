@@ -394,8 +394,9 @@ int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, co
  * kept (from p_j where that is zero everywhere), or from the row behind the last.  Drawn: the lowest token whose inclusive
  * cumulative weight exceeds sample_u times the total.  Greedy: p is one-hot at the largest logit, the lowest index of equals.
  * The weights that a token is drawn from and their sums are fp64.  Whether a draft is kept, and accept_probs, come from fp32
- * statistics of the rows: each probability is good to 1.2e-6 of itself, p / q to 2.4e-6.  -inf masks a token, NaN counts as -inf; a row with +inf has its weight on those; a draft outside the
- * vocabulary is not kept; a row with no number above -inf keeps no draft and draws -1.
+ * statistics of the rows: each probability is good to 1.2e-6 of itself, p / q to 2.4e-6.
+ * -inf masks a token, NaN counts as -inf; a row with +inf has its weight on those; a draft outside the vocabulary is not kept; a
+ * row with no number above -inf keeps no draft and draws -1.
  *   tokens       int64 [n_seqs, max_q_len]: the kept drafts, the drawn token, -1 behind it
  *   num_accepted int32 [n_seqs];  accept_probs fp32 [n_drafts]: min(1, p / q) of every draft, kept or not
  * max_q_len bounds query_lens (a longer sequence has its first max_q_len rows verified; 0: nothing is done or written).  A
