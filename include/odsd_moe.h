@@ -40,6 +40,8 @@
  *   odsd_linear        F.linear around the block               demo/src/layers/attention.py:169-288
  *   odsd_rotary        q_norm / k_norm, rotary_emb, store      demo/src/layers/attention.py:209-228
  *   odsd_verify_drafts  acceptance of a verify step            demo/src/execution/cb_executor.py:261-300
+ *   odsd_kv_store_fp8, odsd_paged_attention_fp8, odsd_copy_blocks, odsd_adjust_logits   (no counterpart: the reference's cache is
+ *                      16 bits wide, never forks or moves blocks, and its acceptance is greedy)
  */
 #ifndef ODSD_MOE_H
 #define ODSD_MOE_H
@@ -56,8 +58,8 @@ extern "C" {
  * 113: odsd_moe_static_init
  * 114: odsd_moe_stack_forward, odsd_moe_stack_forward_events
  * 115: odsd_route_dispatch_host_counts
- * (odsd_linear, odsd_linear_plan, odsd_rotary and odsd_verify_drafts came under the same number: a host that may meet an
- * older library looks their symbols up) */
+ * (odsd_linear, odsd_linear_plan, odsd_rotary, odsd_verify_drafts, odsd_kv_store_fp8, odsd_paged_attention_fp8, odsd_copy_blocks and
+ * odsd_adjust_logits came under the same number: a host that may meet an older library looks their symbols up) */
 #define ODSD_VERSION 115
 
 typedef enum odsd_status {
@@ -311,6 +313,56 @@ size_t odsd_paged_attention_workspace_bytes(int32_t n_seqs, int32_t max_q_len, i
                                             int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                             int32_t max_blocks);
 
+/* ---- 8-bit KV cache -------------------------------------------------------------------------- */
+/* A cache of e4m3 numbers with a power-of-two scale for each block and KV head, one for K and one for V:
+ *   k_cache  [n_blocks, num_kv_heads, block_size, head_dim]
+ *   v_cache  [n_blocks, num_kv_heads, head_dim, block_size]     (transposed: what the attention multiplies by, as it lies)
+ *   scales   fp32 [n_blocks, num_kv_heads, 2]: K's, V's; 0: the block holds nothing (a new cache is zeroed)
+ * A value is its code times the scale.  head_dim 64 or 128; block_size a multiple of 16, 1024 at most; n_blocks * block_size and n_blocks *
+ * num_kv_heads below 2^31; caches 16-byte, scales 8-byte aligned.
+ *
+ * odsd_kv_store_fp8: rows of this step's keys and values to their slots, as odsd_kv_store: for i in [0, N)
+ *   row = src_index ? src_index[i] : i (then N == n_src);  slot = slot_mapping[i], block slot / block_size, token slot % block_size
+ * key / value [n_src, num_kv_heads, head_dim], a head's elements consecutive, tokens and heads any number of elements apart (16-byte aligned
+ * rows run the fast kernel), dtype ODSD_DT_BF16 or ODSD_DT_F16.  Rows without a slot (negative, beyond the cache) or without a row (src_index
+ * out of range) are not stored; of two with one slot the later is.
+ *   Scale of a block: the smallest power of two, 2^-64 at least, by which the largest |x| of the call's rows is 448 at most; the block's
+ *   present scale if that is larger.  When the scale rises, the codes of the rows that stay are rounded again (exact but for those below
+ *   2^-6 then).  A call that writes a block's token 0 starts the block anew: its scale is that of the call's rows alone, and codes of other
+ *   tokens are given up.  Rounding to nearest, ties to even; infinities become +-448 and do not count for the scale, NaN stays NaN.
+ * The same call gives the same bits.  (No counterpart in the reference.) */
+int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int64_t key_head_stride, const void *value,
+                      int64_t value_token_stride, int64_t value_head_stride, void *k_cache, void *v_cache, float *scales,
+                      const int32_t *slot_mapping, const int32_t *src_index, int32_t N, int32_t n_src,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t n_blocks, int32_t dtype,
+                      void *stream);
+
+/* odsd_paged_attention over that cache: the same queries, tables, lengths and masks, q and out of `dtype` (ODSD_DT_BF16 or ODSD_DT_F16).
+ * Position p of sequence s is token p % block_size of block block_tables[s][p / block_size]; an entry that is negative or beyond the cache reads
+ * block 0.  Rows that attend nothing (a context of 0) are zeros.  Products of the codes with q and sums in fp32; the weights (softmax times the
+ * scale of V, relative to the row's largest) are rounded to q's type once, the result once.  What a block holds behind a sequence's
+ * last key is never used, and a NaN reaches the rows that attend it only.  out 8-byte aligned.
+ * workspace: odsd_paged_attention_fp8_workspace_bytes(...) bytes (0: the call is refused), 16-byte aligned. */
+int odsd_paged_attention_fp8(const void *q, const void *k_cache, const void *v_cache, const float *scales,
+                             const int32_t *block_tables, const int32_t *context_lens, const int32_t *q_lens,
+                             int32_t n_seqs, int32_t max_q_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, int32_t max_blocks, int32_t n_blocks, float softmax_scale, int32_t dtype,
+                             void *out, void *workspace, size_t workspace_bytes, void *stream);
+size_t odsd_paged_attention_fp8_workspace_bytes(int32_t n_seqs, int32_t max_q_len, int32_t num_heads, int32_t num_kv_heads,
+                                                int32_t head_dim, int32_t block_size, int32_t max_blocks);
+
+/* Copies of whole blocks within every tensor of a cache (any type; K, V and scales of all layers together): block src[i] to block dst[i].
+ *   tensors      HOST array of n_tensors (ODSD_COPY_TENSORS at most) device pointers: [layers][n_blocks] blocks of block_bytes bytes, a
+ *                layer's blocks consecutive, layers layer_bytes apart;  block_bytes, layer_bytes, layers: HOST arrays
+ *   src, dst     HOST int32 [n_pairs] in [0, n_blocks): read before the call returns (and so frozen in a graph that captures it).  No block is
+ *                named twice in dst, or in both (the CALLER'S duty: copies run in any order); one may be in src more than once
+ *   block_tables device int32 [n_entries] or NULL: entries that equal src[i] become dst[i] (no block is in src twice then)
+ * (No counterpart in the reference.) */
+#define ODSD_COPY_TENSORS 16
+int odsd_copy_blocks(void *const *tensors, const int64_t *block_bytes, const int64_t *layer_bytes, const int32_t *layers,
+                     int32_t n_tensors, const int32_t *src, const int32_t *dst, int32_t n_pairs, int32_t n_blocks,
+                     int32_t *block_tables, int64_t n_entries, void *stream);
+
 /* Causal attention of a prefill step: variable-length sequences packed one after the other, keys
  * and values taken from the step's own k / v (no cache read).
  *   q [total_q, num_heads, head_dim], k / v [total_k, num_kv_heads, head_dim], contiguous
@@ -380,6 +432,29 @@ int odsd_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, co
                 const double *inv_freq, const void *q_weight, const void *k_weight, float eps, void *q_out,
                 void *k_out, void *k_cache, void *v_cache, const int32_t *slot_mapping,
                 const int32_t *src_index, int32_t n_store, int64_t num_slots, void *stream);
+
+/* Penalties for repeated tokens, biases and masks on the rows that odsd_verify_drafts takes next:
+ *   logits       [n_rows, vocab], rows logits_stride apart, ODSD_DT_F32 / BF16 / F16; out of the same type, rows out_stride apart (the same
+ *                rows as logits, or none of them)
+ *   query_lens   int32 [n_seqs] or NULL (one row each, n_rows == n_seqs): rows of each sequence, one after the other; rows behind the last
+ *                sequence's are not written
+ *   tokens       [n_seqs, max_tokens], rows token_stride apart, int32 or int64 (token_bytes 4 or 8), or NULL: prompt and output so far;
+ *                token_lens int32 [n_seqs] of them (NULL: max_tokens), of which the first prompt_lens[s] (NULL: none) are the prompt
+ *   draft_tokens int64 [n_drafts] or NULL: query_lens[s] - 1 for sequence s; row j of a sequence has seen its first j drafts as output
+ *   repetition, frequency, presence   fp32 [n_seqs], or NULL: repetition_all (> 0), frequency_all, presence_all for all
+ *   bias_tokens int32, bias_values fp32 [n_seqs, n_bias]: added to the logits of those tokens (of a token named twice the later entry)
+ *   mask         int32 [n_mask] rows of mask_stride words, or NULL: bit t % 32 of word t / 32 clear: token t is not allowed.  Row i has mask
+ *                mask_rows[i] (NULL: i); out of [0, n_mask): no mask
+ * In fp32, in this order, rounded once:  x > 0 ? x / repetition : x * repetition  for tokens of the prompt, the output or the drafts;  x -
+ * (frequency * n + presence [n > 0])  with n the times in output and drafts;  x + bias;  -inf where the mask forbids.  Tokens outside [0, vocab)
+ * count as none.  NaN stays NaN where the mask allows it.  (No counterpart in the reference: its acceptance is greedy.) */
+int odsd_adjust_logits(const void *logits, int64_t logits_stride, void *out, int64_t out_stride, int32_t dtype, int32_t n_rows,
+                       int32_t vocab, const int32_t *query_lens, int32_t n_seqs, const void *tokens, int32_t token_bytes,
+                       int64_t token_stride, int32_t max_tokens, const int32_t *token_lens, const int32_t *prompt_lens,
+                       const int64_t *draft_tokens, int32_t n_drafts, const float *repetition, float repetition_all,
+                       const float *frequency, float frequency_all, const float *presence, float presence_all,
+                       const int32_t *bias_tokens, const float *bias_values, int32_t n_bias, const int32_t *mask,
+                       int64_t mask_stride, int32_t n_mask, const int32_t *mask_rows, void *stream);
 
 /* Verification of drafted tokens against the target's probabilities from given random numbers (speculative sampling);
  * without drafts, the sampling of a decode step.

@@ -15,7 +15,9 @@ from .cache import LRUStrategy, W4ExpertCache, cache_capacity
 from .kv import (SequenceSlots, apply_rotary, attention_for_context, build_decode_context, build_prefill_context,
                  build_verify_context, get_attention_context, paged_attention, rotary_store_kvcache, store_kvcache,
                  varlen_attention)
-from .verify import VerifyResult, verify_drafts
+from .kv_fp8 import KVCacheFP8, paged_attention_fp8, store_kvcache_fp8
+from .blocks import BlockPool, copy_cache_blocks
+from .verify import VerifyResult, adjust_logits, verify_drafts
 
 __all__ = [
     "AttentionOutput", "ExpertID", "ExpertPlacement", "LayerOutput", "MoEConfig", "RoutingResult",
@@ -28,4 +30,5 @@ __all__ = [
     "SequenceSlots", "build_verify_context", "build_prefill_context", "build_decode_context",
     "get_attention_context", "attention_for_context", "paged_attention", "store_kvcache", "varlen_attention",
     "apply_rotary", "rotary_store_kvcache", "VerifyResult", "verify_drafts",
+    "KVCacheFP8", "store_kvcache_fp8", "paged_attention_fp8", "BlockPool", "copy_cache_blocks", "adjust_logits",
 ]

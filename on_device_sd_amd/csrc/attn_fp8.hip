@@ -1,0 +1,449 @@
+// Causal attention over the 8-bit paged cache: decode, verify, and a chunk of a prompt.
+//
+// With query row i, key j of block b(j), codes kc, vc and the block's scales sk, sv of the KV head:
+//   s_ij = scale * sk(b(j)) * sum_d q_id kc_jd                       (j <= L - ql + token of i)
+//   o_i  = sum_j exp(s_ij) sv(b(j)) vc_j / sum_j exp(s_ij)
+// The scale of V joins the exponent: w_ij = 2^(s_ij log2 e + log2 sv - m_i) is what the matrix product takes, m_i the running
+// maximum of that exponent, and l_i sums w_ij / sv in fp32: nothing depends on how far the scales of two blocks are apart, and w stays
+// within what fp16 holds.  Codes become 16-bit operands of q's type in registers (exact); products and sums are fp32; w is rounded to
+// q's type once (half a step, as in the kernels over 16-bit keys), the result once.
+//
+// A unit -- up to 16, 32 or 64 query rows of a (sequence, KV head) -- and the way units are cut into shares of keys are those of attn_list.h.
+// Each of the four wavefronts takes 64 keys of every 256 for all rows of the unit, with no barrier and no LDS in the loop: the cache
+// holds what the matrix instructions want as it lies.  A lane's 16 bytes of a K row are the k indices of two products (the query's
+// fragments have the same order); V is stored transposed, so 16 bytes are 16 keys of one dimension, and the rows of S^T = K Q^T are
+// dealt so that a lane (c, kq) gets the scores of keys 16 kq .. 16 kq + 15 of query row c: those of its own V bytes, as the B operand of
+// O^T = V^T P^T, and all in one block, whose scales are lane values.  The next tile's bytes are requested into the registers that the
+// present one has just left.
+#include "attn_list.h"
+#include "fp8.h"
+
+#define FP8_WG 512           // workgroups that share the keys: two per CU (one with 64 rows)
+#define FP8_STEP 256         // keys of a list step, 64 per wavefront
+#define FP8_WHOLE 512        // no sequence longer: nothing is split
+
+struct AttnFp8Params : AttnParams {
+    const float *scales;     // [n_blocks, KVH, 2]
+    int n_blocks;
+};
+
+template <typename T, int HD, int RB, bool ALIGNED, bool SPLIT>
+__global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const AttnFp8Params p) {
+    typedef typename AttnT<T>::V8 V8;
+    constexpr int NJ = HD / 32;          // 32-dim steps of the score product
+    constexpr int NC = HD / 64;          // 16-byte pieces of a K row per lane
+    constexpr int NDB = HD / 16;         // 16-dim blocks of the output
+    constexpr int ROWS = 16 * RB, XROW = HD + 4;
+    constexpr int MOST = ALIGNED ? 64 : 16;              // tiles whose blocks are looked up at a time
+    __shared__ __attribute__((aligned(16))) float xch[4 * 16 * XROW];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, kq = lane >> 4;
+
+    const ListPlan pl = list_plan<false, SPLIT, RB != 4 || !SPLIT, RB == 4>(p, ROWS, FP8_STEP, FP8_STEP, blockIdx.x);
+    if (!pl.found) return;
+    const int first_pos = pl.me * pl.share;
+    int pos = first_pos;                                   // list position of the next step
+    const int end = min(pl.total, pos + pl.share);
+    SeqAt sq = pl.at;
+    int unit = (pos - sq.first) / sq.steps;                // unit of the sequence, step inside the unit
+    int step = (pos - sq.first) - unit * sq.steps;
+
+    const int bs = p.block_size;
+    const uint32_t block_bytes = (uint32_t)(bs * HD);
+    const char *kc = (const char *)p.k_cache, *vc = (const char *)p.v_cache;
+    // K: the rows of product t are keys 16 (m / 4) + 4 t + m % 4; V: 16 keys of dimension 16 db + c
+    const uint32_t k_lane = (uint32_t)((ALIGNED ? 16 * (c >> 2) + (c & 3) : (c & 3)) * HD + 16 * kq);
+    const uint32_t v_lane = (uint32_t)(c * bs + (ALIGNED ? 16 * kq : 0));
+
+    while (pos < end) {
+        // ---- one piece: steps step .. step + n - 1 of one unit ----------------------------------------
+        const int n = min(end - pos, sq.steps - step);
+        const int kvh = unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);      // row groups with the most keys first
+        const int L = sq.L, ql = sq.ql;
+        const int rows_total = ql * p.Gq, row0 = rg * ROWS;
+        const int rows_here = min(ROWS, rows_total - row0);
+        const int32_t *bt = p.block_tables + (size_t)sq.seq * p.max_blocks;
+
+        V8 qf[RB][NJ];
+        int kmax[RB];                                      // last position that row attends
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int row = row0 + 16 * rb + c;
+            const bool ok = row < rows_total;
+            const int tok = ok ? row / p.Gq : 0, hq = ok ? row - tok * p.Gq : 0;
+            kmax[rb] = ok ? L - ql + tok : -1;
+            const uint16_t *qp = (const uint16_t *)p.q + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + 16 * kq;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {                 // dims 64 (j / 2) + 16 kq + 8 (j % 2) ..
+                uint4_t raw = {0u, 0u, 0u, 0u};
+                if (ok) raw = *(const uint4_t *)(qp + 64 * (j >> 1) + 8 * (j & 1));
+                qf[rb][j] = __builtin_bit_cast(V8, raw);
+            }
+        }
+        const int kmin = L - ql + row0 / p.Gq;            // the unit's first row: tiles that end at or before it need no mask
+
+        float m_run[RB], l_run[RB];
+        float4_t o[RB][NDB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            m_run[rb] = -INFINITY;
+            l_run[rb] = 0.0f;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) o[rb][db] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+
+        int key_end = step + n == sq.steps ? L : pl.g * (step + n);
+        if (RB == 4 && sq.rg > 1)                          // (no further than the unit's last row sees)
+            key_end = min(key_end, L - ql + min(ql, (row0 + ROWS - 1) / p.Gq + 1));
+        for (int key0 = pl.g * step + 64 * wave; key0 < key_end; key0 += MOST * FP8_STEP) {
+            const int nt = min(MOST, (key_end - key0 + FP8_STEP - 1) / FP8_STEP);
+            // the blocks of this wavefront's next tiles, one tile (ALIGNED: it lies in one block) or one group of 16 keys per lane;
+            // an entry that is negative or beyond the cache reads block 0, keys past the last one its group
+            const int kp = min(ALIGNED ? key0 + FP8_STEP * lane : key0 + FP8_STEP * (lane >> 2) + 16 * (lane & 3),
+                               ALIGNED ? (L - 1) & ~63 : (L - 1) & ~15);
+            const int blk = kp / bs;
+            const int32_t b = bt[min(blk, p.max_blocks - 1)];
+            const uint32_t gk_l = (b >= 0 && b < p.n_blocks && blk < p.max_blocks ? (uint32_t)b : 0u) * (uint32_t)p.KVH + (uint32_t)kvh;
+            const uint32_t off_l = (uint32_t)(kp - blk * bs);
+            const float2_t s2 = *(const float2_t *)(p.scales + 2 * (size_t)gk_l);
+            const float sc_l = p.scale_log2e * fmaxf(s2.x, FP8_MIN_SCALE), sv_l = fmaxf(s2.y, FP8_MIN_SCALE);
+            const float ev_l = __builtin_amdgcn_logf(sv_l), iv_l = __builtin_amdgcn_rcpf(sv_l);
+
+            uint4_t kreg[4][NC], vreg[NDB];
+            auto k_from = [&](const int i) {
+                const char *at;
+                if constexpr (ALIGNED)
+                    at = kc + (uint64_t)(uint32_t)lane_value((int)gk_l, i) * block_bytes + (uint32_t)lane_value((int)off_l, i) * (uint32_t)HD + k_lane;
+                else
+                    at = kc + (uint64_t)(uint32_t)__shfl((int)gk_l, 4 * i + (c >> 2), ODSD_WAVE) * block_bytes +
+                         (uint32_t)__shfl((int)off_l, 4 * i + (c >> 2), ODSD_WAVE) * (uint32_t)HD + k_lane;
+                return at;
+            };
+            auto v_from = [&](const int i) {
+                const char *at;
+                if constexpr (ALIGNED)
+                    at = vc + (uint64_t)(uint32_t)lane_value((int)gk_l, i) * block_bytes + (uint32_t)lane_value((int)off_l, i) + v_lane;
+                else
+                    at = vc + (uint64_t)(uint32_t)__shfl((int)gk_l, 4 * i + kq, ODSD_WAVE) * block_bytes +
+                         (uint32_t)__shfl((int)off_l, 4 * i + kq, ODSD_WAVE) + v_lane;
+                return at;
+            };
+            auto fetch_k = [&](const char *at, const int t) {
+#pragma unroll
+                for (int h = 0; h < NC; ++h) kreg[t][h] = __builtin_nontemporal_load((const uint4_t *)(at + 4 * t * HD + 64 * h));
+            };
+            auto fetch_v = [&](const char *at, const int db) {
+                vreg[db] = __builtin_nontemporal_load((const uint4_t *)(at + (uint32_t)(16 * db * bs)));
+            };
+            // one tile.  FETCH: there is a next one, whose bytes are requested as registers come free (the scheduling barriers keep
+            // the compiler from widening all of a tile first, which costs 64 registers)
+            auto tile = [&](auto fetch_c, const int i) {
+                const int k0 = key0 + FP8_STEP * i;
+                float sc, ev, iv;
+                if constexpr (ALIGNED) {
+                    sc = __uint_as_float((uint32_t)lane_value((int)__float_as_uint(sc_l), i));
+                    ev = __uint_as_float((uint32_t)lane_value((int)__float_as_uint(ev_l), i));
+                    iv = __uint_as_float((uint32_t)lane_value((int)__float_as_uint(iv_l), i));
+                } else {
+                    sc = __shfl(sc_l, 4 * i + kq, ODSD_WAVE);
+                    ev = __shfl(ev_l, 4 * i + kq, ODSD_WAVE);
+                    iv = __shfl(iv_l, 4 * i + kq, ODSD_WAVE);
+                }
+                float4_t st[RB][4];
+                const char *next = nullptr;
+                if constexpr (decltype(fetch_c)::value) next = k_from(i + 1);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) st[rb][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < NC; ++h) {
+                        const V8 lo = fp8_widen8<T>(kreg[t][h].x, kreg[t][h].y), hi = fp8_widen8<T>(kreg[t][h].z, kreg[t][h].w);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            st[rb][t] = AttnT<T>::mfma(lo, qf[rb][2 * h], st[rb][t]);
+                            st[rb][t] = AttnT<T>::mfma(hi, qf[rb][2 * h + 1], st[rb][t]);
+                        }
+                    }
+                    if constexpr (decltype(fetch_c)::value) fetch_k(next, t);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if constexpr (decltype(fetch_c)::value) next = v_from(i + 1);
+                const bool masked = k0 + 63 > kmin;
+                V8 pf[RB][2];
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    // lane (c, kq) holds keys k0 + 16 kq + 4 t + i of query row c
+                    float a[16];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        a[4 * t] = st[rb][t].x; a[4 * t + 1] = st[rb][t].y; a[4 * t + 2] = st[rb][t].z; a[4 * t + 3] = st[rb][t].w;
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) a[e] = k0 + 16 * kq + e <= kmax[rb] ? a[e] : -INFINITY;
+                    }
+                    float mx = a[0];
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, a[e]);
+                    mx = fmaf(mx, sc, ev);
+                    // The reference point moves only when a weight of the wavefront would pass 2^8 (weights up to 256 are as exact in
+                    // fp16 / bf16 as those below 1, and the sums are fp32): most tiles need no exchange between lanes
+                    if (__any(mx > m_run[rb] + 8.0f)) {
+                        mx = fmaxf(mx, __shfl_xor(mx, 16, ODSD_WAVE));
+                        mx = fmaxf(mx, __shfl_xor(mx, 32, ODSD_WAVE));
+                        const float m_new = fmaxf(m_run[rb], mx);
+                        // a row with nothing to attend yet keeps m = -inf: use 0 as the reference point then
+                        const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - (m_new == -INFINITY ? 0.0f : m_new));
+                        l_run[rb] *= alpha;
+                        m_run[rb] = m_new;
+#pragma unroll
+                        for (int db = 0; db < NDB; ++db) {
+                            o[rb][db].x *= alpha; o[rb][db].y *= alpha; o[rb][db].z *= alpha; o[rb][db].w *= alpha;
+                        }
+                    }
+                    const float ref = m_run[rb] == -INFINITY ? ev : ev - m_run[rb];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) a[e] = __builtin_amdgcn_exp2f(fmaf(a[e], sc, ref));      // masked -> 0
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) sum += (a[e] + a[e + 1]) + (a[e + 2] + a[e + 3]);
+                    l_run[rb] = fmaf(sum, iv, l_run[rb]);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        pf[rb][u] = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(a[8 * u], a[8 * u + 1]), AttnT<T>::pack2(a[8 * u + 2], a[8 * u + 3]),
+                                                                   AttnT<T>::pack2(a[8 * u + 4], a[8 * u + 5]), AttnT<T>::pack2(a[8 * u + 6], a[8 * u + 7])});
+                }
+                if (masked) {
+                    // Bytes of V past the last key are what a block held before: they count as zeros.  A NaN of a key that some
+                    // rows see and others do not must not reach the others as 0 * NaN: such codes are counted for the rows that
+                    // see them by a product of their own, and taken out.
+                    uint32_t keep[4], bad = 0u;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int left = L - (k0 + 16 * kq) - 4 * w;
+                        keep[w] = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+                    }
+#pragma unroll
+                    for (int db = 0; db < NDB; ++db) {
+                        vreg[db].x &= keep[0]; vreg[db].y &= keep[1]; vreg[db].z &= keep[2]; vreg[db].w &= keep[3];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) bad |= (vreg[db][w] & 0x7f7f7f7fu) + 0x01010101u;
+                    }
+                    if (__any((bad & 0x80808080u) != 0u)) {
+#pragma unroll
+                        for (int db = 0; db < NDB; ++db) {
+                            uint32_t ones[4];              // 1.0 where the code is no number
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const uint32_t f = (((vreg[db][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                                ones[w] = f * 0x38u;
+                                vreg[db][w] &= ~(f * 0xffu);
+                            }
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb) {
+                                float4_t cnt = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) {
+                                    float s[8];
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) s[e] = k0 + 16 * kq + 8 * u + e <= kmax[rb] ? 1.0f : 0.0f;
+                                    const V8 sees = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(s[0], s[1]), AttnT<T>::pack2(s[2], s[3]),
+                                                                                   AttnT<T>::pack2(s[4], s[5]), AttnT<T>::pack2(s[6], s[7])});
+                                    cnt = AttnT<T>::mfma(fp8_widen8<T>(ones[2 * u], ones[2 * u + 1]), sees, cnt);
+                                }
+#pragma unroll
+                                for (int i4 = 0; i4 < 4; ++i4)
+                                    if (cnt[i4] > 0.0f) o[rb][db][i4] = __builtin_nanf("");
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) {
+                    const V8 lo = fp8_widen8<T>(vreg[db].x, vreg[db].y), hi = fp8_widen8<T>(vreg[db].z, vreg[db].w);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        o[rb][db] = AttnT<T>::mfma(lo, pf[rb][0], o[rb][db]);
+                        o[rb][db] = AttnT<T>::mfma(hi, pf[rb][1], o[rb][db]);
+                    }
+                    if constexpr (decltype(fetch_c)::value) fetch_v(next, db);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            {
+                const char *ka = k_from(0), *va = v_from(0);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) fetch_k(ka, t);
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) fetch_v(va, db);
+            }
+            int i = 0;
+            for (; i + 1 < nt; ++i) tile(std::true_type{}, i);
+            tile(std::false_type{}, i);
+        }
+
+        // ---- the four wavefronts' sums, through LDS, 16 rows at a time ------------------------------------
+        const bool whole = n == sq.steps;
+        // (a piece that begins where its workgroup's share begins goes to the workgroup's first slot)
+        float *part = p.part + (size_t)(2 * pl.me + (pos > first_pos ? 1 : 0)) * (ROWS * XROW);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            __syncthreads();                               // the area is free
+            float *xr = xch + (wave * 16 + c) * XROW;
+            float l = l_run[rb];
+            l += __shfl_xor(l, 16, ODSD_WAVE);
+            l += __shfl_xor(l, 32, ODSD_WAVE);
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) *(float4_t *)(xr + 16 * db + 4 * kq) = o[rb][db];
+            if (kq == 0) {
+                xr[HD] = m_run[rb];
+                xr[HD + 1] = l;
+            }
+            __syncthreads();
+            for (int it = tid; it < min(16, rows_here - 16 * rb) * (HD / 4); it += 256) {
+                const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
+                const float *xs = xch + row * XROW;
+                float m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) m = fmaxf(m, xs[w * 16 * XROW + HD]);
+                const float ref = m == -INFINITY ? 0.0f : m;
+                float ls = 0.0f;
+                float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(xs[w * 16 * XROW + HD] - ref);      // -inf -> 0
+                    const float4_t v = *(const float4_t *)(xs + w * 16 * XROW + d);
+                    ls += f * xs[w * 16 * XROW + HD + 1];
+                    acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+                }
+                const int r = 16 * rb + row;
+                if (whole) {
+                    const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
+                    const int tok = (row0 + r) / p.Gq, hq = row0 + r - tok * p.Gq;
+                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                    *(u32x2 *)((uint16_t *)p.out + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + d) =
+                        u32x2{AttnT<T>::pack2(acc.x * inv, acc.y * inv), AttnT<T>::pack2(acc.z * inv, acc.w * inv)};
+                } else {
+                    *(float4_t *)(part + r * XROW + d) = acc;
+                    if (d == 0) {
+                        part[r * XROW + HD] = m;
+                        part[r * XROW + HD + 1] = ls;
+                    }
+                }
+            }
+        }
+        pos += n;
+        if (pos < end) next_unit(p, sq, unit, step, ROWS, pl.g);
+    }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------
+// What a call does, from its shape alone; the size function and the launch both ask here.
+struct AttnFp8Plan {
+    int rows;                     // per unit
+    int64_t rg, units;            // row groups per (sequence, KV head), units
+    int n_wg, shares;             // workgroups that share the list, those that can get a share
+    bool split;                   // units may be split: partial results and a merge
+    size_t bytes;                 // workspace that splitting takes
+};
+static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t max_keys, int kvh, int head_dim) {
+    AttnFp8Plan pl;
+    const int64_t rows = max_q * gq;
+    pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    pl.rg = (rows + pl.rows - 1) / pl.rows;
+    pl.units = n_seqs * kvh * pl.rg;
+    pl.n_wg = pl.rows == 64 ? FP8_WG / 2 : FP8_WG;
+    const int64_t steps = (max_keys + FP8_STEP - 1) / FP8_STEP;
+    // (list positions are 32 bits wide)
+    pl.split = !(max_keys <= FP8_WHOLE || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
+    pl.shares = (int)min(pl.units * steps, (int64_t)pl.n_wg);
+    pl.bytes = pl.split ? odsd_round_up((size_t)2 * pl.shares * pl.rows * (head_dim + 4) * sizeof(float), 256) : 0;
+    return pl;
+}
+static bool attn_fp8_shape_ok(int64_t n_seqs, int64_t max_q_len, int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks) {
+    return n_seqs > 0 && max_q_len > 0 && num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 &&
+           (head_dim == 64 || head_dim == 128) && block_size > 0 && block_size % 16 == 0 && block_size <= FP8_MAX_BLOCK && max_blocks > 0 &&
+           (max_q_len * (num_heads / num_kv_heads) + 63) / 64 <= 65535 && n_seqs * num_kv_heads <= 0x7fffffffLL &&
+           n_seqs * num_kv_heads * ((max_q_len * (num_heads / num_kv_heads) + 63) / 64) <= (1LL << 24) - 1;
+}
+
+extern "C" size_t odsd_paged_attention_fp8_workspace_bytes(int32_t n_seqs, int32_t max_q_len, int32_t num_heads,
+                                                           int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                                           int32_t max_blocks) {
+    if (!attn_fp8_shape_ok(n_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size, max_blocks)) return 0;
+    const AttnFp8Plan pl = attn_fp8_plan(n_seqs, max_q_len, num_heads / num_kv_heads, (int64_t)max_blocks * block_size, num_kv_heads, head_dim);
+    return pl.split ? pl.bytes : 256;
+}
+
+extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, const void *v_cache, const float *scales,
+                                        const int32_t *block_tables, const int32_t *context_lens, const int32_t *q_lens,
+                                        int32_t n_seqs, int32_t max_q_len, int32_t num_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, int32_t block_size, int32_t max_blocks, int32_t n_blocks,
+                                        float softmax_scale, int32_t dtype, void *out, void *workspace,
+                                        size_t workspace_bytes, void *stream) {
+    if (n_seqs < 0 || max_q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || block_size <= 0 ||
+        block_size % 16 || max_blocks <= 0 || n_blocks <= 0 || !(softmax_scale > 0.0f) || !(softmax_scale < INFINITY))
+        return ODSD_ERR_SHAPE;
+    if (dtype != ODSD_DT_BF16 && dtype != ODSD_DT_F16) return ODSD_ERR_DTYPE;
+    if (n_seqs == 0) return (head_dim == 64 || head_dim == 128) && block_size <= FP8_MAX_BLOCK ? ODSD_OK : ODSD_ERR_UNSUPPORTED;
+    if (!attn_fp8_shape_ok(n_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size, max_blocks) ||
+        (int64_t)n_blocks * num_kv_heads > 0x7fffffffLL)
+        return ODSD_ERR_UNSUPPORTED;
+    if (!q || !k_cache || !v_cache || !scales || !block_tables || !context_lens || !out) return ODSD_ERR_NULL;
+    if (!odsd_aligned16(q) || !odsd_aligned16(k_cache) || !odsd_aligned16(v_cache) || ((uintptr_t)scales & 7u) || ((uintptr_t)out & 7u))
+        return ODSD_ERR_ALIGN;
+    const int64_t max_keys = (int64_t)max_blocks * block_size;
+    const AttnFp8Plan pl = attn_fp8_plan(n_seqs, max_q_len, num_heads / num_kv_heads, max_keys, num_kv_heads, head_dim);
+    AttnFp8Params p{};
+    p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
+    p.q_lens = q_lens; p.context_lens = context_lens; p.block_tables = block_tables;
+    p.n_seqs = n_seqs; p.H = num_heads; p.KVH = num_kv_heads; p.Gq = num_heads / num_kv_heads;
+    p.max_blocks = max_blocks; p.block_size = block_size;
+    p.scale_log2e = softmax_scale * 1.4426950408889634f;
+    p.scales = scales; p.n_blocks = n_blocks;
+    p.max_keys = (int)min(max_keys, (int64_t)1 << 30);
+    p.max_rg = (int)pl.rg;
+    if (pl.split) {
+        if (!workspace) return ODSD_ERR_NULL;
+        if (!odsd_aligned16(workspace)) return ODSD_ERR_ALIGN;
+        if (workspace_bytes < pl.bytes) return ODSD_ERR_WORKSPACE;
+        p.part = (float *)workspace;
+        p.n_wg = pl.n_wg;
+    } else {
+        p.n_wg = (int)pl.units;
+        p.whole = (int)pl.rg;
+    }
+    const unsigned grid = (unsigned)(pl.split ? pl.shares : p.n_wg);
+    const dim3 mgrid((unsigned)(n_seqs * num_kv_heads), (unsigned)pl.rg, (unsigned)((pl.rows * head_dim + 1023) / 1024));
+    hipStream_t st = (hipStream_t)stream;
+    const bool aligned = block_size % 64 == 0;
+#define FP8_GO(T, HDV, RBV)                                                                               \
+    do {                                                                                                  \
+        if (RBV == 4 && !pl.split) {                                                                      \
+            if (aligned) attn_fp8_kernel<T, HDV, RBV, true, RBV != 4><<<grid, 256, 0, st>>>(p);           \
+            else attn_fp8_kernel<T, HDV, RBV, false, RBV != 4><<<grid, 256, 0, st>>>(p);                  \
+        } else if (aligned) attn_fp8_kernel<T, HDV, RBV, true, true><<<grid, 256, 0, st>>>(p);            \
+        else attn_fp8_kernel<T, HDV, RBV, false, true><<<grid, 256, 0, st>>>(p);                          \
+        if (pl.split) attn_merge_kernel<T, HDV, 16 * RBV, FP8_STEP, FP8_STEP><<<mgrid, 256, 0, st>>>(p);  \
+    } while (0)
+#define FP8_GO_RB(T, HDV)                                                                                 \
+    do {                                                                                                  \
+        if (pl.rows == 16) FP8_GO(T, HDV, 1);                                                             \
+        else if (pl.rows == 32) FP8_GO(T, HDV, 2);                                                        \
+        else FP8_GO(T, HDV, 4);                                                                           \
+    } while (0)
+    if (dtype == ODSD_DT_F16) {
+        if (head_dim == 128) FP8_GO_RB(half_t, 128);
+        else FP8_GO_RB(half_t, 64);
+    } else {
+        if (head_dim == 128) FP8_GO_RB(__bf16, 128);
+        else FP8_GO_RB(__bf16, 64);
+    }
+#undef FP8_GO_RB
+#undef FP8_GO
+    ODSD_CHECK_LAUNCH();
+    return ODSD_OK;
+}

@@ -20,6 +20,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
+from .kv_fp8 import KVCacheFP8, paged_attention_fp8
 from .ops import _ptr, _raw_device, _same_device, _stream, _wrote
 
 
@@ -383,8 +384,13 @@ def attention_for_context(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     """The branch of ``Qwen3Attention.forward`` after the KV store (attention.py:229-282): a prefill
     context (it carries ``cu_seqlens_q``) attends the step's own packed k / v, a decode or verify
     context reads the paged cache.  q: [n_tokens, num_heads, head_dim]; k, v: [n_tokens,
-    num_kv_heads, head_dim] (unused for decode / verify)."""
+    num_kv_heads, head_dim] (unused for decode / verify).  An 8-bit cache (``KVCacheFP8``) is given
+    as k_cache, with v_cache None."""
     if "cu_seqlens_q" in context:
         return varlen_attention(q, k, v, context["cu_seqlens_q"], context["cu_seqlens_k"],
                                 context["max_seqlen_q"], context["max_seqlen_k"], softmax_scale)
+    if isinstance(k_cache, KVCacheFP8):
+        if v_cache is not None or k_cache.k.shape[-3:-1] != (num_kv_heads, block_size):
+            raise ValueError("an 8-bit cache holds both k and v, and its heads and block size are those of the call")
+        return paged_attention_fp8(q, k_cache, context, softmax_scale)
     return paged_attention(q, k_cache, v_cache, context, num_kv_heads, block_size, softmax_scale)
