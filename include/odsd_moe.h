@@ -330,12 +330,14 @@ size_t odsd_paged_attention_workspace_bytes(int32_t n_seqs, int32_t max_q_len, i
  *   present scale if that is larger.  When the scale rises, the codes of the rows that stay are rounded again (exact but for those below
  *   2^-6 then).  A call that writes a block's token 0 starts the block anew: its scale is that of the call's rows alone, and codes of other
  *   tokens are given up.  Rounding to nearest, ties to even; infinities become +-448 and do not count for the scale, NaN stays NaN.
- * The same call gives the same bits.  (No counterpart in the reference.) */
+ * The same call gives the same bits.  workspace: odsd_kv_store_fp8_workspace_bytes(N) bytes (256: none is used, NULL will do), 4-byte aligned.
+ * (No counterpart in the reference.) */
 int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int64_t key_head_stride, const void *value,
                       int64_t value_token_stride, int64_t value_head_stride, void *k_cache, void *v_cache, float *scales,
                       const int32_t *slot_mapping, const int32_t *src_index, int32_t N, int32_t n_src,
                       int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t n_blocks, int32_t dtype,
-                      void *stream);
+                      void *workspace, size_t workspace_bytes, void *stream);
+size_t odsd_kv_store_fp8_workspace_bytes(int32_t N);
 
 /* odsd_paged_attention over that cache: the same queries, tables, lengths and masks, q and out of `dtype` (ODSD_DT_BF16 or ODSD_DT_F16).
  * Position p of sequence s is token p % block_size of block block_tables[s][p / block_size]; an entry that is negative or beyond the cache reads

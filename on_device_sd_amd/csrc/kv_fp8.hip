@@ -6,8 +6,17 @@
 // A (block, head) is written by one workgroup, K and V by one each, so scale and codes need no atomics and the same call gives the same
 // bits.  The rows of a block may stand anywhere in slot_mapping: the workgroup of the first of them (the leader) looks through the list
 // and notes which row goes to which token of the block (of two with one slot the last).  Rows that follow one of the same block, which
-// is what a prompt's are, end at once.
+// is what a prompt's are, end at once.  In a long list the leader looks only into those chunks of 256 entries whose bitmap, made by a
+// launch of its own, has the block's bit.
+// Many rows of a block (a prompt) are read once and stay in registers between their maximum and their codes; V's codes are turned
+// through LDS, four rows of four dimensions at a time, and leave as 16 bytes of a dimension.  A few rows (decode) write V's bytes one by one.
 #include "fp8.h"
+
+#define KV8_CHUNK 256          // list entries with one bitmap
+#define KV8_BITS 256           // bits of a bitmap
+#define KV8_LONG 4096          // a longer list has bitmaps
+#define KV8_WINDOW 256         // tokens of a block that are turned at a time
+#define KV8_FEW 16             // rows of a block that are not turned
 
 struct KvFp8Params {
     const uint16_t *key, *value;
@@ -15,50 +24,94 @@ struct KvFp8Params {
     uint8_t *k_cache, *v_cache;
     float *scales;                                             // [n_blocks, KVH, 2]
     const int32_t *slots, *src;
-    int N, n_src, KVH, HD, bs, n_blocks;
-    int per_wg;                                                // list entries of a workgroup
+    uint32_t *bitmaps;                                         // [KV8_BITS / 32][n_chunks], or null
+    int N, n_src, KVH, bs, n_blocks, n_chunks;
+    int per_wg;                                                // list entries of a workgroup, at most 64
 };
+
+__device__ __forceinline__ uint32_t kv_bit(const int block) { return ((uint32_t)block * 0x9e3779b1u) >> 24; }      // of KV8_BITS
+// whether list entry i names a slot and a row that exist; its slot
+__device__ __forceinline__ bool kv_entry(const KvFp8Params &p, const int i, int &slot) {
+    slot = p.slots[i];
+    const bool row = !p.src || (p.src[i] >= 0 && p.src[i] < p.n_src);
+    return slot >= 0 && slot / p.bs < p.n_blocks && row;
+}
+
+__global__ __launch_bounds__(KV8_CHUNK) void kv_bitmap_kernel(const KvFp8Params p) {
+    __shared__ uint32_t bits[KV8_BITS / 32];
+    const int i = blockIdx.x * KV8_CHUNK + threadIdx.x;
+    if (threadIdx.x < KV8_BITS / 32) bits[threadIdx.x] = 0u;
+    __syncthreads();
+    int slot;
+    if (i < p.N && kv_entry(p, i, slot)) {
+        const uint32_t b = kv_bit(slot / p.bs);
+        atomicOr(&bits[b >> 5], 1u << (b & 31));
+    }
+    __syncthreads();
+    if (threadIdx.x < KV8_BITS / 32) p.bitmaps[(size_t)threadIdx.x * p.n_chunks + blockIdx.x] = bits[threadIdx.x];
+}
 
 template <typename T> __device__ __forceinline__ float kv_value(uint16_t b);
 template <> __device__ __forceinline__ float kv_value<__bf16>(uint16_t b) { return bf16_to_f32(b); }
 template <> __device__ __forceinline__ float kv_value<half_t>(uint16_t b) { return (float)__builtin_bit_cast(half_t, b); }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void kv_load8(const uint16_t *p, float (&x)[8]) {
-    if constexpr (VEC) {
-        const uint4_t w = *(const uint4_t *)p;
+template <bool VEC>
+__device__ __forceinline__ uint4_t kv_load8(const uint16_t *p) {
+    if constexpr (VEC) return *(const uint4_t *)p;
+    uint4_t w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = kv_value<T>((uint16_t)(w[i] & 0xffffu));
-            x[2 * i + 1] = kv_value<T>((uint16_t)(w[i] >> 16));
-        }
-    } else {
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    return w;
+}
+template <typename T>
+__device__ __forceinline__ float kv_amax8(const uint4_t w, float amax) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = kv_value<T>(p[i]);
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(kv_value<T>((uint16_t)(w[i >> 1] >> (16 * (i & 1)))));
+        amax = a <= 3.4028234663852886e38f ? fmaxf(amax, a) : amax;      // infinities and NaN do not count
     }
+    return amax;
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename T>
+__device__ __forceinline__ u32x2 kv_codes8(const uint4_t w, const float inv) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = kv_value<T>((uint16_t)(w[i >> 1] >> (16 * (i & 1)))) * inv;
+    return u32x2{fp8_pack4(x[0], x[1], x[2], x[3]), fp8_pack4(x[4], x[5], x[6], x[7])};
 }
 
-template <typename T, bool VEC>
+template <typename T, int HD, bool VEC>
 __global__ __launch_bounds__(256) void kv_store_fp8_kernel(const KvFp8Params p) {
+    constexpr int NP = HD / 8;                           // pieces of 8 values of a row
+    constexpr int HELD = KV8_WINDOW * NP / 256;          // pieces of a window per thread
+    constexpr int ROW = HD + 8;                          // bytes of a row in LDS: 16 rows on, other banks
     __shared__ int row_of[FP8_MAX_BLOCK];      // list entry that goes to a token of the block, -1: none
-    __shared__ int present[FP8_MAX_BLOCK];     // tokens that get one
+    __shared__ uint16_t present[FP8_MAX_BLOCK];          // tokens that get one
     __shared__ int first, count;
     __shared__ float red[4];
-    const int tid = threadIdx.x, h = blockIdx.y;
+    __shared__ __attribute__((aligned(16))) uint8_t turn[KV8_WINDOW * ROW];
+    const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
-    const uint16_t *x = is_v ? p.value : p.key;
-    const int64_t token = is_v ? p.value_token : p.key_token, head = is_v ? p.value_head : p.key_head;
-    const int bs = p.bs, HD = p.HD, NP = HD / 8;
-    const int begin = blockIdx.x * p.per_wg, end = min(p.N, begin + p.per_wg);
-    for (int e = begin; e < end; ++e) {
-        const int slot = p.slots[e];
-        if (slot < 0) continue;
-        const int block = slot / bs, base = block * bs;
-        if (block >= p.n_blocks) continue;
-        if (e > 0) {
-            const int before = p.slots[e - 1];
-            if (before >= base && before - base < bs && (!p.src || (p.src[e - 1] >= 0 && p.src[e - 1] < p.n_src))) continue;
+    const uint16_t *x = (is_v ? p.value : p.key) + (int64_t)h * (is_v ? p.value_head : p.key_head);
+    const int64_t token = is_v ? p.value_token : p.key_token;
+    const int bs = p.bs;
+    const int begin = blockIdx.x * p.per_wg;
+    // entries that may be leaders: those whose neighbour in front is of another block
+    uint64_t leaders;
+    int slot_l = -1;
+    {
+        const int e = begin + lane;
+        bool may = false;
+        if (lane < p.per_wg && e < p.N && kv_entry(p, e, slot_l)) {
+            int before;
+            may = e == 0 || !kv_entry(p, e - 1, before) || before / bs != slot_l / bs;
         }
+        leaders = __ballot(may);
+    }
+    for (; leaders; leaders &= leaders - 1) {
+        const int l = __builtin_ctzll(leaders), e = begin + l;
+        const int block = __builtin_amdgcn_readlane(slot_l, l) / bs, base = block * bs;
         // ---- the block's rows ------------------------------------------------------------------------
         __syncthreads();                        // the arrays are free
         for (int i = tid; i < bs; i += 256) row_of[i] = -1;
@@ -67,36 +120,54 @@ __global__ __launch_bounds__(256) void kv_store_fp8_kernel(const KvFp8Params p) 
             count = 0;
         }
         __syncthreads();
-        for (int i = tid; i < p.N; i += 256) {
-            const int at = p.slots[i] - base;
-            if (p.slots[i] >= base && at < bs && (!p.src || (p.src[i] >= 0 && p.src[i] < p.n_src))) {
+        auto look = [&](const int i) {          // (block is a block of the cache, so its slots need no check)
+            const int slot = p.slots[i], at = slot - base;
+            if (slot >= base && at < bs && (!p.src || (p.src[i] >= 0 && p.src[i] < p.n_src))) {
                 atomicMax(&row_of[at], i);
                 atomicMin(&first, i);
             }
+        };
+        if (p.bitmaps) {
+            const uint32_t bit = kv_bit(block);
+            const uint32_t *maps = p.bitmaps + (size_t)(bit >> 5) * p.n_chunks;
+            for (int c0 = 0; c0 < p.n_chunks; c0 += 64) {
+                const bool has = c0 + lane < p.n_chunks && (maps[c0 + lane] >> (bit & 31)) & 1;
+                for (uint64_t todo = __ballot(has); todo; todo &= todo - 1) {
+                    const int i = (c0 + __builtin_ctzll(todo)) * KV8_CHUNK + tid;
+                    if (i < p.N) look(i);
+                }
+            }
+        } else {
+            for (int i = tid; i < p.N; i += 256) look(i);
         }
         __syncthreads();
-        if (first != e) continue;               // (another workgroup's, or a row that does not exist)
+        if (first != e) continue;               // (another workgroup's)
         for (int i = tid; i < bs; i += 256)
-            if (row_of[i] >= 0) present[atomicAdd(&count, 1)] = i;
+            if (row_of[i] >= 0) present[atomicAdd(&count, 1)] = (uint16_t)i;
         __syncthreads();
         const int rows = count;
-        auto source = [&](const int r) {        // the row that goes to token r
-            const int i = row_of[r];
-            return x + (int64_t)(p.src ? p.src[i] : i) * token + (int64_t)h * head;
+        const bool turned = rows > KV8_FEW, held = turned && bs <= KV8_WINDOW;
+        auto source = [&](const int i) { return x + (int64_t)(p.src ? p.src[i] : i) * token; };
+        // the pieces of a window: piece tid + 256 u of row (tid + 256 u) / NP
+        uint4_t hold[HELD];
+        auto load_window = [&](const int w0) {
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                const int r = w0 + (tid + 256 * u) / NP, i = r < bs ? row_of[r] : -1;
+                hold[u] = i >= 0 ? kv_load8<VEC>(source(i) + 8 * (tid % NP)) : uint4_t{0u, 0u, 0u, 0u};
+            }
         };
         // ---- the scale -------------------------------------------------------------------------------
         float amax = 0.0f;
-        for (int i = tid; i < rows * NP; i += 256) {
-            float v[8];
-            kv_load8<T, VEC>(source(present[i / NP]) + 8 * (i % NP), v);
+        if (held) {
+            load_window(0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float a = fabsf(v[j]);
-                amax = a <= 3.4028234663852886e38f ? fmaxf(amax, a) : amax;      // infinities and NaN do not count
-            }
+            for (int u = 0; u < HELD; ++u) amax = kv_amax8<T>(hold[u], amax);
+        } else {
+            for (int i = tid; i < rows * NP; i += 256) amax = kv_amax8<T>(kv_load8<VEC>(source(row_of[present[i / NP]]) + 8 * (i % NP)), amax);
         }
         amax = wave_max(amax);
-        if ((tid & 63) == 0) red[tid >> 6] = amax;
+        if (lane == 0) red[tid >> 6] = amax;
         __syncthreads();
         amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const int64_t bh = (int64_t)block * p.KVH + h;
@@ -117,28 +188,78 @@ __global__ __launch_bounds__(256) void kv_store_fp8_kernel(const KvFp8Params p) 
         __syncthreads();                        // (every thread has read the scale; the codes are there before the new ones come)
         if (tid == 0) *scale_at = scale;
         // ---- the codes -------------------------------------------------------------------------------
-        for (int i = tid; i < rows * NP; i += 256) {
-            const int r = present[i / NP], d = 8 * (i % NP);
-            float v[8];
-            kv_load8<T, VEC>(source(r) + d, v);
-            const uint32_t lo = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-            const uint32_t hi = fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-            if (!is_v) {
-                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                *(u32x2 *)(codes + r * HD + d) = u32x2{lo, hi};
-            } else {
+        if (!turned) {
+            for (int i = tid; i < rows * NP; i += 256) {
+                const int r = present[i / NP], d = 8 * (i % NP);
+                const u32x2 c = kv_codes8<T>(kv_load8<VEC>(source(row_of[r]) + d), inv);
+                if (!is_v) {
+                    *(u32x2 *)(codes + r * HD + d) = c;
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) codes[(d + j) * bs + r] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+                    for (int j = 0; j < 8; ++j) codes[(d + j) * bs + r] = (uint8_t)(c[j >> 2] >> (8 * (j & 3)));
+                }
+            }
+            continue;
+        }
+        for (int w0 = 0; w0 < bs; w0 += KV8_WINDOW) {
+            if (!held) load_window(w0);
+            if (is_v) __syncthreads();          // the last window has left LDS
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                const int r = (tid + 256 * u) / NP, d = 8 * (tid % NP);
+                const u32x2 c = kv_codes8<T>(hold[u], inv);
+                if (is_v) *(u32x2 *)(turn + r * ROW + d) = c;
+                else if (w0 + r < bs && row_of[w0 + r] >= 0) *(u32x2 *)(codes + (w0 + r) * HD + d) = c;
+            }
+            if (!is_v) continue;
+            __syncthreads();
+            // 16 tokens of 4 dimensions a turn
+            const int here = min(KV8_WINDOW, bs - w0);
+            for (int i = tid; i < here / 16 * (HD / 4); i += 256) {
+                const int r0 = 16 * (i / (HD / 4)), d = 4 * (i % (HD / 4));
+                uint32_t there = 0u;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) there |= row_of[w0 + r0 + r] >= 0 ? 1u << r : 0u;
+                if (!there) continue;
+                uint4_t out[4];                 // [dimension], four tokens a word
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[r] = *(const uint32_t *)(turn + (r0 + 4 * q + r) * ROW + d);
+                    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+                    const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), e4 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+                    out[0][q] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+                    out[1][q] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                    out[2][q] = __builtin_amdgcn_perm(e4, c, 0x05040100u);
+                    out[3][q] = __builtin_amdgcn_perm(e4, c, 0x07060302u);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint8_t *to = codes + (d + j) * bs + w0 + r0;
+                    if (there == 0xffffu) {
+                        *(uint4_t *)to = out[j];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (there >> r & 1) to[r] = (uint8_t)(out[j][r >> 2] >> (8 * (r & 3)));
+                    }
+                }
             }
         }
     }
+}
+
+extern "C" size_t odsd_kv_store_fp8_workspace_bytes(int32_t N) {
+    if (N < 0 || N > (1 << 28)) return 0;
+    return N <= KV8_LONG ? 256 : odsd_round_up((size_t)((N + KV8_CHUNK - 1) / KV8_CHUNK) * (KV8_BITS / 8), 256);
 }
 
 extern "C" int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int64_t key_head_stride, const void *value,
                                  int64_t value_token_stride, int64_t value_head_stride, void *k_cache, void *v_cache,
                                  float *scales, const int32_t *slot_mapping, const int32_t *src_index, int32_t N,
                                  int32_t n_src, int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t n_blocks,
-                                 int32_t dtype, void *stream) {
+                                 int32_t dtype, void *workspace, size_t workspace_bytes, void *stream) {
     if (N < 0 || n_src < 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || block_size % 16 || n_blocks < 0 ||
         (!src_index && N != n_src))
         return ODSD_ERR_SHAPE;
@@ -152,24 +273,36 @@ extern "C" int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int6
     if (!odsd_aligned16(k_cache) || !odsd_aligned16(v_cache) || ((uintptr_t)scales & 7u) || (((uintptr_t)key | (uintptr_t)value) & 1u))
         return ODSD_ERR_ALIGN;
     KvFp8Params p{};
+    hipStream_t st = (hipStream_t)stream;
     p.key = (const uint16_t *)key; p.value = (const uint16_t *)value;
     p.key_token = key_token_stride; p.key_head = key_head_stride; p.value_token = value_token_stride; p.value_head = value_head_stride;
     p.k_cache = (uint8_t *)k_cache; p.v_cache = (uint8_t *)v_cache; p.scales = scales;
     p.slots = slot_mapping; p.src = src_index;
-    p.N = N; p.n_src = n_src; p.KVH = num_kv_heads; p.HD = head_dim; p.bs = block_size; p.n_blocks = n_blocks;
-    // enough workgroups for the chip, no more than 64 entries each
-    p.per_wg = (int)max((int64_t)1, min((int64_t)64, (int64_t)N * num_kv_heads / 1024));
+    p.N = N; p.n_src = n_src; p.KVH = num_kv_heads; p.bs = block_size; p.n_blocks = n_blocks;
+    if (N > KV8_LONG) {
+        if (!workspace) return ODSD_ERR_NULL;
+        if ((uintptr_t)workspace & 3u) return ODSD_ERR_ALIGN;
+        if (workspace_bytes < odsd_kv_store_fp8_workspace_bytes(N)) return ODSD_ERR_WORKSPACE;
+        p.bitmaps = (uint32_t *)workspace;
+        p.n_chunks = (N + KV8_CHUNK - 1) / KV8_CHUNK;
+        kv_bitmap_kernel<<<(unsigned)p.n_chunks, KV8_CHUNK, 0, st>>>(p);
+    }
+    // enough workgroups for the chip; no more entries each than a block of a prompt takes, or than a wavefront has lanes
+    p.per_wg = (int)max((int64_t)1, min((int64_t)min(64, block_size), (int64_t)N * num_kv_heads / 1024));
     const dim3 grid((unsigned)((N + p.per_wg - 1) / p.per_wg), (unsigned)num_kv_heads, 2);
     const bool vec = !(((uintptr_t)key | (uintptr_t)value) & 15u) &&
                      !((key_token_stride | key_head_stride | value_token_stride | value_head_stride) & 7);
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == ODSD_DT_BF16) {
-        if (vec) kv_store_fp8_kernel<__bf16, true><<<grid, 256, 0, st>>>(p);
-        else kv_store_fp8_kernel<__bf16, false><<<grid, 256, 0, st>>>(p);
-    } else {
-        if (vec) kv_store_fp8_kernel<half_t, true><<<grid, 256, 0, st>>>(p);
-        else kv_store_fp8_kernel<half_t, false><<<grid, 256, 0, st>>>(p);
-    }
+#define KV8_GO(T)                                                                        \
+    do {                                                                                 \
+        if (head_dim == 128) {                                                           \
+            if (vec) kv_store_fp8_kernel<T, 128, true><<<grid, 256, 0, st>>>(p);         \
+            else kv_store_fp8_kernel<T, 128, false><<<grid, 256, 0, st>>>(p);            \
+        } else if (vec) kv_store_fp8_kernel<T, 64, true><<<grid, 256, 0, st>>>(p);       \
+        else kv_store_fp8_kernel<T, 64, false><<<grid, 256, 0, st>>>(p);                 \
+    } while (0)
+    if (dtype == ODSD_DT_BF16) KV8_GO(__bf16);
+    else KV8_GO(half_t);
+#undef KV8_GO
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
 }

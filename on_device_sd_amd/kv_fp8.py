@@ -15,6 +15,7 @@ from . import _lib
 from .ops import _ptr, _raw_device, _same_device, _stream, _wrote
 
 _E4M3 = torch.float8_e4m3fn
+_SHORT_LIST = 4096                                      # rows that the store takes without a workspace
 _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
@@ -103,9 +104,13 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, cache: KVCacheFP8,
     if vs[2] != 1:
         value = value.contiguous()
         vs = value.stride()
-    rc = _lib.load().odsd_kv_store_fp8(key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], cache.k.data_ptr(),
-                                       cache.v.data_ptr(), cache.scales.data_ptr(), slot_mapping.data_ptr(), _ptr(src_index), N, n, heads,
-                                       head_dim, block_size, blocks, code, _stream())
+    lib, ws, nbytes = _lib.load(), None, 0
+    if N > _SHORT_LIST:
+        nbytes = lib.odsd_kv_store_fp8_workspace_bytes(N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=key.device)
+    rc = lib.odsd_kv_store_fp8(key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], cache.k.data_ptr(), cache.v.data_ptr(),
+                               cache.scales.data_ptr(), slot_mapping.data_ptr(), _ptr(src_index), N, n, heads, head_dim, block_size, blocks,
+                               code, _ptr(ws), nbytes, _stream())
     if rc:
         _lib.check(rc, "odsd_kv_store_fp8")
     _wrote(cache.k, cache.v, cache.scales)

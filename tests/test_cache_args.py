@@ -13,13 +13,17 @@ P = 1 << 20
 
 def test_store_status_codes():
     lib = _lib.load()
-    f = lambda N=4, n=4, H=2, D=64, bs=16, nb=8, dt=1, key=P, val=P, k=P, v=P, sc=P, slots=P, src=None, st=128: \
-        lib.odsd_kv_store_fp8(key, st, D, val, st, D, k, v, sc, slots, src, N, n, H, D, bs, nb, dt, None)  # noqa: E731
+    f = lambda N=4, n=4, H=2, D=64, bs=16, nb=8, dt=1, key=P, val=P, k=P, v=P, sc=P, slots=P, src=None, st=128, ws=P, b=1 << 30: \
+        lib.odsd_kv_store_fp8(key, st, D, val, st, D, k, v, sc, slots, src, N, n, H, D, bs, nb, dt, ws, b, None)  # noqa: E731
     assert f(N=-1) == f(n=-1) == f(H=0) == f(D=0) == f(bs=0) == f(bs=24) == f(nb=-1) == f(N=3) == 2
     assert f(dt=0) == f(dt=3) == 7
     assert f(D=96) == f(bs=1040) == f(nb=1 << 27) == f(nb=1 << 26, H=64) == f(N=1 << 29, n=1 << 29) == 3
     assert f(key=None) == f(val=None) == f(k=None) == f(v=None) == f(sc=None) == f(slots=None) == 1
     assert f(k=P + 8) == f(v=P + 1) == f(sc=P + 4) == f(key=P + 1) == 4
+    many = dict(N=5000, n=5000)
+    assert f(ws=None, **many) == 1 and f(ws=P + 2, **many) == 4 and f(b=256, **many) == 5
+    size = lib.odsd_kv_store_fp8_workspace_bytes
+    assert size(0) == size(4096) == 256 and size(4097) > 256 and size(-1) == size(1 << 29) == 0
     assert f(N=0, n=0, key=None) == f(nb=0, k=None) == f(N=0, src=P, key=None) == 0
 
 
