@@ -3,18 +3,24 @@
 //   x = x - (f n + p [n > 0])         n: how often among the output and the drafts before the row
 //   x = x + bias;   a mask bit that is clear: x = -inf;   rounded once, to the logits' type
 //
-// A workgroup has one sequence and a slice of the vocabulary, and goes over it twice.  First all rows are copied, 16 bytes a thread, with -inf where
-// the mask forbids: nearly every logit is done then.  (In place and without a mask there is nothing to copy.)  Meanwhile it has
-// looked through the sequence's tokens and counted those of its slice in LDS; the tokens that have occurred, are drafted or have a
-// bias are listed, and each thread then computes its tokens of the list in all rows, adding to the count the drafts that stand before.  No table of
-// counts lives between steps, so drafts that are not kept leave nothing to undo.  The logits are read and written once: that traffic is
-// the bound; the tokens (read again by every slice, from L2) and the listed logits (from L2 or the memory-side cache) are little next to it.
+// A workgroup has one sequence and a share of the vocabulary, every so many granules of 128 tokens (the words that are used most have
+// neighbouring numbers).  It looks through the sequence's tokens once, counts its own in LDS and lists those that have occurred, are
+// drafted or have a bias.  Then it goes through the sequence's rows, adding to the counts the draft that stands before each: a row's
+// share comes in 16 bytes a thread, the listed logits are changed in LDS, and it leaves 16 bytes a thread with -inf where the mask forbids.
+// No table of counts lives between steps, so drafts that are not kept leave nothing to undo.  The traffic of the logits, once in and once
+// out, is the bound; the tokens (read again for every share, from L2) are little next to it.  (Changing the listed logits in memory after a copy
+// of the rows took 102 us for 449 rows of 131072, 4096 tokens each, of which the copy is 50: a logit is 2 bytes of the 64 that move.)
+// In place and without a mask only the listed logits are read and written.
 #include "common.h"
 #include <type_traits>
 
 #define ADJ_SEEN 0x80000000u     // has occurred
 #define ADJ_DRAFT 0x40000000u    // is drafted, and may occur in later rows
 #define ADJ_BIAS 0x20000000u     // has a bias; the other bits count
+#define ADJ_BIASES 128           // biases of a share that are kept in LDS
+#define ADJ_GRANULE 128          // tokens, a power of two
+#define ADJ_MOST 4096            // tokens of a share at most
+#define ADJ_ROWS 64              // rows whose drafts and masks are looked up at a time
 
 struct AdjParams {
     const void *logits;
@@ -32,7 +38,8 @@ struct AdjParams {
     const int32_t *mask;                       // rows of mask_stride words
     int64_t mask_stride;
     const int32_t *mask_rows;                  // [n_rows] or null
-    int n_seqs, n_rows, n_drafts, vocab, token_bytes, max_tokens, n_bias, n_mask, slice, slices;
+    int n_seqs, n_rows, n_drafts, vocab, token_bytes, max_tokens, n_bias, n_mask;
+    int shares, share_bits, most;              // shares of the vocabulary, a power of two; tokens of a share at most
     int dense, sparse;                         // rows have to be copied; some tokens may differ
 };
 
@@ -57,18 +64,26 @@ __device__ __forceinline__ int64_t adj_token(const void *p, const int bytes, con
     return bytes == 8 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
 }
 
-template <typename T>
+template <typename T, bool MASK>
 __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
-    extern __shared__ uint32_t lds[];          // counts [slice], the list [slice] in 16 bits
-    __shared__ int sums[8], listed;
+    extern __shared__ uint4_t lds4[];          // two rows of the share (dense), counts [most], the list [most] in 16 bits
+    uint32_t *lds = (uint32_t *)lds4 + (p.dense ? 2 * p.most * (int)sizeof(T) / 4 : 0);
+    __shared__ int sums[8], listed, biases;
+    __shared__ int bias_token[ADJ_BIASES], bias_entry[ADJ_BIASES], draft_of[ADJ_ROWS], mask_at[ADJ_ROWS];       // entries that name a token of the share, in no order
     uint32_t *counts = lds;
-    uint16_t *list = (uint16_t *)(lds + p.slice);
+    uint16_t *list = (uint16_t *)(lds + p.most);
     const int tid = threadIdx.x;
-    const int s = blockIdx.x / p.slices, v0 = (blockIdx.x - s * p.slices) * p.slice;
-    const int here = min(p.slice, p.vocab - v0);
+    const int s = blockIdx.x >> p.share_bits, share = blockIdx.x & (p.shares - 1);
+    // token i of the share is token at(i) of the vocabulary, from vocab on there is none; mine(t): which of the share's it is, or -1
+    auto at = [&](const int i) { return ((i / ADJ_GRANULE << p.share_bits) + share) * ADJ_GRANULE + i % ADJ_GRANULE; };
+    auto mine = [&](const int64_t t) -> int {
+        if (t < 0 || t >= p.vocab) return -1;
+        const int g = (int)t / ADJ_GRANULE;
+        return (g & (p.shares - 1)) == share ? (g >> p.share_bits) * ADJ_GRANULE + (int)t % ADJ_GRANULE : -1;
+    };
     if (p.sparse) {
-        if (tid == 0) listed = 0;
-        for (int i = tid; i < here; i += 256) counts[i] = 0u;
+        if (tid == 0) listed = biases = 0;
+        for (int i = tid; i < p.most; i += 256) counts[i] = 0u;
     }
     // the sequence's first row and first draft
     int row = s, draft = 0, rows = 1;
@@ -102,101 +117,202 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
         if (p.tokens) {
             const int len = min(max(p.token_lens ? p.token_lens[s] : p.max_tokens, 0), p.max_tokens);
             const int prompt = p.prompt_lens ? p.prompt_lens[s] : 0;
-            for (int i = tid; i < len; i += 256) {
-                const int64_t t = adj_token(p.tokens, p.token_bytes, s * p.token_stride + i) - v0;
-                if (t >= 0 && t < here) {
-                    if (i >= prompt) atomicAdd(&counts[t], 1u);
-                    atomicOr(&counts[t], ADJ_SEEN);
+            for (int i0 = tid; i0 < len; i0 += 8 * 256) {      // (eight loads on their way at a time)
+                int64_t t[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) t[u] = adj_token(p.tokens, p.token_bytes, s * p.token_stride + min(i0 + 256 * u, len - 1));
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int i = i0 + 256 * u < len ? mine(t[u]) : -1;
+                    if (i >= 0) {
+                        if (i0 + 256 * u >= prompt) atomicAdd(&counts[i], 1u);
+                        atomicOr(&counts[i], ADJ_SEEN);
+                    }
                 }
             }
         }
         for (int i = tid; i < drafts; i += 256) {
-            const int64_t t = adj_token(p.drafts, 8, draft + i) - v0;
-            if (t >= 0 && t < here) atomicOr(&counts[t], ADJ_DRAFT);
+            const int t = mine(adj_token(p.drafts, 8, draft + i));
+            if (t >= 0) atomicOr(&counts[t], ADJ_DRAFT);
         }
         for (int i = tid; i < p.n_bias; i += 256) {
-            const int t = p.bias_tokens[(int64_t)s * p.n_bias + i];
-            if (t >= v0 && t - v0 < here) atomicOr(&counts[t - v0], ADJ_BIAS);
-        }
-    }
-    // ---- all rows, as they are or forbidden ------------------------------------------------------------
-    const T *in = (const T *)p.logits + (int64_t)row * p.ld + v0;
-    T *to = (T *)p.out + (int64_t)row * p.ldo + v0;
-    auto mask_of = [&](const int j) -> const int32_t * {
-        const int m = p.mask ? p.mask_rows ? p.mask_rows[row + j] : row + j : -1;
-        return m >= 0 && m < p.n_mask ? p.mask + m * p.mask_stride : nullptr;
-    };
-    if (p.dense) {
-        constexpr int TPG = 16 / (int)sizeof(T);           // tokens of a group: 16 bytes, rows at any element
-        const int groups = here / TPG;
-        for (int j = 0; j < rows; ++j) {
-            const T *x = in + j * p.ld;
-            T *y = to + j * p.ldo;
-            const int32_t *mask = mask_of(j);
-            for (int g0 = tid; g0 < groups; g0 += 4 * 256) {
-                uint4_t raw[4];
-                uint32_t bits[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int g = min(g0 + 256 * u, groups - 1);
-                    raw[u] = *(const raw_t *)(x + g * TPG);
-                    bits[u] = mask ? (uint32_t)mask[(v0 + g * TPG) >> 5] >> ((v0 + g * TPG) & 31) : ~0u;
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int g = g0 + 256 * u;
-                    if (mask) {
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            if constexpr (sizeof(T) == 4) {
-                                raw[u][w] = (bits[u] >> w) & 1 ? raw[u][w] : 0xff800000u;
-                            } else {
-                                constexpr uint32_t INF = std::is_same<T, half_t>::value ? 0xfc00u : 0xff80u;
-                                const uint32_t lo = (bits[u] >> (2 * w)) & 1 ? raw[u][w] & 0xffffu : INF;
-                                const uint32_t hi = (bits[u] >> (2 * w + 1)) & 1 ? raw[u][w] & 0xffff0000u : INF << 16;
-                                raw[u][w] = lo | hi;
-                            }
-                        }
-                    }
-                    if (g < groups) *(raw_t *)(y + g * TPG) = raw[u];
+            const int t = mine(p.bias_tokens[(int64_t)s * p.n_bias + i]);
+            if (t >= 0) {
+                atomicOr(&counts[t], ADJ_BIAS);
+                const int k = atomicAdd(&biases, 1);
+                if (k < ADJ_BIASES) {
+                    bias_token[k] = t;
+                    bias_entry[k] = i;
                 }
             }
-            const int i = groups * TPG + tid;              // what is left of a row that is no whole number of groups
-            if (i < here) y[i] = !mask || ((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1) ? x[i] : AdjIO<T>::put(-INFINITY);
         }
     }
-    if (!p.sparse) return;
-    __syncthreads();                           // counts and biases are there, and so are the copies of this workgroup
-    for (int i = tid; i < here; i += 256)
-        if (counts[i]) list[atomicAdd(&listed, 1)] = (uint16_t)i;
-    __syncthreads();
+    const T *in = (const T *)p.logits + (int64_t)row * p.ld;
+    T *to = (T *)p.out + (int64_t)row * p.ldo;
+    auto mask_row = [&](const int j) {         // of the masks, or -1
+        const int m = p.mask_rows ? p.mask_rows[row + j] : row + j;
+        return m >= 0 && m < p.n_mask ? m : -1;
+    };
+    int n_listed = 0;
+    if (p.sparse) {
+        __syncthreads();                       // counts and biases are there
+        for (int i = tid; i < p.most; i += 256)
+            if (counts[i]) list[atomicAdd(&listed, 1)] = (uint16_t)i;
+        __syncthreads();
+        n_listed = listed;
+    }
     const float r = p.repetition ? p.repetition[s] : p.repetition_all;
     const float f = p.frequency ? p.frequency[s] : p.frequency_all;
     const float pr = p.presence ? p.presence[s] : p.presence_all;
-    for (int k = tid; k < listed; k += 256) {
-        const int i = (int)list[k];
-        const uint32_t n = counts[i];
-        const bool drafted = n & ADJ_DRAFT, biased = n & ADJ_BIAS;
-        bool seen = n & ADJ_SEEN;
-        uint32_t times = n & (ADJ_BIAS - 1);
-        float add = 0.0f;
-        if (biased) {                          // the last of the entries that name the token
-            int b = p.n_bias - 1;
-            while (p.bias_tokens[(int64_t)s * p.n_bias + b] != v0 + i) --b;
-            add = p.bias_values[(int64_t)s * p.n_bias + b];
+    // the bias of token i: the last of the entries that name it
+    auto bias_of = [&](const int i) {
+        int last = -1;
+        if (biases <= ADJ_BIASES) {
+            for (int b = 0; b < biases; ++b) last = bias_token[b] == i ? max(last, bias_entry[b]) : last;
+        } else {
+            const int v = at(i);
+            for (int b = 0; b < p.n_bias; ++b) last = p.bias_tokens[(int64_t)s * p.n_bias + b] == v ? b : last;
         }
-        for (int j = 0; j < rows; ++j) {
-            if (drafted && j > 0 && j - 1 < drafts && adj_token(p.drafts, 8, draft + j - 1) == v0 + i) {
-                ++times;
-                seen = true;
+        return p.bias_values[(int64_t)s * p.n_bias + last];
+    };
+    auto changed = [&](float x, const uint32_t n, const float add) {
+        const uint32_t times = n & (ADJ_BIAS - 1);
+        if (n & ADJ_SEEN) x = x > 0.0f ? x / r : x * r;
+        if (times) x = x - (f * (float)times + pr);
+        return n & ADJ_BIAS ? x + add : x;
+    };
+    // token i of the share in all rows, straight in memory
+    auto column = [&](const int i, uint32_t n) {
+        const int v = at(i);
+        const float add = n & ADJ_BIAS ? bias_of(i) : 0.0f;
+        for (int j0 = 0; j0 < rows; j0 += 4) {             // (four rows' loads on their way at a time)
+            T raw[4];
+            int64_t before[4];
+            bool allowed[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = min(j0 + u, rows - 1);
+                const int m = MASK ? mask_row(j) : -1;
+                raw[u] = in[j * p.ld + v];
+                allowed[u] = m < 0 || ((p.mask[m * p.mask_stride + (v >> 5)] >> (v & 31)) & 1);
+                before[u] = n & ADJ_DRAFT && j > 0 && j <= drafts ? adj_token(p.drafts, 8, draft + j - 1) : -1;
             }
-            const int32_t *mask = mask_of(j);
-            float x = AdjIO<T>::get(in[j * p.ld + i]);
-            if (seen) x = x > 0.0f ? x / r : x * r;
-            if (times) x = x - (f * (float)times + pr);
-            if (biased) x += add;
-            if (mask && !((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1)) x = -INFINITY;
-            to[j * p.ldo + i] = AdjIO<T>::put(x);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (j0 + u >= rows) break;
+                if (before[u] == v) n = (n + 1u) | ADJ_SEEN;
+                to[(j0 + u) * p.ldo + v] = AdjIO<T>::put(allowed[u] ? changed(AdjIO<T>::get(raw[u]), n, add) : -INFINITY);
+            }
+        }
+    };
+    if (!p.dense) {                            // in place, and no mask: nothing else changes
+        for (int k = tid; k < n_listed; k += 256) column(list[k], counts[list[k]]);
+        return;
+    }
+    constexpr int TPG = 16 / (int)sizeof(T);   // tokens of a group: 16 bytes, rows at any element
+    constexpr int U = ADJ_MOST / TPG / 256;    // groups of a thread
+    constexpr int R = 2;                       // rows at a time
+    // what the vocabulary has behind its last whole group
+    const int tail = p.vocab - p.vocab % TPG + tid;
+    if (tid < TPG && tail < p.vocab && mine(tail) >= 0) column(mine(tail), p.sparse ? counts[mine(tail)] : 0u);
+    if (p.vocab < TPG) return;
+    uint4_t raw[R][U], next[R][U];
+    uint32_t bits[R][U], next_bits[R][U];
+    // of a thread's only token of the list, where no thread has more
+    const bool few = n_listed <= 256;
+    const int my_i = few && tid < n_listed ? list[tid] : 0, my_v = at(my_i), per = p.most / TPG;
+    uint32_t my_n = few && tid < n_listed ? counts[my_i] : 0u;
+    const float my_add = my_n & ADJ_BIAS ? bias_of(my_i) : 0.0f;
+    for (int c0 = 0; c0 < rows; c0 += ADJ_ROWS) {
+        __syncthreads();                       // nobody reads the last rows' drafts and masks any more
+        if (tid < ADJ_ROWS) {
+            const int j = c0 + tid;
+            const int64_t t = j > 0 && j <= drafts ? adj_token(p.drafts, 8, draft + j - 1) : -1;
+            draft_of[tid] = t >= 0 && t < p.vocab ? (int)t : -1;
+            mask_at[tid] = MASK && j < rows ? mask_row(j) : -1;
+        }
+        __syncthreads();
+        const int end = min(rows, c0 + ADJ_ROWS);
+        // (what the next turn needs is requested a turn ahead, loads without branches in between: the compiler then knows how many
+        // younger ones it may leave on their way)
+        auto load = [&](uint4_t (&w)[R][U], uint32_t (&b)[R][U], const int j) {
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                const int jq = min(j + q, end - 1), m = MASK ? mask_at[jq - c0] : -1;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int v = min(at(TPG * (tid + 256 * u)), p.vocab - TPG);
+                    w[q][u] = *(const raw_t *)(in + jq * p.ld + v);
+                    if constexpr (MASK) b[q][u] = (uint32_t)p.mask[max(m, 0) * p.mask_stride + (v >> 5)] >> (v & 31) | (m < 0 ? ~0u : 0u);
+                }
+            }
+        };
+        load(raw, bits, c0);
+        for (int j = c0; j < end; j += R) {
+            load(next, next_bits, j + R);
+            if (n_listed) {
+                if (j > c0) __syncthreads();   // the last rows have left LDS
+#pragma unroll
+                for (int q = 0; q < R; ++q)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (tid + 256 * u < per) lds4[q * per + tid + 256 * u] = raw[q][u];
+                __syncthreads();
+                T *one = (T *)lds4;
+                if (few) {
+#pragma unroll
+                    for (int q = 0; q < R; ++q) {
+                        if (my_n && draft_of[min(j + q, end - 1) - c0] == my_v && j + q < end) my_n = (my_n + 1u) | ADJ_SEEN;
+                        if (my_n) one[q * p.most + my_i] = AdjIO<T>::put(changed(AdjIO<T>::get(one[q * p.most + my_i]), my_n, my_add));
+                    }
+                } else {
+                    for (int k = tid; k < n_listed; k += 256) {
+                        const int i = list[k];
+                        uint32_t n = counts[i];
+                        const float add = n & ADJ_BIAS ? bias_of(i) : 0.0f;
+#pragma unroll
+                        for (int q = 0; q < R; ++q) {
+                            if (j + q < end && draft_of[j + q - c0] == at(i)) counts[i] = n = (n + 1u) | ADJ_SEEN;
+                            one[q * p.most + i] = AdjIO<T>::put(changed(AdjIO<T>::get(one[q * p.most + i]), n, add));
+                        }
+                    }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int q = 0; q < R; ++q)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (tid + 256 * u < per) raw[q][u] = lds4[q * per + tid + 256 * u];
+            }
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                T *y = to + (j + q) * p.ldo;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int i = TPG * (tid + 256 * u), v = at(i);
+                    if constexpr (MASK) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            if constexpr (sizeof(T) == 4) {
+                                raw[q][u][w] = (bits[q][u] >> w) & 1 ? raw[q][u][w] : 0xff800000u;
+                            } else {
+                                constexpr uint32_t INF = std::is_same<T, half_t>::value ? 0xfc00u : 0xff80u;
+                                const uint32_t lo = (bits[q][u] >> (2 * w)) & 1 ? raw[q][u][w] & 0xffffu : INF;
+                                const uint32_t hi = (bits[q][u] >> (2 * w + 1)) & 1 ? raw[q][u][w] & 0xffff0000u : INF << 16;
+                                raw[q][u][w] = lo | hi;
+                            }
+                        }
+                    }
+                    if (j + q < end && i < p.most && v + TPG <= p.vocab) *(raw_t *)(y + v) = raw[q][u];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < R; ++q)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    raw[q][u] = next[q][u];
+                    if constexpr (MASK) bits[q][u] = next_bits[q][u];
+                }
         }
     }
 }
@@ -230,21 +346,28 @@ extern "C" int odsd_adjust_logits(const void *logits, int64_t logits_stride, voi
     p.bias_tokens = bias_tokens; p.bias_values = bias_values; p.n_bias = n_bias;
     p.mask = mask; p.mask_stride = mask_stride; p.n_mask = n_mask; p.mask_rows = mask_rows;
     p.n_seqs = n_seqs; p.n_rows = n_rows; p.vocab = vocab;
-    // slices: enough workgroups for the chip, of 1024 to 8192 tokens
-    int64_t slice = ((int64_t)vocab * n_seqs / 1024 + 255) / 256 * 256;
-    slice = max((int64_t)1024, min((int64_t)8192, slice));
-    p.slice = (int)slice;
-    p.slices = (int)((vocab + slice - 1) / slice);
-    if ((int64_t)n_seqs * p.slices >= (1LL << 24) || max_tokens + (int64_t)n_drafts >= (1 << 29)) return ODSD_ERR_UNSUPPORTED;
+    // shares: enough workgroups for the chip, of 1024 to 4096 tokens
+    const int64_t granules = ((int64_t)vocab + ADJ_GRANULE - 1) / ADJ_GRANULE;
+    auto tokens_of = [&](const int bits) { return ((granules + (1LL << bits) - 1) >> bits) * ADJ_GRANULE; };
+    while (tokens_of(p.share_bits) > 1024 && (tokens_of(p.share_bits) > ADJ_MOST || ((int64_t)n_seqs << p.share_bits) < 1024)) ++p.share_bits;
+    p.shares = 1 << p.share_bits;
+    p.most = (int)tokens_of(p.share_bits);
+    if ((int64_t)n_seqs * p.shares >= (1LL << 24) || max_tokens + (int64_t)n_drafts >= (1 << 29)) return ODSD_ERR_UNSUPPORTED;
     p.sparse = p.tokens || n_drafts || n_bias;
     p.dense = out != logits || out_stride != logits_stride || mask;
     if (!p.sparse && !p.dense) return ODSD_OK;
-    const unsigned grid = (unsigned)(n_seqs * p.slices);
-    const size_t bytes = p.sparse ? (size_t)slice * 6 : 0;
+    const unsigned grid = (unsigned)n_seqs << p.share_bits;
+    const size_t elt = dtype == ODSD_DT_F32 ? 4 : 2, bytes = p.sparse ? (size_t)p.most * (6 + (p.dense ? 2 * elt : 0)) : 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == ODSD_DT_F32) adjust_logits_kernel<float><<<grid, 256, bytes, st>>>(p);
-    else if (dtype == ODSD_DT_BF16) adjust_logits_kernel<__bf16><<<grid, 256, bytes, st>>>(p);
-    else adjust_logits_kernel<half_t><<<grid, 256, bytes, st>>>(p);
+#define ADJ_GO(T)                                                                 \
+    do {                                                                          \
+        if (mask && n_mask) adjust_logits_kernel<T, true><<<grid, 256, bytes, st>>>(p);     \
+        else adjust_logits_kernel<T, false><<<grid, 256, bytes, st>>>(p);         \
+    } while (0)
+    if (dtype == ODSD_DT_F32) ADJ_GO(float);
+    else if (dtype == ODSD_DT_BF16) ADJ_GO(__bf16);
+    else ADJ_GO(half_t);
+#undef ADJ_GO
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
 }
