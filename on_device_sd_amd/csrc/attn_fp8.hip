@@ -17,20 +17,220 @@
 // present one has just left.
 #include "attn_list.h"
 #include "fp8.h"
+#include "w4_gemm.h"
 
-#define FP8_WG 512           // workgroups that share the keys: two per CU (one with 64 rows)
+#define FP8_WG 512           // workgroups that share the keys: two per CU
 #define FP8_STEP 256         // keys of a list step, 64 per wavefront
 #define FP8_WHOLE 512        // no sequence longer: nothing is split
 
 struct AttnFp8Params : AttnParams {
     const float *scales;     // [n_blocks, KVH, 2]
     int n_blocks;
+    uint32_t gq_inverse;     // ceil(2^32 / Gq), 0 for 1
 };
+// query token of a row: row / Gq (exact: rows * Gq stays below 2^32)
+__device__ __forceinline__ int fp8_token(const AttnFp8Params &p, const int row) {
+    return p.gq_inverse ? (int)__umulhi((uint32_t)row, p.gq_inverse) : row;
+}
 
-template <typename T, int HD, int RB, bool ALIGNED, bool SPLIT>
-__global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const AttnFp8Params p) {
+// ---- 64 keys of 16 RB query rows ------------------------------------------------------------------------
+// Lane (c, kq) has the raw scores st[rb][t] of keys k0 + 16 kq + 4 t + i of query row 16 rb + c.  Returns the weights as the B operands of
+// O^T = V^T P^T and keeps the rows' reference points, this lane's part of their sums, and O^T.  sc, ev, iv: of the block of the lane's
+// keys, scale * sk * log2 e, log2 sv and 1 / sv.
+template <typename T, int RB, int NDB>
+__device__ __forceinline__ void fp8_weights(const float4_t (&st)[RB][4], const float sc, const float ev, const float iv, const bool masked,
+                                            const int k, const int (&kmax)[RB], float (&m_run)[RB], float (&l_run)[RB],
+                                            float4_t (&o)[RB][NDB], typename AttnT<T>::V8 (&pf)[RB][2]) {
     typedef typename AttnT<T>::V8 V8;
-    constexpr int NJ = HD / 32;          // 32-dim steps of the score product
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float a[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            a[4 * t] = st[rb][t].x; a[4 * t + 1] = st[rb][t].y; a[4 * t + 2] = st[rb][t].z; a[4 * t + 3] = st[rb][t].w;
+        }
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) a[e] = k + e <= kmax[rb] ? a[e] : -INFINITY;
+        }
+        float mx = a[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, a[e]);
+        mx = fmaf(mx, sc, ev);
+        // The reference point moves only when a weight of the wavefront would pass 2^8 (weights up to 256 are as exact in fp16 / bf16 as
+        // those below 1, and the sums are fp32): most tiles need no exchange between lanes
+        if (__any(mx > m_run[rb] + 8.0f)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16, ODSD_WAVE));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, ODSD_WAVE));
+            const float m_new = fmaxf(m_run[rb], mx);
+            // a row with nothing to attend yet keeps m = -inf: use 0 as the reference point then
+            const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - (m_new == -INFINITY ? 0.0f : m_new));
+            l_run[rb] *= alpha;
+            m_run[rb] = m_new;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) {
+                o[rb][db].x *= alpha; o[rb][db].y *= alpha; o[rb][db].z *= alpha; o[rb][db].w *= alpha;
+            }
+        }
+        const float ref = m_run[rb] == -INFINITY ? ev : ev - m_run[rb];
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) a[e] = __builtin_amdgcn_exp2f(fmaf(a[e], sc, ref));      // masked -> 0
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) sum += (a[e] + a[e + 1]) + (a[e + 2] + a[e + 3]);
+        l_run[rb] = fmaf(sum, iv, l_run[rb]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            pf[rb][u] = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(a[8 * u], a[8 * u + 1]), AttnT<T>::pack2(a[8 * u + 2], a[8 * u + 3]),
+                                                       AttnT<T>::pack2(a[8 * u + 4], a[8 * u + 5]), AttnT<T>::pack2(a[8 * u + 6], a[8 * u + 7])});
+    }
+}
+// Codes of V, 16 keys of one dimension from key k on, of a masked tile.  Bytes past the last key are what a block held before: they count as
+// zeros.  A NaN of a key that some rows see and others do not must not reach the others as 0 * NaN: fp8_nan_rows counts such codes for the
+// rows that see them by a product of its own, and takes them out.
+__device__ __forceinline__ uint4_t fp8_keep(uint4_t v, const int k, const int L) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int left = L - k - 4 * w;
+        v[w] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t fp8_nan_bits(const uint4_t v) {
+    return ((((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u)) |
+            (((v.z & 0x7f7f7f7fu) + 0x01010101u) | ((v.w & 0x7f7f7f7fu) + 0x01010101u))) & 0x80808080u;
+}
+template <typename T, int RB, int NDB>
+__device__ __forceinline__ void fp8_nan_rows(uint4_t &v, const int db, const int k, const int (&kmax)[RB], float4_t (&o)[RB][NDB]) {
+    typedef typename AttnT<T>::V8 V8;
+    uint32_t ones[4];                              // 1.0 where the code is no number
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t f = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+        ones[w] = f * 0x38u;
+        v[w] &= ~(f * 0xffu);
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float4_t cnt = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float s[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = k + 8 * u + e <= kmax[rb] ? 1.0f : 0.0f;
+            const V8 sees = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(s[0], s[1]), AttnT<T>::pack2(s[2], s[3]),
+                                                           AttnT<T>::pack2(s[4], s[5]), AttnT<T>::pack2(s[6], s[7])});
+            cnt = AttnT<T>::mfma(fp8_widen8<T>(ones[2 * u], ones[2 * u + 1]), sees, cnt);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (cnt[i] > 0.0f) o[rb][db][i] = __builtin_nanf("");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// fragments of the unit's query rows from row0 on, and the last position that each attends
+template <typename T, int HD, int RB>
+__device__ __forceinline__ void fp8_queries(const AttnFp8Params &p, const SeqAt &sq, const int kvh, const int row0, const int lane,
+                                            typename AttnT<T>::V8 (&qf)[RB][HD / 32], int (&kmax)[RB]) {
+    const int c = lane & 15, kq = lane >> 4, rows_total = sq.ql * p.Gq;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int row = row0 + 16 * rb + c;
+        const bool ok = row < rows_total;
+        const int tok = ok ? fp8_token(p, row) : 0, hq = ok ? row - tok * p.Gq : 0;
+        kmax[rb] = ok ? sq.L - sq.ql + tok : -1;
+        const uint16_t *qp = (const uint16_t *)p.q + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + 16 * kq;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {                // dims 64 (j / 2) + 16 kq + 8 (j % 2) ..
+            uint4_t raw = {0u, 0u, 0u, 0u};
+            if (ok) raw = *(const uint4_t *)(qp + 64 * (j >> 1) + 8 * (j & 1));
+            qf[rb][j] = __builtin_bit_cast(typename AttnT<T>::V8, raw);
+        }
+    }
+}
+// block of the KV head (block * KVH + kvh) and token of it of position kp; an entry that is negative or beyond the cache reads block 0
+__device__ __forceinline__ void fp8_locate(const AttnFp8Params &p, const int32_t *bt, const int kvh, const int kp, uint32_t &gk, uint32_t &off) {
+    const int blk = kp / p.block_size;
+    const int32_t b = bt[min(blk, p.max_blocks - 1)];
+    gk = (b >= 0 && b < p.n_blocks && blk < p.max_blocks ? (uint32_t)b : 0u) * (uint32_t)p.KVH + (uint32_t)kvh;
+    off = (uint32_t)(kp - blk * p.block_size);
+}
+// its scales as the scores want them: scale * sk * log2 e, log2 sv, 1 / sv
+__device__ __forceinline__ void fp8_scales(const AttnFp8Params &p, const uint32_t gk, float &sc, float &ev, float &iv) {
+    const float2_t s2 = *(const float2_t *)(p.scales + 2 * (size_t)gk);
+    const float sv = fmaxf(s2.y, FP8_MIN_SCALE);
+    sc = p.scale_log2e * fmaxf(s2.x, FP8_MIN_SCALE);
+    ev = __builtin_amdgcn_logf(sv);
+    iv = __builtin_amdgcn_rcpf(sv);
+}
+// The sums of WK wavefronts that had other keys of the same rows (and of WR groups of them, with other rows), 16 rows of each group at
+// a time through LDS; `whole`: the unit is done, otherwise the results go to `part`.
+template <typename T, int HD, int RB, int WR>
+__device__ __forceinline__ void fp8_finish(const AttnFp8Params &p, const SeqAt &sq, const int kvh, const int row0, const int tid, const bool whole,
+                                           float *part, const float (&m_run)[RB], const float (&l_run)[RB], const float4_t (&o)[RB][HD / 16],
+                                           float *xch) {
+    constexpr int WK = 4 / WR, XROW = HD + 4, TPR = 16 / WR, PIECES = HD / 4 / TPR;      // threads of a row, float4 each
+    const int lane = tid & 63, wave = tid >> 6, c = lane & 15, kq = lane >> 4;
+    const int rows_here = min(16 * RB * WR, sq.ql * p.Gq - row0);
+    const int x = tid / TPR;                               // this thread's row of the 16 WR
+    const float *xs = xch + ((x >> 4) * WK * 16 + (x & 15)) * XROW;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        __syncthreads();                                   // the area is free
+        float *xr = xch + (wave * 16 + c) * XROW;          // wavefront: group wave / WK, keys wave % WK
+        float l = l_run[rb];
+        l += __shfl_xor(l, 16, ODSD_WAVE);
+        l += __shfl_xor(l, 32, ODSD_WAVE);
+#pragma unroll
+        for (int db = 0; db < HD / 16; ++db) *(float4_t *)(xr + 16 * db + 4 * kq) = o[rb][db];
+        if (kq == 0) {
+            xr[HD] = m_run[rb];
+            xr[HD + 1] = l;
+        }
+        __syncthreads();
+        const int r = 16 * RB * (x >> 4) + 16 * rb + (x & 15);
+        if (r >= rows_here) continue;
+        float m = -INFINITY, f[WK], ls = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) m = fmaxf(m, xs[w * 16 * XROW + HD]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(xs[w * 16 * XROW + HD] - ref);      // -inf -> 0
+            ls += f[w] * xs[w * 16 * XROW + HD + 1];
+        }
+        if (whole) {
+            const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) f[w] *= inv;
+        }
+        const int tok = fp8_token(p, row0 + r), hq = row0 + r - tok * p.Gq;
+        uint16_t *to = (uint16_t *)p.out + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD;
+        float *pr = part + r * XROW;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int d = 4 * (tid % TPR + TPR * i);
+            float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float4_t v = *(const float4_t *)(xs + w * 16 * XROW + d);
+                acc.x += f[w] * v.x; acc.y += f[w] * v.y; acc.z += f[w] * v.z; acc.w += f[w] * v.w;
+            }
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            if (whole) *(u32x2 *)(to + d) = u32x2{AttnT<T>::pack2(acc.x, acc.y), AttnT<T>::pack2(acc.z, acc.w)};
+            else *(float4_t *)(pr + d) = acc;
+        }
+        if (!whole && tid % TPR == 0) {
+            pr[HD] = m;
+            pr[HD + 1] = ls;
+        }
+    }
+}
+
+// ---- up to 32 rows: the keys straight to registers --------------------------------------------------------
+template <typename T, int HD, int RB, bool ALIGNED>
+__global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p) {
+    typedef typename AttnT<T>::V8 V8;
     constexpr int NC = HD / 64;          // 16-byte pieces of a K row per lane
     constexpr int NDB = HD / 16;         // 16-dim blocks of the output
     constexpr int ROWS = 16 * RB, XROW = HD + 4;
@@ -40,13 +240,13 @@ __global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const At
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, kq = lane >> 4;
 
-    const ListPlan pl = list_plan<false, SPLIT, RB != 4 || !SPLIT, RB == 4>(p, ROWS, FP8_STEP, FP8_STEP, blockIdx.x);
+    const ListPlan pl = list_plan<false, true, true>(p, ROWS, FP8_STEP, FP8_STEP, blockIdx.x);
     if (!pl.found) return;
     const int first_pos = pl.me * pl.share;
     int pos = first_pos;                                   // list position of the next step
     const int end = min(pl.total, pos + pl.share);
     SeqAt sq = pl.at;
-    int unit = (pos - sq.first) / sq.steps;                // unit of the sequence, step inside the unit
+    int unit = sq.steps == 1 ? pos - sq.first : (pos - sq.first) / sq.steps;      // unit of the sequence, step inside the unit
     int step = (pos - sq.first) - unit * sq.steps;
 
     const int bs = p.block_size;
@@ -59,30 +259,13 @@ __global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const At
     while (pos < end) {
         // ---- one piece: steps step .. step + n - 1 of one unit ----------------------------------------
         const int n = min(end - pos, sq.steps - step);
-        const int kvh = unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);      // row groups with the most keys first
-        const int L = sq.L, ql = sq.ql;
-        const int rows_total = ql * p.Gq, row0 = rg * ROWS;
-        const int rows_here = min(ROWS, rows_total - row0);
+        const int kvh = sq.rg == 1 ? unit : unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);
+        const int L = sq.L, row0 = rg * ROWS;
         const int32_t *bt = p.block_tables + (size_t)sq.seq * p.max_blocks;
-
-        V8 qf[RB][NJ];
-        int kmax[RB];                                      // last position that row attends
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const int row = row0 + 16 * rb + c;
-            const bool ok = row < rows_total;
-            const int tok = ok ? row / p.Gq : 0, hq = ok ? row - tok * p.Gq : 0;
-            kmax[rb] = ok ? L - ql + tok : -1;
-            const uint16_t *qp = (const uint16_t *)p.q + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + 16 * kq;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {                 // dims 64 (j / 2) + 16 kq + 8 (j % 2) ..
-                uint4_t raw = {0u, 0u, 0u, 0u};
-                if (ok) raw = *(const uint4_t *)(qp + 64 * (j >> 1) + 8 * (j & 1));
-                qf[rb][j] = __builtin_bit_cast(V8, raw);
-            }
-        }
-        const int kmin = L - ql + row0 / p.Gq;            // the unit's first row: tiles that end at or before it need no mask
-
+        V8 qf[RB][HD / 32];
+        int kmax[RB];
+        fp8_queries<T, HD, RB>(p, sq, kvh, row0, lane, qf, kmax);
+        const int kmin = L - sq.ql + fp8_token(p, row0);         // the unit's first row: tiles that end at or before it need no mask
         float m_run[RB], l_run[RB];
         float4_t o[RB][NDB];
 #pragma unroll
@@ -92,23 +275,16 @@ __global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const At
 #pragma unroll
             for (int db = 0; db < NDB; ++db) o[rb][db] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-
-        int key_end = step + n == sq.steps ? L : pl.g * (step + n);
-        if (RB == 4 && sq.rg > 1)                          // (no further than the unit's last row sees)
-            key_end = min(key_end, L - ql + min(ql, (row0 + ROWS - 1) / p.Gq + 1));
+        const int key_end = step + n == sq.steps ? L : pl.g * (step + n);
         for (int key0 = pl.g * step + 64 * wave; key0 < key_end; key0 += MOST * FP8_STEP) {
             const int nt = min(MOST, (key_end - key0 + FP8_STEP - 1) / FP8_STEP);
             // the blocks of this wavefront's next tiles, one tile (ALIGNED: it lies in one block) or one group of 16 keys per lane;
-            // an entry that is negative or beyond the cache reads block 0, keys past the last one its group
-            const int kp = min(ALIGNED ? key0 + FP8_STEP * lane : key0 + FP8_STEP * (lane >> 2) + 16 * (lane & 3),
-                               ALIGNED ? (L - 1) & ~63 : (L - 1) & ~15);
-            const int blk = kp / bs;
-            const int32_t b = bt[min(blk, p.max_blocks - 1)];
-            const uint32_t gk_l = (b >= 0 && b < p.n_blocks && blk < p.max_blocks ? (uint32_t)b : 0u) * (uint32_t)p.KVH + (uint32_t)kvh;
-            const uint32_t off_l = (uint32_t)(kp - blk * bs);
-            const float2_t s2 = *(const float2_t *)(p.scales + 2 * (size_t)gk_l);
-            const float sc_l = p.scale_log2e * fmaxf(s2.x, FP8_MIN_SCALE), sv_l = fmaxf(s2.y, FP8_MIN_SCALE);
-            const float ev_l = __builtin_amdgcn_logf(sv_l), iv_l = __builtin_amdgcn_rcpf(sv_l);
+            // keys past the last one are its group's
+            uint32_t gk_l, off_l;
+            float sc_l, ev_l, iv_l;
+            fp8_locate(p, bt, kvh, min(ALIGNED ? key0 + FP8_STEP * lane : key0 + FP8_STEP * (lane >> 2) + 16 * (lane & 3),
+                                       ALIGNED ? (L - 1) & ~63 : (L - 1) & ~15), gk_l, off_l);
+            fp8_scales(p, gk_l, sc_l, ev_l, iv_l);
 
             uint4_t kreg[4][NC], vreg[NDB];
             auto k_from = [&](const int i) {
@@ -134,7 +310,7 @@ __global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const At
                 for (int h = 0; h < NC; ++h) kreg[t][h] = __builtin_nontemporal_load((const uint4_t *)(at + 4 * t * HD + 64 * h));
             };
             auto fetch_v = [&](const char *at, const int db) {
-                vreg[db] = __builtin_nontemporal_load((const uint4_t *)(at + (uint32_t)(16 * db * bs)));
+                vreg[db] = *(const uint4_t *)(at + (uint32_t)(16 * db * bs));
             };
             // one tile.  FETCH: there is a next one, whose bytes are requested as registers come free (the scheduling barriers keep
             // the compiler from widening all of a tile first, which costs 64 registers)
@@ -172,93 +348,17 @@ __global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const At
                 if constexpr (decltype(fetch_c)::value) next = v_from(i + 1);
                 const bool masked = k0 + 63 > kmin;
                 V8 pf[RB][2];
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    // lane (c, kq) holds keys k0 + 16 kq + 4 t + i of query row c
-                    float a[16];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        a[4 * t] = st[rb][t].x; a[4 * t + 1] = st[rb][t].y; a[4 * t + 2] = st[rb][t].z; a[4 * t + 3] = st[rb][t].w;
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) a[e] = k0 + 16 * kq + e <= kmax[rb] ? a[e] : -INFINITY;
-                    }
-                    float mx = a[0];
-#pragma unroll
-                    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, a[e]);
-                    mx = fmaf(mx, sc, ev);
-                    // The reference point moves only when a weight of the wavefront would pass 2^8 (weights up to 256 are as exact in
-                    // fp16 / bf16 as those below 1, and the sums are fp32): most tiles need no exchange between lanes
-                    if (__any(mx > m_run[rb] + 8.0f)) {
-                        mx = fmaxf(mx, __shfl_xor(mx, 16, ODSD_WAVE));
-                        mx = fmaxf(mx, __shfl_xor(mx, 32, ODSD_WAVE));
-                        const float m_new = fmaxf(m_run[rb], mx);
-                        // a row with nothing to attend yet keeps m = -inf: use 0 as the reference point then
-                        const float alpha = __builtin_amdgcn_exp2f(m_run[rb] - (m_new == -INFINITY ? 0.0f : m_new));
-                        l_run[rb] *= alpha;
-                        m_run[rb] = m_new;
-#pragma unroll
-                        for (int db = 0; db < NDB; ++db) {
-                            o[rb][db].x *= alpha; o[rb][db].y *= alpha; o[rb][db].z *= alpha; o[rb][db].w *= alpha;
-                        }
-                    }
-                    const float ref = m_run[rb] == -INFINITY ? ev : ev - m_run[rb];
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) a[e] = __builtin_amdgcn_exp2f(fmaf(a[e], sc, ref));      // masked -> 0
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) sum += (a[e] + a[e + 1]) + (a[e + 2] + a[e + 3]);
-                    l_run[rb] = fmaf(sum, iv, l_run[rb]);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        pf[rb][u] = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(a[8 * u], a[8 * u + 1]), AttnT<T>::pack2(a[8 * u + 2], a[8 * u + 3]),
-                                                                   AttnT<T>::pack2(a[8 * u + 4], a[8 * u + 5]), AttnT<T>::pack2(a[8 * u + 6], a[8 * u + 7])});
-                }
+                fp8_weights<T, RB, NDB>(st, sc, ev, iv, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
                 if (masked) {
-                    // Bytes of V past the last key are what a block held before: they count as zeros.  A NaN of a key that some
-                    // rows see and others do not must not reach the others as 0 * NaN: such codes are counted for the rows that
-                    // see them by a product of their own, and taken out.
-                    uint32_t keep[4], bad = 0u;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int left = L - (k0 + 16 * kq) - 4 * w;
-                        keep[w] = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-                    }
+                    uint32_t bad = 0u;
 #pragma unroll
                     for (int db = 0; db < NDB; ++db) {
-                        vreg[db].x &= keep[0]; vreg[db].y &= keep[1]; vreg[db].z &= keep[2]; vreg[db].w &= keep[3];
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) bad |= (vreg[db][w] & 0x7f7f7f7fu) + 0x01010101u;
+                        vreg[db] = fp8_keep(vreg[db], k0 + 16 * kq, L);
+                        bad |= fp8_nan_bits(vreg[db]);
                     }
-                    if (__any((bad & 0x80808080u) != 0u)) {
+                    if (__any(bad != 0u)) {
 #pragma unroll
-                        for (int db = 0; db < NDB; ++db) {
-                            uint32_t ones[4];              // 1.0 where the code is no number
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                const uint32_t f = (((vreg[db][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                                ones[w] = f * 0x38u;
-                                vreg[db][w] &= ~(f * 0xffu);
-                            }
-#pragma unroll
-                            for (int rb = 0; rb < RB; ++rb) {
-                                float4_t cnt = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                    float s[8];
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e) s[e] = k0 + 16 * kq + 8 * u + e <= kmax[rb] ? 1.0f : 0.0f;
-                                    const V8 sees = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(s[0], s[1]), AttnT<T>::pack2(s[2], s[3]),
-                                                                                   AttnT<T>::pack2(s[4], s[5]), AttnT<T>::pack2(s[6], s[7])});
-                                    cnt = AttnT<T>::mfma(fp8_widen8<T>(ones[2 * u], ones[2 * u + 1]), sees, cnt);
-                                }
-#pragma unroll
-                                for (int i4 = 0; i4 < 4; ++i4)
-                                    if (cnt[i4] > 0.0f) o[rb][db][i4] = __builtin_nanf("");
-                                __builtin_amdgcn_sched_barrier(0);
-                            }
-                        }
+                        for (int db = 0; db < NDB; ++db) fp8_nan_rows<T, RB, NDB>(vreg[db], db, k0 + 16 * kq, kmax, o);
                     }
                 }
 #pragma unroll
@@ -285,56 +385,176 @@ __global__ __launch_bounds__(256, RB == 4 ? 1 : 2) void attn_fp8_kernel(const At
             tile(std::false_type{}, i);
         }
 
-        // ---- the four wavefronts' sums, through LDS, 16 rows at a time ------------------------------------
-        const bool whole = n == sq.steps;
         // (a piece that begins where its workgroup's share begins goes to the workgroup's first slot)
-        float *part = p.part + (size_t)(2 * pl.me + (pos > first_pos ? 1 : 0)) * (ROWS * XROW);
+        fp8_finish<T, HD, RB, 1>(p, sq, kvh, row0, tid, n == sq.steps, p.part + (size_t)(2 * pl.me + (pos > first_pos ? 1 : 0)) * (ROWS * XROW),
+                                 m_run, l_run, o, xch);
+        pos += n;
+        if (pos < end) next_unit(p, sq, unit, step, ROWS, pl.g);
+    }
+}
+
+// ---- more rows: the keys through LDS -----------------------------------------------------------------------
+// Steps of 128 keys, copied to LDS as they are (asynchronously, the next step's while this one is worked on) for all four wavefronts.  A
+// wavefront has 32 rows; WR of them next to each other, the others have other keys of a step (two of 64; with WR = 4 every one both).
+// 16-byte pieces are stored XORed with bits of their row, so that the 16 rows that are read together lie in all banks: K rows (keys
+// 16 a + 4 t + b, a and b from the lane) by a and the upper bit of b, V rows (dimensions) by their number / 2.
+#define FP8_TILE 128         // keys of a step
+#define FP8_TILES 32         // steps whose blocks are looked up at a time
+
+template <typename T, int HD, int WR, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Params p) {
+    typedef typename AttnT<T>::V8 V8;
+    constexpr int RB = 2, WK = 4 / WR, ROWS = 16 * RB * WR, XROW = HD + 4;
+    constexpr int NC = HD / 64, NDB = HD / 16, NP = HD / 16;       // NP: pieces of a K row
+    constexpr int TILEB = FP8_TILE * HD;                  // bytes of K (and of V) of a step
+    constexpr int COPIES = TILEB / 1024 / 4;              // copies of K (and of V) per wavefront
+    __shared__ __attribute__((aligned(16))) char lds[2 * 2 * TILEB];
+    __shared__ uint32_t at_block[FP8_TILES * 8], at_token[FP8_TILES * 8];      // of every 16 keys
+    __shared__ float4_t at_scale[FP8_TILES * 8];
+    static_assert(2 * 2 * TILEB >= 4 * 16 * XROW * 4, "the exchange area is in the tiles");
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, kq = lane >> 4, wr = wave / WK, wk = wave % WK;
+
+    const ListPlan pl = list_plan<false, SPLIT, !SPLIT, true>(p, ROWS, FP8_TILE, FP8_TILE, blockIdx.x);
+    if (!pl.found) return;
+    const int first_pos = pl.me * pl.share;
+    int pos = first_pos;
+    const int end = min(pl.total, pos + pl.share);
+    SeqAt sq = pl.at;
+    int unit = sq.steps == 1 ? pos - sq.first : (pos - sq.first) / sq.steps;
+    int step = (pos - sq.first) - unit * sq.steps;
+    const int bs = p.block_size;
+    const uint32_t block_bytes = (uint32_t)(bs * HD);
+
+    // copies: K rows RPC i + lane / NP of the tile, V rows 8 i + lane / 8 (dimensions)
+    constexpr int RPC = 64 / NP;
+    const int k_row = lane / NP, k_slot = lane % NP, v_row = lane >> 3, v_slot = lane & 7;
+    // fragments
+    const int ka = c >> 2, kb = c & 3;
+    uint32_t k_at[NC];
+#pragma unroll
+    for (int h = 0; h < NC; ++h) {
+        const int f = HD == 128 ? (kb >> 1) + 2 * ka : ka;
+        k_at[h] = (uint32_t)((16 * ka + kb) * HD + ((kq + 4 * h) ^ f) * 16);
+    }
+
+    while (pos < end) {
+        const int n = min(end - pos, sq.steps - step);
+        const int kvh = sq.rg == 1 ? unit : unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);      // row groups with the most keys first
+        const int L = sq.L, row0 = rg * ROWS;
+        const int32_t *bt = p.block_tables + (size_t)sq.seq * p.max_blocks;
+        V8 qf[RB][HD / 32];
+        int kmax[RB];
+        fp8_queries<T, HD, RB>(p, sq, kvh, row0 + 16 * RB * wr, lane, qf, kmax);
+        const int kmin = L - sq.ql + fp8_token(p, row0 + 16 * RB * wr);     // of the wavefront's first row
+        const bool active = row0 + 16 * RB * wr < sq.ql * p.Gq;
+        float m_run[RB], l_run[RB];
+        float4_t o[RB][NDB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            __syncthreads();                               // the area is free
-            float *xr = xch + (wave * 16 + c) * XROW;
-            float l = l_run[rb];
-            l += __shfl_xor(l, 16, ODSD_WAVE);
-            l += __shfl_xor(l, 32, ODSD_WAVE);
+            m_run[rb] = -INFINITY;
+            l_run[rb] = 0.0f;
 #pragma unroll
-            for (int db = 0; db < NDB; ++db) *(float4_t *)(xr + 16 * db + 4 * kq) = o[rb][db];
-            if (kq == 0) {
-                xr[HD] = m_run[rb];
-                xr[HD + 1] = l;
+            for (int db = 0; db < NDB; ++db) o[rb][db] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        int key_end = step + n == sq.steps ? L : pl.g * (step + n);
+        if (sq.rg > 1)                                     // (no further than the unit's last row sees)
+            key_end = min(key_end, L - sq.ql + min(sq.ql, fp8_token(p, row0 + ROWS - 1) + 1));
+        for (int key0 = pl.g * step; key0 < key_end; key0 += FP8_TILES * FP8_TILE) {
+            const int nt = min(FP8_TILES, (key_end - key0 + FP8_TILE - 1) / FP8_TILE);
+            __syncthreads();                               // tables and tiles are free
+            uint32_t gk = 0u, off;
+            if (tid < 8 * nt) {
+                fp8_locate(p, bt, kvh, min(key0 + 16 * tid, (L - 1) & ~15), gk, off);
+                at_block[tid] = gk;
+                at_token[tid] = off;
             }
             __syncthreads();
-            for (int it = tid; it < min(16, rows_here - 16 * rb) * (HD / 4); it += 256) {
-                const int row = it / (HD / 4), d = 4 * (it % (HD / 4));
-                const float *xs = xch + row * XROW;
-                float m = -INFINITY;
+            // (Q has come in before the table entries; without this the compiler would wait for it, and with it for every copy, at
+            // its first use)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) m = fmaxf(m, xs[w * 16 * XROW + HD]);
-                const float ref = m == -INFINITY ? 0.0f : m;
-                float ls = 0.0f;
-                float4_t acc = {0.f, 0.f, 0.f, 0.f};
+            for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(xs[w * 16 * XROW + HD] - ref);      // -inf -> 0
-                    const float4_t v = *(const float4_t *)(xs + w * 16 * XROW + d);
-                    ls += f * xs[w * 16 * XROW + HD + 1];
-                    acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+                for (int j = 0; j < HD / 32; ++j) asm volatile("" : "+v"(qf[rb][j]));
+            auto copy = [&](const int i) {
+                char *dst = lds + (i & 1) * (2 * TILEB);
+#pragma unroll
+                for (int u = 0; u < COPIES; ++u) {
+                    const int r = RPC * (COPIES * wave + u) + k_row;       // key of the tile
+                    const int g = 8 * i + r / 16, a = (r >> 4) & 3, f = HD == 128 ? ((r >> 1) & 1) + 2 * a : a;
+                    dma16_from_to_lds((const char *)p.k_cache + (uint64_t)at_block[g] * block_bytes + at_token[g] * (uint32_t)HD +
+                                          (uint32_t)((r & 15) * HD + (k_slot ^ f) * 16),
+                                      (lds_void *)(dst + 1024 * (COPIES * wave + u)));
                 }
-                const int r = 16 * rb + row;
-                if (whole) {
-                    const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
-                    const int tok = (row0 + r) / p.Gq, hq = row0 + r - tok * p.Gq;
-                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                    *(u32x2 *)((uint16_t *)p.out + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + d) =
-                        u32x2{AttnT<T>::pack2(acc.x * inv, acc.y * inv), AttnT<T>::pack2(acc.z * inv, acc.w * inv)};
-                } else {
-                    *(float4_t *)(part + r * XROW + d) = acc;
-                    if (d == 0) {
-                        part[r * XROW + HD] = m;
-                        part[r * XROW + HD + 1] = ls;
+#pragma unroll
+                for (int u = 0; u < COPIES; ++u) {
+                    const int d = 8 * (COPIES * wave + u) + v_row, g = 8 * i + (v_slot ^ ((d >> 1) & 7));
+                    dma16_from_to_lds((const char *)p.v_cache + (uint64_t)at_block[g] * block_bytes + at_token[g] + (uint32_t)(d * bs),
+                                      (lds_void *)(dst + TILEB + 1024 * (COPIES * wave + u)));
+                }
+            };
+            copy(0);
+            if (tid < 8 * nt) {                            // (the scales are wanted behind the first barrier only)
+                float sc, ev, iv;
+                fp8_scales(p, gk, sc, ev, iv);
+                at_scale[tid] = float4_t{sc, ev, iv, 0.f};
+            }
+            for (int i = 0; i < nt; ++i) {
+                ODSD_WAIT_VMCNT_LGKM0(0);                  // this wavefront's copies of step i have landed
+                __builtin_amdgcn_s_barrier();              // ... everybody's, and all are done with step i - 1
+                if (i + 1 < nt) copy(i + 1);
+                if (!active) continue;
+                const char *kt = lds + (i & 1) * (2 * TILEB), *vt = kt + TILEB;
+#pragma unroll
+                for (int sub = 0; sub < (WK == 1 ? 2 : 1); ++sub) {
+                    const int half = WK == 1 ? sub : wk, k0 = key0 + FP8_TILE * i + 64 * half;
+                    const float4_t sc = at_scale[8 * i + 4 * half + kq];
+                    // (the next fragment is read while this one is multiplied; the scheduling barriers keep the compiler from reading and
+                    // widening all of them first, whose registers would push others out to memory)
+                    auto k_piece = [&](const int x) { return *(const uint4_t *)(kt + k_at[x % NC] + (64 * half + 4 * (x / NC)) * HD); };
+                    float4_t st[RB][4];
+                    uint4_t w = k_piece(0), wn = w;
+#pragma unroll
+                    for (int x = 0; x < 4 * NC; ++x) {
+                        const int t = x / NC, h = x % NC;
+                        if (x + 1 < 4 * NC) wn = k_piece(x + 1);
+                        const V8 lo = fp8_widen8<T>(w.x, w.y), hi = fp8_widen8<T>(w.z, w.w);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            st[rb][t] = AttnT<T>::mfma(lo, qf[rb][2 * h], h == 0 ? float4_t{0.f, 0.f, 0.f, 0.f} : st[rb][t]);
+                            st[rb][t] = AttnT<T>::mfma(hi, qf[rb][2 * h + 1], st[rb][t]);
+                        }
+                        w = wn;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    const bool masked = k0 + 63 > kmin;
+                    const char *v_at = vt + c * FP8_TILE + ((4 * half + kq) ^ (c >> 1)) * 16;
+                    V8 pf[RB][2];
+                    w = *(const uint4_t *)v_at;
+                    fp8_weights<T, RB, NDB>(st, sc.x, sc.y, sc.z, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int db = 0; db < NDB; ++db) {
+                        if (db + 1 < NDB) wn = *(const uint4_t *)(v_at + 16 * (db + 1) * FP8_TILE);
+                        if (masked) {
+                            w = fp8_keep(w, k0 + 16 * kq, L);
+                            if (__any(fp8_nan_bits(w) != 0u)) fp8_nan_rows<T, RB, NDB>(w, db, k0 + 16 * kq, kmax, o);
+                        }
+                        const V8 lo = fp8_widen8<T>(w.x, w.y), hi = fp8_widen8<T>(w.z, w.w);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            o[rb][db] = AttnT<T>::mfma(lo, pf[rb][0], o[rb][db]);
+                            o[rb][db] = AttnT<T>::mfma(hi, pf[rb][1], o[rb][db]);
+                        }
+                        w = wn;
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
         }
+        fp8_finish<T, HD, RB, WR>(p, sq, kvh, row0, tid, n == sq.steps, p.part + (size_t)(2 * pl.me + (pos > first_pos ? 1 : 0)) * (ROWS * XROW),
+                                  m_run, l_run, o, (float *)lds);
         pos += n;
         if (pos < end) next_unit(p, sq, unit, step, ROWS, pl.g);
     }
@@ -352,11 +572,12 @@ struct AttnFp8Plan {
 static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t max_keys, int kvh, int head_dim) {
     AttnFp8Plan pl;
     const int64_t rows = max_q * gq;
-    pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     pl.rg = (rows + pl.rows - 1) / pl.rows;
     pl.units = n_seqs * kvh * pl.rg;
-    pl.n_wg = pl.rows == 64 ? FP8_WG / 2 : FP8_WG;
-    const int64_t steps = (max_keys + FP8_STEP - 1) / FP8_STEP;
+    const int step = pl.rows <= 32 ? FP8_STEP : FP8_TILE;
+    const int64_t steps = (max_keys + step - 1) / step;
+    pl.n_wg = FP8_WG;
     // (list positions are 32 bits wide)
     pl.split = !(max_keys <= FP8_WHOLE || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
     pl.shares = (int)min(pl.units * steps, (int64_t)pl.n_wg);
@@ -366,7 +587,8 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
 static bool attn_fp8_shape_ok(int64_t n_seqs, int64_t max_q_len, int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks) {
     return n_seqs > 0 && max_q_len > 0 && num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 &&
            (head_dim == 64 || head_dim == 128) && block_size > 0 && block_size % 16 == 0 && block_size <= FP8_MAX_BLOCK && max_blocks > 0 &&
-           (max_q_len * (num_heads / num_kv_heads) + 63) / 64 <= 65535 && n_seqs * num_kv_heads <= 0x7fffffffLL &&
+           (max_q_len * (num_heads / num_kv_heads) + 63) / 64 <= 65535 &&
+           ((max_q_len + 128) * (num_heads / num_kv_heads) + 128) * (num_heads / num_kv_heads) < (1LL << 32) && n_seqs * num_kv_heads <= 0x7fffffffLL &&
            n_seqs * num_kv_heads * ((max_q_len * (num_heads / num_kv_heads) + 63) / 64) <= (1LL << 24) - 1;
 }
 
@@ -404,6 +626,7 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     p.max_blocks = max_blocks; p.block_size = block_size;
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.scales = scales; p.n_blocks = n_blocks;
+    p.gq_inverse = p.Gq > 1 ? (uint32_t)(((1ULL << 32) + (uint64_t)p.Gq - 1) / (uint64_t)p.Gq) : 0u;
     p.max_keys = (int)min(max_keys, (int64_t)1 << 30);
     p.max_rg = (int)pl.rg;
     if (pl.split) {
@@ -422,18 +645,22 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     const bool aligned = block_size % 64 == 0;
 #define FP8_GO(T, HDV, RBV)                                                                               \
     do {                                                                                                  \
-        if (RBV == 4 && !pl.split) {                                                                      \
-            if (aligned) attn_fp8_kernel<T, HDV, RBV, true, RBV != 4><<<grid, 256, 0, st>>>(p);           \
-            else attn_fp8_kernel<T, HDV, RBV, false, RBV != 4><<<grid, 256, 0, st>>>(p);                  \
-        } else if (aligned) attn_fp8_kernel<T, HDV, RBV, true, true><<<grid, 256, 0, st>>>(p);            \
-        else attn_fp8_kernel<T, HDV, RBV, false, true><<<grid, 256, 0, st>>>(p);                          \
+        if (aligned) attn_fp8_kernel<T, HDV, RBV, true><<<grid, 256, 0, st>>>(p);                         \
+        else attn_fp8_kernel<T, HDV, RBV, false><<<grid, 256, 0, st>>>(p);                                \
         if (pl.split) attn_merge_kernel<T, HDV, 16 * RBV, FP8_STEP, FP8_STEP><<<mgrid, 256, 0, st>>>(p);  \
+    } while (0)
+#define FP8_GO_TILE(T, HDV, WRV)                                                                          \
+    do {                                                                                                  \
+        if (pl.split) attn_fp8_tile_kernel<T, HDV, WRV, true><<<grid, 256, 0, st>>>(p);                   \
+        else attn_fp8_tile_kernel<T, HDV, WRV, false><<<grid, 256, 0, st>>>(p);                           \
+        if (pl.split) attn_merge_kernel<T, HDV, 32 * WRV, FP8_TILE, FP8_TILE><<<mgrid, 256, 0, st>>>(p);  \
     } while (0)
 #define FP8_GO_RB(T, HDV)                                                                                 \
     do {                                                                                                  \
         if (pl.rows == 16) FP8_GO(T, HDV, 1);                                                             \
         else if (pl.rows == 32) FP8_GO(T, HDV, 2);                                                        \
-        else FP8_GO(T, HDV, 4);                                                                           \
+        else if (pl.rows == 64) FP8_GO_TILE(T, HDV, 2);                                                   \
+        else FP8_GO_TILE(T, HDV, 4);                                                                      \
     } while (0)
     if (dtype == ODSD_DT_F16) {
         if (head_dim == 128) FP8_GO_RB(half_t, 128);
@@ -443,6 +670,7 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
         else FP8_GO_RB(__bf16, 64);
     }
 #undef FP8_GO_RB
+#undef FP8_GO_TILE
 #undef FP8_GO
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
