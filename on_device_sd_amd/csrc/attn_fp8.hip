@@ -85,53 +85,70 @@ __device__ __forceinline__ void fp8_weights(const float4_t (&st)[RB][4], const f
                                                        AttnT<T>::pack2(a[8 * u + 4], a[8 * u + 5]), AttnT<T>::pack2(a[8 * u + 6], a[8 * u + 7])});
     }
 }
-// Codes of V, 16 keys of one dimension from key k on, of a masked tile.  Bytes past the last key are what a block held before: they count as
-// zeros.  A NaN of a key that some rows see and others do not must not reach the others as 0 * NaN: fp8_nan_rows counts such codes for the
-// rows that see them by a product of its own, and takes them out.
-__device__ __forceinline__ uint4_t fp8_keep(uint4_t v, const int k, const int L) {
+// Codes of V, 16 keys of one dimension from key k on, of a tile in which some row does not see some key.  Bytes past the last key are what a
+// block held before: they count as zeros.  A NaN of a key that some rows see and others do not must not reach the others as 0 * NaN: before
+// the tile's weights are there fp8_nan_rows counts such codes for the rows that see them, by a product of its own, and makes their sums
+// NaN; in the product itself they are zeros.
+__device__ __forceinline__ uint4_t fp8_keep(const int k, const int L) {
+    uint4_t keep;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         const int left = L - k - 4 * w;
-        v[w] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        keep[w] = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+    }
+    return keep;
+}
+__device__ __forceinline__ uint32_t fp8_nan_bits(const uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint4_t fp8_clean(uint4_t v, const uint4_t keep) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t f = fp8_nan_bits(v[w]);
+        v[w] &= keep[w] & ~((f << 1) - (f >> 7));
     }
     return v;
 }
-__device__ __forceinline__ uint32_t fp8_nan_bits(const uint4_t v) {
-    return ((((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u)) |
-            (((v.z & 0x7f7f7f7fu) + 0x01010101u) | ((v.w & 0x7f7f7f7fu) + 0x01010101u))) & 0x80808080u;
-}
-template <typename T, int RB, int NDB>
-__device__ __forceinline__ void fp8_nan_rows(uint4_t &v, const int db, const int k, const int (&kmax)[RB], float4_t (&o)[RB][NDB]) {
+template <typename T, int RB, int NDB, typename PIECE>
+__device__ __forceinline__ void fp8_nan_rows(const PIECE &piece, const uint4_t keep, const int k, const int (&kmax)[RB], float4_t (&o)[RB][NDB]) {
     typedef typename AttnT<T>::V8 V8;
-    uint32_t ones[4];                              // 1.0 where the code is no number
+    uint32_t any = 0u;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const uint32_t f = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-        ones[w] = f * 0x38u;
-        v[w] &= ~(f * 0xffu);
+    for (int db = 0; db < NDB; ++db) {
+        const uint4_t v = piece(db);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) any |= fp8_nan_bits(v[w] & keep[w]);
     }
+    if (!__any(any != 0u)) return;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        float4_t cnt = {0.f, 0.f, 0.f, 0.f};
+        V8 sees[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             float s[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] = k + 8 * u + e <= kmax[rb] ? 1.0f : 0.0f;
-            const V8 sees = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(s[0], s[1]), AttnT<T>::pack2(s[2], s[3]),
-                                                           AttnT<T>::pack2(s[4], s[5]), AttnT<T>::pack2(s[6], s[7])});
-            cnt = AttnT<T>::mfma(fp8_widen8<T>(ones[2 * u], ones[2 * u + 1]), sees, cnt);
+            sees[u] = __builtin_bit_cast(V8, uint4_t{AttnT<T>::pack2(s[0], s[1]), AttnT<T>::pack2(s[2], s[3]),
+                                                     AttnT<T>::pack2(s[4], s[5]), AttnT<T>::pack2(s[6], s[7])});
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (cnt[i] > 0.0f) o[rb][db][i] = __builtin_nanf("");
-        __builtin_amdgcn_sched_barrier(0);
+        for (int db = 0; db < NDB; ++db) {
+            uint4_t ones = piece(db);                      // 1.0 where the code is no number
+#pragma unroll
+            for (int w = 0; w < 4; ++w) ones[w] = (fp8_nan_bits(ones[w] & keep[w]) >> 7) * 0x38u;
+            float4_t cnt = AttnT<T>::mfma(fp8_widen8<T>(ones[0], ones[1]), sees[0], float4_t{0.f, 0.f, 0.f, 0.f});
+            cnt = AttnT<T>::mfma(fp8_widen8<T>(ones[2], ones[3]), sees[1], cnt);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (cnt[i] > 0.0f) o[rb][db][i] = __builtin_nanf("");
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 }
 // fragments of the unit's query rows from row0 on, and the last position that each attends
 template <typename T, int HD, int RB>
-__device__ __forceinline__ void fp8_queries(const AttnFp8Params &p, const SeqAt &sq, const int kvh, const int row0, const int lane,
+__device__ __forceinline__ void fp8_queries(const AttnFp8Params &p, const SeqAt &sq, const int kvh, const int row0, int lane,
                                             typename AttnT<T>::V8 (&qf)[RB][HD / 32], int (&kmax)[RB]) {
+    asm volatile("" : "+v"(lane));                         // (computed here, not kept from piece to piece)
     const int c = lane & 15, kq = lane >> 4, rows_total = sq.ql * p.Gq;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
@@ -166,10 +183,11 @@ __device__ __forceinline__ void fp8_scales(const AttnFp8Params &p, const uint32_
 // The sums of WK wavefronts that had other keys of the same rows (and of WR groups of them, with other rows), 16 rows of each group at
 // a time through LDS; `whole`: the unit is done, otherwise the results go to `part`.
 template <typename T, int HD, int RB, int WR>
-__device__ __forceinline__ void fp8_finish(const AttnFp8Params &p, const SeqAt &sq, const int kvh, const int row0, const int tid, const bool whole,
+__device__ __forceinline__ void fp8_finish(const AttnFp8Params &p, const SeqAt &sq, const int kvh, const int row0, int tid, const bool whole,
                                            float *part, const float (&m_run)[RB], const float (&l_run)[RB], const float4_t (&o)[RB][HD / 16],
                                            float *xch) {
     constexpr int WK = 4 / WR, XROW = HD + 4, TPR = 16 / WR, PIECES = HD / 4 / TPR;      // threads of a row, float4 each
+    asm volatile("" : "+v"(tid));                          // (what follows from it is computed here, not kept through the loop over the keys)
     const int lane = tid & 63, wave = tid >> 6, c = lane & 15, kq = lane >> 4;
     const int rows_here = min(16 * RB * WR, sq.ql * p.Gq - row0);
     const int x = tid / TPR;                               // this thread's row of the 16 WR
@@ -326,6 +344,14 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
                     ev = __shfl(ev_l, 4 * i + kq, ODSD_WAVE);
                     iv = __shfl(iv_l, 4 * i + kq, ODSD_WAVE);
                 }
+                const bool masked = k0 + 63 > kmin;
+                if (masked) {
+                    const uint4_t keep = fp8_keep(k0 + 16 * kq, L);
+                    fp8_nan_rows<T, RB, NDB>([&](const int db) { return vreg[db]; }, keep, k0 + 16 * kq, kmax, o);
+#pragma unroll
+                    for (int db = 0; db < NDB; ++db) vreg[db] = fp8_clean(vreg[db], keep);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 float4_t st[RB][4];
                 const char *next = nullptr;
                 if constexpr (decltype(fetch_c)::value) next = k_from(i + 1);
@@ -346,21 +372,8 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if constexpr (decltype(fetch_c)::value) next = v_from(i + 1);
-                const bool masked = k0 + 63 > kmin;
                 V8 pf[RB][2];
                 fp8_weights<T, RB, NDB>(st, sc, ev, iv, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
-                if (masked) {
-                    uint32_t bad = 0u;
-#pragma unroll
-                    for (int db = 0; db < NDB; ++db) {
-                        vreg[db] = fp8_keep(vreg[db], k0 + 16 * kq, L);
-                        bad |= fp8_nan_bits(vreg[db]);
-                    }
-                    if (__any(bad != 0u)) {
-#pragma unroll
-                        for (int db = 0; db < NDB; ++db) fp8_nan_rows<T, RB, NDB>(vreg[db], db, k0 + 16 * kq, kmax, o);
-                    }
-                }
 #pragma unroll
                 for (int db = 0; db < NDB; ++db) {
                     const V8 lo = fp8_widen8<T>(vreg[db].x, vreg[db].y), hi = fp8_widen8<T>(vreg[db].z, vreg[db].w);
@@ -401,10 +414,10 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
 #define FP8_TILE 128         // keys of a step
 #define FP8_TILES 32         // steps whose blocks are looked up at a time
 
-template <typename T, int HD, int WR, bool SPLIT>
+template <typename T, int HD, int RB, int WR, bool ALIGNED, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Params p) {
     typedef typename AttnT<T>::V8 V8;
-    constexpr int RB = 2, WK = 4 / WR, ROWS = 16 * RB * WR, XROW = HD + 4;
+    constexpr int WK = 4 / WR, ROWS = 16 * RB * WR, XROW = HD + 4;
     constexpr int NC = HD / 64, NDB = HD / 16, NP = HD / 16;       // NP: pieces of a K row
     constexpr int TILEB = FP8_TILE * HD;                  // bytes of K (and of V) of a step
     constexpr int COPIES = TILEB / 1024 / 4;              // copies of K (and of V) per wavefront
@@ -427,9 +440,19 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
     const int bs = p.block_size;
     const uint32_t block_bytes = (uint32_t)(bs * HD);
 
-    // copies: K rows RPC i + lane / NP of the tile, V rows 8 i + lane / 8 (dimensions)
+    // copies: K rows RPC i + lane / NP of the tile, V rows 8 i + lane / 8 (dimensions); where a lane's pieces begin, in the tile's block
+    // (ALIGNED: the whole tile lies in one) or in the block of the lane's 16 keys
     constexpr int RPC = 64 / NP;
     const int k_row = lane / NP, k_slot = lane % NP, v_row = lane >> 3, v_slot = lane & 7;
+    uint32_t k_from[COPIES], v_from[COPIES], v_group[COPIES];
+#pragma unroll
+    for (int u = 0; u < COPIES; ++u) {
+        const int r = RPC * (COPIES * wave + u) + k_row, a = (r >> 4) & 3, f = HD == 128 ? ((r >> 1) & 1) + 2 * a : a;
+        const int d = 8 * (COPIES * wave + u) + v_row;
+        v_group[u] = (uint32_t)(v_slot ^ ((d >> 1) & 7));
+        k_from[u] = (uint32_t)((ALIGNED ? r : r & 15) * HD + (k_slot ^ f) * 16);
+        v_from[u] = (uint32_t)(d * bs) + (ALIGNED ? 16u * v_group[u] : 0u);
+    }
     // fragments
     const int ka = c >> 2, kb = c & 3;
     uint32_t k_at[NC];
@@ -478,20 +501,28 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) asm volatile("" : "+v"(qf[rb][j]));
             auto copy = [&](const int i) {
-                char *dst = lds + (i & 1) * (2 * TILEB);
+                char *dst = lds + (i & 1) * (2 * TILEB) + 1024 * COPIES * wave;
+                if constexpr (ALIGNED) {
+                    const uint32_t gk1 = __builtin_amdgcn_readfirstlane(at_block[8 * i]), off1 = __builtin_amdgcn_readfirstlane(at_token[8 * i]);
+                    const global_char *kb1 = scalar_base((const global_char *)p.k_cache + (uint64_t)gk1 * block_bytes + off1 * (uint32_t)HD);
+                    const global_char *vb1 = scalar_base((const global_char *)p.v_cache + (uint64_t)gk1 * block_bytes + off1);
 #pragma unroll
-                for (int u = 0; u < COPIES; ++u) {
-                    const int r = RPC * (COPIES * wave + u) + k_row;       // key of the tile
-                    const int g = 8 * i + r / 16, a = (r >> 4) & 3, f = HD == 128 ? ((r >> 1) & 1) + 2 * a : a;
-                    dma16_from_to_lds((const char *)p.k_cache + (uint64_t)at_block[g] * block_bytes + at_token[g] * (uint32_t)HD +
-                                          (uint32_t)((r & 15) * HD + (k_slot ^ f) * 16),
-                                      (lds_void *)(dst + 1024 * (COPIES * wave + u)));
-                }
+                    for (int u = 0; u < COPIES; ++u) dma16_to_lds(kb1, k_from[u], (lds_void *)(dst + 1024 * u));
 #pragma unroll
-                for (int u = 0; u < COPIES; ++u) {
-                    const int d = 8 * (COPIES * wave + u) + v_row, g = 8 * i + (v_slot ^ ((d >> 1) & 7));
-                    dma16_from_to_lds((const char *)p.v_cache + (uint64_t)at_block[g] * block_bytes + at_token[g] + (uint32_t)(d * bs),
-                                      (lds_void *)(dst + TILEB + 1024 * (COPIES * wave + u)));
+                    for (int u = 0; u < COPIES; ++u) dma16_to_lds(vb1, v_from[u], (lds_void *)(dst + TILEB + 1024 * u));
+                } else {
+#pragma unroll
+                    for (int u = 0; u < COPIES; ++u) {
+                        const int g = 8 * i + (RPC * (COPIES * wave + u) + k_row) / 16;
+                        dma16_from_to_lds((const char *)p.k_cache + (uint64_t)at_block[g] * block_bytes + (at_token[g] * (uint32_t)HD + k_from[u]),
+                                          (lds_void *)(dst + 1024 * u));
+                    }
+#pragma unroll
+                    for (int u = 0; u < COPIES; ++u) {
+                        const int g = 8 * i + (int)v_group[u];
+                        dma16_from_to_lds((const char *)p.v_cache + (uint64_t)at_block[g] * block_bytes + (at_token[g] + v_from[u]),
+                                          (lds_void *)(dst + TILEB + 1024 * u));
+                    }
                 }
             };
             copy(0);
@@ -506,50 +537,70 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
                 if (i + 1 < nt) copy(i + 1);
                 if (!active) continue;
                 const char *kt = lds + (i & 1) * (2 * TILEB), *vt = kt + TILEB;
-#pragma unroll
-                for (int sub = 0; sub < (WK == 1 ? 2 : 1); ++sub) {
-                    const int half = WK == 1 ? sub : wk, k0 = key0 + FP8_TILE * i + 64 * half;
+                // 64 keys.  While a fragment is multiplied the next one is widened and the one behind it read; the scheduling barriers keep
+                // the compiler from doing that for all of them first, whose registers would push others out to memory.  MASKED: some row
+                // does not see some key
+                auto keys64 = [&](auto masked_c, const int half, const int k0) {
+                    constexpr bool MASKED = decltype(masked_c)::value;
                     const float4_t sc = at_scale[8 * i + 4 * half + kq];
-                    // (the next fragment is read while this one is multiplied; the scheduling barriers keep the compiler from reading and
-                    // widening all of them first, whose registers would push others out to memory)
+                    const char *v_at = vt + c * FP8_TILE + ((4 * half + kq) ^ (c >> 1)) * 16;
                     auto k_piece = [&](const int x) { return *(const uint4_t *)(kt + k_at[x % NC] + (64 * half + 4 * (x / NC)) * HD); };
+                    auto v_piece = [&](const int db) { return *(const uint4_t *)(v_at + 16 * db * FP8_TILE); };
+                    uint4_t keep;
+                    if constexpr (MASKED) {
+                        keep = fp8_keep(k0 + 16 * kq, L);
+                        fp8_nan_rows<T, RB, NDB>(v_piece, keep, k0 + 16 * kq, kmax, o);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                     float4_t st[RB][4];
-                    uint4_t w = k_piece(0), wn = w;
+                    uint4_t w = k_piece(0);
+                    V8 lo = fp8_widen8<T>(w.x, w.y), hi = fp8_widen8<T>(w.z, w.w);
+                    w = k_piece(1);
 #pragma unroll
                     for (int x = 0; x < 4 * NC; ++x) {
                         const int t = x / NC, h = x % NC;
-                        if (x + 1 < 4 * NC) wn = k_piece(x + 1);
-                        const V8 lo = fp8_widen8<T>(w.x, w.y), hi = fp8_widen8<T>(w.z, w.w);
+                        const uint4_t next = x + 2 < 4 * NC ? k_piece(x + 2) : v_piece(x + 2 - 4 * NC);
 #pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            st[rb][t] = AttnT<T>::mfma(lo, qf[rb][2 * h], h == 0 ? float4_t{0.f, 0.f, 0.f, 0.f} : st[rb][t]);
-                            st[rb][t] = AttnT<T>::mfma(hi, qf[rb][2 * h + 1], st[rb][t]);
+                        for (int rb = 0; rb < RB; ++rb) st[rb][t] = AttnT<T>::mfma(lo, qf[rb][2 * h], h == 0 ? float4_t{0.f, 0.f, 0.f, 0.f} : st[rb][t]);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) st[rb][t] = AttnT<T>::mfma(hi, qf[rb][2 * h + 1], st[rb][t]);
+                        if (x + 1 < 4 * NC) {
+                            lo = fp8_widen8<T>(w.x, w.y);
+                            hi = fp8_widen8<T>(w.z, w.w);
+                            w = next;
                         }
-                        w = wn;
                         __builtin_amdgcn_sched_barrier(0);
-                    }
-                    const bool masked = k0 + 63 > kmin;
-                    const char *v_at = vt + c * FP8_TILE + ((4 * half + kq) ^ (c >> 1)) * 16;
-                    V8 pf[RB][2];
-                    w = *(const uint4_t *)v_at;
-                    fp8_weights<T, RB, NDB>(st, sc.x, sc.y, sc.z, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
-                    __builtin_amdgcn_sched_barrier(0);
+                        if (x + 1 == 4 * NC) {
+                            V8 pf[RB][2];
+                            fp8_weights<T, RB, NDB>(st, sc.x, sc.y, sc.z, MASKED, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
+                            __builtin_amdgcn_sched_barrier(0);
+                            // (w is V's first piece, next its second)
+                            uint4_t wn = next;
+                            auto widen = [&]() {
+                                if constexpr (MASKED) w = fp8_clean(w, keep);
+                                lo = fp8_widen8<T>(w.x, w.y);
+                                hi = fp8_widen8<T>(w.z, w.w);
+                                w = wn;
+                            };
+                            widen();
 #pragma unroll
-                    for (int db = 0; db < NDB; ++db) {
-                        if (db + 1 < NDB) wn = *(const uint4_t *)(v_at + 16 * (db + 1) * FP8_TILE);
-                        if (masked) {
-                            w = fp8_keep(w, k0 + 16 * kq, L);
-                            if (__any(fp8_nan_bits(w) != 0u)) fp8_nan_rows<T, RB, NDB>(w, db, k0 + 16 * kq, kmax, o);
-                        }
-                        const V8 lo = fp8_widen8<T>(w.x, w.y), hi = fp8_widen8<T>(w.z, w.w);
+                            for (int db = 0; db < NDB; ++db) {
+                                if (db + 2 < NDB) wn = v_piece(db + 2);
 #pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            o[rb][db] = AttnT<T>::mfma(lo, pf[rb][0], o[rb][db]);
-                            o[rb][db] = AttnT<T>::mfma(hi, pf[rb][1], o[rb][db]);
+                                for (int rb = 0; rb < RB; ++rb) o[rb][db] = AttnT<T>::mfma(lo, pf[rb][0], o[rb][db]);
+#pragma unroll
+                                for (int rb = 0; rb < RB; ++rb) o[rb][db] = AttnT<T>::mfma(hi, pf[rb][1], o[rb][db]);
+                                if (db + 1 < NDB) widen();
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
                         }
-                        w = wn;
-                        __builtin_amdgcn_sched_barrier(0);
                     }
+                };
+#pragma unroll
+                for (int sub = 0; sub < (WK == 1 ? 2 : 1); ++sub) {
+                    const int half = WK == 1 ? sub : wk, k0 = key0 + FP8_TILE * i + 64 * half;
+                    if (k0 + 63 > kmin) keys64(std::true_type{}, half, k0);
+                    else keys64(std::false_type{}, half, k0);
                 }
             }
         }
@@ -575,7 +626,7 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
     pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     pl.rg = (rows + pl.rows - 1) / pl.rows;
     pl.units = n_seqs * kvh * pl.rg;
-    const int step = pl.rows <= 32 ? FP8_STEP : FP8_TILE;
+    const int step = pl.rows <= 16 ? FP8_STEP : FP8_TILE;
     const int64_t steps = (max_keys + step - 1) / step;
     pl.n_wg = FP8_WG;
     // (list positions are 32 bits wide)
@@ -642,25 +693,28 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     const unsigned grid = (unsigned)(pl.split ? pl.shares : p.n_wg);
     const dim3 mgrid((unsigned)(n_seqs * num_kv_heads), (unsigned)pl.rg, (unsigned)((pl.rows * head_dim + 1023) / 1024));
     hipStream_t st = (hipStream_t)stream;
-    const bool aligned = block_size % 64 == 0;
+    const bool aligned = block_size % (pl.rows <= 16 ? 64 : FP8_TILE) == 0;       // a tile lies in one block
 #define FP8_GO(T, HDV, RBV)                                                                               \
     do {                                                                                                  \
         if (aligned) attn_fp8_kernel<T, HDV, RBV, true><<<grid, 256, 0, st>>>(p);                         \
         else attn_fp8_kernel<T, HDV, RBV, false><<<grid, 256, 0, st>>>(p);                                \
         if (pl.split) attn_merge_kernel<T, HDV, 16 * RBV, FP8_STEP, FP8_STEP><<<mgrid, 256, 0, st>>>(p);  \
     } while (0)
-#define FP8_GO_TILE(T, HDV, WRV)                                                                          \
+#define FP8_GO_TILE(T, HDV, RBV, WRV)                                                                          \
     do {                                                                                                  \
-        if (pl.split) attn_fp8_tile_kernel<T, HDV, WRV, true><<<grid, 256, 0, st>>>(p);                   \
-        else attn_fp8_tile_kernel<T, HDV, WRV, false><<<grid, 256, 0, st>>>(p);                           \
-        if (pl.split) attn_merge_kernel<T, HDV, 32 * WRV, FP8_TILE, FP8_TILE><<<mgrid, 256, 0, st>>>(p);  \
+        if (pl.split) {                                                                                   \
+            if (aligned) attn_fp8_tile_kernel<T, HDV, RBV, WRV, true, true><<<grid, 256, 0, st>>>(p);       \
+            else attn_fp8_tile_kernel<T, HDV, RBV, WRV, false, true><<<grid, 256, 0, st>>>(p);              \
+            attn_merge_kernel<T, HDV, 16 * RBV * WRV, FP8_TILE, FP8_TILE><<<mgrid, 256, 0, st>>>(p);            \
+        } else if (aligned) attn_fp8_tile_kernel<T, HDV, RBV, WRV, true, false><<<grid, 256, 0, st>>>(p);   \
+        else attn_fp8_tile_kernel<T, HDV, RBV, WRV, false, false><<<grid, 256, 0, st>>>(p);                 \
     } while (0)
 #define FP8_GO_RB(T, HDV)                                                                                 \
     do {                                                                                                  \
         if (pl.rows == 16) FP8_GO(T, HDV, 1);                                                             \
-        else if (pl.rows == 32) FP8_GO(T, HDV, 2);                                                        \
-        else if (pl.rows == 64) FP8_GO_TILE(T, HDV, 2);                                                   \
-        else FP8_GO_TILE(T, HDV, 4);                                                                      \
+        else if (pl.rows == 32) FP8_GO_TILE(T, HDV, 1, 2);                                                \
+        else if (pl.rows == 64) FP8_GO_TILE(T, HDV, 2, 2);                                                \
+        else FP8_GO_TILE(T, HDV, 2, 4);                                                                      \
     } while (0)
     if (dtype == ODSD_DT_F16) {
         if (head_dim == 128) FP8_GO_RB(half_t, 128);
