@@ -8,13 +8,21 @@
 // within what fp16 holds.  Codes become 16-bit operands of q's type in registers (exact); products and sums are fp32; w is rounded to
 // q's type once (half a step, as in the kernels over 16-bit keys), the result once.
 //
-// A unit -- up to 16, 32 or 64 query rows of a (sequence, KV head) -- and the way units are cut into shares of keys are those of attn_list.h.
-// Each of the four wavefronts takes 64 keys of every 256 for all rows of the unit, with no barrier and no LDS in the loop: the cache
-// holds what the matrix instructions want as it lies.  A lane's 16 bytes of a K row are the k indices of two products (the query's
-// fragments have the same order); V is stored transposed, so 16 bytes are 16 keys of one dimension, and the rows of S^T = K Q^T are
-// dealt so that a lane (c, kq) gets the scores of keys 16 kq .. 16 kq + 15 of query row c: those of its own V bytes, as the B operand of
-// O^T = V^T P^T, and all in one block, whose scales are lane values.  The next tile's bytes are requested into the registers that the
-// present one has just left.
+// A unit -- up to 16, 32, 64 or 128 query rows of a (sequence, KV head) -- and the way units are cut into shares of keys are those of
+// attn_list.h.  V is stored transposed, so 16 bytes are 16 keys of one dimension, and the rows of S^T = K Q^T are dealt so that a lane
+// (c, kq) gets the scores of keys 16 kq .. 16 kq + 15 of query row c: those of its own V bytes, as the B operand of O^T = V^T P^T, and all in
+// one block, whose scales are lane values.  A lane's 16 bytes of a K row are the k indices of two products; the query's fragments have the
+// same order.  The cache holds what the matrix instructions want as it lies.
+//
+// Up to 16 rows (a token of each sequence) bytes bound it: no barrier and no LDS in the loop, the next tile's bytes requested into the registers
+// that the present one has just left.  More rows would read each key once per wavefront that has it, and widening it once per 16 rows is what
+// they wait for: the keys go through LDS, a step is copied while the one before is worked on, and a wavefront has 32 rows for every code
+// it widens.  (32 / 4 heads of 128, 8 tokens of 32 sequences of up to 2000 keys: 42 us with keys straight to registers, 30 through LDS; a
+// chunk of 2048 tokens at 4096 keys 397 and 226.)
+//
+// Measured, 32 / 4 heads of 128, bf16, in a graph: a token each of 64 sequences of 750 to 3000 keys 29 us, 4.2 TB/s of codes; 4 tokens each of 64
+// sequences of 8000 to 8192 keys 114 us, 4.7 TB/s; a chunk of 512 tokens each of 8 sequences of 8192 keys 514 us, 990 TFLOP/s.  A short call is a
+// list, a lookup, a tile and a merge, each waiting for the one before: one sequence of 777 keys 8.0 us.
 #include "attn_list.h"
 #include "fp8.h"
 #include "w4_gemm.h"
@@ -245,13 +253,13 @@ __device__ __forceinline__ void fp8_finish(const AttnFp8Params &p, const SeqAt &
     }
 }
 
-// ---- up to 32 rows: the keys straight to registers --------------------------------------------------------
-template <typename T, int HD, int RB, bool ALIGNED>
+// ---- up to 16 rows: the keys straight to registers --------------------------------------------------------
+template <typename T, int HD, bool ALIGNED>
 __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p) {
     typedef typename AttnT<T>::V8 V8;
     constexpr int NC = HD / 64;          // 16-byte pieces of a K row per lane
     constexpr int NDB = HD / 16;         // 16-dim blocks of the output
-    constexpr int ROWS = 16 * RB, XROW = HD + 4;
+    constexpr int ROWS = 16, XROW = HD + 4;
     constexpr int MOST = ALIGNED ? 64 : 16;              // tiles whose blocks are looked up at a time
     __shared__ __attribute__((aligned(16))) float xch[4 * 16 * XROW];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -280,19 +288,14 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
         const int kvh = sq.rg == 1 ? unit : unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);
         const int L = sq.L, row0 = rg * ROWS;
         const int32_t *bt = p.block_tables + (size_t)sq.seq * p.max_blocks;
-        V8 qf[RB][HD / 32];
-        int kmax[RB];
-        fp8_queries<T, HD, RB>(p, sq, kvh, row0, lane, qf, kmax);
+        V8 qf[1][HD / 32];
+        int kmax[1];
+        fp8_queries<T, HD, 1>(p, sq, kvh, row0, lane, qf, kmax);
         const int kmin = L - sq.ql + fp8_token(p, row0);         // the unit's first row: tiles that end at or before it need no mask
-        float m_run[RB], l_run[RB];
-        float4_t o[RB][NDB];
+        float m_run[1] = {-INFINITY}, l_run[1] = {0.0f};
+        float4_t o[1][NDB];
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            m_run[rb] = -INFINITY;
-            l_run[rb] = 0.0f;
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) o[rb][db] = float4_t{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int db = 0; db < NDB; ++db) o[0][db] = float4_t{0.f, 0.f, 0.f, 0.f};
         const int key_end = step + n == sq.steps ? L : pl.g * (step + n);
         for (int key0 = pl.g * step + 64 * wave; key0 < key_end; key0 += MOST * FP8_STEP) {
             const int nt = min(MOST, (key_end - key0 + FP8_STEP - 1) / FP8_STEP);
@@ -347,41 +350,34 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
                 const bool masked = k0 + 63 > kmin;
                 if (masked) {
                     const uint4_t keep = fp8_keep(k0 + 16 * kq, L);
-                    fp8_nan_rows<T, RB, NDB>([&](const int db) { return vreg[db]; }, keep, k0 + 16 * kq, kmax, o);
+                    fp8_nan_rows<T, 1, NDB>([&](const int db) { return vreg[db]; }, keep, k0 + 16 * kq, kmax, o);
 #pragma unroll
                     for (int db = 0; db < NDB; ++db) vreg[db] = fp8_clean(vreg[db], keep);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                float4_t st[RB][4];
+                float4_t st[1][4];
                 const char *next = nullptr;
                 if constexpr (decltype(fetch_c)::value) next = k_from(i + 1);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) st[rb][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+                    st[0][t] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int h = 0; h < NC; ++h) {
                         const V8 lo = fp8_widen8<T>(kreg[t][h].x, kreg[t][h].y), hi = fp8_widen8<T>(kreg[t][h].z, kreg[t][h].w);
-#pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            st[rb][t] = AttnT<T>::mfma(lo, qf[rb][2 * h], st[rb][t]);
-                            st[rb][t] = AttnT<T>::mfma(hi, qf[rb][2 * h + 1], st[rb][t]);
-                        }
+                        st[0][t] = AttnT<T>::mfma(lo, qf[0][2 * h], st[0][t]);
+                        st[0][t] = AttnT<T>::mfma(hi, qf[0][2 * h + 1], st[0][t]);
                     }
                     if constexpr (decltype(fetch_c)::value) fetch_k(next, t);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if constexpr (decltype(fetch_c)::value) next = v_from(i + 1);
-                V8 pf[RB][2];
-                fp8_weights<T, RB, NDB>(st, sc, ev, iv, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
+                V8 pf[1][2];
+                fp8_weights<T, 1, NDB>(st, sc, ev, iv, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
 #pragma unroll
                 for (int db = 0; db < NDB; ++db) {
                     const V8 lo = fp8_widen8<T>(vreg[db].x, vreg[db].y), hi = fp8_widen8<T>(vreg[db].z, vreg[db].w);
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        o[rb][db] = AttnT<T>::mfma(lo, pf[rb][0], o[rb][db]);
-                        o[rb][db] = AttnT<T>::mfma(hi, pf[rb][1], o[rb][db]);
-                    }
+                    o[0][db] = AttnT<T>::mfma(lo, pf[0][0], o[0][db]);
+                    o[0][db] = AttnT<T>::mfma(hi, pf[0][1], o[0][db]);
                     if constexpr (decltype(fetch_c)::value) fetch_v(next, db);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -399,7 +395,7 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
         }
 
         // (a piece that begins where its workgroup's share begins goes to the workgroup's first slot)
-        fp8_finish<T, HD, RB, 1>(p, sq, kvh, row0, tid, n == sq.steps, p.part + (size_t)(2 * pl.me + (pos > first_pos ? 1 : 0)) * (ROWS * XROW),
+        fp8_finish<T, HD, 1, 1>(p, sq, kvh, row0, tid, n == sq.steps, p.part + (size_t)(2 * pl.me + (pos > first_pos ? 1 : 0)) * (ROWS * XROW),
                                  m_run, l_run, o, xch);
         pos += n;
         if (pos < end) next_unit(p, sq, unit, step, ROWS, pl.g);
@@ -629,8 +625,13 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
     const int step = pl.rows <= 16 ? FP8_STEP : FP8_TILE;
     const int64_t steps = (max_keys + step - 1) / step;
     pl.n_wg = FP8_WG;
-    // (list positions are 32 bits wide)
-    pl.split = !(max_keys <= FP8_WHOLE || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
+    // Whole units need no merge (4 to 6 us) and leave no pieces; split ones level mixed lengths out and fill the chip.  (32 / 4 heads of 128, whole /
+    // split, us.  16 rows: 64 sequences of 512 keys 9.9 / 13.9, 1024 15.1 / 18.8, 2048 25.1 / 28.6, 750 to 3001 31.6 / 29.4; 128 of 1024 25.4 /
+    // 29.1; 16 of 1024 12.0 / 10.0; one of 777 10.0 / 8.0.  64 rows: 32 sequences of 512 keys 14.6 / 21.2, 1024 20.4 / 23.8, 2048 31.9 / 28.9;
+    // 64 of 2048 41.7 / 45.1, 512 to 2048 33.9 / 39.3; 8 of 2048 30.6 / 22.0.  32 rows: 64 of 2048 33.2 / 37.2, 8 of 4096 37.9 / 18.6.  128 rows: 4
+    // sequences of 8192 keys 279 / 286, one 160 / 86.)  List positions are 32 bits wide.
+    const int64_t whole = pl.rows <= 16 ? (pl.units >= 256 ? 2048 : pl.units >= 128 ? 1024 : FP8_WHOLE) : max((int64_t)FP8_WHOLE, 12 * pl.units);
+    pl.split = !(max_keys <= whole || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
     pl.shares = (int)min(pl.units * steps, (int64_t)pl.n_wg);
     pl.bytes = pl.split ? odsd_round_up((size_t)2 * pl.shares * pl.rows * (head_dim + 4) * sizeof(float), 256) : 0;
     return pl;
@@ -694,11 +695,11 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     const dim3 mgrid((unsigned)(n_seqs * num_kv_heads), (unsigned)pl.rg, (unsigned)((pl.rows * head_dim + 1023) / 1024));
     hipStream_t st = (hipStream_t)stream;
     const bool aligned = block_size % (pl.rows <= 16 ? 64 : FP8_TILE) == 0;       // a tile lies in one block
-#define FP8_GO(T, HDV, RBV)                                                                               \
+#define FP8_GO(T, HDV)                                                                                    \
     do {                                                                                                  \
-        if (aligned) attn_fp8_kernel<T, HDV, RBV, true><<<grid, 256, 0, st>>>(p);                         \
-        else attn_fp8_kernel<T, HDV, RBV, false><<<grid, 256, 0, st>>>(p);                                \
-        if (pl.split) attn_merge_kernel<T, HDV, 16 * RBV, FP8_STEP, FP8_STEP><<<mgrid, 256, 0, st>>>(p);  \
+        if (aligned) attn_fp8_kernel<T, HDV, true><<<grid, 256, 0, st>>>(p);                              \
+        else attn_fp8_kernel<T, HDV, false><<<grid, 256, 0, st>>>(p);                                     \
+        if (pl.split) attn_merge_kernel<T, HDV, 16, FP8_STEP, FP8_STEP><<<mgrid, 256, 0, st>>>(p);        \
     } while (0)
 #define FP8_GO_TILE(T, HDV, RBV, WRV)                                                                          \
     do {                                                                                                  \
@@ -711,7 +712,7 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     } while (0)
 #define FP8_GO_RB(T, HDV)                                                                                 \
     do {                                                                                                  \
-        if (pl.rows == 16) FP8_GO(T, HDV, 1);                                                             \
+        if (pl.rows == 16) FP8_GO(T, HDV);                                                                \
         else if (pl.rows == 32) FP8_GO_TILE(T, HDV, 1, 2);                                                \
         else if (pl.rows == 64) FP8_GO_TILE(T, HDV, 2, 2);                                                \
         else FP8_GO_TILE(T, HDV, 2, 4);                                                                      \
