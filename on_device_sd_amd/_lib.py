@@ -67,7 +67,7 @@ SIGNATURES = {
     "odsd_paged_attention_workspace_bytes": (C.c_size_t, [C.c_int32] * 7),
     "odsd_kv_store_fp8": (C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64] + [_P] * 5 + [C.c_int32] * 7 + [_P, C.c_size_t, _P]),
     "odsd_kv_store_fp8_workspace_bytes": (C.c_size_t, [C.c_int32]),
-    "odsd_paged_attention_fp8": (C.c_int, [_P] * 7 + [C.c_int32] * 8 + [C.c_float, C.c_int32, _P, _P, C.c_size_t, _P]),
+    "odsd_paged_attention_fp8": (C.c_int, [_P] * 7 + [C.c_int32] * 9 + [C.c_float, C.c_int32, _P, _P, C.c_size_t, _P]),
     "odsd_paged_attention_fp8_workspace_bytes": (C.c_size_t, [C.c_int32] * 7),
     "odsd_copy_blocks": (C.c_int, [_P] * 4 + [C.c_int32] + [_P] * 2 + [C.c_int32] * 2 + [_P, C.c_int64, _P]),
     "odsd_adjust_logits": (C.c_int, [_P, C.c_int64, _P, C.c_int64] + [C.c_int32] * 3 + [_P, C.c_int32, _P, C.c_int32, C.c_int64, C.c_int32,

@@ -110,9 +110,10 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     } else if (p.sparse) {
         __syncthreads();
     }
+    // (no row and no draft past those that there are, whatever the lengths say: their sums may have wrapped)
+    if (rows == 0 || (uint32_t)row >= (uint32_t)p.n_rows) return;
     rows = min(rows, p.n_rows - row);
-    if (rows <= 0) return;
-    const int drafts = p.drafts ? max(min(rows - 1, p.n_drafts - draft), 0) : 0;
+    const int drafts = p.drafts && (uint32_t)draft < (uint32_t)p.n_drafts ? min(rows - 1, p.n_drafts - draft) : 0;
     if (p.sparse) {
         if (p.tokens) {
             const int len = min(max(p.token_lens ? p.token_lens[s] : p.max_tokens, 0), p.max_tokens);

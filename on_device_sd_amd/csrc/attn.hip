@@ -768,7 +768,7 @@ extern "C" int odsd_paged_attention(const void *q, const void *k_cache, const vo
     AttnParams p{};
     p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
     p.q_lens = q_lens; p.context_lens = context_lens; p.block_tables = block_tables;
-    p.n_seqs = n_seqs; p.H = num_heads; p.KVH = num_kv_heads; p.max_blocks = max_blocks;
+    p.n_seqs = n_seqs; p.n_tokens = 0x7fffffff; p.H = num_heads; p.KVH = num_kv_heads; p.max_blocks = max_blocks;
     p.block_size = block_size; p.num_slots = num_slots;
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     return attn_stream_launch(p, dtype, head_dim, max_q_len, (int64_t)max_blocks * block_size, block_size % 32 == 0,
@@ -798,7 +798,7 @@ extern "C" int odsd_varlen_attention(const void *q, const void *k, const void *v
     AttnParams p{};
     p.q = q; p.k_cache = k; p.v_cache = v; p.out = out;
     p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k;
-    p.n_seqs = n_seqs; p.H = num_heads; p.KVH = num_kv_heads;
+    p.n_seqs = n_seqs; p.n_tokens = 0x7fffffff; p.H = num_heads; p.KVH = num_kv_heads;
     p.block_size = 32; p.max_blocks = (max_seqlen_k + 31) / 32; p.num_slots = 0;
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     const int64_t rows = (int64_t)max_seqlen_q * (num_heads / num_kv_heads);

@@ -161,9 +161,11 @@ __device__ __forceinline__ void fp8_queries(const AttnFp8Params &p, const SeqAt 
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const int row = row0 + 16 * rb + c;
-        const bool ok = row < rows_total;
-        const int tok = ok ? fp8_token(p, row) : 0, hq = ok ? row - tok * p.Gq : 0;
-        kmax[rb] = ok ? sq.L - sq.ql + tok : -1;
+        int tok = fp8_token(p, row);
+        const bool ok = row < rows_total && (uint32_t)(sq.q0 + tok) < (uint32_t)p.n_tokens;
+        tok = ok ? tok : 0;
+        const int hq = ok ? row - tok * p.Gq : 0;
+        kmax[rb] = ok ? min(sq.L - sq.ql + tok, p.max_keys - 1) : -1;
         const uint16_t *qp = (const uint16_t *)p.q + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + 16 * kq;
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {                // dims 64 (j / 2) + 16 kq + 8 (j % 2) ..
@@ -215,7 +217,8 @@ __device__ __forceinline__ void fp8_finish(const AttnFp8Params &p, const SeqAt &
         }
         __syncthreads();
         const int r = 16 * RB * (x >> 4) + 16 * rb + (x & 15);
-        if (r >= rows_here) continue;
+        const int tok = fp8_token(p, row0 + r), hq = row0 + r - tok * p.Gq;
+        if (r >= rows_here || (uint32_t)(sq.q0 + tok) >= (uint32_t)p.n_tokens) continue;
         float m = -INFINITY, f[WK], ls = 0.0f;
 #pragma unroll
         for (int w = 0; w < WK; ++w) m = fmaxf(m, xs[w * 16 * XROW + HD]);
@@ -230,7 +233,6 @@ __device__ __forceinline__ void fp8_finish(const AttnFp8Params &p, const SeqAt &
 #pragma unroll
             for (int w = 0; w < WK; ++w) f[w] *= inv;
         }
-        const int tok = fp8_token(p, row0 + r), hq = row0 + r - tok * p.Gq;
         uint16_t *to = (uint16_t *)p.out + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD;
         float *pr = part + r * XROW;
 #pragma unroll
@@ -286,12 +288,12 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_kernel(const AttnFp8Params p)
         // ---- one piece: steps step .. step + n - 1 of one unit ----------------------------------------
         const int n = min(end - pos, sq.steps - step);
         const int kvh = sq.rg == 1 ? unit : unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);
-        const int L = sq.L, row0 = rg * ROWS;
+        const int L = min(sq.L, p.max_keys), row0 = rg * ROWS;       // (what is past the table is not attended)
         const int32_t *bt = p.block_tables + (size_t)sq.seq * p.max_blocks;
         V8 qf[1][HD / 32];
         int kmax[1];
         fp8_queries<T, HD, 1>(p, sq, kvh, row0, lane, qf, kmax);
-        const int kmin = L - sq.ql + fp8_token(p, row0);         // the unit's first row: tiles that end at or before it need no mask
+        const int kmin = min(sq.L - sq.ql + fp8_token(p, row0), p.max_keys - 1);       // of the unit's first row: tiles that end at or before it need no mask
         float m_run[1] = {-INFINITY}, l_run[1] = {0.0f};
         float4_t o[1][NDB];
 #pragma unroll
@@ -461,12 +463,12 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
     while (pos < end) {
         const int n = min(end - pos, sq.steps - step);
         const int kvh = sq.rg == 1 ? unit : unit / sq.rg, rg = sq.rg - 1 - (unit - kvh * sq.rg);      // row groups with the most keys first
-        const int L = sq.L, row0 = rg * ROWS;
+        const int L = min(sq.L, p.max_keys), row0 = rg * ROWS;       // (what is past the table is not attended)
         const int32_t *bt = p.block_tables + (size_t)sq.seq * p.max_blocks;
         V8 qf[RB][HD / 32];
         int kmax[RB];
         fp8_queries<T, HD, RB>(p, sq, kvh, row0 + 16 * RB * wr, lane, qf, kmax);
-        const int kmin = L - sq.ql + fp8_token(p, row0 + 16 * RB * wr);     // of the wavefront's first row
+        const int kmin = min(sq.L - sq.ql + fp8_token(p, row0 + 16 * RB * wr), p.max_keys - 1);     // of the wavefront's first row
         const bool active = row0 + 16 * RB * wr < sq.ql * p.Gq;
         float m_run[RB], l_run[RB];
         float4_t o[RB][NDB];
@@ -479,7 +481,7 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
         }
         int key_end = step + n == sq.steps ? L : pl.g * (step + n);
         if (sq.rg > 1)                                     // (no further than the unit's last row sees)
-            key_end = min(key_end, L - sq.ql + min(sq.ql, fp8_token(p, row0 + ROWS - 1) + 1));
+            key_end = min(key_end, sq.L - sq.ql + min(sq.ql, fp8_token(p, row0 + ROWS - 1) + 1));
         for (int key0 = pl.g * step; key0 < key_end; key0 += FP8_TILES * FP8_TILE) {
             const int nt = min(FP8_TILES, (key_end - key0 + FP8_TILE - 1) / FP8_TILE);
             __syncthreads();                               // tables and tiles are free
@@ -654,15 +656,15 @@ extern "C" size_t odsd_paged_attention_fp8_workspace_bytes(int32_t n_seqs, int32
 
 extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, const void *v_cache, const float *scales,
                                         const int32_t *block_tables, const int32_t *context_lens, const int32_t *q_lens,
-                                        int32_t n_seqs, int32_t max_q_len, int32_t num_heads, int32_t num_kv_heads,
+                                        int32_t n_tokens, int32_t n_seqs, int32_t max_q_len, int32_t num_heads, int32_t num_kv_heads,
                                         int32_t head_dim, int32_t block_size, int32_t max_blocks, int32_t n_blocks,
                                         float softmax_scale, int32_t dtype, void *out, void *workspace,
                                         size_t workspace_bytes, void *stream) {
-    if (n_seqs < 0 || max_q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || block_size <= 0 ||
+    if (n_tokens < 0 || n_seqs < 0 || max_q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || block_size <= 0 ||
         block_size % 16 || max_blocks <= 0 || n_blocks <= 0 || !(softmax_scale > 0.0f) || !(softmax_scale < INFINITY))
         return ODSD_ERR_SHAPE;
     if (dtype != ODSD_DT_BF16 && dtype != ODSD_DT_F16) return ODSD_ERR_DTYPE;
-    if (n_seqs == 0) return (head_dim == 64 || head_dim == 128) && block_size <= FP8_MAX_BLOCK ? ODSD_OK : ODSD_ERR_UNSUPPORTED;
+    if (n_seqs == 0 || n_tokens == 0) return (head_dim == 64 || head_dim == 128) && block_size <= FP8_MAX_BLOCK ? ODSD_OK : ODSD_ERR_UNSUPPORTED;
     if (!attn_fp8_shape_ok(n_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size, max_blocks) ||
         (int64_t)n_blocks * num_kv_heads > 0x7fffffffLL)
         return ODSD_ERR_UNSUPPORTED;
@@ -674,7 +676,7 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     AttnFp8Params p{};
     p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
     p.q_lens = q_lens; p.context_lens = context_lens; p.block_tables = block_tables;
-    p.n_seqs = n_seqs; p.H = num_heads; p.KVH = num_kv_heads; p.Gq = num_heads / num_kv_heads;
+    p.n_seqs = n_seqs; p.n_tokens = n_tokens; p.H = num_heads; p.KVH = num_kv_heads; p.Gq = num_heads / num_kv_heads;
     p.max_blocks = max_blocks; p.block_size = block_size;
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.scales = scales; p.n_blocks = n_blocks;

@@ -27,7 +27,7 @@ __device__ __forceinline__ SeqCost seq_cost(const AttnParams &p, const int s, co
             c.L = p.context_lens[s];
             c.ql = p.q_lens ? p.q_lens[s] : 1;
         }
-        c.ql = max(c.ql, 0);
+        c.ql = min(max(c.ql, 0), p.n_tokens);
         c.rg = min((c.ql * p.Gq + rows_per_unit - 1) / rows_per_unit, p.max_rg);
         seq_steps(p, c, g);
     }
@@ -243,6 +243,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const int tok = r / p.Gq, hq = r - tok * p.Gq;
+    if ((uint32_t)(sq.q0 + tok) >= (uint32_t)p.n_tokens) return;
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     *(u32x2 *)((uint16_t *)p.out + ((size_t)(sq.q0 + tok) * p.H + kvh * p.Gq + hq) * HD + d) =
         u32x2{AttnT<T>::pack2(acc.x * inv, acc.y * inv), AttnT<T>::pack2(acc.z * inv, acc.w * inv)};

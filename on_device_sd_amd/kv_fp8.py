@@ -122,7 +122,7 @@ def paged_attention_fp8(q: torch.Tensor, cache: KVCacheFP8, context: Dict[str, t
     (bfloat16 / float16), ``context`` with ``block_tables`` int32 [n_seqs, max_blocks], ``context_lens`` int32 [n_seqs] and, for a verify
     step or a chunk of a prompt, ``verify_query_lens`` int32 [n_seqs].  Query j of a sequence attends positions 0 .. context_len -
     query_len + j; a sequence without keys gets zeros.  ``max_q_len`` bounds the query lengths (default: the context's
-    ``max_query_len``, else n_tokens)."""
+    ``max_query_len``, else n_tokens): rows of a sequence past it, and rows behind the last sequence's, hold nothing in particular."""
     dev = q.get_device()
     _same_device(dev, cache.k, cache.v, cache.scales)
     if dev != _raw_device():
@@ -170,7 +170,7 @@ def paged_attention_fp8(q: torch.Tensor, cache: KVCacheFP8, context: Dict[str, t
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     scale = head_dim ** -0.5 if softmax_scale is None else softmax_scale
     rc = lib.odsd_paged_attention_fp8(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(),
-                                      lens.data_ptr(), _ptr(q_lens), n_seqs, most, num_heads, kv_heads, head_dim, block_size, max_blocks,
+                                      lens.data_ptr(), _ptr(q_lens), n_tokens, n_seqs, most, num_heads, kv_heads, head_dim, block_size, max_blocks,
                                       blocks, scale, code, out.data_ptr(), ws.data_ptr(), nbytes, _stream())
     if rc:
         _lib.check(rc, "odsd_paged_attention_fp8")

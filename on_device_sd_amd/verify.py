@@ -150,6 +150,22 @@ def _lens_on(t: Optional[torch.Tensor], n_seqs: int, what: str, logits: torch.Te
     return t.contiguous()
 
 
+def _half_alike(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices of one shape and dtype, rows dense, share elements without being the same."""
+    rows, cols = a.shape
+    if a.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+    (sa, ca), (sb, _) = a.stride(), b.stride()
+    off = b.storage_offset() - a.storage_offset()
+    if rows == 1:
+        sa = sb = cols
+    if ca != 1 and cols > 1:                                # (its rows are copied first)
+        return False
+    if off == 0 and sa == sb or off >= (rows - 1) * sa + cols or -off >= (rows - 1) * sb + cols:
+        return False
+    return sa != sb or not cols <= off % max(sa, 1) <= sa - cols
+
+
 def adjust_logits(logits: torch.Tensor, context: Dict, *, tokens: Optional[torch.Tensor] = None,
                   token_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
                   draft_tokens: Optional[torch.Tensor] = None, repetition: Union[float, torch.Tensor] = 1.0,
@@ -246,6 +262,8 @@ def adjust_logits(logits: torch.Tensor, context: Dict, *, tokens: Optional[torch
             raise ValueError("out must have the shape and dtype of logits")
         if out.numel() and (out.stride(1) != 1 and vocab > 1 or out.stride(0) < vocab and rows > 1):
             raise ValueError("the rows of out must be dense")
+        if _half_alike(logits, out):
+            raise ValueError("out must be logits itself, or share no element with it")
     else:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
     if rows == 0 or vocab == 0 or n_seqs == 0:

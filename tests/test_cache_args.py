@@ -29,15 +29,15 @@ def test_store_status_codes():
 
 def test_attention_status_codes():
     lib = _lib.load()
-    f = lambda S=2, mq=3, H=8, KV=2, D=64, bs=16, mb=4, nb=8, scale=0.1, dt=1, q=P, k=P, v=P, sc=P, bt=P, cl=P, out=P, ws=P, n=1 << 30: \
-        lib.odsd_paged_attention_fp8(q, k, v, sc, bt, cl, None, S, mq, H, KV, D, bs, mb, nb, scale, dt, out, ws, n, None)  # noqa: E731
-    assert f(S=-1) == f(mq=0) == f(H=7) == f(KV=0) == f(bs=8) == f(mb=0) == f(nb=0) == f(scale=0.0) == f(scale=float("nan")) == f(scale=float("inf")) == 2
+    f = lambda S=2, mq=3, H=8, KV=2, D=64, bs=16, mb=4, nb=8, scale=0.1, dt=1, q=P, k=P, v=P, sc=P, bt=P, cl=P, out=P, ws=P, n=1 << 30, T=6: \
+        lib.odsd_paged_attention_fp8(q, k, v, sc, bt, cl, None, T, S, mq, H, KV, D, bs, mb, nb, scale, dt, out, ws, n, None)  # noqa: E731
+    assert f(T=-1) == f(S=-1) == f(mq=0) == f(H=7) == f(KV=0) == f(bs=8) == f(mb=0) == f(nb=0) == f(scale=0.0) == f(scale=float("nan")) == f(scale=float("inf")) == 2
     assert f(dt=0) == f(dt=5) == 7
     assert f(D=96) == f(bs=1040) == f(nb=1 << 30) == f(mq=1 << 21) == f(S=1 << 28) == f(S=1 << 20, mq=1024) == 3
     assert f(q=None) == f(k=None) == f(v=None) == f(sc=None) == f(bt=None) == f(cl=None) == f(out=None) == f(mb=400, ws=None) == 1
     assert f(q=P + 8) == f(k=P + 8) == f(v=P + 8) == f(sc=P + 4) == f(out=P + 4) == f(mb=400, ws=P + 8) == 4
     assert f(mb=400, n=16) == 5
-    assert f(S=0, q=None) == 0 and f(S=0, D=96) == 3
+    assert f(S=0, q=None) == f(T=0, q=None) == 0 and f(S=0, D=96) == 3
     size = lib.odsd_paged_attention_fp8_workspace_bytes
     assert size(2, 3, 8, 2, 64, 16, 4) == 256 and size(2, 3, 8, 2, 64, 16, 400) > 256
     assert size(2, 3, 8, 2, 96, 16, 4) == size(2, 3, 8, 2, 64, 24, 4) == size(0, 3, 8, 2, 64, 16, 4) == size(1 << 28, 3, 8, 2, 64, 16, 4) == 0
@@ -208,3 +208,14 @@ def test_pool_random_walk():
             assert [store[x] for x in _tokens(pool, s)] == text[id(s)]
         assert pool.num_free == pool.holders.count(0) == len(pool._free)
         assert sum(pool.holders) == sum(len(s.block_table) for s in live)
+
+
+def test_rows_half_alike():
+    from on_device_sd_amd.verify import _half_alike
+    buf = torch.zeros(20, 50)
+    a = buf[:8, :20]
+    for b, alike in ((a, False), (buf[8:16, :20], False), (buf[:8, 20:40], False), (buf[:8, 30:], False), (buf[1:9, :20], True), (buf[:8, 19:39], True),
+                     (buf[:8, 10:30], True), (buf.view(-1)[:160].view(8, 20), True), (buf[::2][:8, :20], True), (torch.zeros(8, 20), False),
+                     (buf.view(-1)[800:960].view(8, 20), False), (buf.view(-1)[35:435].view(8, 50)[:, :20], True)):
+        assert _half_alike(a, b) == alike == _half_alike(b, a), (b.shape, b.stride(), b.storage_offset())
+    assert not _half_alike(buf[:1, :20], buf[:1, 20:40]) and _half_alike(buf[:1, :20], buf[:1, 1:21]) and not _half_alike(a[:0], buf[:0, 1:21])

@@ -96,6 +96,30 @@ def test_padded_and_plain_batches(dev):
     check(dev, [1] * 64, 131072, torch.bfloat16, history=2000)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("mask", [None, "shared"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_many_rows_of_a_sequence(dev, dtype, mask, in_place):
+    """more rows than are looked up at a time, with drafts that repeat; few and many tokens that have occurred"""
+    check(dev, [130, 1, 65, 64], 1500, dtype, history=40, mask=mask, bias=3, in_place=in_place)
+    check(dev, [129, 66], 9000, dtype, history=6000, mask=mask, bias=700, in_place=in_place, token_dtype=torch.int32)
+
+
+def test_query_lengths_past_the_rows(dev):
+    """rows and drafts past those that there are stay out of it, whatever the lengths say, and the first sequence has its own"""
+    V, i32 = 300, lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    all_ = torch.randn(12, V, generator=torch.Generator(device=dev).manual_seed(1), device=dev)
+    x = all_[:4]
+    tokens = torch.randint(0, V, (3, 50), generator=torch.Generator(device=dev).manual_seed(2), device=dev)
+    drafts = torch.arange(2, device=dev)
+    want = odsd.adjust_logits(x[:2], {"verify_query_lens": i32(2)}, tokens=tokens[:1], draft_tokens=drafts[:1], repetition=2.0, frequency=0.5)
+    for told in ((2, 7, 3), (2, 2 ** 31 - 1, 2 ** 31 - 1), (2, -5, 9)):
+        out = torch.full((12, V), 7.0, device=dev)
+        got = odsd.adjust_logits(x, {"verify_query_lens": i32(*told)}, tokens=tokens, draft_tokens=drafts, repetition=2.0, frequency=0.5, out=out[:4])
+        torch.cuda.synchronize()
+        assert torch.equal(got[:2], want) and bool((out[4:] == 7.0).all())
+
+
 def test_special_numbers(dev):
     inf, nan = float("inf"), float("nan")
     x = torch.tensor([[inf, -inf, nan, 0.0, -0.0, 3.0, nan]], device=dev)

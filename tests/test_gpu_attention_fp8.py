@@ -179,6 +179,46 @@ def test_odd_lengths_and_tables(dev):
     assert torch.equal(odsd.paged_attention_fp8(*a[1:])[:10], a[0][:10])
 
 
+@pytest.mark.parametrize("L, blocks", [(100, 2), (3000, 5), (70000, 200), (1 << 30, 40)])
+@pytest.mark.parametrize("q_len, heads", [(1, 2), (3, 2), (6, 8), (9, 16)])
+def test_a_context_past_its_table(dev, L, blocks, q_len, heads):
+    """positions that the table has no entry for are not attended: every row sees the keys of the table's entries (-1 reads block 0)"""
+    bs, D = 16, 64
+    cache, tables = make(dev, 2, D, bs, [blocks * bs, 40], 4)
+    q = torch.randn(q_len + 1, heads, D, generator=torch.Generator(device=dev).manual_seed(5), device=dev).to(torch.bfloat16)
+    ctx = {"block_tables": tables, "context_lens": torch.tensor([L, 40], dtype=torch.int32, device=dev), "max_query_len": q_len,
+           "verify_query_lens": torch.tensor([q_len, 1], dtype=torch.int32, device=dev)}
+    got = odsd.paged_attention_fp8(q, cache, ctx).double().cpu().numpy()
+    width = tables.shape[1] * bs
+    ends = [min(L - q_len + 1 + j, width) for j in range(q_len)] + [40]
+    rows = tables[[0] * q_len + [1]]
+    want, mag, top = expected(q, cache, rows, ends, [1] * (q_len + 1), D ** -0.5)
+    off = np.abs(got - want)
+    assert np.array_equal(np.isnan(off), np.isnan(want)) and not (off > bound(want, mag, top, torch.bfloat16, D, width)).any()
+
+
+@pytest.mark.parametrize("L", [300, 6000])
+@pytest.mark.parametrize("heads, most", [(2, 4), (8, 8), (32, 8)])
+@pytest.mark.parametrize("told", [[3, 9, 4], [3, 1 << 30, 1 << 30], [3, -2, 7]])
+def test_query_lengths_past_the_rows(dev, L, heads, most, told):
+    """q and out have 5 rows: nothing behind them is touched, and the first sequence, whose length is right, has its results"""
+    D, n = 64, 5
+    cache, tables = make(dev, 2, D, 64, [L, L, L], 6)
+    q = torch.randn(40, heads, D, generator=torch.Generator(device=dev).manual_seed(7), device=dev).to(torch.bfloat16)
+    out = torch.full((40, heads, D), 7.0, dtype=torch.bfloat16, device=dev)
+    lens, q_lens = (torch.tensor(t, dtype=torch.int32, device=dev) for t in ([L] * 3, told))
+    lib = odsd._lib.load()
+    size = lib.odsd_paged_attention_fp8_workspace_bytes(3, most, heads, 2, D, 64, tables.shape[1])
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    rc = lib.odsd_paged_attention_fp8(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(),
+                                      lens.data_ptr(), q_lens.data_ptr(), n, 3, most, heads, 2, D, 64, tables.shape[1], cache.k.shape[0],
+                                      D ** -0.5, odsd._lib.DT_BF16, out.data_ptr(), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0 and bool((out[n:] == 7.0).all())
+    want, mag, top = expected(q[:3], cache, tables[:1], [L], [3], D ** -0.5)
+    assert (np.abs(out[:3].double().cpu().numpy() - want) <= bound(want, mag, top, torch.bfloat16, D, L)).all()
+
+
 def test_a_cache_past_32_bits(dev):
     """blocks whose bytes begin beyond 2^32"""
     H, D, bs = 8, 128, 256
