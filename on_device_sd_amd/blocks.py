@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import dataclasses
+from array import array
 from typing import Dict, List, Optional, Sequence, Union
 
 import torch
@@ -21,17 +22,14 @@ _TENSORS = 16                                              # ODSD_COPY_TENSORS
 Blocks = Union[Sequence[int], torch.Tensor]
 
 
-def _block_list(blocks: Blocks) -> torch.Tensor:
+def _block_list(blocks: Blocks) -> List[int]:
     if isinstance(blocks, torch.Tensor):
         if blocks.is_cuda:
             raise TypeError("block numbers must be on the host: they are checked, and travel with the launch")
         if blocks.is_floating_point() or blocks.is_complex() or blocks.dtype == torch.bool:
             raise TypeError(f"block numbers must be whole numbers, got {blocks.dtype}")
-        blocks = blocks.flatten()
-        if blocks.dtype != torch.int32:
-            blocks = blocks.to(torch.int64)
-        return blocks.contiguous()
-    return torch.tensor(list(blocks), dtype=torch.int64)
+        return blocks.flatten().tolist()
+    return list(blocks)
 
 
 def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blocks: Blocks, dst_blocks: Blocks, block_dim: int = 0,
@@ -55,9 +53,9 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         with torch.cuda.device(dev):
             return copy_cache_blocks(tensors, src_blocks, dst_blocks, block_dim, block_tables)
     src, dst = _block_list(src_blocks), _block_list(dst_blocks)
-    n = src.numel()
-    if dst.numel() != n:
-        raise ValueError(f"{n} sources for {dst.numel()} destinations")
+    n = len(src)
+    if len(dst) != n:
+        raise ValueError(f"{n} sources for {len(dst)} destinations")
     if tensors[0].dim() <= block_dim:
         raise ValueError(f"a cache {tuple(tensors[0].shape)} has no dimension {block_dim} of blocks")
     num_blocks = tensors[0].shape[block_dim]
@@ -68,17 +66,17 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         raise ValueError("block_tables must be contiguous int32")
     if n == 0:
         return
-    from_, to = src.tolist(), dst.tolist()
-    if min(min(from_), min(to)) < 0 or max(max(from_), max(to)) >= num_blocks:
+    if min(src) < 0 or min(dst) < 0 or max(src) >= num_blocks or max(dst) >= num_blocks:
         raise ValueError(f"block numbers must be in [0, {num_blocks})")
-    places = set(to)
-    if len(places) != n or not places.isdisjoint(from_):
+    places = set(dst)
+    if len(places) != n or not places.isdisjoint(src):
         raise ValueError("every destination must be named once, and be no source")
-    if block_tables is not None and len(set(from_)) != n:
+    if block_tables is not None and len(set(src)) != n:
         raise ValueError("a block that moves has one destination")
     if num_blocks >> 31:
         raise _lib.OdsdError(f"copy_cache_blocks: unsupported sizes: {num_blocks} blocks")
-    src, dst = src.to(torch.int32), dst.to(torch.int32)
+    from_, to = array("i", src), array("i", dst)            # (no whole number: TypeError)
+    from_at, to_at = from_.buffer_info()[0], to.buffer_info()[0]
     lib = _lib.load()
     tensors_, tables = [t for t in tensors if t.numel()], block_tables
     for at in range(0, max(len(tensors_), 1), _TENSORS):
@@ -87,7 +85,7 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         layers = [t.shape[0] if block_dim else 1 for t in some]
         layer_bytes = [t.numel() // l * t.element_size() for t, l in zip(some, layers)]
         rc = lib.odsd_copy_blocks((C.c_void_p * k)(*[t.data_ptr() for t in some]), (C.c_int64 * k)(*[b // num_blocks for b in layer_bytes]),
-                                  (C.c_int64 * k)(*layer_bytes), (C.c_int32 * k)(*layers), k, src.data_ptr(), dst.data_ptr(), n, num_blocks,
+                                  (C.c_int64 * k)(*layer_bytes), (C.c_int32 * k)(*layers), k, from_at, to_at, n, num_blocks,
                                   _ptr(tables), 0 if tables is None else tables.numel(), _stream())
         if rc:
             _lib.check(rc, "odsd_copy_blocks")

@@ -10,7 +10,7 @@
 // launch of its own, has the block's bit.
 // Many rows of a block (a prompt) are read once and stay in registers between their maximum and their codes; V's codes are turned
 // through LDS, four rows of four dimensions at a time, and leave as 16 bytes of a dimension.  A few rows (decode) write V's bytes one by one.
-// Traffic bounds a prompt, 3 bytes a value: 32767 tokens of 8 heads of 128, 201 MB, 60 us (and 5 for the bitmaps), 3.3 TB/s.  The 16
+// Traffic bounds a prompt, 3 bytes a value: 32767 tokens of 8 heads of 128, 201 MB, 58 us (and 5 for the bitmaps), 3.5 TB/s.  The 16
 // loads of a thread have no branch between them (rows that are not there load the leader's and count as zeros): with one each 76 us.
 // Three workgroups to a CU; with four the registers do not suffice (87).  A decode step is a chain of four trips to memory: 64 rows 5.7 us.
 #include "fp8.h"
@@ -62,7 +62,7 @@ template <> __device__ __forceinline__ float kv_value<half_t>(uint16_t b) { retu
 
 template <bool VEC>
 __device__ __forceinline__ uint4_t kv_load8(const uint16_t *p) {
-    if constexpr (VEC) return *(const uint4_t *)p;
+    if constexpr (VEC) return __builtin_nontemporal_load((const uint4_t *)p);
     uint4_t w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;

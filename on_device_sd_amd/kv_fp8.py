@@ -153,13 +153,13 @@ def paged_attention_fp8(q: torch.Tensor, cache: KVCacheFP8, context: Dict[str, t
                 raise ValueError(f"max_q_len={most} is below the longest query ({max(host)} tokens)")
             if min(host) < 0 or sum(host) > n_tokens:
                 raise ValueError(f"query lengths {host} do not fit {n_tokens} tokens")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q = q.contiguous()
+    out = torch.empty_like(q)
     if n_seqs == 0 or n_tokens == 0:
         return out
     max_blocks = tables.shape[1]
     if max_blocks == 0:                                     # nobody has a key
         return out.zero_()
-    q = q.contiguous()
     tables, lens, q_lens = (t if t is None or (t.get_device() == dev and t.dtype == torch.int32 and t.is_contiguous())
                             else t.to(device=q.device, dtype=torch.int32).contiguous() for t in (tables, lens, q_lens))
     lib = _lib.load()
@@ -167,7 +167,7 @@ def paged_attention_fp8(q: torch.Tensor, cache: KVCacheFP8, context: Dict[str, t
     if nbytes == 0:
         raise _lib.OdsdError(f"attention over the 8-bit cache: unsupported shape: {n_seqs} sequences of up to {most} queries, {num_heads} / "
                              f"{kv_heads} heads of {head_dim}, blocks of {block_size}")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(nbytes // 2)                           # (of two-byte numbers)
     scale = head_dim ** -0.5 if softmax_scale is None else softmax_scale
     rc = lib.odsd_paged_attention_fp8(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(),
                                       lens.data_ptr(), _ptr(q_lens), n_tokens, n_seqs, most, num_heads, kv_heads, head_dim, block_size, max_blocks,

@@ -265,7 +265,7 @@ def adjust_logits(logits: torch.Tensor, context: Dict, *, tokens: Optional[torch
         if _half_alike(logits, out):
             raise ValueError("out must be logits itself, or share no element with it")
     else:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     if rows == 0 or vocab == 0 or n_seqs == 0:
         return out
     ldo = out.stride(0) if rows > 1 else vocab
