@@ -629,10 +629,11 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
     pl.n_wg = FP8_WG;
     // Whole units need no merge (4 to 6 us) and leave no pieces; split ones level mixed lengths out and fill the chip.  (32 / 4 heads of 128, whole /
     // split, us.  16 rows: 64 sequences of 512 keys 9.9 / 13.9, 1024 15.1 / 18.8, 2048 25.1 / 28.6, 750 to 3001 31.6 / 29.4; 128 of 1024 25.4 /
-    // 29.1; 16 of 1024 12.0 / 10.0; one of 777 10.0 / 8.0.  64 rows: 32 sequences of 512 keys 14.6 / 21.2, 1024 20.4 / 23.8, 2048 31.9 / 28.9;
+    // 29.1; 16 of 1024 12.0 / 10.0; one of 777 10.0 / 8.0: what a CU reads a microsecond bounds a unit, so heads of 64 stay whole for twice the keys, 14 /
+    // 2 heads, one of 1024 5.3 / 6.7, 2048 7.6 / 7.3; 64 of 2048 9.7 / 12.3; 128 of 4096 23.1 / 28.0.  64 rows: 32 sequences of 512 keys 14.6 / 21.2, 1024 20.4 / 23.8, 2048 31.9 / 28.9;
     // 64 of 2048 41.7 / 45.1, 512 to 2048 33.9 / 39.3; 8 of 2048 30.6 / 22.0.  32 rows: 64 of 2048 33.2 / 37.2, 8 of 4096 37.9 / 18.6.  128 rows: 4
     // sequences of 8192 keys 279 / 286, one 160 / 86.)  List positions are 32 bits wide.
-    const int64_t whole = pl.rows <= 16 ? (pl.units >= 256 ? 2048 : pl.units >= 128 ? 1024 : FP8_WHOLE) : max((int64_t)FP8_WHOLE, 12 * pl.units);
+    const int64_t whole = pl.rows <= 16 ? (pl.units >= 256 ? 2048 : pl.units >= 128 ? 1024 : FP8_WHOLE) * 128 / head_dim : max((int64_t)FP8_WHOLE, 12 * pl.units);
     pl.split = !(max_keys <= whole || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
     pl.shares = (int)min(pl.units * steps, (int64_t)pl.n_wg);
     pl.bytes = pl.split ? odsd_round_up((size_t)2 * pl.shares * pl.rows * (head_dim + 4) * sizeof(float), 256) : 0;
