@@ -12,7 +12,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _ptr, _raw_device, _same_device, _stream, _wrote
+from .ops import _NO_WORKSPACE, _ptr, _raw_device, _same_device, _stream, _wrote
 
 _E4M3 = torch.float8_e4m3fn
 _SHORT_LIST = 4096                                      # rows that the store takes without a workspace
@@ -167,11 +167,11 @@ def paged_attention_fp8(q: torch.Tensor, cache: KVCacheFP8, context: Dict[str, t
     if nbytes == 0:
         raise _lib.OdsdError(f"attention over the 8-bit cache: unsupported shape: {n_seqs} sequences of up to {most} queries, {num_heads} / "
                              f"{kv_heads} heads of {head_dim}, blocks of {block_size}")
-    ws = q.new_empty(nbytes // 2)                           # (of two-byte numbers)
+    ws = None if nbytes == _NO_WORKSPACE else q.new_empty(nbytes // 2)       # (of two-byte numbers)
     scale = head_dim ** -0.5 if softmax_scale is None else softmax_scale
     rc = lib.odsd_paged_attention_fp8(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(),
                                       lens.data_ptr(), _ptr(q_lens), n_tokens, n_seqs, most, num_heads, kv_heads, head_dim, block_size, max_blocks,
-                                      blocks, scale, code, out.data_ptr(), ws.data_ptr(), nbytes, _stream())
+                                      blocks, scale, code, out.data_ptr(), _ptr(ws), nbytes, _stream())
     if rc:
         _lib.check(rc, "odsd_paged_attention_fp8")
     return out

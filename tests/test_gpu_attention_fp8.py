@@ -110,6 +110,17 @@ def test_bound_from_the_tokens(dev):
     check(dev, 8, 2, 64, 32, [100, 40, 700], [3, 4, 2], torch.bfloat16, extra=200)         # tables far longer than the contexts
 
 
+@pytest.mark.parametrize("n_seqs, heads, H, D, q, lens", [
+    (32, 4, 4, 64, 1, (2048, 1, 2033)), (32, 4, 4, 64, 1, (2064, 0, 700)), (64, 4, 4, 64, 1, (4096, 5)), (64, 4, 4, 64, 1, (4112, 16)),
+    (32, 8, 4, 128, 1, (1024, 17)), (32, 8, 4, 128, 1, (1040, 1000)), (1, 8, 4, 128, 1, (512,)), (1, 8, 4, 128, 1, (528,)), (1, 8, 1, 64, 1, (1040,)),
+    (12, 28, 4, 64, 3, (576, 60)), (12, 28, 4, 64, 3, (592, 3)), (16, 16, 4, 64, 9, (768, 9)), (16, 16, 4, 64, 9, (784, 500)),
+    (4, 64, 4, 64, 16, (512, 100)), (4, 64, 4, 64, 16, (528, 528))])
+def test_whole_and_split_units(dev, n_seqs, heads, H, D, q, lens):
+    """tables just within and just past the length up to which units are not split, for every number of rows"""
+    lens = [lens[i % len(lens)] for i in range(n_seqs)]
+    check(dev, heads, H, D, 16, lens, [q] * n_seqs, torch.bfloat16, explicit=q > 1, context_more={"max_query_len": q})
+
+
 def test_many_sequences(dev):
     rng = np.random.default_rng(7)
     lens = [int(n) for n in rng.integers(0, 700, 700)]
