@@ -8,8 +8,9 @@
 // drafted or have a bias.  Then it goes through the sequence's rows, adding to the counts the draft that stands before each: a row's
 // share comes in 16 bytes a thread, the listed logits are changed in LDS, and it leaves 16 bytes a thread with -inf where the mask forbids.
 // No table of counts lives between steps, so drafts that are not kept leave nothing to undo.  The traffic of the logits, once in and once
-// out, is the bound; the tokens (read again for every share, from L2) are little next to it.  (Changing the listed logits in memory after a copy
-// of the rows took 102 us for 449 rows of 131072, 4096 tokens each, of which the copy is 50: a logit is 2 bytes of the 64 that move.)
+// out, is the bound; the tokens (read again for every share, from L2) are little next to it: 449 rows of 131072 in bf16, 4096 tokens a sequence,
+// 65 us, 3.6 TB/s (a copy of the rows 45).  Changing the listed logits in memory after a copy took 102: a logit is 2 bytes of the 64 that move.
+// Asking for the first rows before the tokens are looked through gains nothing (66), nor do nontemporal loads or stores (67).
 // In place and without a mask only the listed logits are read and written.
 #include "common.h"
 #include <type_traits>
@@ -20,6 +21,7 @@
 #define ADJ_BIASES 128           // biases of a share that are kept in LDS
 #define ADJ_GRANULE 128          // tokens, a power of two
 #define ADJ_MOST 4096            // tokens of a share at most
+#define ADJ_FEW 1024             // workgroups up to which a sequence's rows go to several
 #define ADJ_ROWS 64              // rows whose drafts and masks are looked up at a time
 
 struct AdjParams {
@@ -69,7 +71,8 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     extern __shared__ uint4_t lds4[];          // two rows of the share (dense), counts [most], the list [most] in 16 bits
     uint32_t *lds = (uint32_t *)lds4 + (p.dense ? 2 * p.most * (int)sizeof(T) / 4 : 0);
     __shared__ int sums[8], listed, biases;
-    __shared__ int bias_token[ADJ_BIASES], bias_entry[ADJ_BIASES], draft_of[ADJ_ROWS], mask_at[ADJ_ROWS];       // entries that name a token of the share, in no order
+    __shared__ int bias_token[ADJ_BIASES], bias_entry[ADJ_BIASES];       // entries that name a token of the share, in no order
+    __shared__ int draft_of[ADJ_ROWS], mask_at[ADJ_ROWS];
     uint32_t *counts = lds;
     uint16_t *list = (uint16_t *)(lds + p.most);
     const int tid = threadIdx.x;
@@ -114,6 +117,10 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     if (rows == 0 || (uint32_t)row >= (uint32_t)p.n_rows) return;
     rows = min(rows, p.n_rows - row);
     const int drafts = p.drafts && (uint32_t)draft < (uint32_t)p.n_drafts ? min(rows - 1, p.n_drafts - draft) : 0;
+    // the rows of this workgroup
+    constexpr int R = 2;                       // rows at a time
+    const int per_group = ((rows + (int)gridDim.y - 1) / (int)gridDim.y + R - 1) / R * R, from = (int)blockIdx.y * per_group, until = min(rows, from + per_group);
+    if (from >= rows) return;
     if (p.sparse) {
         if (p.tokens) {
             const int len = min(max(p.token_lens ? p.token_lens[s] : p.max_tokens, 0), p.max_tokens);
@@ -134,7 +141,9 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
         }
         for (int i = tid; i < drafts; i += 256) {
             const int t = mine(adj_token(p.drafts, 8, draft + i));
-            if (t >= 0) atomicOr(&counts[t], ADJ_DRAFT);
+            if (t < 0) continue;
+            if (i + 1 < from) atomicAdd(&counts[t], 1u);          // (draft i stands before row i + 1)
+            if (i + 1 < until) atomicOr(&counts[t], i + 1 < from ? ADJ_SEEN : ADJ_DRAFT);
         }
         for (int i = tid; i < p.n_bias; i += 256) {
             const int t = mine(p.bias_tokens[(int64_t)s * p.n_bias + i]);
@@ -182,17 +191,17 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
         if (times) x = x - (f * (float)times + pr);
         return n & ADJ_BIAS ? x + add : x;
     };
-    // token i of the share in all rows, straight in memory
+    // token i of the share in the workgroup's rows, straight in memory
     auto column = [&](const int i, uint32_t n) {
         const int v = at(i);
         const float add = n & ADJ_BIAS ? bias_of(i) : 0.0f;
-        for (int j0 = 0; j0 < rows; j0 += 4) {             // (four rows' loads on their way at a time)
+        for (int j0 = from; j0 < until; j0 += 4) {         // (four rows' loads on their way at a time)
             T raw[4];
             int64_t before[4];
             bool allowed[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int j = min(j0 + u, rows - 1);
+                const int j = min(j0 + u, until - 1);
                 const int m = MASK ? mask_row(j) : -1;
                 raw[u] = in[j * p.ld + v];
                 allowed[u] = m < 0 || ((p.mask[m * p.mask_stride + (v >> 5)] >> (v & 31)) & 1);
@@ -200,7 +209,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if (j0 + u >= rows) break;
+                if (j0 + u >= until) break;
                 if (before[u] == v) n = (n + 1u) | ADJ_SEEN;
                 to[(j0 + u) * p.ldo + v] = AdjIO<T>::put(allowed[u] ? changed(AdjIO<T>::get(raw[u]), n, add) : -INFINITY);
             }
@@ -212,7 +221,6 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     }
     constexpr int TPG = 16 / (int)sizeof(T);   // tokens of a group: 16 bytes, rows at any element
     constexpr int U = ADJ_MOST / TPG / 256;    // groups of a thread
-    constexpr int R = 2;                       // rows at a time
     // what the vocabulary has behind its last whole group
     const int tail = p.vocab - p.vocab % TPG + tid;
     if (tid < TPG && tail < p.vocab && mine(tail) >= 0) column(mine(tail), p.sparse ? counts[mine(tail)] : 0u);
@@ -224,7 +232,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     const int my_i = few && tid < n_listed ? list[tid] : 0, my_v = at(my_i), per = p.most / TPG;
     uint32_t my_n = few && tid < n_listed ? counts[my_i] : 0u;
     const float my_add = my_n & ADJ_BIAS ? bias_of(my_i) : 0.0f;
-    for (int c0 = 0; c0 < rows; c0 += ADJ_ROWS) {
+    for (int c0 = from; c0 < until; c0 += ADJ_ROWS) {
         __syncthreads();                       // nobody reads the last rows' drafts and masks any more
         if (tid < ADJ_ROWS) {
             const int j = c0 + tid;
@@ -233,7 +241,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
             mask_at[tid] = MASK && j < rows ? mask_row(j) : -1;
         }
         __syncthreads();
-        const int end = min(rows, c0 + ADJ_ROWS);
+        const int end = min(until, c0 + ADJ_ROWS);
         // (what the next turn needs is requested a turn ahead, loads without branches in between: the compiler then knows how many
         // younger ones it may leave on their way)
         auto load = [&](uint4_t (&w)[R][U], uint32_t (&b)[R][U], const int j) {
@@ -357,7 +365,12 @@ extern "C" int odsd_adjust_logits(const void *logits, int64_t logits_stride, voi
     p.sparse = p.tokens || n_drafts || n_bias;
     p.dense = out != logits || out_stride != logits_stride || mask;
     if (!p.sparse && !p.dense) return ODSD_OK;
-    const unsigned grid = (unsigned)n_seqs << p.share_bits;
+    // Few sequences: their rows are dealt out too, two to a workgroup at least, and each looks through the tokens for itself.  (Rows of one
+    // workgroup / so, us: one sequence of 5 rows of 50257 fp32 9.2 / 6.5, of 41 35.4 / 11.6; 4 of 5 rows of 131072 bf16 9.9 / 9.3; up to 2048
+    // workgroups 16 of 9 rows of 131072 21.2 / 25.3.)
+    const int64_t wgs = (int64_t)n_seqs << p.share_bits;
+    const int64_t groups = query_lens ? max((int64_t)1, min((int64_t)ADJ_FEW / wgs, ((int64_t)n_rows + 1) / 2)) : 1;
+    const dim3 grid((unsigned)wgs, (unsigned)groups);
     const size_t elt = dtype == ODSD_DT_F32 ? 4 : 2, bytes = p.sparse ? (size_t)p.most * (6 + (p.dense ? 2 * elt : 0)) : 0;
     hipStream_t st = (hipStream_t)stream;
 #define ADJ_GO(T)                                                                 \
