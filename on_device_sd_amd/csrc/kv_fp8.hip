@@ -3,16 +3,19 @@
 // Powers of two, so that a row stored earlier keeps its value when a later one raises the scale: the codes are divided by a power of
 // two, which only those lose bits by that fall below e4m3's normal numbers.
 //
-// A (block, head) is written by one workgroup, K and V by one each, so scale and codes need no atomics and the same call gives the same
-// bits.  The rows of a block may stand anywhere in slot_mapping: the workgroup of the first of them (the leader) looks through the list
-// and notes which row goes to which token of the block (of two with one slot the last).  Rows that follow one of the same block, which
-// is what a prompt's are, end at once.  In a long list the leader looks only into those chunks of 256 entries whose bitmap, made by a
+// A (block, head) is written by one workgroup, K and V each by one wavefront or workgroup, so scale and codes need no atomics and the same
+// call gives the same bits.  The rows of a block may stand anywhere in slot_mapping: the workgroup of the first of them (the leader) looks through
+// the list and notes which row goes to which token of the block (of two with one slot the last).  Rows that follow one of the same block,
+// which is what a prompt's are, end at once.  In a long list the leader looks only into those chunks of 256 entries whose bitmap, made by a
 // launch of its own, has the block's bit.
 // Many rows of a block (a prompt) are read once and stay in registers between their maximum and their codes; V's codes are turned
-// through LDS, four rows of four dimensions at a time, and leave as 16 bytes of a dimension.  A few rows (decode) write V's bytes one by one.
+// through LDS, four rows of four dimensions at a time, and leave as 16 bytes of a dimension.  A few rows write V's bytes one by one.
 // Traffic bounds a prompt, 3 bytes a value: 32767 tokens of 8 heads of 128, 201 MB, 58 us (and 5 for the bitmaps), 3.5 TB/s.  The 16
 // loads of a thread have no branch between them (rows that are not there load the leader's and count as zeros): with one each 76 us.
-// Three workgroups to a CU; with four the registers do not suffice (87).  A decode step is a chain of four trips to memory: 64 rows 5.7 us.
+// Three workgroups to a CU; with four the registers do not suffice (87).
+// A decode step is a chain of four trips to memory, 64 rows of 8 heads 5.1 us, and then a number of workgroups: where the leader's sixteenth neighbour
+// behind is no row of its block, a workgroup looks through the list once for several heads, and its wavefronts take a K or V each.  (A workgroup for each
+// K and V / so: 128 rows 14.7 / 6.2, 512 44 / 20; a prompt of 2000, whose leaders wait for no other workgroup, 14.4 / 15.9.)
 #include "fp8.h"
 #include <type_traits>
 
@@ -22,6 +25,7 @@
 #define KV8_LONG 4096          // a longer list has bitmaps
 #define KV8_WINDOW 256         // tokens of a block that are turned at a time
 #define KV8_FEW 16             // rows of a block that are not turned
+#define KV8_WGS 512            // workgroups that a list of few rows a block goes to (1024: 256 rows of 8 heads 13.1 us for 11.0)
 
 struct KvFp8Params {
     const uint16_t *key, *value;
@@ -32,6 +36,8 @@ struct KvFp8Params {
     uint32_t *bitmaps;                                         // [KV8_BITS / 32][n_chunks], or null
     int N, n_src, KVH, bs, n_blocks, n_chunks;
     int per_wg;                                                // list entries of a workgroup
+    int run_wgs;                                               // workgroups that have a head's K or V each; behind them those for few rows of a block,
+    int few_groups, few_heads, few_entries;                    // which have a range of entries and some heads
 };
 
 __device__ __forceinline__ uint32_t kv_bit(const int block) { return ((uint32_t)block * 0x9e3779b1u) >> 24; }      // of KV8_BITS
@@ -40,6 +46,13 @@ __device__ __forceinline__ bool kv_entry(const KvFp8Params &p, const int i, int 
     slot = p.slots[i];
     const bool row = !p.src || (p.src[i] >= 0 && p.src[i] < p.n_src);
     return slot >= 0 && slot / p.bs < p.n_blocks && row;
+}
+
+// Whether a block whose first entry is e has a run of rows: its leader is looked for by the workgroups of a head's K or V, otherwise by
+// those for few rows.
+__device__ __forceinline__ bool kv_run(const KvFp8Params &p, const int e, const int block) {
+    int slot;
+    return e + KV8_FEW < p.N && kv_entry(p, e + KV8_FEW, slot) && slot / p.bs == block;
 }
 
 __global__ __launch_bounds__(KV8_CHUNK) void kv_bitmap_kernel(const KvFp8Params p) {
@@ -54,6 +67,17 @@ __global__ __launch_bounds__(KV8_CHUNK) void kv_bitmap_kernel(const KvFp8Params 
     }
     __syncthreads();
     if (threadIdx.x < KV8_BITS / 32) p.bitmaps[(size_t)threadIdx.x * p.n_chunks + blockIdx.x] = bits[threadIdx.x];
+}
+
+// n times 16 codes of a block times `ratio`, a power of two (0: the block held nothing, whatever its bytes are)
+__device__ __forceinline__ void kv_rescale(uint8_t *codes, const int n, const float ratio, const int first, const int step) {
+#pragma unroll 1
+    for (int i = first; i < n; i += step) {
+        uint4_t w = *(const uint4_t *)(codes + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = ratio > 0.0f ? fp8_rescale4(w[j], ratio) : 0u;
+        *(uint4_t *)(codes + 16 * i) = w;
+    }
 }
 
 template <typename T> __device__ __forceinline__ float kv_value(uint16_t b);
@@ -111,11 +135,116 @@ __device__ __forceinline__ u32x2 kv_codes8(const uint4_t w, const float scale) {
     for (int i = 0; i < 8; ++i) x[i] = kv_value<T>((uint16_t)(w[i >> 1] >> (16 * (i & 1)))) * inv;
     return u32x2{fp8_pack4(x[0], x[1], x[2], x[3]), fp8_pack4(x[4], x[5], x[6], x[7])};
 }
+// codes of eight dimensions of a token to their place
+template <int HD>
+__device__ __forceinline__ void kv_put(uint8_t *codes, const int bs, const bool is_v, const int r, const int d, const u32x2 c) {
+    if (!is_v) {
+        *(u32x2 *)(codes + r * HD + d) = c;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) codes[(d + j) * bs + r] = (uint8_t)(c[j >> 2] >> (8 * (j & 3)));
+    }
+}
 __device__ __forceinline__ uint32_t kv_wave_top(uint32_t m) {
     m = max(m & 0xffffu, m >> 16);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, ODSD_WAVE));
     return m;
+}
+
+// Blocks without a run of rows, in short lists: the leader's workgroup has several heads, and a wavefront takes one of their Ks and Vs after
+// the other, with nothing to wait for between them.
+template <typename T, int HD, bool VEC>
+__device__ __forceinline__ void kv_store_few(const KvFp8Params &p, const int wg, int *row_of, int *first, int *count, uint16_t *present) {
+    constexpr int NP = HD / 8, HELD = KV8_FEW * NP / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), bs = p.bs;
+    const int range = wg / p.few_groups, h0 = (wg - range * p.few_groups) * p.few_heads, heads = min(p.few_heads, p.KVH - h0);
+    const int begin = range * p.few_entries, stop = min(p.N, begin + p.few_entries);
+    for (int e0 = begin; e0 < stop; e0 += 64) {
+        const int le = e0 + lane;
+        int slot_l = -1, before;
+        bool may = false;
+        if (le < stop && kv_entry(p, le, slot_l)) {
+            const int block = slot_l / bs;
+            may = (le == 0 || !kv_entry(p, le - 1, before) || before / bs != block) && !kv_run(p, le, block);
+        }
+        for (uint64_t leaders = __ballot(may); leaders; leaders &= leaders - 1) {
+            const int l = __builtin_ctzll(leaders), e = e0 + l;
+            const int block = __builtin_amdgcn_readlane(slot_l, l) / bs, base = block * bs;
+            __syncthreads();                    // the arrays are free
+            for (int i = tid; i < bs; i += KV8_THREADS) row_of[i] = -1;
+            if (tid == 0) {
+                *first = 0x7fffffff;
+                *count = 0;
+            }
+            __syncthreads();
+            for (int i = tid; i < p.N; i += KV8_THREADS) {
+                const int slot = p.slots[i], at = slot - base;
+                if (slot >= base && at < bs && (!p.src || (p.src[i] >= 0 && p.src[i] < p.n_src))) {
+                    atomicMax(&row_of[at], i);
+                    atomicMin(first, i);
+                }
+            }
+            __syncthreads();
+            if (*first != e) continue;          // (another entry's)
+            for (int i = tid; i < bs; i += KV8_THREADS)
+                if (row_of[i] >= 0) present[atomicAdd(count, 1)] = (uint16_t)i;
+            __syncthreads();
+            const int rows = *count, pieces = rows * NP;
+            const bool anew = row_of[0] >= 0, held = rows <= KV8_FEW;
+            for (int t = wave; t < 2 * heads; t += KV8_THREADS / 64) {
+                const int h = h0 + (t >> 1);
+                const bool is_v = t & 1;
+                const uint16_t *x = (is_v ? p.value : p.key) + (int64_t)h * (is_v ? p.value_head : p.key_head);
+                const int64_t token = is_v ? p.value_token : p.key_token, bh = (int64_t)block * p.KVH + h;
+                float *scale_at = p.scales + 2 * bh + (is_v ? 1 : 0);
+                const float was = *scale_at;
+                auto load = [&](const int i) {
+                    const int from = row_of[present[i / NP]];
+                    return kv_load8<VEC>(x + (int64_t)(p.src ? p.src[from] : from) * token + 8 * (i % NP));
+                };
+                uint4_t hold[HELD];
+#pragma unroll
+                for (int u = 0; u < HELD; ++u) {
+                    hold[u] = uint4_t{0u, 0u, 0u, 0u};
+                    if (held && lane + 64 * u < pieces) hold[u] = load(lane + 64 * u);
+                }
+                auto top_of = [&](auto finite_c) {
+                    constexpr bool FINITE = decltype(finite_c)::value;
+                    uint32_t m = 0u;
+                    if (held) {
+#pragma unroll
+                        for (int u = 0; u < HELD; ++u) m = kv_top8<T, FINITE>(hold[u], m);
+                    } else {
+#pragma unroll 1
+                        for (int i = lane; i < pieces; i += 64) m = kv_top8<T, FINITE>(load(i), m);
+                    }
+                    return kv_wave_top(m);
+                };
+                uint32_t top = top_of(std::false_type{});
+                const bool finite = top < KvBits<T>::INF;
+                if (!finite) top = top_of(std::true_type{});
+                const float old = anew ? 0.0f : was, scale = fmaxf(old, fp8_scale_of(kv_value<T>((uint16_t)top)));
+                uint8_t *codes = (is_v ? p.v_cache : p.k_cache) + bh * bs * HD;
+                if (!anew && old < scale) {
+                    kv_rescale(codes, bs * HD / 16, old / scale, lane, 64);
+                    __threadfence_block();      // (the codes are there before the new ones come)
+                }
+                if (lane == 0) *scale_at = scale;
+                auto put = [&](const int i, const uint4_t w) {
+                    kv_put<HD>(codes, bs, is_v, present[i / NP], 8 * (i % NP), finite ? kv_codes8<T, true>(w, scale) : kv_codes8<T, false>(w, scale));
+                };
+                if (held) {
+#pragma unroll
+                    for (int u = 0; u < HELD; ++u)
+                        if (lane + 64 * u < pieces) put(lane + 64 * u, hold[u]);
+                } else {
+#pragma unroll 1
+                    for (int i = lane; i < pieces; i += 64) put(i, load(i));
+                }
+            }
+        }
+    }
 }
 
 template <typename T, int HD, bool VEC>
@@ -130,6 +259,7 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
     __shared__ __attribute__((aligned(16))) uint8_t turn[KV8_WINDOW * ROW];
     uint16_t *present = (uint16_t *)turn;      // tokens that get a row, in no order; where V is turned only until then
     const int tid = threadIdx.x, lane = tid & 63, row0 = tid / NP, piece = tid % NP;
+    if ((int)blockIdx.x >= p.run_wgs) return kv_store_few<T, HD, VEC>(p, (int)blockIdx.x - p.run_wgs, row_of, &first, &count, present);
     const int which = blockIdx.x / 2, h = which % p.KVH;
     const bool is_v = blockIdx.x & 1;
     const uint16_t *x = (is_v ? p.value : p.key) + (int64_t)h * (is_v ? p.value_head : p.key_head);
@@ -146,7 +276,8 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
         bool may = false;
         if (e < stop && kv_entry(p, e, slot_l)) {
             int before;
-            may = e == 0 || !kv_entry(p, e - 1, before) || before / bs != slot_l / bs;
+            const int block = slot_l / bs;
+            may = (e == 0 || !kv_entry(p, e - 1, before) || before / bs != block) && (p.bitmaps || kv_run(p, e, block));
         }
         leaders = __ballot(may);
     }
@@ -242,14 +373,7 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
         const float scale = fmaxf(old, fp8_scale_of(amax));
         uint8_t *codes = (is_v ? p.v_cache : p.k_cache) + bh * bs * HD;
         if (!anew && old < scale) {
-            const float ratio = old / scale;    // a power of two (0: the block held nothing, whatever its bytes are)
-#pragma unroll 1
-            for (int i = tid; i < bs * HD / 16; i += KV8_THREADS) {
-                uint4_t w = *(const uint4_t *)(codes + 16 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = ratio > 0.0f ? fp8_rescale4(w[j], ratio) : 0u;
-                *(uint4_t *)(codes + 16 * i) = w;
-            }
+            kv_rescale(codes, bs * HD / 16, old / scale, tid, KV8_THREADS);
         }
         __syncthreads();                        // (the codes are there before the new ones come)
         if (tid == 0) *scale_at = scale;
@@ -259,13 +383,7 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
             for (int i = tid; i < rows * NP; i += KV8_THREADS) {
                 const int r = present[i / NP], d = 8 * (i % NP);
                 const uint4_t w = kv_load8<VEC>(source(row_of[r]) + d);
-                const u32x2 c = finite ? kv_codes8<T, true>(w, scale) : kv_codes8<T, false>(w, scale);
-                if (!is_v) {
-                    *(u32x2 *)(codes + r * HD + d) = c;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) codes[(d + j) * bs + r] = (uint8_t)(c[j >> 2] >> (8 * (j & 3)));
-                }
+                kv_put<HD>(codes, bs, is_v, r, d, finite ? kv_codes8<T, true>(w, scale) : kv_codes8<T, false>(w, scale));
             }
             continue;
         }
@@ -362,9 +480,19 @@ extern "C" int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int6
     // Enough workgroups for the chip; no more entries each than a block of a prompt takes, so that every one has about one leader (a workgroup
     // that has none holds its place for two trips to memory: with 64 entries each and blocks of 256 three of four, 94 us where this took 76).
     p.per_wg = (int)max((int64_t)1, min((int64_t)min(256, block_size), (int64_t)N * num_kv_heads / 1024));
+    int64_t few = 0;
+    if (N <= KV8_LONG) {
+        p.per_wg = max(p.per_wg, min(KV8_FEW, N));            // (a run has more than KV8_FEW entries)
+        const int64_t heads = ((int64_t)N * num_kv_heads + KV8_WGS - 1) / KV8_WGS;
+        p.few_heads = (int)min((int64_t)num_kv_heads, max((int64_t)2, heads));
+        p.few_groups = (num_kv_heads + p.few_heads - 1) / p.few_heads;
+        p.few_entries = (int)max((int64_t)1, (int64_t)N * p.few_groups / KV8_WGS);
+        few = ((int64_t)N + p.few_entries - 1) / p.few_entries * p.few_groups;
+    }
     const int64_t wgs = ((int64_t)N + p.per_wg - 1) / p.per_wg * num_kv_heads * 2;
-    if (wgs >= (1LL << 24)) return ODSD_ERR_UNSUPPORTED;
-    const unsigned grid = (unsigned)wgs;
+    if (wgs + few >= (1LL << 24)) return ODSD_ERR_UNSUPPORTED;
+    p.run_wgs = (int)wgs;
+    const unsigned grid = (unsigned)(wgs + few);
     if (N > KV8_LONG) {
         if (!workspace) return ODSD_ERR_NULL;
         if ((uintptr_t)workspace & 3u) return ODSD_ERR_ALIGN;

@@ -79,7 +79,7 @@ def test_rows_in_any_order(dev, N):
     check(filled(dev, nb, H, bs, D, N), *rows(dev, n, H, D, torch.bfloat16, N), slots, src)
 
 
-@pytest.mark.parametrize("N", [300, 20000])
+@pytest.mark.parametrize("N", [300, 480, 4080, 20000])
 def test_all_blocks_side_by_side(dev, N):
     """one token for every block in turn: every workgroup's entries are of other blocks"""
     H, D, bs = 1, 64, 32
