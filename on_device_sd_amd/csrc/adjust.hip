@@ -9,8 +9,9 @@
 // share comes in 16 bytes a thread, the listed logits are changed in LDS, and it leaves 16 bytes a thread with -inf where the mask forbids.
 // No table of counts lives between steps, so drafts that are not kept leave nothing to undo.  The traffic of the logits, once in and once
 // out, is the bound; the tokens (read again for every share, from L2) are little next to it: 449 rows of 131072 in bf16, 4096 tokens a sequence,
-// 65 us, 3.6 TB/s (a copy of the rows 45).  Changing the listed logits in memory after a copy took 102: a logit is 2 bytes of the 64 that move.
-// Asking for the first rows before the tokens are looked through gains nothing (66), nor do nontemporal loads or stores (67).
+// 63 us, 3.9 TB/s (a copy of the rows 45).  Changing the listed logits in memory after a copy took 102: a logit is 2 bytes of the 64 that move.
+// Asking for the first rows before the tokens are looked through gains nothing, nor do nontemporal loads or stores (1 to 2 us more).  One row
+// a sequence is a chain of some ten waits a workgroup, two rounds of them for 64 sequences of 131072: 20 us where the bytes take 7.
 // In place and without a mask only the listed logits are read and written.
 #include "common.h"
 #include <type_traits>
@@ -86,8 +87,12 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     };
     if (p.sparse) {
         if (tid == 0) listed = biases = 0;
-        for (int i = tid; i < p.most; i += 256) counts[i] = 0u;
+        for (int i = tid; i < p.most / 4; i += 256) ((uint4_t *)counts)[i] = uint4_t{0u, 0u, 0u, 0u};
     }
+    // flags of token i of the share; whoever sets the first lists it
+    auto mark = [&](const int i, const uint32_t flags) {
+        if (atomicOr(&counts[i], flags) == 0u) list[atomicAdd(&listed, 1)] = (uint16_t)i;
+    };
     // the sequence's first row and first draft
     int row = s, draft = 0, rows = 1;
     if (p.q_lens) {
@@ -133,8 +138,8 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
                 for (int u = 0; u < 8; ++u) {
                     const int i = i0 + 256 * u < len ? mine(t[u]) : -1;
                     if (i >= 0) {
+                        mark(i, ADJ_SEEN);
                         if (i0 + 256 * u >= prompt) atomicAdd(&counts[i], 1u);
-                        atomicOr(&counts[i], ADJ_SEEN);
                     }
                 }
             }
@@ -142,13 +147,14 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
         for (int i = tid; i < drafts; i += 256) {
             const int t = mine(adj_token(p.drafts, 8, draft + i));
             if (t < 0) continue;
-            if (i + 1 < from) atomicAdd(&counts[t], 1u);          // (draft i stands before row i + 1)
-            if (i + 1 < until) atomicOr(&counts[t], i + 1 < from ? ADJ_SEEN : ADJ_DRAFT);
+            if (i + 1 >= until) continue;      // (draft i stands before row i + 1)
+            mark(t, i + 1 < from ? ADJ_SEEN : ADJ_DRAFT);
+            if (i + 1 < from) atomicAdd(&counts[t], 1u);
         }
         for (int i = tid; i < p.n_bias; i += 256) {
             const int t = mine(p.bias_tokens[(int64_t)s * p.n_bias + i]);
             if (t >= 0) {
-                atomicOr(&counts[t], ADJ_BIAS);
+                mark(t, ADJ_BIAS);
                 const int k = atomicAdd(&biases, 1);
                 if (k < ADJ_BIASES) {
                     bias_token[k] = t;
@@ -165,10 +171,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjParams p) {
     };
     int n_listed = 0;
     if (p.sparse) {
-        __syncthreads();                       // counts and biases are there
-        for (int i = tid; i < p.most; i += 256)
-            if (counts[i]) list[atomicAdd(&listed, 1)] = (uint16_t)i;
-        __syncthreads();
+        __syncthreads();                       // counts, list and biases are there
         n_listed = listed;
     }
     const float r = p.repetition ? p.repetition[s] : p.repetition_all;
