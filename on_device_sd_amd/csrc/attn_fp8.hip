@@ -28,6 +28,7 @@
 #include "w4_gemm.h"
 
 #define FP8_WG 512           // workgroups that share the keys: two per CU
+#define FP8_JOIN 8           // threads that share the merge of a row's pieces where units are few
 #define FP8_STEP 256         // keys of a list step, 64 per wavefront
 #define FP8_WHOLE 512        // no sequence longer: nothing is split
 
@@ -616,6 +617,7 @@ struct AttnFp8Plan {
     int64_t rg, units;            // row groups per (sequence, KV head), units
     int n_wg, shares;             // workgroups that share the list, those that can get a share
     bool split;                   // units may be split: partial results and a merge
+    int join;                     // threads that share the merge of a row's pieces
     size_t bytes;                 // workspace that splitting takes
 };
 static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t max_keys, int kvh, int head_dim) {
@@ -635,6 +637,9 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
     // sequences of 8192 keys 279 / 286, one 160 / 86.)  List positions are 32 bits wide.
     const int64_t whole = pl.rows <= 16 ? (pl.units >= 256 ? 2048 : pl.units >= 128 ? 1024 : FP8_WHOLE) * 128 / head_dim : max((int64_t)FP8_WHOLE, 12 * pl.units);
     pl.split = !(max_keys <= whole || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
+    // Few units are many pieces each, which are long to walk for one thread (one / eight, us: 4 units of 16 rows and 32768 keys 31.2 / 16.2, 16 of
+    // 16384 22.9 / 19.2, 64 of 4096 19.6 / 19.9; 4 of 64 rows and 32768 keys 39.8 / 24.9, 32 of 16384 45.9 / 46.5, 128 of 4096 46.1 / 52.2).
+    pl.join = pl.units <= 32 ? FP8_JOIN : 1;
     pl.shares = (int)min(pl.units * steps, (int64_t)pl.n_wg);
     pl.bytes = pl.split ? odsd_round_up((size_t)2 * pl.shares * pl.rows * (head_dim + 4) * sizeof(float), 256) : 0;
     return pl;
@@ -695,23 +700,29 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
         p.whole = (int)pl.rg;
     }
     const unsigned grid = (unsigned)(pl.split ? pl.shares : p.n_wg);
-    const dim3 mgrid((unsigned)(n_seqs * num_kv_heads), (unsigned)pl.rg, (unsigned)((pl.rows * head_dim + 1023) / 1024));
+    const dim3 mgrid((unsigned)(n_seqs * num_kv_heads), (unsigned)pl.rg, (unsigned)((pl.rows * head_dim * pl.join + 1023) / 1024));
     hipStream_t st = (hipStream_t)stream;
     const bool aligned = block_size % (pl.rows <= 16 ? 64 : FP8_TILE) == 0;       // a tile lies in one block
+#define FP8_MERGE(T, HDV, ROWSV, STEPV)                                                                   \
+    do {                                                                                                  \
+        if (!pl.split) break;                                                                             \
+        if (pl.join > 1) attn_merge_kernel<T, HDV, ROWSV, STEPV, STEPV, false, FP8_JOIN><<<mgrid, 256, 0, st>>>(p); \
+        else attn_merge_kernel<T, HDV, ROWSV, STEPV, STEPV><<<mgrid, 256, 0, st>>>(p);                    \
+    } while (0)
 #define FP8_GO(T, HDV)                                                                                    \
     do {                                                                                                  \
         if (aligned) attn_fp8_kernel<T, HDV, true><<<grid, 256, 0, st>>>(p);                              \
         else attn_fp8_kernel<T, HDV, false><<<grid, 256, 0, st>>>(p);                                     \
-        if (pl.split) attn_merge_kernel<T, HDV, 16, FP8_STEP, FP8_STEP><<<mgrid, 256, 0, st>>>(p);        \
+        FP8_MERGE(T, HDV, 16, FP8_STEP);                                                                  \
     } while (0)
 #define FP8_GO_TILE(T, HDV, RBV, WRV)                                                                          \
     do {                                                                                                  \
         if (pl.split) {                                                                                   \
             if (aligned) attn_fp8_tile_kernel<T, HDV, RBV, WRV, true, true><<<grid, 256, 0, st>>>(p);       \
             else attn_fp8_tile_kernel<T, HDV, RBV, WRV, false, true><<<grid, 256, 0, st>>>(p);              \
-            attn_merge_kernel<T, HDV, 16 * RBV * WRV, FP8_TILE, FP8_TILE><<<mgrid, 256, 0, st>>>(p);            \
         } else if (aligned) attn_fp8_tile_kernel<T, HDV, RBV, WRV, true, false><<<grid, 256, 0, st>>>(p);   \
         else attn_fp8_tile_kernel<T, HDV, RBV, WRV, false, false><<<grid, 256, 0, st>>>(p);                 \
+        FP8_MERGE(T, HDV, 16 * RBV * WRV, FP8_TILE);                                                      \
     } while (0)
 #define FP8_GO_RB(T, HDV)                                                                                 \
     do {                                                                                                  \
@@ -730,6 +741,7 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
 #undef FP8_GO_RB
 #undef FP8_GO_TILE
 #undef FP8_GO
+#undef FP8_MERGE
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
 }

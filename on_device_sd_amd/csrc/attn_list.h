@@ -176,10 +176,11 @@ __device__ __forceinline__ void next_unit(const AttnParams &p, SeqAt &sq, int &u
 // does the work.  (For launches that allow for many row groups, which need not be there: 64 sequences of 8
 // queries with the query lengths bounded by the 512 tokens of the call only, 900 keys: 131072 workgroups
 // otherwise, 96 us the call.)
-template <typename T, int HD, int ROWS, int FINE, int COARSE, bool BY_SHARE = false>
+// G: threads that share the walk over a row's pieces, and join what they have through LDS (1024 / HD / G rows to a workgroup then)
+template <typename T, int HD, int ROWS, int FINE, int COARSE, bool BY_SHARE = false, int G = 1>
 __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
     constexpr int XROW = HD + 4;
-    constexpr int TPR = HD / 4, RPW = 256 / TPR;
+    constexpr int TPR = HD / 4, RPW = 256 / TPR / G;
     int kvh, rg, a;                                                // a: list position of the unit's first step
     const ListPlan pl = list_plan<!BY_SHARE, true, false>(p, ROWS, FINE, COARSE, BY_SHARE ? blockIdx.x + 1 : blockIdx.x / p.KVH);
     const SeqAt &sq = pl.at;
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
     }
     const int wa = a / pl.share, wb = (a + sq.steps - 1) / pl.share;
     if (wa == wb || (BY_SHARE && wa != (int)blockIdx.x)) return;
-    const int row = (int)blockIdx.z * RPW + (int)threadIdx.x / TPR, d = 4 * ((int)threadIdx.x % TPR);
+    const int row = (int)blockIdx.z * RPW + (int)threadIdx.x / TPR % RPW, d = 4 * ((int)threadIdx.x % TPR), g = (int)threadIdx.x / (TPR * RPW);
     const int r = rg * ROWS + row;
     if (row >= ROWS || r >= sq.ql * p.Gq) return;
     const float *base = p.part + row * XROW;
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
     float m = -INFINITY, l = 0.0f;
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
     constexpr int SB = 4;
-    for (int w0 = wa; w0 <= wb; w0 += SB) {
+    for (int w0 = wa + SB * g; w0 <= wb; w0 += SB * G) {
         float ms[SB], ls[SB];
         float4_t os[SB];
 #pragma unroll
@@ -240,6 +241,27 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
             acc.x += f * os[u].x; acc.y += f * os[u].y; acc.z += f * os[u].z; acc.w += f * os[u].w;
         }
         m = mb;
+    }
+    if constexpr (G > 1) {
+        __shared__ float2_t ml[G][RPW * TPR];
+        __shared__ float4_t os[G][RPW * TPR];
+        const int at = (int)threadIdx.x % (RPW * TPR);
+        ml[g][at] = float2_t{m, l};
+        os[g][at] = acc;
+        __syncthreads();
+        if (g > 0) return;
+#pragma unroll
+        for (int u = 1; u < G; ++u) m = fmaxf(m, ml[u][at].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        l = 0.0f;
+        acc = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            const float f = __builtin_amdgcn_exp2f(ml[u][at].x - ref);
+            const float4_t o = os[u][at];
+            l += f * ml[u][at].y;
+            acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+        }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const int tok = r / p.Gq, hq = r - tok * p.Gq;

@@ -247,7 +247,8 @@ __device__ __forceinline__ void kv_store_few(const KvFp8Params &p, const int wg,
     }
 }
 
-template <typename T, int HD, bool VEC>
+// LONG: the list has bitmaps, and no workgroups for few rows
+template <typename T, int HD, bool VEC, bool LONG>
 __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp8Params p) {
     constexpr int NP = HD / 8;                           // pieces of 8 values of a row
     constexpr int HELD = KV8_WINDOW * NP / KV8_THREADS;          // pieces of a window per thread
@@ -259,7 +260,9 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
     __shared__ __attribute__((aligned(16))) uint8_t turn[KV8_WINDOW * ROW];
     uint16_t *present = (uint16_t *)turn;      // tokens that get a row, in no order; where V is turned only until then
     const int tid = threadIdx.x, lane = tid & 63, row0 = tid / NP, piece = tid % NP;
-    if ((int)blockIdx.x >= p.run_wgs) return kv_store_few<T, HD, VEC>(p, (int)blockIdx.x - p.run_wgs, row_of, &first, &count, present);
+    if constexpr (!LONG) {
+        if ((int)blockIdx.x >= p.run_wgs) return kv_store_few<T, HD, VEC>(p, (int)blockIdx.x - p.run_wgs, row_of, &first, &count, present);
+    }
     const int which = blockIdx.x / 2, h = which % p.KVH;
     const bool is_v = blockIdx.x & 1;
     const uint16_t *x = (is_v ? p.value : p.key) + (int64_t)h * (is_v ? p.value_head : p.key_head);
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
         if (e < stop && kv_entry(p, e, slot_l)) {
             int before;
             const int block = slot_l / bs;
-            may = (e == 0 || !kv_entry(p, e - 1, before) || before / bs != block) && (p.bitmaps || kv_run(p, e, block));
+            may = (e == 0 || !kv_entry(p, e - 1, before) || before / bs != block) && (LONG || kv_run(p, e, block));
         }
         leaders = __ballot(may);
     }
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
                 atomicMin(&first, i);
             }
         };
-        if (p.bitmaps) {
+        if constexpr (LONG) {
             const uint32_t bit = kv_bit(block);
             const uint32_t *maps = p.bitmaps + (size_t)(bit >> 5) * p.n_chunks;
             for (int c0 = 0; c0 < p.n_chunks; c0 += 64) {
@@ -503,17 +506,23 @@ extern "C" int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int6
     }
     const bool vec = !(((uintptr_t)key | (uintptr_t)value) & 15u) &&
                      !((key_token_stride | key_head_stride | value_token_stride | value_head_stride) & 7);
-#define KV8_GO(T)                                                                           \
-    do {                                                                                    \
-        if (head_dim == 128) {                                                              \
-            if (vec) kv_store_fp8_kernel<T, 128, true><<<grid, KV8_THREADS, 0, st>>>(p);    \
-            else kv_store_fp8_kernel<T, 128, false><<<grid, KV8_THREADS, 0, st>>>(p);       \
-        } else if (vec) kv_store_fp8_kernel<T, 64, true><<<grid, KV8_THREADS, 0, st>>>(p);  \
-        else kv_store_fp8_kernel<T, 64, false><<<grid, KV8_THREADS, 0, st>>>(p);            \
+#define KV8_GO_LONG(T, HDV, VECV)                                                                        \
+    do {                                                                                                 \
+        if (p.bitmaps) kv_store_fp8_kernel<T, HDV, VECV, true><<<grid, KV8_THREADS, 0, st>>>(p);         \
+        else kv_store_fp8_kernel<T, HDV, VECV, false><<<grid, KV8_THREADS, 0, st>>>(p);                  \
+    } while (0)
+#define KV8_GO(T)                                                                                        \
+    do {                                                                                                 \
+        if (head_dim == 128) {                                                                           \
+            if (vec) KV8_GO_LONG(T, 128, true);                                                          \
+            else KV8_GO_LONG(T, 128, false);                                                             \
+        } else if (vec) KV8_GO_LONG(T, 64, true);                                                        \
+        else KV8_GO_LONG(T, 64, false);                                                                  \
     } while (0)
     if (dtype == ODSD_DT_BF16) KV8_GO(__bf16);
     else KV8_GO(half_t);
 #undef KV8_GO
+#undef KV8_GO_LONG
     ODSD_CHECK_LAUNCH();
     return ODSD_OK;
 }

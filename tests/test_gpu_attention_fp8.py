@@ -95,7 +95,8 @@ def test_verify_and_chunks(dev, dtype, heads, H, D, bs, most):
 
 
 @pytest.mark.parametrize("heads, H, D, q, L, bs", [(32, 4, 128, 1, 9000, 256), (8, 2, 64, 1, 20001, 16), (32, 8, 128, 6, 5003, 64),
-                                                  (16, 2, 128, 8, 6007, 48), (8, 1, 128, 100, 3001, 256), (4, 4, 64, 300, 1777, 32)])
+                                                  (16, 2, 128, 8, 6007, 48), (8, 1, 128, 100, 3001, 256), (4, 4, 64, 300, 1777, 32),
+                                                  (16, 1, 128, 8, 9001, 64), (8, 1, 64, 4, 30000, 256), (3, 1, 128, 1, 40000, 128)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_long_sequences_are_shared_out(dev, heads, H, D, q, L, bs, dtype):
     """units are cut into pieces whose results are joined; short sequences beside them"""
