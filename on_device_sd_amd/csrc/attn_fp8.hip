@@ -537,16 +537,16 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
                 if (!active) continue;
                 const char *kt = lds + (i & 1) * (2 * TILEB), *vt = kt + TILEB;
                 // 64 keys.  While a fragment is multiplied the next one is widened and the one behind it read; the scheduling barriers keep
-                // the compiler from doing that for all of them first, whose registers would push others out to memory.  MASKED: some row
-                // does not see some key
-                auto keys64 = [&](auto masked_c, const int half, const int k0) {
-                    constexpr bool MASKED = decltype(masked_c)::value;
+                // the compiler from doing that for all of them first, whose registers would push others out to memory.  masked: some row
+                // does not see some key.  (One body for both: with one each the accumulators are copied where they meet, and some
+                // registers go to memory.)
+                auto keys64 = [&](const bool masked, const int half, const int k0) {
                     const float4_t sc = at_scale[8 * i + 4 * half + kq];
                     const char *v_at = vt + c * FP8_TILE + ((4 * half + kq) ^ (c >> 1)) * 16;
                     auto k_piece = [&](const int x) { return *(const uint4_t *)(kt + k_at[x % NC] + (64 * half + 4 * (x / NC)) * HD); };
                     auto v_piece = [&](const int db) { return *(const uint4_t *)(v_at + 16 * db * FP8_TILE); };
-                    uint4_t keep;
-                    if constexpr (MASKED) {
+                    uint4_t keep = {0u, 0u, 0u, 0u};
+                    if (masked) {
                         keep = fp8_keep(k0 + 16 * kq, L);
                         fp8_nan_rows<T, RB, NDB>(v_piece, keep, k0 + 16 * kq, kmax, o);
                         __builtin_amdgcn_sched_barrier(0);
@@ -571,12 +571,12 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
                         __builtin_amdgcn_sched_barrier(0);
                         if (x + 1 == 4 * NC) {
                             V8 pf[RB][2];
-                            fp8_weights<T, RB, NDB>(st, sc.x, sc.y, sc.z, MASKED, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
+                            fp8_weights<T, RB, NDB>(st, sc.x, sc.y, sc.z, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
                             __builtin_amdgcn_sched_barrier(0);
                             // (w is V's first piece, next its second)
                             uint4_t wn = next;
                             auto widen = [&]() {
-                                if constexpr (MASKED) w = fp8_clean(w, keep);
+                                if (masked) w = fp8_clean(w, keep);
                                 lo = fp8_widen8<T>(w.x, w.y);
                                 hi = fp8_widen8<T>(w.z, w.w);
                                 w = wn;
@@ -598,8 +598,7 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
 #pragma unroll
                 for (int sub = 0; sub < (WK == 1 ? 2 : 1); ++sub) {
                     const int half = WK == 1 ? sub : wk, k0 = key0 + FP8_TILE * i + 64 * half;
-                    if (k0 + 63 > kmin) keys64(std::true_type{}, half, k0);
-                    else keys64(std::false_type{}, half, k0);
+                    keys64(k0 + 63 > kmin, half, k0);
                 }
             }
         }
