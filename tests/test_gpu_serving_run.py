@@ -158,3 +158,38 @@ def test_on_another_stream(dev):
     want = odsd.paged_attention_fp8(q, twin, context)
     assert torch.equal(a, want) and torch.equal(b, odsd.adjust_logits(want.flatten(1).float(), {}, repetition=2.0, tokens=slots.view(2, 2000)))
     assert torch.equal(cache.k.view(torch.uint8), twin.k.view(torch.uint8)) and torch.equal(cache.scales, twin.scales)
+
+
+def test_two_at_once(dev):
+    """the same calls on two streams, neither waiting for the other: every one has its own workspace"""
+    g = torch.Generator(device=dev).manual_seed(4)
+    n, new = 3, 6000
+    key = torch.randn(2, new, H, D, generator=g, device=dev).to(torch.bfloat16)
+    slots = torch.stack([torch.randperm(400 * BS, generator=g, device=dev)[:new].to(torch.int32) for _ in range(2)])
+    tables = torch.arange(375, dtype=torch.int32, device=dev).view(n, 125)
+    q = torch.randn(2, n, HQ, D, generator=g, device=dev).to(torch.bfloat16)
+    logits = torch.randn(2, n, 5000, generator=g, device=dev)
+    tokens = torch.randint(0, 5000, (2, n, 700), generator=g, device=dev)
+    context = {"block_tables": tables, "context_lens": torch.tensor([2000, 1500, 7], dtype=torch.int32, device=dev)}
+
+    def step(i, cache):
+        odsd.store_kvcache_fp8(key[i], key[i], cache, slots[i])
+        odsd.copy_cache_blocks([cache], [0, 1, 2], [397, 398, 399])
+        return odsd.paged_attention_fp8(q[i], cache, context), odsd.adjust_logits(logits[i], {}, tokens=tokens[i], repetition=1.5, frequency=0.25)
+
+    caches = [[odsd.KVCacheFP8.zeros(400, H, BS, D, dev) for _ in range(2)] for _ in range(2)]
+    want = [step(i, caches[0][i]) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i, caches[1][i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(caches[0][i].k.view(torch.uint8), caches[1][i].k.view(torch.uint8)) and torch.equal(caches[0][i].scales, caches[1][i].scales)
+        for a, x in got[i]:
+            assert torch.equal(torch.isnan(a), torch.isnan(want[i][0])) and torch.equal(a.nan_to_num(), want[i][0].nan_to_num()) and torch.equal(x, want[i][1])
