@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 DT_F32 = 0
 DT_BF16 = 1
 DT_F16 = 2
+ERR_SHAPE = 2                          # ODSD_ERR_SHAPE
 TABLE_COLS = 4
 
 

@@ -66,8 +66,6 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         raise ValueError("block_tables must be contiguous int32")
     if n == 0:
         return
-    if min(src) < 0 or min(dst) < 0 or max(src) >= num_blocks or max(dst) >= num_blocks:
-        raise ValueError(f"block numbers must be in [0, {num_blocks})")
     places = set(dst)
     if len(places) != n or not places.isdisjoint(src):
         raise ValueError("every destination must be named once, and be no source")
@@ -75,7 +73,11 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         raise ValueError("a block that moves has one destination")
     if num_blocks >> 31:
         raise _lib.OdsdError(f"copy_cache_blocks: unsupported sizes: {num_blocks} blocks")
-    from_, to = array("i", src), array("i", dst)            # (no whole number: TypeError)
+    outside = f"block numbers must be in [0, {num_blocks})"
+    try:
+        from_, to = array("i", src), array("i", dst)        # (no whole number: TypeError)
+    except OverflowError:
+        raise ValueError(outside) from None
     from_at, to_at = from_.buffer_info()[0], to.buffer_info()[0]
     lib = _lib.load()
     tensors_, tables = [t for t in tensors if t.numel()], block_tables
@@ -87,6 +89,8 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         rc = lib.odsd_copy_blocks((C.c_void_p * k)(*[t.data_ptr() for t in some]), (C.c_int64 * k)(*[b // num_blocks for b in layer_bytes]),
                                   (C.c_int64 * k)(*layer_bytes), (C.c_int32 * k)(*layers), k, from_at, to_at, n, num_blocks,
                                   _ptr(tables), 0 if tables is None else tables.numel(), _stream())
+        if rc == _lib.ERR_SHAPE:                            # (every number is looked at before anything is launched)
+            raise ValueError(outside)
         if rc:
             _lib.check(rc, "odsd_copy_blocks")
         tables = None
