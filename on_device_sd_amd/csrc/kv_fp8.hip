@@ -14,8 +14,9 @@
 // loads of a thread have no branch between them (rows that are not there load the leader's and count as zeros): with one each 76 us.
 // Three workgroups to a CU; with four the registers do not suffice (87).
 // A decode step is a chain of four trips to memory, 64 rows of 8 heads 5.1 us, and then a number of workgroups: where the leader's sixteenth neighbour
-// behind is no row of its block, a workgroup looks through the list once for several heads, and its wavefronts take a K or V each.  (A workgroup for each
-// K and V / so: 128 rows 14.7 / 6.2, 512 44 / 20; a prompt of 2000, whose leaders wait for no other workgroup, 14.4 / 15.9.)
+// behind is no row of its block, a workgroup looks through the list once for several heads, and its wavefronts take one K or V after the other, the
+// next one's rows on their way meanwhile.  (A workgroup for each K and V / so: 128 rows 14.7 / 6.4, 512 44 / 18, 1024 of 4 heads 48 / 15.  Without
+// asking ahead 1024 take 20, and 64 rows 5.0 instead of 5.3.)
 #include "fp8.h"
 #include <type_traits>
 
@@ -52,7 +53,7 @@ __device__ __forceinline__ bool kv_entry(const KvFp8Params &p, const int i, int 
 // those for few rows.
 __device__ __forceinline__ bool kv_run(const KvFp8Params &p, const int e, const int block) {
     int slot;
-    return e + KV8_FEW < p.N && kv_entry(p, e + KV8_FEW, slot) && slot / p.bs == block;
+    return p.run_wgs > 0 && e + KV8_FEW < p.N && kv_entry(p, e + KV8_FEW, slot) && slot / p.bs == block;
 }
 
 __global__ __launch_bounds__(KV8_CHUNK) void kv_bitmap_kernel(const KvFp8Params p) {
@@ -192,29 +193,42 @@ __device__ __forceinline__ void kv_store_few(const KvFp8Params &p, const int wg,
             __syncthreads();
             const int rows = *count, pieces = rows * NP;
             const bool anew = row_of[0] >= 0, held = rows <= KV8_FEW;
-            for (int t = wave; t < 2 * heads; t += KV8_THREADS / 64) {
+            auto source = [&](const int i) {        // the row of piece i
+                const int from = row_of[present[i / NP]];
+                return p.src ? p.src[from] : from;
+            };
+            int64_t rows_at[HELD];              // of this lane's pieces, where they can be held
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) rows_at[u] = held && lane + 64 * u < pieces ? source(lane + 64 * u) : 0;
+            // a K or V: what is asked for (`ask`) while the one before is worked on (`put`)
+            struct Task {
+                uint4_t hold[HELD];
+                float was;
+            };
+            auto ask = [&](Task &k, const int t) {
+                const int h = h0 + (t >> 1);
+                const bool is_v = t & 1;
+                const uint16_t *x = (is_v ? p.value : p.key) + (int64_t)h * (is_v ? p.value_head : p.key_head);
+                const int64_t token = is_v ? p.value_token : p.key_token;
+                k.was = p.scales[2 * ((int64_t)block * p.KVH + h) + (is_v ? 1 : 0)];
+#pragma unroll
+                for (int u = 0; u < HELD; ++u) {
+                    k.hold[u] = uint4_t{0u, 0u, 0u, 0u};
+                    if (held && lane + 64 * u < pieces) k.hold[u] = kv_load8<VEC>(x + rows_at[u] * token + 8 * ((lane + 64 * u) % NP));
+                }
+            };
+            auto put = [&](const Task &k, const int t) {
                 const int h = h0 + (t >> 1);
                 const bool is_v = t & 1;
                 const uint16_t *x = (is_v ? p.value : p.key) + (int64_t)h * (is_v ? p.value_head : p.key_head);
                 const int64_t token = is_v ? p.value_token : p.key_token, bh = (int64_t)block * p.KVH + h;
-                float *scale_at = p.scales + 2 * bh + (is_v ? 1 : 0);
-                const float was = *scale_at;
-                auto load = [&](const int i) {
-                    const int from = row_of[present[i / NP]];
-                    return kv_load8<VEC>(x + (int64_t)(p.src ? p.src[from] : from) * token + 8 * (i % NP));
-                };
-                uint4_t hold[HELD];
-#pragma unroll
-                for (int u = 0; u < HELD; ++u) {
-                    hold[u] = uint4_t{0u, 0u, 0u, 0u};
-                    if (held && lane + 64 * u < pieces) hold[u] = load(lane + 64 * u);
-                }
+                auto load = [&](const int i) { return kv_load8<VEC>(x + source(i) * token + 8 * (i % NP)); };
                 auto top_of = [&](auto finite_c) {
                     constexpr bool FINITE = decltype(finite_c)::value;
                     uint32_t m = 0u;
                     if (held) {
 #pragma unroll
-                        for (int u = 0; u < HELD; ++u) m = kv_top8<T, FINITE>(hold[u], m);
+                        for (int u = 0; u < HELD; ++u) m = kv_top8<T, FINITE>(k.hold[u], m);
                     } else {
 #pragma unroll 1
                         for (int i = lane; i < pieces; i += 64) m = kv_top8<T, FINITE>(load(i), m);
@@ -224,24 +238,33 @@ __device__ __forceinline__ void kv_store_few(const KvFp8Params &p, const int wg,
                 uint32_t top = top_of(std::false_type{});
                 const bool finite = top < KvBits<T>::INF;
                 if (!finite) top = top_of(std::true_type{});
-                const float old = anew ? 0.0f : was, scale = fmaxf(old, fp8_scale_of(kv_value<T>((uint16_t)top)));
+                const float old = anew ? 0.0f : k.was, scale = fmaxf(old, fp8_scale_of(kv_value<T>((uint16_t)top)));
                 uint8_t *codes = (is_v ? p.v_cache : p.k_cache) + bh * bs * HD;
                 if (!anew && old < scale) {
                     kv_rescale(codes, bs * HD / 16, old / scale, lane, 64);
                     __threadfence_block();      // (the codes are there before the new ones come)
                 }
-                if (lane == 0) *scale_at = scale;
-                auto put = [&](const int i, const uint4_t w) {
+                if (lane == 0) p.scales[2 * bh + (is_v ? 1 : 0)] = scale;
+                auto store = [&](const int i, const uint4_t w) {
                     kv_put<HD>(codes, bs, is_v, present[i / NP], 8 * (i % NP), finite ? kv_codes8<T, true>(w, scale) : kv_codes8<T, false>(w, scale));
                 };
                 if (held) {
 #pragma unroll
                     for (int u = 0; u < HELD; ++u)
-                        if (lane + 64 * u < pieces) put(lane + 64 * u, hold[u]);
+                        if (lane + 64 * u < pieces) store(lane + 64 * u, k.hold[u]);
                 } else {
 #pragma unroll 1
-                    for (int i = lane; i < pieces; i += 64) put(i, load(i));
+                    for (int i = lane; i < pieces; i += 64) store(i, load(i));
                 }
+            };
+            constexpr int W = KV8_THREADS / 64;
+            Task k[2];
+            if (wave < 2 * heads) ask(k[0], wave);
+            for (int t = wave; t < 2 * heads; t += 2 * W) {
+                if (t + W < 2 * heads) ask(k[1], t + W);
+                put(k[0], t);
+                if (t + 2 * W < 2 * heads) ask(k[0], t + 2 * W);
+                if (t + W < 2 * heads) put(k[1], t + W);
             }
         }
     }
@@ -485,14 +508,15 @@ extern "C" int odsd_kv_store_fp8(const void *key, int64_t key_token_stride, int6
     p.per_wg = (int)max((int64_t)1, min((int64_t)min(256, block_size), (int64_t)N * num_kv_heads / 1024));
     int64_t few = 0;
     if (N <= KV8_LONG) {
-        p.per_wg = max(p.per_wg, min(KV8_FEW, N));            // (a run has more than KV8_FEW entries)
+        p.per_wg = 64;                                        // (leaders of runs stand further apart than others)
         const int64_t heads = ((int64_t)N * num_kv_heads + KV8_WGS - 1) / KV8_WGS;
         p.few_heads = (int)min((int64_t)num_kv_heads, max((int64_t)2, heads));
         p.few_groups = (num_kv_heads + p.few_heads - 1) / p.few_heads;
         p.few_entries = (int)max((int64_t)1, (int64_t)N * p.few_groups / KV8_WGS);
         few = ((int64_t)N + p.few_entries - 1) / p.few_entries * p.few_groups;
     }
-    const int64_t wgs = ((int64_t)N + p.per_wg - 1) / p.per_wg * num_kv_heads * 2;
+    // (a block of few tokens has no run)
+    const int64_t wgs = few && block_size <= KV8_FEW ? 0 : ((int64_t)N + p.per_wg - 1) / p.per_wg * num_kv_heads * 2;
     if (wgs + few >= (1LL << 24)) return ODSD_ERR_UNSUPPORTED;
     p.run_wgs = (int)wgs;
     const unsigned grid = (unsigned)(wgs + few);
