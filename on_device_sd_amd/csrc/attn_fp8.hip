@@ -538,9 +538,8 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
                 const char *kt = lds + (i & 1) * (2 * TILEB), *vt = kt + TILEB;
                 // 64 keys.  While a fragment is multiplied the next one is widened and the one behind it read; the scheduling barriers keep
                 // the compiler from doing that for all of them first, whose registers would push others out to memory.  masked: some row
-                // does not see some key.  (One body for both: with one each the accumulators are copied where they meet, and some
-                // registers go to memory.)
-                auto keys64 = [&](const bool masked, const int half, const int k0) {
+                // does not see some key.
+                auto keys64 = [&](const auto masked, const int half, const int k0) {
                     const float4_t sc = at_scale[8 * i + 4 * half + kq];
                     const char *v_at = vt + c * FP8_TILE + ((4 * half + kq) ^ (c >> 1)) * 16;
                     auto k_piece = [&](const int x) { return *(const uint4_t *)(kt + k_at[x % NC] + (64 * half + 4 * (x / NC)) * HD); };
@@ -598,7 +597,11 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
 #pragma unroll
                 for (int sub = 0; sub < (WK == 1 ? 2 : 1); ++sub) {
                     const int half = WK == 1 ? sub : wk, k0 = key0 + FP8_TILE * i + 64 * half;
-                    keys64(k0 + 63 > kmin, half, k0);
+                    // (One body for both costs a branch here and there, two copy the accumulators where they meet and put some registers in
+                    // memory: 128 rows, whose tiles are nearly all full, a chunk 228 / 220 us; 64 rows, verify of 32 x 8 28.7 / 29.6.)
+                    if constexpr (WR < 4) keys64(k0 + 63 > kmin, half, k0);
+                    else if (k0 + 63 > kmin) keys64(std::true_type{}, half, k0);
+                    else keys64(std::false_type{}, half, k0);
                 }
             }
         }
@@ -637,8 +640,9 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
     const int64_t whole = pl.rows <= 16 ? (pl.units >= 256 ? 2048 : pl.units >= 128 ? 1024 : FP8_WHOLE) * 128 / head_dim : max((int64_t)FP8_WHOLE, 12 * pl.units);
     pl.split = !(max_keys <= whole || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
     // Few units are many pieces each, which are long to walk for one thread (one / eight, us: 4 units of 16 rows and 32768 keys 31.2 / 16.2, 16 of
-    // 16384 22.9 / 19.2, 64 of 4096 19.6 / 19.9; 4 of 64 rows and 32768 keys 39.8 / 24.9, 32 of 16384 45.9 / 46.5, 128 of 4096 46.1 / 52.2).
-    pl.join = pl.units <= 32 ? FP8_JOIN : 1;
+    // 16384 22.9 / 19.2, 64 of 4096 19.6 / 19.9; 4 of 64 rows and 32768 keys 39.8 / 24.9, 32 of 16384 45.9 / 46.5, 128 of 4096 46.1 / 52.2; one
+    // sequence of 777 keys, four pieces a unit, 8.0 / 8.3).
+    pl.join = pl.units <= 32 && steps > FP8_JOIN ? FP8_JOIN : 1;
     pl.shares = (int)min(pl.units * steps, (int64_t)pl.n_wg);
     pl.bytes = pl.split ? odsd_round_up((size_t)2 * pl.shares * pl.rows * (head_dim + 4) * sizeof(float), 256) : 0;
     return pl;
