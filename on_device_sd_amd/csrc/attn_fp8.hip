@@ -21,7 +21,7 @@
 // chunk of 2048 tokens at 4096 keys 397 and 226.)
 //
 // Measured, 32 / 4 heads of 128, bf16, in a graph: a token each of 64 sequences of 750 to 3000 keys 29 us, 4.2 TB/s of codes; 4 tokens each of 64
-// sequences of 8000 to 8192 keys 114 us, 4.7 TB/s; a chunk of 512 tokens each of 8 sequences of 8192 keys 514 us, 990 TFLOP/s.  A short call is a
+// sequences of 8000 to 8192 keys 114 us, 4.7 TB/s; a chunk of 512 tokens each of 8 sequences of 8192 keys 506 us, 1000 TFLOP/s.  A short call is a
 // list, a lookup, a tile and a merge, each waiting for the one before: one sequence of 777 keys 8.0 us.
 #include "attn_list.h"
 #include "fp8.h"
@@ -531,6 +531,10 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
                 at_scale[tid] = float4_t{sc, ev, iv, 0.f};
             }
             for (int i = 0; i < nt; ++i) {
+                // (128 rows: a wavefront that has got as far as a step's first product with V goes in front of the SIMD's other one until the step
+                // ends; the two then want the matrix pipe and the vector unit at different times: a chunk 236 / 226 us, 2048 tokens of one
+                // sequence 140 / 129.  In front during every product 227, during those with K 232, with V 231.)
+                if constexpr (WR == 4) __builtin_amdgcn_s_setprio(0);
                 ODSD_WAIT_VMCNT_LGKM0(0);                  // this wavefront's copies of step i have landed
                 __builtin_amdgcn_s_barrier();              // ... everybody's, and all are done with step i - 1
                 if (i + 1 < nt) copy(i + 1);
@@ -572,6 +576,7 @@ __global__ __launch_bounds__(256, 2) void attn_fp8_tile_kernel(const AttnFp8Para
                             V8 pf[RB][2];
                             fp8_weights<T, RB, NDB>(st, sc.x, sc.y, sc.z, masked, k0 + 16 * kq, kmax, m_run, l_run, o, pf);
                             __builtin_amdgcn_sched_barrier(0);
+                            if constexpr (WR == 4) __builtin_amdgcn_s_setprio(1);
                             // (w is V's first piece, next its second)
                             uint4_t wn = next;
                             auto widen = [&]() {
