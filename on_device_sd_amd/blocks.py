@@ -131,7 +131,8 @@ class BlockPool:
 
     def append(self, seqs: Sequence[SequenceSlots], counts: Sequence[int]) -> None:
         """Room for ``counts[i]`` more tokens of each sequence, whose num_tokens grows by them.  A part-filled last block that another
-        sequence holds too is replaced by a copy (all copies in one launch).  Too few free blocks: RuntimeError, nothing is changed."""
+        sequence holds too is replaced by a copy (all copies in one launch).  Too few free blocks: RuntimeError.  A call that raises, for
+        those or for a copy that is refused, changes nothing."""
         if len(seqs) != len(counts) or any(c < 0 for c in counts):
             raise ValueError("every sequence needs a count of new tokens, 0 or more")
         if len({id(s) for s in seqs}) != len(seqs):
@@ -158,24 +159,22 @@ class BlockPool:
             need += new + copies
         if need > len(self._free):
             raise RuntimeError(f"{need} blocks are needed, {len(self._free)} are free")
-        src, dst = [], []
-        for s, c, copies, new in plan:
-            if copies:
+        free = iter(self._free[:-need - 1:-1])             # in the order in which they are taken
+        plan = [(s, c, next(free) if copies else None, [next(free) for _ in range(new)]) for s, c, copies, new in plan]
+        copied = [(s.block_table[s.num_tokens // self.block_size], to) for s, _, to, _ in plan if to is not None]
+        if copied and self.caches:                         # (before the books change: a copy that is refused leaves them as they were)
+            copy_cache_blocks(self.caches, [b for b, _ in copied], [to for _, to in copied], self.block_dim)
+        del self._free[len(self._free) - need:]
+        for s, c, to, new in plan:
+            if to is not None:
                 at = s.num_tokens // self.block_size
-                b, to = s.block_table[at], self._take()
-                src.append(b)
-                dst.append(to)
+                self._drop([s.block_table[at]])
                 s.block_table[at] = to
-                self._drop([b])
-            s.block_table.extend(self._take() for _ in range(new))
+                self.holders[to] = 1
+            for b in new:
+                self.holders[b] = 1
+            s.block_table.extend(new)
             s.num_tokens += c
-        if src and self.caches:
-            copy_cache_blocks(self.caches, src, dst, self.block_dim)
-
-    def _take(self) -> int:
-        b = self._free.pop()
-        self.holders[b] = 1
-        return b
 
     def fork(self, seq: SequenceSlots) -> SequenceSlots:
         """Another sequence with the same tokens so far, in the same blocks; whichever writes to the last one first gets a copy."""
