@@ -32,6 +32,21 @@ def _block_list(blocks: Blocks) -> List[int]:
     return list(blocks)
 
 
+def _tensors_of(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], block_dim: int) -> List[torch.Tensor]:
+    if block_dim not in (0, 1):
+        raise ValueError("block_dim is 0, or 1 behind a dimension of layers")
+    tensors: List[torch.Tensor] = []
+    for c in caches:
+        tensors += [c.k, c.v, c.scales] if isinstance(c, KVCacheFP8) else [c]
+    return tensors
+
+
+def _check_caches(tensors: Sequence[torch.Tensor], num_blocks: int, block_dim: int) -> None:
+    for t in tensors:
+        if t.dim() <= block_dim or t.shape[block_dim] != num_blocks or not t.is_contiguous():
+            raise ValueError(f"a cache {tuple(t.shape)}: caches must be contiguous, with {num_blocks} blocks along dimension {block_dim}")
+
+
 def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blocks: Blocks, dst_blocks: Blocks, block_dim: int = 0,
                       block_tables: Optional[torch.Tensor] = None) -> None:
     """Block ``src_blocks[i]`` of every cache to block ``dst_blocks[i]``, in one launch (16 tensors and 384 pairs of them each).
@@ -40,13 +55,9 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
     blocks), and ``KVCacheFP8``.  The lists are the host's (sequences or CPU tensors) and are read before the call returns: a graph
     that captures it copies these blocks at every replay.  A destination is named once and is no source (else ValueError).
     ``block_tables`` (int32, on the GPU, contiguous): entries that name a source name its destination afterwards: the blocks move."""
-    tensors: List[torch.Tensor] = []
-    for c in caches:
-        tensors += [c.k, c.v, c.scales] if isinstance(c, KVCacheFP8) else [c]
+    tensors = _tensors_of(caches, block_dim)
     if not tensors:
         raise ValueError("no cache to copy in")
-    if block_dim not in (0, 1):
-        raise ValueError("block_dim is 0, or 1 behind a dimension of layers")
     dev = tensors[0].get_device()
     _same_device(dev, *tensors, block_tables)
     if dev != _raw_device():
@@ -59,9 +70,7 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
     if tensors[0].dim() <= block_dim:
         raise ValueError(f"a cache {tuple(tensors[0].shape)} has no dimension {block_dim} of blocks")
     num_blocks = tensors[0].shape[block_dim]
-    for t in tensors:
-        if t.dim() <= block_dim or t.shape[block_dim] != num_blocks or not t.is_contiguous():
-            raise ValueError(f"caches must be contiguous, with {num_blocks} blocks along dimension {block_dim}")
+    _check_caches(tensors, num_blocks, block_dim)
     if block_tables is not None and (block_tables.dtype != torch.int32 or not block_tables.is_contiguous()):
         raise ValueError("block_tables must be contiguous int32")
     if n == 0:
@@ -105,10 +114,10 @@ class BlockPool:
     def __init__(self, num_blocks: int, block_size: int, caches: Sequence[Union[torch.Tensor, KVCacheFP8]] = (), block_dim: int = 0):
         if num_blocks < 0 or block_size <= 0:
             raise ValueError(f"a pool of {num_blocks} blocks of {block_size} tokens")
-        for c in caches:
-            t = c.k if isinstance(c, KVCacheFP8) else c
-            if t.dim() <= block_dim or t.shape[block_dim] != num_blocks:
-                raise ValueError(f"a cache {tuple(t.shape)} has not {num_blocks} blocks along dimension {block_dim}")
+        tensors = _tensors_of(caches, block_dim)
+        _check_caches(tensors, num_blocks, block_dim)
+        if len({t.device for t in tensors}) > 1:
+            raise ValueError("the caches of a pool are on one device")
         self.num_blocks, self.block_size, self.caches, self.block_dim = num_blocks, block_size, list(caches), block_dim
         self.holders = [0] * num_blocks                    # sequences that hold a block
         self._free = list(range(num_blocks - 1, -1, -1))   # the lowest comes last, and is taken first

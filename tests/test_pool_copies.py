@@ -45,3 +45,17 @@ def test_blocks_are_taken_in_order():
     pool.append([a, c, d, b], [7, 1, 1, 5])          # (the last to write keeps the block)
     assert [a.block_table, c.block_table, d.block_table, b.block_table] == [[0, 2, 3, 4], [0, 5], [0, 1], [6, 7]]
     assert pool.holders == [3, 1, 1, 1, 1, 1, 1, 1, 0, 0, 0, 0] and pool._free == [11, 10, 9, 8]
+
+
+def test_caches_that_could_not_be_copied_are_refused():
+    c8 = lambda k=(6, 2, 16, 64), v=(6, 2, 64, 16), s=(6, 2, 2): odsd.KVCacheFP8(*(torch.zeros(t) for t in (k, v, s)))  # noqa: E731
+    rows = torch.zeros(6, 4, 8)
+    for caches in ([rows.transpose(1, 2)], [rows, torch.zeros(12, 4, 8)[::2]], [c8(v=(5, 2, 64, 16))], [c8(s=(7, 2, 2))], [rows, c8(k=(5, 2, 16, 64))],
+                   [rows, torch.zeros((6, 4), device="meta")], [torch.zeros(())]):
+        with pytest.raises(ValueError):
+            odsd.BlockPool(6, 16, caches)
+    for caches, dim in (([rows], 0), ([c8(), rows], 0), ([torch.zeros(3, 6, 4)], 1), ([], 0)):
+        assert odsd.BlockPool(6, 16, caches, dim).num_free == 6
+    for dim in (2, -1):
+        with pytest.raises(ValueError):
+            odsd.BlockPool(6, 16, [torch.zeros(6, 6, 6)], dim)
