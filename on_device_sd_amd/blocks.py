@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import dataclasses
 from array import array
-from typing import Dict, List, Optional, Sequence, Union
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -30,6 +30,23 @@ def _block_list(blocks: Blocks) -> List[int]:
             raise TypeError(f"block numbers must be whole numbers, got {blocks.dtype}")
         return blocks.flatten().tolist()
     return list(blocks)
+
+
+def _block_pairs(src_blocks: Blocks, dst_blocks: Blocks, moves: bool) -> Tuple[array, array]:
+    """Both lists as the library takes them.  They are compared as numbers: two tensors that hold the same number are not equal to a set."""
+    try:
+        src, dst = (array("i", _block_list(blocks)) for blocks in (src_blocks, dst_blocks))      # (no whole number: TypeError)
+    except OverflowError:
+        raise ValueError("block numbers must be those of blocks of the caches") from None
+    n = len(src)
+    if len(dst) != n:
+        raise ValueError(f"{n} sources for {len(dst)} destinations")
+    places = set(dst)
+    if len(places) != n or not places.isdisjoint(src):
+        raise ValueError("every destination must be named once, and be no source")
+    if moves and len(set(src)) != n:
+        raise ValueError("a block that moves has one destination")
+    return src, dst
 
 
 def _tensors_of(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], block_dim: int) -> List[torch.Tensor]:
@@ -63,10 +80,8 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
     if dev != _raw_device():
         with torch.cuda.device(dev):
             return copy_cache_blocks(tensors, src_blocks, dst_blocks, block_dim, block_tables)
-    src, dst = _block_list(src_blocks), _block_list(dst_blocks)
+    src, dst = _block_pairs(src_blocks, dst_blocks, block_tables is not None)
     n = len(src)
-    if len(dst) != n:
-        raise ValueError(f"{n} sources for {len(dst)} destinations")
     if tensors[0].dim() <= block_dim:
         raise ValueError(f"a cache {tuple(tensors[0].shape)} has no dimension {block_dim} of blocks")
     num_blocks = tensors[0].shape[block_dim]
@@ -75,19 +90,9 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         raise ValueError("block_tables must be contiguous int32")
     if n == 0:
         return
-    places = set(dst)
-    if len(places) != n or not places.isdisjoint(src):
-        raise ValueError("every destination must be named once, and be no source")
-    if block_tables is not None and len(set(src)) != n:
-        raise ValueError("a block that moves has one destination")
     if num_blocks >> 31:
         raise _lib.OdsdError(f"copy_cache_blocks: unsupported sizes: {num_blocks} blocks")
-    outside = f"block numbers must be in [0, {num_blocks})"
-    try:
-        from_, to = array("i", src), array("i", dst)        # (no whole number: TypeError)
-    except OverflowError:
-        raise ValueError(outside) from None
-    from_at, to_at = from_.buffer_info()[0], to.buffer_info()[0]
+    from_at, to_at = src.buffer_info()[0], dst.buffer_info()[0]
     lib = _lib.load()
     tensors_, tables = [t for t in tensors if t.numel()], block_tables
     for at in range(0, max(len(tensors_), 1), _TENSORS):
@@ -99,7 +104,7 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
                                   (C.c_int64 * k)(*layer_bytes), (C.c_int32 * k)(*layers), k, from_at, to_at, n, num_blocks,
                                   _ptr(tables), 0 if tables is None else tables.numel(), _stream())
         if rc == _lib.ERR_SHAPE:                            # (every number is looked at before anything is launched)
-            raise ValueError(outside)
+            raise ValueError(f"block numbers must be in [0, {num_blocks})")
         if rc:
             _lib.check(rc, "odsd_copy_blocks")
         tables = None
