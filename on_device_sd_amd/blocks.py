@@ -94,10 +94,11 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
         raise _lib.OdsdError(f"copy_cache_blocks: unsupported sizes: {num_blocks} blocks")
     from_at, to_at = src.buffer_info()[0], dst.buffer_info()[0]
     lib = _lib.load()
-    tensors_, tables = [t for t in tensors if t.numel()], block_tables
+    tensors_ = [t for t in tensors if t.numel()]
     for at in range(0, max(len(tensors_), 1), _TENSORS):
         some = tensors_[at:at + _TENSORS]
         k = len(some)
+        tables = block_tables if at + _TENSORS >= len(tensors_) else None      # (the last launch has them: where one is refused nothing has moved)
         layers = [t.shape[0] if block_dim else 1 for t in some]
         layer_bytes = [t.numel() // l * t.element_size() for t, l in zip(some, layers)]
         rc = lib.odsd_copy_blocks((C.c_void_p * k)(*[t.data_ptr() for t in some]), (C.c_int64 * k)(*[b // num_blocks for b in layer_bytes]),
@@ -107,7 +108,6 @@ def copy_cache_blocks(caches: Sequence[Union[torch.Tensor, KVCacheFP8]], src_blo
             raise ValueError(f"block numbers must be in [0, {num_blocks})")
         if rc:
             _lib.check(rc, "odsd_copy_blocks")
-        tables = None
     _wrote(*tensors, block_tables)
 
 
