@@ -70,6 +70,9 @@ __global__ __launch_bounds__(KV8_CHUNK) void kv_bitmap_kernel(const KvFp8Params 
     if (threadIdx.x < KV8_BITS / 32) p.bitmaps[(size_t)threadIdx.x * p.n_chunks + blockIdx.x] = bits[threadIdx.x];
 }
 
+// what the codes under one scale are multiplied by for the next; 0: the block held nothing.  A quotient that fp32 does not hold as a
+// normal number leaves of every number zero, and so does the smallest one that it does hold: with a 0 a NaN would go too.
+__device__ __forceinline__ float kv_ratio(const float old, const float scale) { return old > 0.0f ? fmaxf(old / scale, 1.17549435e-38f) : 0.0f; }
 // n times 16 codes of a block times `ratio`, a power of two (0: the block held nothing, whatever its bytes are)
 __device__ __forceinline__ void kv_rescale(uint8_t *codes, const int n, const float ratio, const int first, const int step) {
 #pragma unroll 1
@@ -241,7 +244,7 @@ __device__ __forceinline__ void kv_store_few(const KvFp8Params &p, const int wg,
                 const float old = anew ? 0.0f : k.was, scale = fmaxf(old, fp8_scale_of(kv_value<T>((uint16_t)top)));
                 uint8_t *codes = (is_v ? p.v_cache : p.k_cache) + bh * bs * HD;
                 if (!anew && old < scale) {
-                    kv_rescale(codes, bs * HD / 16, old / scale, lane, 64);
+                    kv_rescale(codes, bs * HD / 16, kv_ratio(old, scale), lane, 64);
                     __threadfence_block();      // (the codes are there before the new ones come)
                 }
                 if (lane == 0) p.scales[2 * bh + (is_v ? 1 : 0)] = scale;
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(KV8_THREADS, 3) void kv_store_fp8_kernel(const KvFp
         const float scale = fmaxf(old, fp8_scale_of(amax));
         uint8_t *codes = (is_v ? p.v_cache : p.k_cache) + bh * bs * HD;
         if (!anew && old < scale) {
-            kv_rescale(codes, bs * HD / 16, old / scale, tid, KV8_THREADS);
+            kv_rescale(codes, bs * HD / 16, kv_ratio(old, scale), tid, KV8_THREADS);
         }
         __syncthreads();                        // (the codes are there before the new ones come)
         if (tid == 0) *scale_at = scale;
