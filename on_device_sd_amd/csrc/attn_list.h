@@ -200,14 +200,16 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
     if (wa == wb || (BY_SHARE && wa != (int)blockIdx.x)) return;
     const int row = (int)blockIdx.z * RPW + (int)threadIdx.x / TPR % RPW, d = 4 * ((int)threadIdx.x % TPR), g = (int)threadIdx.x / (TPR * RPW);
     const int r = rg * ROWS + row;
-    if (row >= ROWS || r >= sq.ql * p.Gq) return;
+    const bool there = row < ROWS && r < sq.ql * p.Gq;
+    // (G > 1: all threads of a workgroup that has a row come to the barrier below)
+    if (G == 1 ? !there : rg * ROWS + (int)blockIdx.z * RPW >= sq.ql * p.Gq) return;
     const float *base = p.part + row * XROW;
     const size_t slot = (size_t)ROWS * XROW;
     auto piece = [&](const int w) { return base + (size_t)(2 * w + (w == wa && a > wa * pl.share ? 1 : 0)) * slot; };
     float m = -INFINITY, l = 0.0f;
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
     constexpr int SB = 4;
-    for (int w0 = wa + SB * g; w0 <= wb; w0 += SB * G) {
+    for (int w0 = wa + SB * g; there && w0 <= wb; w0 += SB * G) {
         float ms[SB], ls[SB];
         float4_t os[SB];
 #pragma unroll
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const AttnParams p) {
         ml[g][at] = float2_t{m, l};
         os[g][at] = acc;
         __syncthreads();
-        if (g > 0) return;
+        if (g > 0 || !there) return;
 #pragma unroll
         for (int u = 1; u < G; ++u) m = fmaxf(m, ml[u][at].x);
         const float ref = m == -INFINITY ? 0.0f : m;
