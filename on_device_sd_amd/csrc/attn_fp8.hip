@@ -655,6 +655,7 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
 static bool attn_fp8_shape_ok(int64_t n_seqs, int64_t max_q_len, int num_heads, int num_kv_heads, int head_dim, int block_size, int max_blocks) {
     return n_seqs > 0 && max_q_len > 0 && num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 &&
            (head_dim == 64 || head_dim == 128) && block_size > 0 && block_size % 16 == 0 && block_size <= FP8_MAX_BLOCK && max_blocks > 0 &&
+           (int64_t)max_blocks * block_size <= (1LL << 30) &&                     // (a position and a list step behind it are 31 bits)
            (max_q_len * (num_heads / num_kv_heads) + 63) / 64 <= 65535 &&
            ((max_q_len + 128) * (num_heads / num_kv_heads) + 128) * (num_heads / num_kv_heads) < (1LL << 32) && n_seqs * num_kv_heads <= 0x7fffffffLL &&
            n_seqs * num_kv_heads * ((max_q_len * (num_heads / num_kv_heads) + 63) / 64) <= (1LL << 24) - 1;
@@ -695,7 +696,7 @@ extern "C" int odsd_paged_attention_fp8(const void *q, const void *k_cache, cons
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.scales = scales; p.n_blocks = n_blocks;
     p.gq_inverse = p.Gq > 1 ? (uint32_t)(((1ULL << 32) + (uint64_t)p.Gq - 1) / (uint64_t)p.Gq) : 0u;
-    p.max_keys = (int)min(max_keys, (int64_t)1 << 30);
+    p.max_keys = (int)max_keys;
     p.max_rg = (int)pl.rg;
     if (pl.split) {
         if (!workspace) return ODSD_ERR_NULL;

@@ -162,11 +162,12 @@ def paged_attention_fp8(q: torch.Tensor, cache: KVCacheFP8, context: Dict[str, t
         return out.zero_()
     tables, lens, q_lens = (t if t is None or (t.get_device() == dev and t.dtype == torch.int32 and t.is_contiguous())
                             else t.to(device=q.device, dtype=torch.int32).contiguous() for t in (tables, lens, q_lens))
-    lib = _lib.load()
-    nbytes = lib.odsd_paged_attention_fp8_workspace_bytes(n_seqs, most, num_heads, kv_heads, head_dim, block_size, max_blocks)
+    lib, nbytes = _lib.load(), 0
+    if not (n_tokens | n_seqs | most | num_heads | max_blocks) >> 31:        # (sizes are 31 bits in the library)
+        nbytes = lib.odsd_paged_attention_fp8_workspace_bytes(n_seqs, most, num_heads, kv_heads, head_dim, block_size, max_blocks)
     if nbytes == 0:
         raise _lib.OdsdError(f"attention over the 8-bit cache: unsupported shape: {n_seqs} sequences of up to {most} queries, {num_heads} / "
-                             f"{kv_heads} heads of {head_dim}, blocks of {block_size}")
+                             f"{kv_heads} heads of {head_dim}, {max_blocks} blocks of {block_size}")
     ws = None if nbytes == _NO_WORKSPACE else q.new_empty(nbytes // 2)       # (of two-byte numbers)
     scale = head_dim ** -0.5 if softmax_scale is None else softmax_scale
     rc = lib.odsd_paged_attention_fp8(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), tables.data_ptr(),
