@@ -183,11 +183,12 @@ __device__ __forceinline__ void fp8_locate(const AttnFp8Params &p, const int32_t
     gk = (b >= 0 && b < p.n_blocks && blk < p.max_blocks ? (uint32_t)b : 0u) * (uint32_t)p.KVH + (uint32_t)kvh;
     off = (uint32_t)(kp - blk * p.block_size);
 }
-// its scales as the scores want them: scale * sk * log2 e, log2 sv, 1 / sv
+// its scales as the scores want them: scale * sk * log2 e, log2 sv, 1 / sv.  A product that fp32 does not hold counts as the smallest or the largest
+// normal number: -inf stands for a key that is not seen, and -inf * 0 would be no number (nor 0 * inf, of a score of 0).
 __device__ __forceinline__ void fp8_scales(const AttnFp8Params &p, const uint32_t gk, float &sc, float &ev, float &iv) {
     const float2_t s2 = *(const float2_t *)(p.scales + 2 * (size_t)gk);
     const float sv = fmaxf(s2.y, FP8_MIN_SCALE);
-    sc = p.scale_log2e * fmaxf(s2.x, FP8_MIN_SCALE);
+    sc = __builtin_amdgcn_fmed3f(p.scale_log2e * fmaxf(s2.x, FP8_MIN_SCALE), 1.17549435e-38f, 3.40282347e38f);
     ev = __builtin_amdgcn_logf(sv);
     iv = __builtin_amdgcn_rcpf(sv);
 }
