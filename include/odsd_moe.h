@@ -296,7 +296,8 @@ int odsd_kv_store(const void *key, const void *value, int64_t key_stride, int64_
  *   query j of sequence s attends positions 0 .. context_lens[s] - q_lens[s] + j; query head h
  *   reads KV head h / (num_heads / num_kv_heads); scores scaled by softmax_scale (> 0); fp32 softmax
  *   out          [n_tokens, num_heads, head_dim] in the dtype of q (ODSD_DT_BF16 or ODSD_DT_F16)
- * max_q_len: an upper bound of q_lens (sizes the launch); head_dim 64 or 128.
+ * max_q_len: an upper bound of q_lens (sizes the launch); head_dim 64 or 128.  q and out have as many rows as q_lens name (the
+ * CALLER'S duty: the call does not know how many there are).
  * workspace: odsd_paged_attention_workspace_bytes(...) bytes (with few sequences the keys of one
  * sequence are shared out between workgroups, whose partial results land there).
  * Stands in for Qwen3Attention._fallback_decode_attention and the flash_attn_with_kvcache call

@@ -21,7 +21,8 @@ struct AttnParams {
     // variable-length mode (prefill): q / k / v rows of sequence s are q[cu_q[s] ..], k[cu_k[s] ..]
     // (contiguous, no block table); both null in paged mode
     const int32_t *cu_q, *cu_k;
-    int n_tokens;              // query rows that there are: no row past them is read or written, whatever the lengths say
+    int n_tokens;              // query rows that there are.  The kernels over the 8-bit cache read and write no row past them, whatever the lengths
+                               // say; those over 16-bit keys do not look (0x7fffffff): there the lengths' sum is the caller's duty
     int max_keys, max_rg;      // streaming kernels: the keys and row groups of a sequence that the launch is sized for
     int n_wg;                  // workgroups that share the work
     int whole;                 // no unit is split and a workgroup's number says which is its own: row groups per
