@@ -342,10 +342,12 @@ size_t odsd_kv_store_fp8_workspace_bytes(int32_t N);
 
 /* odsd_paged_attention over that cache: the same queries, tables, lengths and masks, q and out of `dtype` (ODSD_DT_BF16 or ODSD_DT_F16).
  * Position p of sequence s is token p % block_size of block block_tables[s][p / block_size]; an entry that is negative or beyond the cache reads
- * block 0; positions past the table's end (max_blocks * block_size, 2^30 at most) are not attended.  Rows that attend nothing (a context of 0) are zeros.  q and out have n_tokens rows: those
- * behind the last sequence's are left as they are, and none past n_tokens is touched, whatever q_lens says.  Products of the codes with q and sums in fp32; the weights (softmax times the
- * scale of V, relative to the row's largest) are rounded to q's type once, the result once.  What a block holds behind a sequence's
- * last key is never used, and a NaN reaches the rows that attend it only.  out 8-byte aligned.
+ * block 0; positions past the table's end (max_blocks * block_size, 2^30 at most) are not attended.  Rows that attend nothing (a context of 0)
+ * are zeros.  q and out have n_tokens rows: those behind the last sequence's are left as they are, and none past n_tokens is touched, whatever
+ * q_lens says.  Products of the codes with q and sums in fp32; the weights (softmax times the scale of V, relative to the row's largest) are
+ * rounded to q's type once (fp16: below 2^-14 in steps of 2^-24), the result once.  The scales of V that a row meets may be 2^80 apart: V up to
+ * 2^24, and any fp16, beside blocks of zeros.  What a block holds behind a sequence's last key is never used, and a NaN reaches the rows
+ * that attend it only.  out 8-byte aligned.
  * workspace: odsd_paged_attention_fp8_workspace_bytes(...) bytes (0: the call is refused), 16-byte aligned. */
 int odsd_paged_attention_fp8(const void *q, const void *k_cache, const void *v_cache, const float *scales,
                              const int32_t *block_tables, const int32_t *context_lens, const int32_t *q_lens,

@@ -4,9 +4,11 @@
 //   s_ij = scale * sk(b(j)) * sum_d q_id kc_jd                       (j <= L - ql + token of i)
 //   o_i  = sum_j exp(s_ij) sv(b(j)) vc_j / sum_j exp(s_ij)
 // The scale of V joins the exponent: w_ij = 2^(s_ij log2 e + log2 sv - m_i) is what the matrix product takes, m_i the running
-// maximum of that exponent, and l_i sums w_ij / sv in fp32: nothing depends on how far the scales of two blocks are apart, and w stays
-// within what fp16 holds.  Codes become 16-bit operands of q's type in registers (exact); products and sums are fp32; w is rounded to
-// q's type once (half a step, as in the kernels over 16-bit keys), the result once.
+// maximum of that exponent, and l_i sums w_ij / sv in fp32.  A w below 2^-126 vanishes; beside the row's largest, 1 or more, it is less than
+// 2^-46 of l_i while the scales of V that the row meets are within 2^80 of each other.  (Blocks of zeros have the smallest scale, 2^-64: V up to
+// 2^24 may stand beside them, and with it all that fp16 holds.)  Codes become 16-bit operands of q's type in registers (exact); products
+// and sums are fp32; w, 2^8 at most, is rounded to q's type once (half a step, as in the kernels over 16-bit keys; fp16 has steps of 2^-24 below
+// 2^-14), the result once.
 //
 // A unit -- up to 16, 32, 64 or 128 query rows of a (sequence, KV head) -- and the way units are cut into shares of keys are those of
 // attn_list.h.  V is stored transposed, so 16 bytes are 16 keys of one dimension, and the rows of S^T = K Q^T are dealt so that a lane
@@ -21,7 +23,7 @@
 // chunk of 2048 tokens at 4096 keys 397 and 226.)
 //
 // Measured, 32 / 4 heads of 128, bf16, in a graph: a token each of 64 sequences of 750 to 3000 keys 29 us, 4.2 TB/s of codes; 4 tokens each of 64
-// sequences of 8000 to 8192 keys 114 us, 4.7 TB/s; a chunk of 512 tokens each of 8 sequences of 8192 keys 506 us, 1000 TFLOP/s.  A short call is a
+// sequences of 8000 to 8192 keys 114 us, 4.7 TB/s; a chunk of 512 tokens each of 8 sequences of 8192 keys 497 us, 1020 TFLOP/s.  A short call is a
 // list, a lookup, a tile and a merge, each waiting for the one before: one sequence of 777 keys 8.0 us.
 #include "attn_list.h"
 #include "fp8.h"
@@ -642,7 +644,8 @@ static AttnFp8Plan attn_fp8_plan(int64_t n_seqs, int64_t max_q, int gq, int64_t 
     // 29.1; 16 of 1024 12.0 / 10.0; one of 777 10.0 / 8.0: what a CU reads a microsecond bounds a unit, so heads of 64 stay whole for twice the keys, 14 /
     // 2 heads, one of 1024 5.3 / 6.7, 2048 7.6 / 7.3; 64 of 2048 9.7 / 12.3; 128 of 4096 23.1 / 28.0.  64 rows: 32 sequences of 512 keys 14.6 / 21.2, 1024 20.4 / 23.8, 2048 31.9 / 28.9;
     // 64 of 2048 41.7 / 45.1, 512 to 2048 33.9 / 39.3; 8 of 2048 30.6 / 22.0.  32 rows: 64 of 2048 33.2 / 37.2, 8 of 4096 37.9 / 18.6.  128 rows: 4
-    // sequences of 8192 keys 279 / 286, one 160 / 86.)  List positions are 32 bits wide.
+    // sequences of 8192 keys 279 / 286, one 160 / 86.)  List positions are 32 bits wide.  What this costs: from 2048 units on nothing is split however
+    // long one of them is (16 rows, 512 sequences of 500 keys 49, with one of 131072 among them 1059; 510 and one, which are split, 89).
     const int64_t whole = pl.rows <= 16 ? (pl.units >= 256 ? 2048 : pl.units >= 128 ? 1024 : FP8_WHOLE) * 128 / head_dim : max((int64_t)FP8_WHOLE, 12 * pl.units);
     pl.split = !(max_keys <= whole || pl.units >= 4 * pl.n_wg || pl.units * steps > (1LL << 30));
     // Few units are many pieces each, which are long to walk for one thread (one / eight, us: 4 units of 16 rows and 32768 keys 31.2 / 16.2, 16 of

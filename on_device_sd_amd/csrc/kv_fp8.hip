@@ -16,7 +16,8 @@
 // A decode step is a chain of four trips to memory, 64 rows of 8 heads 5.1 us, and then a number of workgroups: where the leader's sixteenth neighbour
 // behind is no row of its block, a workgroup looks through the list once for several heads, and its wavefronts take one K or V after the other, the
 // next one's rows on their way meanwhile.  (A workgroup for each K and V / so: 128 rows 14.7 / 6.4, 512 44 / 18, 1024 of 4 heads 48 / 15.  Without
-// asking ahead 1024 take 20, and 64 rows 5.0 instead of 5.3.)
+// asking ahead 1024 take 20, and 64 rows 5.0 instead of 5.3.)  Those are steps in which no scale rises.  Where one does, its wavefront goes through all codes
+// of the block, a load after the other: 64 rows of 4 heads of 128, every scale rising, blocks of 256 20 us for 4.8, of 1024 73 for 5.1, of 16 (8 heads) 5.2 for 4.2.
 #include "fp8.h"
 #include <type_traits>
 
