@@ -181,7 +181,8 @@ def adjust_logits(logits: torch.Tensor, context: Dict, *, tokens: Optional[torch
     float32 [n_seqs].  ``tokens`` int32 / int64 [n_seqs, max_tokens]: what each sequence has so far, ``token_lens`` of them (None: all), the first
     ``prompt_lens`` (None: none) its prompt, which counts for repetition only; row j of a sequence has put out its first j
     ``draft_tokens`` too.  ``bias_tokens`` int32 / ``bias_values`` float32 [n_seqs, m]: added to these tokens' logits (-1: none; of a token
-    named twice the later; hundreds of them: for thousands of forbidden tokens take a mask, the time of long lists grows with their square).  ``mask`` int32 [n, words of 32]: where bit t % 32 of word t // 32 is clear token t gets -inf; row i has mask
+    named twice the later; hundreds of them: for thousands of forbidden tokens take a mask, the time of long lists grows with their
+    square).  ``mask`` int32 [n, words of 32]: where bit t % 32 of word t // 32 is clear token t gets -inf; row i has mask
     ``mask_rows[i]`` (None: i; -1: no mask).  Rows of logits behind the last sequence's are left out: out has there what it had."""
     dev = logits.get_device()
     _same_device(dev, tokens, draft_tokens, bias_tokens, bias_values, mask, mask_rows, out)
